@@ -351,4 +351,32 @@ void LaunchConvertOutput(int obj_kind, double sigmoid, float* out, int nrow, int
 void LaunchPointwiseMetric(int metric_kind, int obj_kind, double sigmoid, const float* score, const float* label, const float* weight, int n, int num_class,
                            double* partial, int partial_capacity, double* out2, cudaStream_t s);
 
+// ------------------------------------------- class scores, leaf products ----
+// Types of the tensors that the operators on class scores and leaf products take (32-bit and 16-bit floats: the codes of device matrices).
+constexpr int kOpFloat32 = 0, kOpFloat16 = 6, kOpBFloat16 = 16;
+constexpr int kMaxTopClasses = 32;
+// Scores [rows x classes] with strides in elements; labels int32 / int64 (label_bits 0: none), negative: no label. The forward
+// call writes log_prob (when not null), log_norm, entropy [rows] and the alternatives [rows x top_k]; the gradient reads the last four.
+struct ClassScoresArgs {
+  const void* scores; int dtype; long long rows, classes, row_stride, class_stride;
+  const void* labels; int label_bits; int top_k;
+  float *log_prob, *log_norm, *entropy, *top_log_prob; int* top_class;
+};
+// Upstream gradients (null: zero); g_top [rows x top_k]; grad has the type of the scores.
+struct ClassGradArgs { const float *g_log_prob, *g_log_norm, *g_entropy, *g_top; void* grad; long long grad_row_stride, grad_class_stride; };
+void LaunchClassLogProbs(const ClassScoresArgs& a, cudaStream_t s);
+void LaunchClassLogProbsGrad(const ClassScoresArgs& a, const ClassGradArgs& g, cudaStream_t s);
+
+// Leaf g owns the rows [begin[g], begin[g + 1]) of 0..rows-1; begin (int32 / int64, leaves + 1 entries) is clamped to them.
+struct LeafWindows { const void* begin; int begin_bits; int leaves; long long rows; };
+// y [rows x outputs] dense, x [rows x features] with a row stride, weight [leaves x outputs x features] with any strides, one type.
+struct LeafProductsArgs {
+  LeafWindows leaves; const void* x; const void* weight; void* y; int dtype; int features, outputs;
+  long long x_stride, weight_leaf_stride, weight_out_stride, weight_in_stride;
+};
+// out [leaves x a_cols x b_cols] dense, of the inputs' type or fp32.
+struct LeafGramArgs { LeafWindows leaves; const void* a; const void* b; void* out; int dtype, out_dtype; int a_cols, b_cols; long long a_stride, b_stride; };
+void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s);
+void LaunchLeafGram(const LeafGramArgs& a, cudaStream_t s);
+
 }  // namespace fb

@@ -43,6 +43,23 @@ void PartitionOp(const uint8_t* rows, int row_stride, const int* idx, int count,
   FB_CUDA(cudaMemcpyAsync(left_count, left_total.get(), sizeof(int), cudaMemcpyDeviceToHost, s));
   FB_CUDA(cudaStreamSynchronize(s));
 }
+// Makes `device` the thread's current device, and the one before that again at the end.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) { FB_CUDA(cudaGetDevice(&before_)); if (device != before_) { FB_CUDA(cudaSetDevice(device)); changed_ = true; } }
+  ~DeviceScope() { if (changed_) cudaSetDevice(before_); }
+ private:
+  int before_ = 0; bool changed_ = false;
+};
+void CheckClassScores(long long rows, long long classes, int label_bits, int top_k) {
+  if (rows < 0 || rows > 0x7fffffffLL || classes < 1 || classes > 0x7fffffffLL) Log::Fatal("class scores: %lld rows x %lld classes are not covered", rows, classes);
+  if (label_bits != 0 && label_bits != 32 && label_bits != 64) Log::Fatal("class scores: labels of %d bits", label_bits);
+  if (top_k < 0 || top_k > kMaxTopClasses || top_k > classes) Log::Fatal("class scores: %d alternatives of %lld classes (at most %d)", top_k, classes, kMaxTopClasses);
+}
+void CheckLeafWindows(int begin_bits, int leaves, long long rows) {
+  if (rows < 0 || rows > 0x7fffffffLL || leaves < 1) Log::Fatal("leaf products: %lld rows in %d leaves are not covered", rows, leaves);
+  if (begin_bits != 32 && begin_bits != 64) Log::Fatal("leaf products: boundaries of %d bits", begin_bits);
+}
 }  // namespace
 
 #define OPS_BEGIN() try {
@@ -207,6 +224,53 @@ int FB_OpBernoulliRowsHost(int n, long long global_offset, unsigned int seed, do
     for (int i = b * kBlock; i < std::min(n, (b + 1) * kBlock); ++i) if (flag[i]) out_idx[w++] = i;
   }
   *out_count = count[nblocks];
+  OPS_END();
+}
+
+// The entry points below run on the caller's stream of `device` and return without waiting; the calling thread's device stays as it was.
+// Class scores [rows x classes] -> per-row log probability of the label, log of the normaliser, entropy, top alternatives.
+int FB_OpClassLogProbs(const void* scores, int dtype, long long rows, long long classes, long long row_stride, long long class_stride, const void* labels, int label_bits,
+                       int top_k, float* log_prob, float* log_norm, float* entropy, float* top_log_prob, int* top_class, int device, void* stream) {
+  OPS_BEGIN();
+  CheckClassScores(rows, classes, label_bits, top_k);
+  DeviceScope scope(device);
+  ClassScoresArgs a{scores, dtype, rows, classes, row_stride, class_stride, labels, label_bits, top_k, log_prob, log_norm, entropy, top_log_prob, top_class};
+  LaunchClassLogProbs(a, static_cast<cudaStream_t>(stream));
+  OPS_END();
+}
+// The gradient in the scores, from the forward results and the gradients of the outputs (null: zero).
+int FB_OpClassLogProbsGrad(const void* scores, int dtype, long long rows, long long classes, long long row_stride, long long class_stride, const void* labels, int label_bits,
+                           int top_k, const float* log_norm, const float* entropy, const int* top_class, const float* g_log_prob, const float* g_log_norm, const float* g_entropy,
+                           const float* g_top, void* grad, long long grad_row_stride, long long grad_class_stride, int device, void* stream) {
+  OPS_BEGIN();
+  CheckClassScores(rows, classes, label_bits, top_k);
+  DeviceScope scope(device);
+  ClassScoresArgs a{scores, dtype, rows, classes, row_stride, class_stride, labels, label_bits, top_k, nullptr, const_cast<float*>(log_norm), const_cast<float*>(entropy),
+                    nullptr, const_cast<int*>(top_class)};
+  ClassGradArgs g{g_log_prob, g_log_norm, g_entropy, g_top, grad, grad_row_stride, grad_class_stride};
+  LaunchClassLogProbsGrad(a, g, static_cast<cudaStream_t>(stream));
+  OPS_END();
+}
+// y_i = W_leaf(i) x_i for rows grouped by leaf.
+int FB_OpLeafProducts(const void* x, long long x_stride, const void* weight, long long weight_leaf_stride, long long weight_out_stride, long long weight_in_stride, const void* begin,
+                      int begin_bits, int leaves, long long rows, int features, int outputs, int dtype, void* y, int device, void* stream) {
+  OPS_BEGIN();
+  CheckLeafWindows(begin_bits, leaves, rows);
+  if (features < 1 || outputs < 1) Log::Fatal("leaf products: at least one feature and one output (got %d, %d)", features, outputs);
+  DeviceScope scope(device);
+  LeafProductsArgs a{{begin, begin_bits, leaves, rows}, x, weight, y, dtype, features, outputs, x_stride, weight_leaf_stride, weight_out_stride, weight_in_stride};
+  LaunchLeafProducts(a, static_cast<cudaStream_t>(stream));
+  OPS_END();
+}
+// P_g = sum over the rows of leaf g of a_i b_i^T.
+int FB_OpLeafGram(const void* a_rows, long long a_stride, const void* b_rows, long long b_stride, const void* begin, int begin_bits, int leaves, long long rows, int a_cols, int b_cols,
+                  int dtype, int out_dtype, void* out, int device, void* stream) {
+  OPS_BEGIN();
+  CheckLeafWindows(begin_bits, leaves, rows);
+  if (a_cols < 1 || b_cols < 1) Log::Fatal("leaf Gram: at least one column on each side (got %d, %d)", a_cols, b_cols);
+  DeviceScope scope(device);
+  LeafGramArgs a{{begin, begin_bits, leaves, rows}, a_rows, b_rows, out, dtype, out_dtype, a_cols, b_cols, a_stride, b_stride};
+  LaunchLeafGram(a, static_cast<cudaStream_t>(stream));
   OPS_END();
 }
 

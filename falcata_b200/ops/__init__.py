@@ -1,8 +1,9 @@
-"""Kernel-level entry points (one function per device kernel) used by the numerics tests.
+"""Operators on torch CUDA tensors, run by the native library's kernels.
 
-Every function takes torch CUDA tensors, runs exactly one kernel of the training path through the
-native library and returns torch tensors. If the native library is missing these raise: there is
-no PyTorch fallback on this path.
+The functions in this file each run exactly one kernel of the training path (on the default stream, waiting for it) and serve
+the numerics tests. The operators on class scores (``class_log_probs`` and its gradient) and on rows grouped by leaf
+(``leaf_products``, ``leaf_gram``) are for programs: they run on the current stream without waiting, can be captured into a
+CUDA graph and are differentiable. If the native library is missing all of them raise: there is no PyTorch fallback on this path.
 """
 from __future__ import annotations
 
@@ -13,6 +14,8 @@ import numpy as np
 import torch
 
 from ..basic import _lib
+from .leaves import leaf_gram, leaf_products
+from .scores import ClassLogProbs, class_log_probs, class_log_probs_grad
 
 
 def _check(ret: int) -> None:

@@ -1,0 +1,62 @@
+"""Argument checks and native calls shared by the operators that run on the caller's stream."""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from ..basic import _lib
+
+_TYPE_CODE = {torch.float32: 0, torch.float16: 6, torch.bfloat16: 16}
+_BOUND: dict = {}
+
+
+def bind(name: str, argtypes: tuple):
+    """The native entry point with its argument types set (once)."""
+    fn = _BOUND.get(name)
+    if fn is None:
+        fn = getattr(_lib(), name)
+        fn.argtypes = argtypes; fn.restype = ctypes.c_int
+        _BOUND[name] = fn
+    return fn
+
+
+def check(ret: int) -> None:
+    if ret != 0:
+        lib = _lib()
+        lib.FB_OpsLastError.restype = ctypes.c_char_p
+        raise RuntimeError(lib.FB_OpsLastError().decode())
+
+
+def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def type_code(name: str, t: torch.Tensor) -> int:
+    code = _TYPE_CODE.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name}: float32, float16 or bfloat16 is wanted, got {t.dtype}")
+    return code
+
+
+def require_tensor(name: str, t: torch.Tensor) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a torch tensor is wanted, got {type(t).__name__}")
+
+
+def one_device(**tensors: Optional[torch.Tensor]) -> None:
+    """All of them on one CUDA device (that of the first)."""
+    first = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name}: a CUDA tensor is wanted, got one on {t.device}")
+        if first is not None and t.device != first.device:
+            raise ValueError(f"{name}: on {t.device}, the other tensors are on {first.device}")
+        first = first if first is not None else t
+
+
+def device_and_stream(device: torch.device) -> Tuple[int, int]:
+    return device.index, torch.cuda.current_stream(device).cuda_stream

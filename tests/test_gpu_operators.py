@@ -1,0 +1,470 @@
+"""Class log probabilities and per-leaf products against plain 64-bit formulas.
+
+Tolerances, from u = 2^-24 (half a step of fp32; a type's own half step is eps / 2):
+* a sum of K positive terms, each e^x with a relative error of a few u (1 + |x|): at most u (K / 32 + 64 + 4 max |x|) relative
+  (no thread adds more than K / 32 terms in a row, the rest is a tree), |x| weighted by the terms themselves, so below 16;
+* log p and log_norm: that, plus u times the size of the scores; the entropy: that times (1 + log K);
+* a gradient p (a + b log p): relative u (64 + 4 |log p|) plus the error of log_norm, plus half a step of its type;
+* a product over F terms: 2 u (F + 8) sum |x w| (a matrix instruction may cut instead of rounding), plus half a step of its type.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda"); g.manual_seed(seed)
+    return g
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _scores(n, k, dtype, layout, seed=0, spread=2.5):
+    g = _gen(seed)
+    if layout == "row":
+        return torch.randn((n, k), generator=g, device="cuda").mul(spread).to(dtype)
+    if layout == "class":                                     # as the training scores lie
+        return torch.randn((k, n), generator=g, device="cuda").mul(spread).to(dtype).t()
+    if layout == "padded":                                    # a window of a larger matrix, off the 16-byte boundary
+        return torch.randn((n, k + 7), generator=g, device="cuda").mul(spread).to(dtype)[:, 3:3 + k]
+    if layout == "strided":                                   # every other class of every third row
+        return torch.randn((3 * n, 2 * k), generator=g, device="cuda").mul(spread).to(dtype)[::3, ::2]
+    raise ValueError(layout)
+
+
+def _reference(scores, labels, top):
+    s = scores.double()
+    k = s.shape[1]
+    none = torch.isneginf(s).all(1)
+    bad = torch.isnan(s).any(1) | torch.isposinf(s).any(1)
+    most = torch.where(none | bad, 0.0, s.max(1).values)
+    log_sum = torch.log(torch.exp(s - most[:, None]).sum(1))
+    lse = most + log_sum
+    logp = torch.where(torch.isneginf(s), s, (s - most[:, None]) - log_sum[:, None])   # not s - lse: at 1e38 a 64-bit lse no longer holds log K
+    plogp = torch.where(torch.isneginf(s), 0.0, torch.exp(logp) * logp)
+    nan = torch.full_like(lse, math.nan)
+    out = {"log_norm": torch.where(bad, nan, lse), "entropy": torch.where(bad, nan, torch.where(none, 0.0, -plogp.sum(1)))}
+    if labels is not None:
+        y = labels.long()
+        lp = logp.gather(1, y.clamp(0, k - 1)[:, None])[:, 0]
+        out["log_prob"] = torch.where(y < 0, 0.0, torch.where(bad | (y >= k), nan, lp))
+    if top:
+        v, c = torch.sort(s, dim=1, descending=True, stable=True)
+        v, c = v[:, :top], c[:, :top]
+        out["top_class"] = torch.where(bad[:, None] | torch.isneginf(v), -1, c).int()
+        out["top_log_prob"] = torch.where(bad[:, None], nan[:, None], torch.where(torch.isneginf(v), v, logp.gather(1, c)))
+    return out, logp
+
+
+def _check_forward(scores, labels, top):
+    from falcata_b200 import ops
+    got = ops.class_log_probs(scores, labels, top_k=top)
+    want, _ = _reference(scores, labels, top)
+    k = scores.shape[1]
+    finite = scores.double()[torch.isfinite(scores)].abs()
+    size = float(finite.max()) if finite.numel() else 0.0
+    tol = U * (k / 32 + 64 + 4 * 16) + 4 * U * size
+    for name, w in want.items():
+        g = getattr(got, name)
+        assert g.shape == w.shape and g.device == scores.device
+        if name == "top_class":
+            assert g.dtype == torch.int32 and torch.equal(g, w)
+            continue
+        assert g.dtype == torch.float32
+        t = tol * (1 + math.log(k)) if name == "entropy" else tol
+        assert torch.allclose(g.double(), w, rtol=U, atol=t, equal_nan=True), (name, float((g.double() - w).nan_to_num(0, 0, 0).abs().max()), t)
+    assert (got.log_prob is None) == (labels is None) and (got.top_class is None) == (top == 0)
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["row", "class", "padded", "strided"])
+@pytest.mark.parametrize("n,k,top", [(1, 1, 1), (5, 2, 2), (1000, 3, 0), (257, 10, 3), (33, 31, 31), (64, 64, 5), (65, 65, 32), (7, 127, 4), (130, 1000, 20), (3, 1025, 1), (9, 4099, 32), (2, 50021, 20)])
+def test_class_log_probs(dtype, layout, n, k, top):
+    scores = _scores(n, k, dtype, layout, seed=n + k)
+    labels = torch.randint(-1, k, (n,), generator=_gen(1), device="cuda")
+    _check_forward(scores, labels.int() if n % 2 else labels, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,top", [(1, 131075, 20), (2, 262147, 32), (40, 70001, 7), (300, 20000, 5)])
+def test_class_log_probs_many_classes(dtype, n, k, top):
+    _check_forward(_scores(n, k, dtype, "padded", seed=3, spread=4.0), torch.randint(0, k, (n,), generator=_gen(2), device="cuda", dtype=torch.int32), top)
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "equal", "blocks", "one", "last"])
+@pytest.mark.parametrize("layout", ["row", "class"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k,top", [(48, 32), (700, 32), (3000, 20), (40000, 32)])
+def test_class_log_probs_orders_and_ties(order, layout, dtype, k, top):
+    """Rows whose order or ties are the worst for a selection: the lowest classes win among equals."""
+    at = torch.arange(k, device="cuda")
+    row = {"rising": at * (8.0 / k), "falling": -at * (8.0 / k), "equal": torch.zeros(k, device="cuda"), "blocks": -(at // 97 % 5).float(),
+           "one": (at == k // 2) * 9.0, "last": (at >= k - top) * 3.0}[order]
+    scores = row.to(dtype).repeat(3, 1)
+    scores[1] = scores[1].flip(0)
+    scores[2] = -0.0 * scores[2]                       # zeros of both signs are equal scores
+    scores[2, ::2] = 0.0
+    _check_forward(scores if layout == "row" else scores.t().contiguous().t(), torch.tensor([0, k - 1, k // 2], device="cuda"), top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["row", "class", "padded"])
+@pytest.mark.parametrize("k,top", [(5, 5), (40, 32), (300, 32), (5000, 20), (60000, 32)])
+def test_class_log_probs_ruled_out_classes(dtype, layout, k, top):
+    """-inf rules a class out; the type's lowest value does not; NaN and +inf spoil their row only."""
+    lowest = torch.finfo(dtype).min
+    s = _scores(12, k, dtype, layout, seed=5)
+    s[1] = -math.inf                                   # nothing left
+    s[2] = -math.inf; s[2, k // 2] = 1.5               # one class left
+    s[3, : k // 2] = -math.inf
+    s[4] = lowest                                      # uniform at the lowest value
+    s[5] = lowest; s[5, 1] = -3.0
+    s[6, k - 1] = math.nan
+    s[7, 0] = math.inf
+    s[8] = -math.inf; s[8, k - 1] = lowest
+    s[9] = -math.inf; s[9, k // 3] = math.nan
+    s[10] = torch.finfo(dtype).max
+    s[11, :: 2] = -math.inf; s[11, 1] = lowest
+    labels = torch.tensor([0, 0, k // 2, 0, 1, 0, 0, 1, k - 1, -1, 2, k], device="cuda")
+    from falcata_b200 import ops
+    got = ops.class_log_probs(s, labels, top_k=top)
+    want, logp = _reference(s, labels, top)
+    assert torch.equal(got.top_class, want["top_class"])
+    for name in ("log_prob", "log_norm", "entropy", "top_log_prob"):
+        g, w = getattr(got, name).double(), want[name]
+        scale = U * (k / 32 + 128) + 4 * U * 16
+        w32 = w.float().double()                       # log probabilities beyond fp32's range are -inf there
+        assert torch.allclose(g, w32, rtol=4 * U, atol=scale * (1 + math.log(k)), equal_nan=True), name
+    up = {"grad_log_prob": torch.ones(12, device="cuda"), "grad_log_norm": torch.full((12,), 0.5, device="cuda"), "grad_entropy": torch.full((12,), -0.25, device="cuda")}
+    grad = ops.class_log_probs_grad(s, got.log_norm, got.entropy, labels=labels, **up).double()
+    p = torch.where(torch.isneginf(logp), 0.0, torch.exp(logp))
+    h = want["entropy"][:, None]
+    ref = 0.5 * p + 0.25 * torch.where(p > 0, p * (logp.nan_to_num(0, 0, 0) + h), 0.0)
+    y = labels.long()
+    for i in range(12):
+        if i == 1:
+            ref[i] = 0.0
+        elif i in (6, 7, 9, 11):
+            ref[i] = math.nan
+        else:
+            ref[i] -= p[i]; ref[i, y[i]] += 1.0
+    assert torch.allclose(grad, ref, rtol=_half_step(dtype), atol=U * (k / 32 + 256) + (6e-8 if dtype == torch.float16 else 0), equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["row", "class", "padded", "strided"])
+@pytest.mark.parametrize("n,k,top", [(1, 1, 1), (6, 2, 2), (300, 10, 3), (33, 64, 32), (31, 65, 4), (70, 1000, 20), (5, 4099, 32), (3, 50021, 5), (2, 131075, 0)])
+def test_class_log_probs_grad(dtype, layout, n, k, top):
+    """Against the formula in 64 bits, and the formula against differences of the loss."""
+    from falcata_b200 import ops
+    s = _scores(n, k, dtype, layout, seed=n * k)
+    labels = torch.randint(-1, k, (n,), generator=_gen(7), device="cuda")
+    g = _gen(8)
+    up = [torch.randn(n, generator=g, device="cuda") for _ in range(3)] + ([torch.randn((n, top), generator=g, device="cuda")] if top else [])
+    out = ops.class_log_probs(s, labels, top_k=top)
+    grad = ops.class_log_probs_grad(s, out.log_norm, out.entropy, labels=labels, top_class=out.top_class, grad_log_prob=up[0], grad_log_norm=up[1], grad_entropy=up[2],
+                                    grad_top_log_prob=up[3] if top else None)
+    assert grad.dtype == dtype and grad.shape == s.shape and grad.stride(0 if layout == "class" and n > 1 and k > 1 else 1) == 1
+
+    def loss(x):
+        logp = torch.log_softmax(x, 1)
+        total = (torch.where(labels < 0, 0.0, logp.gather(1, labels.clamp(min=0)[:, None])[:, 0]) * up[0].double()).sum()
+        total = total + (torch.logsumexp(x, 1) * up[1].double()).sum() - ((logp.exp() * logp).sum(1) * up[2].double()).sum()
+        return total + (logp.gather(1, out.top_class.long()) * up[3].double()).sum() if top else total
+
+    x = s.double().requires_grad_()
+    ref, = torch.autograd.grad(loss(x), x)
+    step = torch.randn(s.shape, generator=g, device="cuda", dtype=torch.float64)
+    slope = (loss(x.detach() + 1e-5 * step) - loss(x.detach() - 1e-5 * step)) / 2e-5
+    assert abs(float(slope - (ref * step).sum())) <= 1e-6 * (1 + float((ref * step).abs().sum()))
+    logp = torch.log_softmax(s.double(), 1)
+    weight = sum(u.abs().double() if u.dim() == 1 else u.abs().double().sum(1) for u in up)[:, None]
+    h = (out.entropy.double() + 1)[:, None]
+    bound = logp.exp() * weight * (h + logp.abs()) * (U * (k / 32 + 128) + 8 * U * (16 + logp.abs()))
+    given = torch.zeros_like(ref); rows = torch.arange(n, device="cuda")
+    given[rows, labels.clamp(min=0)] += up[0].abs().double()
+    if top:
+        given.scatter_add_(1, out.top_class.long(), up[3].abs().double())
+    bound = bound + 8 * U * given + _half_step(dtype) * ref.abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    off = (grad.double() - ref).abs()
+    assert bool((off <= bound).all()), float((off - bound).max())
+
+
+@pytest.mark.parametrize("layout,k", [("row", 10), ("row", 300), ("row", 5000), ("row", 40000), ("class", 10), ("class", 300)])
+@pytest.mark.parametrize("shift", [-3e4, 1e6, 2.0 ** 100])
+def test_class_log_probs_far_from_zero(layout, k, shift):
+    """Scores far from zero: fp32's log_norm no longer holds the probabilities, the results still do."""
+    from falcata_b200 import ops
+    s = _scores(20, k, torch.float32, layout, seed=2) + shift
+    labels = torch.randint(0, k, (20,), generator=_gen(1), device="cuda")
+    got = ops.class_log_probs(s, labels)
+    want, logp = _reference(s, labels, 0)
+    tol = U * (k / 32 + 128)
+    assert torch.allclose(got.log_prob.double(), want["log_prob"], rtol=4 * U, atol=tol) and torch.allclose(got.entropy.double(), want["entropy"], rtol=4 * U, atol=tol * (1 + math.log(k)))
+    assert torch.allclose(got.log_norm.double(), want["log_norm"], rtol=2 * U, atol=tol)
+    grad = ops.class_log_probs_grad(s, got.log_norm, got.entropy, labels=labels, grad_log_prob=torch.ones(20, device="cuda")).double()
+    ref = -logp.exp()
+    ref[torch.arange(20, device="cuda"), labels] += 1
+    assert torch.allclose(grad, ref, rtol=U, atol=U * (k / 32 + 256))
+
+
+def test_class_log_probs_autograd_and_repeated_indices():
+    from falcata_b200 import ops
+    s = _scores(50, 300, torch.float32, "row").requires_grad_()
+    labels = torch.randint(0, 300, (50,), generator=_gen(1), device="cuda")
+    r = ops.class_log_probs(s, labels, top_k=4)
+    (-r.log_prob.mean() - 0.01 * r.entropy.mean() + 0.1 * r.top_log_prob[:, 1:].sum() + 1e-3 * (r.log_norm ** 2).mean()).backward()
+    x = s.detach().double().requires_grad_()
+    logp = torch.log_softmax(x, 1)
+    loss = -logp.gather(1, labels[:, None]).mean() + 0.01 * (logp.exp() * logp).sum(1).mean() + 0.1 * logp.gather(1, r.top_class.long())[:, 1:].sum() + 1e-3 * (torch.logsumexp(x, 1) ** 2).mean()
+    loss.backward()
+    assert torch.allclose(s.grad.double(), x.grad, rtol=1e-5, atol=2e-6)
+    # the same alternative named several times, the label among them, and entries that name none
+    t = torch.tensor([[3, 3, 3, 7], [-1, 5, 5, -1]], dtype=torch.int32, device="cuda")
+    g = torch.tensor([[1.0, 2.0, 4.0, -1.0], [9.0, 1.0, 1.0, 9.0]], device="cuda")
+    for layout in ("row", "class"):
+        sc = _scores(2, 9, torch.float32, layout, seed=3)
+        f = ops.class_log_probs(sc)
+        got = ops.class_log_probs_grad(sc, f.log_norm, f.entropy, labels=torch.tensor([3, 5], device="cuda"), top_class=t, grad_log_prob=torch.tensor([0.5, 0.25], device="cuda"), grad_top_log_prob=g)
+        p = torch.softmax(sc.double(), 1)
+        want = -p * torch.tensor([[6.5], [2.25]], device="cuda")
+        want[0, 3] += 7.5; want[0, 7] -= 1.0; want[1, 5] += 2.25
+        assert torch.allclose(got.double(), want, atol=4e-6)
+    with pytest.raises(RuntimeError):      # differentiable once
+        z = _scores(2, 9, torch.float32, "row").requires_grad_()
+        d, = torch.autograd.grad(ops.class_log_probs(z).entropy.sum(), z, create_graph=True)
+        d.sum().backward()
+
+
+def test_class_log_probs_empty_and_unused():
+    from falcata_b200 import ops
+    s = torch.zeros((0, 5), device="cuda", requires_grad=True)
+    r = ops.class_log_probs(s, torch.zeros(0, dtype=torch.int32, device="cuda"), top_k=2)
+    assert r.log_prob.shape == (0,) and r.top_class.shape == (0, 2)
+    r.log_prob.sum().backward()
+    assert s.grad.shape == (0, 5)
+    wide = torch.randn(1, 20, device="cuda").expand(6, 20)        # a broadcast row
+    assert torch.equal(ops.class_log_probs(wide, top_k=3).top_class, ops.class_log_probs(wide.contiguous(), top_k=3).top_class)
+    w = torch.randn(1, 20, device="cuda", requires_grad=True)
+    y = torch.arange(6, device="cuda")
+    ops.class_log_probs(w.expand(6, 20), y).log_prob.sum().backward()
+    p = torch.softmax(w.detach().double(), 1)
+    want = -6 * p; want[0, :6] += 1
+    assert torch.allclose(w.grad.double(), want, atol=6 * 64 * U)
+
+
+# ------------------------------------------------------------------------------------------------ leaves ----
+def _leaves(n, leaves, seed, empty=True):
+    g = torch.Generator(); g.manual_seed(seed)
+    cuts = torch.sort(torch.randint(0, n + 1, (leaves - 1,), generator=g)).values if leaves > 1 else torch.zeros(0, dtype=torch.long)
+    if empty and leaves > 3:
+        cuts[1] = cuts[0]
+    return torch.cat([torch.zeros(1, dtype=torch.long), cuts, torch.tensor([n])]).to(torch.int32).cuda()
+
+
+def _ref_products(x, w, begin):
+    y = torch.zeros((x.shape[0], w.shape[1]), dtype=torch.float64, device="cuda"); size = torch.zeros_like(y)
+    b = begin.tolist()
+    for g in range(w.shape[0]):
+        y[b[g]:b[g + 1]] = x[b[g]:b[g + 1]].double() @ w[g].double().t()
+        size[b[g]:b[g + 1]] = x[b[g]:b[g + 1]].double().abs() @ w[g].double().abs().t()
+    return y, size
+
+
+def _near(got, want, size, terms, dtype):
+    bound = 2 * U * (terms + 8) * size + _half_step(dtype) * want.abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), float((off - bound).max())
+
+
+SHAPES = [(1, 1, 1, 1), (3, 5, 2, 4), (100, 28, 10, 7), (257, 33, 17, 3), (1000, 136, 1, 31), (513, 100, 100, 5), (64, 130, 257, 2), (2000, 8, 64, 255), (300, 257, 129, 4), (40, 2000, 30, 40),
+          (1200, 64, 256, 3), (700, 200, 520, 2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,f,k,leaves", SHAPES)
+def test_leaf_products(dtype, n, f, k, leaves):
+    from falcata_b200 import ops
+    g = _gen(n + f)
+    x = torch.randn((n, f), generator=g, device="cuda").to(dtype); w = torch.randn((leaves, k, f), generator=g, device="cuda").mul(f ** -0.5).to(dtype)
+    begin = _leaves(n, leaves, seed=k)
+    y = ops.leaf_products(x, w, begin)
+    assert y.dtype == dtype and y.shape == (n, k)
+    want, size = _ref_products(x, w, begin)
+    _near(y, want, size, f, dtype)
+    # the transposed maps: the gradient in x
+    d = torch.randn((n, k), generator=g, device="cuda").to(dtype)
+    want, size = _ref_products(d, w.transpose(1, 2), begin)
+    _near(ops.leaf_products(d, w.transpose(1, 2), begin.long()), want, size, k, dtype)
+    # the gradient in the maps, in the inputs' type and in fp32
+    b = begin.tolist()
+    want = torch.stack([d[lo:hi].double().t() @ x[lo:hi].double() for lo, hi in zip(b[:-1], b[1:])])
+    size = torch.stack([d[lo:hi].double().abs().t() @ x[lo:hi].double().abs() for lo, hi in zip(b[:-1], b[1:])])
+    p = ops.leaf_gram(d, x, begin)
+    assert p.dtype == dtype and p.shape == (leaves, k, f)
+    _near(p, want, size, n, dtype)
+    _near(ops.leaf_gram(d, x, begin, dtype=torch.float32), want, size, n, torch.float32)
+    assert torch.equal(p, ops.leaf_gram(d, x, begin))          # the same sums on every run
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_leaf_products_strides_and_alignment(dtype):
+    from falcata_b200 import ops
+    n, f, k, leaves = 333, 40, 24, 6
+    g = _gen(4)
+    big = torch.randn((n, f + 13), generator=g, device="cuda").to(dtype)
+    wbig = torch.randn((leaves, k + 3, f + 5), generator=g, device="cuda").to(dtype)
+    begin = _leaves(n, leaves, seed=1)
+    for x in (big[:, 8:8 + f], big[:, 3:3 + f], big[:, :f].t().contiguous().t(), big[:1, :f].expand(n, f)):
+        for w in (wbig[:, :k, :f], wbig[:, 1:1 + k, 5:5 + f], wbig[:, :k, :f].transpose(1, 2).contiguous().transpose(1, 2), wbig[:1, :k, :f].expand(leaves, k, f)):
+            want, size = _ref_products(x, w, begin)
+            _near(ops.leaf_products(x, w, begin), want, size, f, dtype)
+        d = big[:, 10:10 + k]
+        b = begin.tolist()
+        want = torch.stack([d[lo:hi].double().t() @ x[lo:hi].double() for lo, hi in zip(b[:-1], b[1:])])
+        size = torch.stack([d[lo:hi].double().abs().t() @ x[lo:hi].double().abs() for lo, hi in zip(b[:-1], b[1:])])
+        _near(ops.leaf_gram(d, x, begin), want, size, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_leaf_products_rows_outside_the_leaves(dtype):
+    """Rows in no leaf: zero outputs, no share in the sums, whatever they hold; boundaries past the rows are clamped."""
+    from falcata_b200 import ops
+    g = _gen(6)
+    x = torch.randn((300, 20), generator=g, device="cuda").to(dtype); w = torch.randn((3, 12, 20), generator=g, device="cuda").to(dtype); d = torch.randn((300, 12), generator=g, device="cuda").to(dtype)
+    x[:10] = math.nan; x[250:] = math.inf; d[:10] = math.nan; d[250:] = math.nan
+    begin = torch.tensor([10, 100, 100, 250], device="cuda")
+    y = ops.leaf_products(x, w, begin)
+    assert bool((y[:10] == 0).all()) and bool((y[250:] == 0).all())
+    want, size = _ref_products(x[10:250], w, begin - 10)
+    _near(y[10:250], want, size, 20, dtype)
+    p = ops.leaf_gram(d, x, begin)
+    assert bool((p[1] == 0).all()) and bool(torch.isfinite(p).all())
+    want = torch.stack([d[lo:hi].double().t() @ x[lo:hi].double() for lo, hi in ((10, 100), (100, 100), (100, 250))])
+    size = torch.stack([d[lo:hi].double().abs().t() @ x[lo:hi].double().abs() for lo, hi in ((10, 100), (100, 100), (100, 250))])
+    _near(p, want, size, 240, dtype)
+    z = ops.leaf_products(x[10:250], w, torch.tensor([-5, 90, 90, 10 ** 6], device="cuda"))
+    assert torch.equal(z, y[10:250])
+    assert ops.leaf_products(x[:0], w, torch.zeros(4, dtype=torch.int32, device="cuda")).shape == (0, 12)
+    assert bool((ops.leaf_gram(d[:0], x[:0], torch.zeros(4, dtype=torch.int32, device="cuda")) == 0).all())
+    assert bool((ops.leaf_products(x, w, torch.zeros(4, dtype=torch.int32, device="cuda")) == 0).all())
+
+
+def test_leaf_products_autograd():
+    from falcata_b200 import ops
+    g = _gen(9)
+    x = torch.randn((400, 30), generator=g, device="cuda", requires_grad=True); w = torch.randn((5, 7, 30), generator=g, device="cuda", requires_grad=True)
+    begin = _leaves(400, 5, seed=2)
+    (ops.leaf_products(x, w, begin) ** 2).sum().backward()
+    xd, wd = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    b = begin.tolist()
+    sum(((xd[b[i]:b[i + 1]] @ wd[i].t()) ** 2).sum() for i in range(5)).backward()
+    assert torch.allclose(x.grad.double(), xd.grad, rtol=1e-5, atol=1e-4) and torch.allclose(w.grad.double(), wd.grad, rtol=1e-5, atol=1e-3)
+    ops.leaf_products(x, w[:1].expand(5, 7, 30), begin).sum().backward()       # one map shared by all leaves, a broadcast gradient
+    assert torch.isfinite(w.grad).all()
+
+
+# -------------------------------------------------------------------------------------- together, streams ----
+def _head_step(x, w, begin, labels):
+    from falcata_b200 import ops
+    r = ops.class_log_probs(ops.leaf_products(x, w, begin), labels, top_k=3)
+    loss = -(r.log_prob.mean() + 0.01 * r.entropy.mean())
+    return (loss, r.top_class) + torch.autograd.grad(loss, (x, w))
+
+
+def test_forest_leaves_with_class_heads():
+    """As they are used together: a forest's leaves group the rows, every leaf has a linear head, the heads' scores give the loss."""
+    import falcata_b200 as fb
+    from falcata_b200 import ops
+    from util import make_multiclass
+    X, y = make_multiclass(n=3000, f=12, k=4)
+    bst = fb.train({"objective": "multiclass", "num_class": 4, "num_leaves": 15, "device_type": "cuda", "verbosity": -1}, fb.Dataset(X, y), 2)
+    Xd = torch.from_numpy(X).cuda()
+    leaf = bst.predict(Xd, pred_leaf=True)[:, 0].long()
+    order = torch.argsort(leaf, stable=True)
+    begin = torch.searchsorted(leaf[order].contiguous(), torch.arange(16, device="cuda")).int()
+    x = Xd[order].contiguous().requires_grad_()
+    w = torch.zeros((15, 4, 12), device="cuda").normal_(0, 0.1, generator=_gen(3)).requires_grad_()
+    labels = torch.from_numpy(y).cuda().int()[order]
+    loss, top, gx, gw = _head_step(x, w, begin, labels)
+    xd, wd = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    s = torch.einsum("nf,nkf->nk", xd, wd[leaf[order]])
+    logp = torch.log_softmax(s, 1)
+    ref = -(logp.gather(1, labels.long()[:, None]).mean() - 0.01 * (logp.exp() * logp).sum(1).mean())
+    rx, rw = torch.autograd.grad(ref, (xd, wd))
+    assert abs(float(loss.detach()) - float(ref.detach())) < 64 * U * 4
+    assert torch.allclose(gx.double(), rx, rtol=1e-4, atol=1e-9 + 256 * U / 3000) and torch.allclose(gw.double(), rw, rtol=1e-4, atol=4096 * U / 15)
+
+
+def test_custom_objective_from_class_log_probs():
+    """The training scores that a custom objective sees are class-major; the gradient goes back without a copy."""
+    import falcata_b200 as fb
+    from falcata_b200 import ops
+    from util import make_multiclass
+    X, y = make_multiclass(n=2000, f=10, k=3)
+    labels = torch.from_numpy(y).cuda().int()
+    seen = []
+
+    def objective(scores, train):
+        r = ops.class_log_probs(scores, labels)
+        grad = ops.class_log_probs_grad(scores, r.log_norm, r.entropy, labels=labels, grad_log_prob=torch.full_like(r.log_prob, -1.0))
+        p = torch.exp(scores - r.log_norm[:, None])
+        seen.append((grad, p - torch.nn.functional.one_hot(labels.long(), 3)))
+        assert grad.t().is_contiguous()
+        return grad.t(), (1.5 * p * (1 - p)).t().contiguous()
+
+    params = {"num_class": 3, "num_leaves": 7, "device_type": "cuda", "verbosity": -1}
+    mine = fb.Booster(dict(params, objective="none"), fb.Dataset(X, y))
+    theirs = fb.Booster(dict(params, objective="multiclass", boost_from_average=False), fb.Dataset(X, y))
+    for _ in range(3):
+        mine.update(fobj=objective); theirs.update()
+    for grad, want in seen:
+        assert torch.allclose(grad, want, atol=64 * U)
+    Xd = torch.from_numpy(X).cuda()
+    assert torch.allclose(mine.predict(Xd, raw_score=True), theirs.predict(Xd, raw_score=True), atol=1e-4)
+
+
+def test_operators_in_a_graph_and_on_streams():
+    """Captured and replayed on new inputs, two graphs and an eager call side by side on two streams: the same results."""
+    g = _gen(11)
+    def inputs(seed):
+        g.manual_seed(seed)
+        return (torch.randn((500, 36), generator=g, device="cuda", requires_grad=True), torch.randn((9, 300, 36), generator=g, device="cuda", requires_grad=True), _leaves(500, 9, seed),
+                torch.randint(0, 300, (500,), generator=g, device="cuda"))
+    sets = [inputs(i) for i in range(3)]
+    want = [_head_step(*s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    captured = []
+    for st in streams:
+        buf = tuple(t.detach().clone().requires_grad_(t.requires_grad) for t in sets[0])
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            _head_step(*buf)
+        torch.cuda.current_stream().wait_stream(st)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            out = _head_step(*buf)
+        captured.append((graph, buf, out))
+    torch.cuda.synchronize()
+    for (graph, buf, out), src in zip(captured, sets[1:]):
+        with torch.no_grad():
+            for b, s in zip(buf, src):
+                b.copy_(s)
+    torch.cuda.synchronize()
+    for rep in range(3):
+        for st, (graph, _, _) in zip(streams, captured):
+            with torch.cuda.stream(st):
+                graph.replay()
+        eager = _head_step(*sets[0])
+        torch.cuda.synchronize()
+        for got, ref in ((captured[0][2], want[1]), (captured[1][2], want[2]), (eager, want[0])):
+            for a, b in zip(got, ref):
+                assert torch.equal(a, b)
