@@ -52,7 +52,7 @@ class DeviceScope {
   int before_ = 0; bool changed_ = false;
 };
 void CheckClassScores(long long rows, long long classes, int label_bits, int top_k) {
-  if (rows < 0 || rows > 0x7fffffffLL || classes < 1 || classes > 0x7fffffffLL) Log::Fatal("class scores: %lld rows x %lld classes are not covered", rows, classes);
+  if (rows < 0 || rows > 0x7fffffffLL || classes < 1 || classes > 0x7ff00000LL) Log::Fatal("class scores: %lld rows x %lld classes are not covered", rows, classes);
   if (label_bits != 0 && label_bits != 32 && label_bits != 64) Log::Fatal("class scores: labels of %d bits", label_bits);
   if (top_k < 0 || top_k > kMaxTopClasses || top_k > classes) Log::Fatal("class scores: %d alternatives of %lld classes (at most %d)", top_k, classes, kMaxTopClasses);
 }
