@@ -176,6 +176,7 @@ struct Entry { float v; int cls; };
 __device__ __forceinline__ bool Before(const Entry& a, const Entry& b) { return a.v > b.v || (a.v == b.v && a.cls < b.cls); }
 // unsigned order of floats; zeros of both signs alike
 __device__ __forceinline__ unsigned int OrderKey(float v) { const unsigned int u = __float_as_uint(v + 0.f); return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u; }
+__device__ __forceinline__ float KeyValue(unsigned int k) { return __uint_as_float((k & 0x80000000u) != 0 ? k & 0x7fffffffu : ~k); }
 
 template <int GROUP>
 struct RowShared {
@@ -216,6 +217,7 @@ struct TopList {
   // by rising class.
   template <typename E>
   __device__ __forceinline__ void Chunk(float most, int tid, E&& each) {
+    float limit = threshold;                    // only scores above it matter
     bool in = most > threshold;                 // later classes lose against equal earlier ones
     const int above = GroupCount<GROUP>(in);
     if (above == 0) return;
@@ -252,10 +254,11 @@ struct TopList {
       GroupSync<GROUP>();
       const unsigned int mine = OrderKey(most);
       in = in && (mine > sh->limit_key || (mine == sh->limit_key && first <= sh->limit_first));
+      limit = nextafterf(KeyValue(sh->limit_key), -INFINITY);
     } else {
       GroupSync<GROUP>();
     }
-    if (in) each([&](float v, int cls) { if (v > threshold) { const int at = atomicAdd(&sh->cand_count, 1); sh->cand[at].v = v; sh->cand[at].cls = cls; } });
+    if (in) each([&](float v, int cls) { if (v > limit) { const int at = atomicAdd(&sh->cand_count, 1); sh->cand[at].v = v; sh->cand[at].cls = cls; } });
     GroupSync<GROUP>();
     const int count = sh->cand_count;
     for (int i = tid; i < count; i += GROUP) {
