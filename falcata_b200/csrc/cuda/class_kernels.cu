@@ -72,24 +72,91 @@ __device__ __forceinline__ uint4 AllRuledOut(const float*) { return make_uint4(0
 __device__ __forceinline__ uint4 AllRuledOut(const __nv_bfloat16*) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
 __device__ __forceinline__ uint4 AllRuledOut(const __half*) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
 
+// Pairs of fp32 values in one 64-bit register: one instruction for two elements.
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 MakeF2(float x, float y) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ void Split(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 Add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 Mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ F2 Fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+__device__ __forceinline__ float Exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }   // 2 ulp; e^x below is 2^(x log2 e)
+constexpr float kLog2E = 1.44269504088896340736f;
+
 // The running sums of a part of a row, relative to its maximum m (-inf: nothing yet; a NaN or +inf among the scores makes s NaN).
 struct Sums {
   float m = -INFINITY, s = 0.f, t = 0.f;
+  __device__ __forceinline__ static float Down(float by) { return Exp2(by * kLog2E); }
   __device__ __forceinline__ void Raise(float to) {     // to > m
-    const float d = fmaxf(m - to, kLowestExponent), f = __expf(d);
+    const float d = fmaxf(m - to, kLowestExponent), f = Down(d);
     t = (t + s * d) * f; s *= f; m = to;
   }
   __device__ __forceinline__ float Base() const { return m == -INFINITY ? 0.f : m; }
-  __device__ __forceinline__ void Add(float v, float base) { const float x = MaxNan(v - base, kLowestExponent), e = __expf(x); s += e; t = fmaf(e, x, t); }
+  __device__ __forceinline__ void Add(float v, float base) { const float x = MaxNan(v - base, kLowestExponent), e = Down(x); s += e; t = fmaf(e, x, t); }
   __device__ __forceinline__ void AddOne(float v) { if (v > m) Raise(v); Add(v, Base()); }
   __device__ __forceinline__ void Join(float m2, float s2, float t2) {
-    if (m2 > m) { Sums o; o.m = m2; o.s = s2; o.t = t2; const float m1 = m, s1 = s, t1 = t; *this = o; m2 = m1; s2 = s1; t2 = t1; }
-    const float d = m2 == -INFINITY ? kLowestExponent : fmaxf(m2 - m, kLowestExponent), f = __expf(d);
+    if (m2 > m) { const float m1 = m, s1 = s, t1 = t; m = m2; s = s2; t = t2; m2 = m1; s2 = s1; t2 = t1; }
+    const float d = m2 == -INFINITY ? kLowestExponent : fmaxf(m2 - m, kLowestExponent), f = Down(d);
     t += (t2 + s2 * d) * f; s += s2 * f;
   }
+  // Over LANES neighbouring lanes: one maximum, one rescaling, then plain sums.
+  template <int LANES = 32>
   __device__ __forceinline__ void JoinLanes() {
-    for (int o = 16; o > 0; o >>= 1) Join(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o), __shfl_xor_sync(0xffffffffu, t, o));
+    float most = m;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (most > m) Raise(most);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); t += __shfl_xor_sync(0xffffffffu, t, o); }
+    m = most;
   }
+};
+// The same for 16 bytes of scores at a time, two sums side by side.
+// In a pair's product e^x * x a ruled-out score must not give 0 * (-inf): 16-bit scores are lifted to a finite low value first, two
+// per instruction. That is exact as long as the maximum is far above that value; near it (kFar) every score is clamped by itself.
+template <typename T> struct FarBelow;
+template <> struct FarBelow<float> { static constexpr float kFar = INFINITY; };
+template <> struct FarBelow<__half> { static constexpr unsigned int kLow = 0xfbfffbffu; static constexpr float kFar = -60000.f; };               // -65504
+template <> struct FarBelow<__nv_bfloat16> { static constexpr unsigned int kLow = 0xf14af14au; static constexpr float kFar = -1e29f; };          // -1.0e30: the distance to any score stays finite
+template <typename T>
+struct PairSums {
+  float m = -INFINITY; F2 s = MakeF2(0.f, 0.f), t = MakeF2(0.f, 0.f);
+  __device__ __forceinline__ void Raise(float to) {
+    const float d = fmaxf(m - to, kLowestExponent), f = Sums::Down(d);
+    const F2 d2 = MakeF2(d, d), f2 = MakeF2(f, f);
+    t = Mul2(Fma2(s, d2, t), f2); s = Mul2(s, f2); m = to;
+  }
+  __device__ __forceinline__ void AddPair(float v0, float v1, F2 minus_base) {
+    const F2 x = Add2(MakeF2(v0, v1), minus_base), u = Mul2(x, MakeF2(kLog2E, kLog2E));
+    float u0, u1; Split(u, u0, u1);
+    const F2 e = MakeF2(Exp2(u0), Exp2(u1));
+    s = Add2(s, e); t = Fma2(e, x, t);
+  }
+  __device__ __forceinline__ void AddPairClamped(float v0, float v1, float base) {
+    const float x0 = MaxNan(v0 - base, kLowestExponent), x1 = MaxNan(v1 - base, kLowestExponent);
+    const F2 e = MakeF2(Sums::Down(x0), Sums::Down(x1));
+    s = Add2(s, e); t = Fma2(e, MakeF2(x0, x1), t);
+  }
+  __device__ __forceinline__ void Add16(uint4 q) {
+    constexpr int N = Pack<T>::N;
+    const float base = m == -INFINITY ? 0.f : m;
+    const T* type = nullptr;
+    float v[N];
+    if constexpr (sizeof(T) == 2) {
+      if (base > FarBelow<T>::kFar) {
+        const unsigned int low = FarBelow<T>::kLow;
+        q.x = Max2(q.x, low, type); q.y = Max2(q.y, low, type); q.z = Max2(q.z, low, type); q.w = Max2(q.w, low, type);
+        Unpack(q, v, type);
+        const F2 minus_base = MakeF2(-base, -base);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) AddPair(v[i], v[i + 1], minus_base);
+        return;
+      }
+    }
+    Unpack(q, v, type);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) AddPairClamped(v[i], v[i + 1], base);
+  }
+  __device__ __forceinline__ Sums Total() const { Sums r; float a, b; Split(s, a, b); r.s = a + b; Split(t, a, b); r.t = a + b; r.m = m; return r; }
 };
 
 // The results of a row from its sums.
@@ -163,227 +230,294 @@ __global__ void __launch_bounds__(kFewThreads) ClassLogProbsFewKernel(ClassScore
 }
 
 // -------------------------------------------------------------------------------------------- contiguous rows ----
-// GROUP threads (a warp or a block) walk a row, or a block cluster's share of one, in chunks of kUnroll 16-byte loads per thread;
-// the next chunk's loads are in flight while one is worked on. Scores before the first 16-byte boundary and behind the last come
-// one by one.
-// Alternatives: the group keeps the list of the best so far and its last score as a threshold. A chunk in which some thread's
-// maximum passes it is looked at again (it is still in registers): the threads that matter are those with one of the top_k
-// largest maxima - no other can hold one of the best - so at most top_k threads add their scores above the threshold to the
-// list, which is then ranked by counting. Work and space are bounded whatever the order of the scores; in random order a
-// chunk adds top_k / (chunks so far) entries.
+// GROUP threads (a warp or a block) walk a row, or a block cluster's share of one, kUnroll 16-byte loads per thread at a time, the
+// next loads (at a row's end: the next row's) in flight while these are worked on. Scores before the first 16-byte boundary and
+// behind the last come one by one.
+// Alternatives: every thread knows the maximum of the scores that it has seen. With V the top_k-th largest of these maxima, only
+// the threads whose maximum reaches V can hold one of the top_k best scores: about top_k of them, so the group reads only
+// those threads' share of the row again (from L2, 1 / 12 of it for 20 alternatives and 256 threads), lists the scores that
+// reach V and ranks that short list by counting. Nothing is done for the alternatives during the walk itself.
 constexpr int kUnroll = 4;
 struct Entry { float v; int cls; };
 __device__ __forceinline__ bool Before(const Entry& a, const Entry& b) { return a.v > b.v || (a.v == b.v && a.cls < b.cls); }
-// unsigned order of floats; zeros of both signs alike
-__device__ __forceinline__ unsigned int OrderKey(float v) { const unsigned int u = __float_as_uint(v + 0.f); return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u; }
-__device__ __forceinline__ float KeyValue(unsigned int k) { return __uint_as_float((k & 0x80000000u) != 0 ? k & 0x7fffffffu : ~k); }
+// Order of scores as unsigned numbers, -inf 0, zeros of both signs alike; types of 16 bits need fewer.
+template <typename T> struct KeyBits { static constexpr int kBits = 16, kShift = 16; };
+template <> struct KeyBits<__half> { static constexpr int kBits = 19, kShift = 13; };
+template <> struct KeyBits<float> { static constexpr int kBits = 32, kShift = 0; };
+template <typename T>
+__device__ __forceinline__ unsigned int OrderKey(float v) {
+  const unsigned int u = __float_as_uint(v + 0.f);
+  return v == -INFINITY ? 0u : ((u & 0x80000000u) != 0 ? ~u : u | 0x80000000u) >> KeyBits<T>::kShift;
+}
 
 template <int GROUP>
 struct RowShared {
-  Entry list[2][kMaxTopClasses];      // the best so far (in the buffer that is `live`)
-  unsigned int key[GROUP]; int first[GROUP];
+  static constexpr int kFlagged = 64, kCandidates = GROUP == 32 ? 128 : 512;
+  Entry list[kMaxTopClasses], cand[kCandidates];
+  unsigned int key[GROUP];
   float part_m[GROUP / 32], part_s[GROUP / 32], part_t[GROUP / 32];
-  int cand_count; unsigned int limit_key; int limit_first, pad;
-  Entry cand[1];                      // top_k threads' scores and the list
+  int flagged[kFlagged];
+  int num_flagged, num_cand, last, have; unsigned int limit;
 };
-template <int GROUP, typename T>
-constexpr int RowSharedBytes(int top_k) { return static_cast<int>(sizeof(RowShared<GROUP>)) + top_k * (kUnroll * Pack<T>::N + 1) * static_cast<int>(sizeof(Entry)); }
 
 template <int GROUP> __device__ __forceinline__ void GroupSync() { if constexpr (GROUP == 32) __syncwarp(); else __syncthreads(); }
-template <int GROUP> __device__ __forceinline__ int GroupCount(bool p) { if constexpr (GROUP == 32) return __popc(__ballot_sync(0xffffffffu, p)); else return __syncthreads_count(p); }
 
-// The `rank`-th largest (1-based) of the group's keys: bit by bit, the largest value that at least `rank` keys reach. Run by one warp.
-template <int GROUP>
-__device__ __forceinline__ unsigned int KthKey(const unsigned int* key, int rank, int lane) {
-  unsigned int mine[GROUP / 32];
-#pragma unroll
-  for (int i = 0; i < GROUP / 32; ++i) mine[i] = key[lane + 32 * i];
+// The `rank`-th largest (1-based) of GROUP numbers of `bits` bits, GROUP / 32 per lane: bit by bit, the largest value that at least
+// `rank` numbers reach (0: there are fewer). Run by one warp.
+template <int PER>
+__device__ __forceinline__ unsigned int KthLargest(const unsigned int (&mine)[PER], int rank, int bits) {
   unsigned int found = 0u;
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = bits - 1; bit >= 0; --bit) {
     const unsigned int probe = found | (1u << bit);
     int c = 0;
+    if constexpr (PER == 1) c = __popc(__ballot_sync(0xffffffffu, mine[0] >= probe));
+    else {
 #pragma unroll
-    for (int i = 0; i < GROUP / 32; ++i) c += mine[i] >= probe ? 1 : 0;
-    if (static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned int>(c))) >= rank) found = probe;
+      for (int i = 0; i < PER; ++i) c += mine[i] >= probe ? 1 : 0;
+      c = __reduce_add_sync(0xffffffffu, c);
+    }
+    if (c >= rank) found = probe;
   }
   return found;
 }
 
-template <int GROUP>
-struct TopList {
-  RowShared<GROUP>* sh; int top_k, live, have; float threshold;
-  __device__ __forceinline__ TopList(RowShared<GROUP>* shared, int k) : sh(shared), top_k(k), live(0), have(0), threshold(-INFINITY) {}
-  // Every thread of the group calls it with the maximum of its scores of the chunk; each(f) calls f(score, class) for all of them,
-  // by rising class.
-  template <typename E>
-  __device__ __forceinline__ void Chunk(float most, int tid, E&& each) {
-    float limit = threshold;                    // only scores above it matter
-    bool in = most > threshold;                 // later classes lose against equal earlier ones
-    const int above = GroupCount<GROUP>(in);
-    if (above == 0) return;
-    if (tid == 0) sh->cand_count = have;
-    for (int i = tid; i < have; i += GROUP) sh->cand[i] = sh->list[live][i];
-    if (above > top_k) {
-      int first = 0x7fffffff;
-      if (in) each([&](float v, int cls) { if (v == most) first = min(first, cls); });
-      sh->key[tid] = in ? OrderKey(most) : 0u; sh->first[tid] = first;
-      GroupSync<GROUP>();
-      if (tid < 32) {
-        const unsigned int kth = KthKey<GROUP>(sh->key, top_k, tid);
-        int higher = 0, equal = 0;
-#pragma unroll
-        for (int i = 0; i < GROUP / 32; ++i) { const unsigned int k = sh->key[tid + 32 * i]; higher += k > kth ? 1 : 0; equal += k == kth ? 1 : 0; }
-        higher = __reduce_add_sync(0xffffffffu, static_cast<unsigned int>(higher)); equal = __reduce_add_sync(0xffffffffu, static_cast<unsigned int>(equal));
-        int last = 0x7fffffff;
-        if (higher + equal > top_k) {           // equal maxima: those of the lowest classes
-          unsigned int order[GROUP / 32];
-#pragma unroll
-          for (int i = 0; i < GROUP / 32; ++i) order[i] = sh->key[tid + 32 * i] == kth ? ~static_cast<unsigned int>(sh->first[tid + 32 * i]) : 0u;
-          unsigned int found = 0u;
-          for (int bit = 31; bit >= 0; --bit) {
-            const unsigned int probe = found | (1u << bit);
-            int c = 0;
-#pragma unroll
-            for (int i = 0; i < GROUP / 32; ++i) c += order[i] >= probe ? 1 : 0;
-            if (static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned int>(c))) >= top_k - higher) found = probe;
-          }
-          last = static_cast<int>(~found);
-        }
-        if (tid == 0) { sh->limit_key = kth; sh->limit_first = last; }
-      }
-      GroupSync<GROUP>();
-      const unsigned int mine = OrderKey(most);
-      in = in && (mine > sh->limit_key || (mine == sh->limit_key && first <= sh->limit_first));
-      limit = nextafterf(KeyValue(sh->limit_key), -INFINITY);
-    } else {
-      GroupSync<GROUP>();
-    }
-    if (in) each([&](float v, int cls) { if (v > limit) { const int at = atomicAdd(&sh->cand_count, 1); sh->cand[at].v = v; sh->cand[at].cls = cls; } });
-    GroupSync<GROUP>();
-    const int count = sh->cand_count;
-    for (int i = tid; i < count; i += GROUP) {
-      const Entry e = sh->cand[i];
-      int rank = 0;
-      for (int j = 0; j < count; ++j) rank += Before(sh->cand[j], e) ? 1 : 0;
-      if (rank < top_k) sh->list[live ^ 1][rank] = e;
-    }
-    GroupSync<GROUP>();
-    live ^= 1; have = min(count, top_k);
-    if (have == top_k) threshold = sh->list[live][top_k - 1].v;
+// A group's share of a row.
+template <typename T>
+struct RowShare {
+  const T* s; const uint4* body; int K, head, tail, v_begin, v_end; bool first, last_part;
+  __device__ __forceinline__ RowShare(const ClassScoresArgs& a, long long row, int part, int parts, int group) {
+    constexpr int N = Pack<T>::N;
+    s = static_cast<const T*>(a.scores) + row * a.row_stride; K = static_cast<int>(a.classes);
+    head = min(K, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(s) & 15)) & 15) / static_cast<int>(sizeof(T)));
+    const int vectors = (K - head) / N;
+    tail = head + vectors * N; body = reinterpret_cast<const uint4*>(s + head);
+    const int each = ((vectors + parts - 1) / parts + group - 1) / group * group;      // whole rounds of the group
+    v_begin = min(vectors, part * each); v_end = min(vectors, v_begin + each);
+    first = part == 0; last_part = part == parts - 1;
   }
 };
 
-// TOP: alternatives are wanted. A warp per row: 8 rows per block. A block per row: gridDim.x = rows * cluster size.
-template <typename T, int GROUP, bool TOP>
-__global__ void __launch_bounds__(256, 3) ClassLogProbsRowKernel(ClassScoresArgs a) {
-  constexpr int N = Pack<T>::N;
-  extern __shared__ __align__(16) unsigned char s_rows_raw[];
-  RowShared<GROUP>& sh = *reinterpret_cast<RowShared<GROUP>*>(s_rows_raw + (GROUP == 32 ? threadIdx.x / 32 * RowSharedBytes<GROUP, T>(a.top_k) : 0));
-  const int tid = threadIdx.x % GROUP;
-  const int parts = GROUP == 32 ? 1 : static_cast<int>(cg::this_cluster().num_blocks()), part = GROUP == 32 ? 0 : static_cast<int>(cg::this_cluster().block_rank());
-  const long long row = GROUP == 32 ? static_cast<long long>(blockIdx.x) * (256 / GROUP) + threadIdx.x / 32 : blockIdx.x / parts;
-  if (GROUP == 32 && row >= a.rows) return;                     // whole warps
-  const T* s = static_cast<const T*>(a.scores) + row * a.row_stride;
-  const T* type = nullptr;
-  const int K = static_cast<int>(a.classes);
-  const int head = min(K, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(s) & 15)) & 15) / static_cast<int>(sizeof(T)));
-  const int vectors = (K - head) / N, tail = head + vectors * N;
-  const int each = ((vectors + parts - 1) / parts + GROUP - 1) / GROUP * GROUP;      // whole rounds of the group
-  const int v_begin = min(vectors, part * each), v_end = min(vectors, v_begin + each);
-  const uint4* body = reinterpret_cast<const uint4*>(s + head);
-  Sums sums;
-  TopList<GROUP> top(&sh, a.top_k);
-  if (part == 0 && head > 0) {
-    const float v = tid < head ? ToFloat(s[tid]) : -INFINITY;
-    if (tid < head) sums.AddOne(v);
-    if constexpr (TOP) top.Chunk(v, tid, [&](auto&& f) { f(v, tid); });
-  }
-  uint4 q[kUnroll], next[kUnroll];
-  auto load = [&](uint4 (&to)[kUnroll], int at) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) { const int i = at + u * GROUP + tid; to[u] = i < v_end ? __ldg(body + i) : AllRuledOut(type); }
-  };
-  load(q, v_begin);
-  for (int at = v_begin; at < v_end; at += GROUP * kUnroll) {
-    load(next, at + GROUP * kUnroll);
-    float most = Max(q[0], type);
-#pragma unroll
-    for (int u = 1; u < kUnroll; ++u) most = MaxNan(most, Max(q[u], type));
-    if (most > sums.m) sums.Raise(most);
-    const float base = sums.Base();
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+template <int GROUP, typename T>
+struct Alternatives {
+  static constexpr int N = Pack<T>::N;
+  RowShared<GROUP>& sh; const RowShare<T>& r; int top_k, tid;
+  // f(score, class) for the scores of the flagged threads and the ends of the row, dealt out over the group
+  template <typename F>
+  __device__ __forceinline__ void Scores(int num_flagged, float head_v, float tail_v, F&& f) const {
+    if (r.first && tid < r.head) f(head_v, tid);
+    if (r.last_part && tid < r.K - r.tail) f(tail_v, r.tail + tid);
+    const int rounds = (r.v_end - r.v_begin + GROUP - 1) / GROUP;
+    for (int e = tid; e < num_flagged * rounds; e += GROUP) {
+      const int i = r.v_begin + (e / num_flagged) * GROUP + sh.flagged[e % num_flagged];
+      if (i >= r.v_end) continue;
+      const uint4 q = __ldg(r.body + i);
       float v[N];
-      Unpack(q[u], v, type);
+      Unpack(q, v, static_cast<const T*>(nullptr));
 #pragma unroll
-      for (int i = 0; i < N; ++i) sums.Add(v[i], base);
+      for (int k = 0; k < N; ++k) f(v[k], r.head + i * N + k);
     }
-    if constexpr (TOP) {
-      top.Chunk(most, tid, [&](auto&& f) {
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          float v[N];
-          Unpack(q[u], v, type);
-#pragma unroll
-          for (int i = 0; i < N; ++i) f(v[i], head + (at + u * GROUP + tid) * N + i);
-        }
-      });
+  }
+  // Ranks the first `count` candidates into the list; returns how many that leaves.
+  __device__ __forceinline__ int Rank(int count) {
+    for (int i = tid; i < count; i += GROUP) {
+      const Entry e = sh.cand[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += Before(sh.cand[j], e) ? 1 : 0;
+      if (rank < top_k) sh.list[rank] = e;
     }
+    GroupSync<GROUP>();
+    return min(count, top_k);
+  }
+  // most: this thread's maximum. All threads; the list is complete on return.
+  __device__ __forceinline__ int Find(float most, float head_v, float tail_v) {
+    constexpr int PER = GROUP / 32;
+    sh.key[tid] = OrderKey<T>(most);
+    GroupSync<GROUP>();
+    if (tid < 32) {
+      unsigned int mine[PER];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = next[u];
-  }
-  if (part == parts - 1 && tail < K) {
-    const float v = tid < K - tail ? ToFloat(s[tail + tid]) : -INFINITY;
-    if (tid < K - tail) sums.AddOne(v);
-    if constexpr (TOP) top.Chunk(v, tid, [&](auto&& f) { f(v, tail + tid); });
-  }
-  sums.JoinLanes();
-  const long long y = LabelOf(a, row);
-  if constexpr (GROUP == 32) {
-    const RowResult res(sums);
-    if (tid == 0) res.Store(a, row, y, y >= 0 && y < K ? ToFloat(s[y]) : 0.f);
-    if constexpr (TOP) if (tid < a.top_k) { const Entry e = sh.list[top.live][tid]; res.StoreTop(a, row * a.top_k + tid, tid < top.have ? e.v : -INFINITY, e.cls); }
-  } else {
-    if ((tid & 31) == 0) { sh.part_m[tid >> 5] = sums.m; sh.part_s[tid >> 5] = sums.s; sh.part_t[tid >> 5] = sums.t; }
-    __syncthreads();
-    sums = Sums();
-    for (int w = 0; w < GROUP / 32; ++w) sums.Join(sh.part_m[w], sh.part_s[w], sh.part_t[w]);
-    if (parts > 1) {
-      // the cluster's first block joins the others' sums and lists, read from their shared memory
-      __syncthreads();
-      if (tid == 0) { sh.part_m[0] = sums.m; sh.part_s[0] = sums.s; sh.part_t[0] = sums.t; sh.cand_count = top.have; sh.limit_first = top.live; }
-      cg::this_cluster().sync();
-      if (part == 0) {
-        int others = 0;
-        for (int p = 1; p < parts; ++p) {
-          const RowShared<GROUP>* o = cg::this_cluster().map_shared_rank(&sh, p);
-          sums.Join(o->part_m[0], o->part_s[0], o->part_t[0]);
-          if constexpr (TOP) {
-            const int n = o->cand_count, from = o->limit_first;
-            for (int i = tid; i < n; i += GROUP) sh.cand[top.have + others + i] = o->list[from][i];
-            others += n;
-          }
-        }
-        if constexpr (TOP) {
-          for (int i = tid; i < top.have; i += GROUP) sh.cand[i] = sh.list[top.live][i];
-          __syncthreads();
-          const int count = top.have + others;
-          for (int i = tid; i < count; i += GROUP) {
-            const Entry e = sh.cand[i];
-            int rank = 0;
-            for (int j = 0; j < count; ++j) rank += Before(sh.cand[j], e) ? 1 : 0;
-            if (rank < a.top_k) sh.list[top.live ^ 1][rank] = e;
-          }
-          __syncthreads();
-          top.live ^= 1; top.have = min(count, a.top_k);
-        }
+      for (int i = 0; i < PER; ++i) mine[i] = sh.key[tid + 32 * i];
+      const unsigned int limit = max(1u, KthLargest<PER>(mine, top_k, KeyBits<T>::kBits));      // key 0: a thread without a score
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const unsigned int in = __ballot_sync(0xffffffffu, mine[i] >= limit);
+        const int at = n + __popc(in & ((1u << tid) - 1u));
+        if (mine[i] >= limit && at < RowShared<GROUP>::kFlagged) sh.flagged[at] = tid + 32 * i;
+        n += __popc(in);
       }
-      cg::this_cluster().sync();         // no block leaves while its shared memory is read
-      if (part != 0) return;
+      if (tid == 0) { sh.limit = limit; sh.num_flagged = n; sh.num_cand = 0; sh.last = 0x7fffffff; }
     }
-    const RowResult res(sums);
-    if (tid == 0) res.Store(a, row, y, y >= 0 && y < K ? ToFloat(s[y]) : 0.f);
-    if constexpr (TOP) if (tid < a.top_k) { const Entry e = sh.list[top.live][tid]; res.StoreTop(a, row * a.top_k + tid, tid < top.have ? e.v : -INFINITY, e.cls); }
+    GroupSync<GROUP>();
+    const unsigned int limit = sh.limit;
+    if (GROUP > 32 && sh.num_flagged > RowShared<GROUP>::kFlagged) Ties(limit);
+    const int last = sh.last, num_flagged = sh.num_flagged;
+    Scores(num_flagged, head_v, tail_v, [&](float v, int cls) {
+      const unsigned int k = OrderKey<T>(v);
+      if (k > limit || (k == limit && cls <= last)) { const int at = atomicAdd(&sh.num_cand, 1); if (at < RowShared<GROUP>::kCandidates) { sh.cand[at].v = v; sh.cand[at].cls = cls; } }
+    });
+    GroupSync<GROUP>();
+    const int count = sh.num_cand;
+    if (count <= RowShared<GROUP>::kCandidates) return Rank(count);
+    return OneByOne(num_flagged, head_v, tail_v);
+  }
+  // Very many equal maxima: of the threads with maximum `limit` only those count that reach it at the lowest classes.
+  __device__ void Ties(unsigned int limit) {
+    constexpr int PER = GROUP / 32;
+    unsigned int order = 0u;
+    const unsigned int mine = sh.key[tid];
+    if (mine == limit) {
+      int at = 0x7fffffff;
+      if (r.first && tid < r.head && OrderKey<T>(ToFloat(r.s[tid])) == limit) at = tid;
+      for (int i = r.v_begin + tid; i < r.v_end && at == 0x7fffffff; i += GROUP) {
+        float v[N];
+        Unpack(__ldg(r.body + i), v, static_cast<const T*>(nullptr));
+#pragma unroll
+        for (int k = N - 1; k >= 0; --k) if (OrderKey<T>(v[k]) == limit) at = r.head + i * N + k;
+      }
+      if (at == 0x7fffffff) at = r.tail + tid;      // its last score
+      order = 0x80000000u - static_cast<unsigned int>(at);
+    }
+    const int higher = __syncthreads_count(mine > limit);
+    sh.key[tid] = order;
+    const bool above = mine > limit;
+    if (tid == 0) sh.num_flagged = 0;
+    __syncthreads();
+    if (tid < 32) {
+      unsigned int all[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) all[i] = sh.key[tid + 32 * i];
+      const unsigned int kth = KthLargest<PER>(all, top_k - higher, 32);
+      if (tid == 0) sh.last = static_cast<int>(0x80000000u - kth);
+    }
+    __syncthreads();
+    if (above || (mine == limit && order >= 0x80000000u - static_cast<unsigned int>(sh.last))) sh.flagged[atomicAdd(&sh.num_flagged, 1)] = tid;
+    __syncthreads();
+  }
+  // More candidates than the list holds (few threads own very many of the best scores): one alternative per pass.
+  __device__ int OneByOne(int num_flagged, float head_v, float tail_v) {
+    Entry before; before.v = INFINITY; before.cls = -1;
+    int t = 0;
+    for (; t < top_k; ++t) {
+      Entry best; best.v = -INFINITY; best.cls = 0x7fffffff;
+      Scores(num_flagged, head_v, tail_v, [&](float v, int cls) { Entry e; e.v = v; e.cls = cls; if (v > -INFINITY && Before(before, e) && Before(e, best)) best = e; });
+      for (int o = 16; o > 0; o >>= 1) {
+        Entry e; e.v = __shfl_xor_sync(0xffffffffu, best.v, o); e.cls = __shfl_xor_sync(0xffffffffu, best.cls, o);
+        if (Before(e, best)) best = e;
+      }
+      if constexpr (GROUP > 32) {
+        if ((tid & 31) == 0) sh.cand[tid >> 5] = best;
+        __syncthreads();
+        best = sh.cand[0];
+        for (int w = 1; w < GROUP / 32; ++w) if (Before(sh.cand[w], best)) best = sh.cand[w];
+        __syncthreads();
+      }
+      if (best.cls == 0x7fffffff) break;
+      if (tid == 0) sh.list[t] = best;
+      before = best;
+    }
+    GroupSync<GROUP>();
+    return t;
+  }
+};
+
+// TOP: alternatives are wanted. Groups walk the rows with the grid's stride; a row belongs to a warp, a block or a cluster.
+template <typename T, int GROUP, bool TOP>
+__global__ void __launch_bounds__(256, TOP ? 3 : 4) ClassLogProbsRowKernel(ClassScoresArgs a) {
+  constexpr int kGroups = 256 / GROUP;
+  __shared__ RowShared<GROUP> s_all[TOP ? kGroups : 1];
+  __shared__ float s_m[8], s_s[8], s_t[8];
+  RowShared<GROUP>& sh = s_all[TOP && GROUP == 32 ? threadIdx.x / 32 : 0];
+  const int tid = threadIdx.x % GROUP;
+  const T* type = nullptr;
+  const int parts = GROUP == 32 ? 1 : static_cast<int>(cg::this_cluster().num_blocks()), part = GROUP == 32 ? 0 : static_cast<int>(cg::this_cluster().block_rank());
+  const long long stride = GROUP == 32 ? static_cast<long long>(gridDim.x) * kGroups : gridDim.x / parts;
+  long long row = GROUP == 32 ? static_cast<long long>(blockIdx.x) * kGroups + threadIdx.x / 32 : blockIdx.x / parts;
+  if (row >= a.rows) return;                     // whole groups
+  uint4 q[kUnroll], next[kUnroll];
+  auto load = [&](uint4 (&to)[kUnroll], const RowShare<T>& r, int at) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) { const int i = at + u * GROUP + tid; to[u] = i < r.v_end ? __ldg(r.body + i) : AllRuledOut(type); }
+  };
+  RowShare<T> r(a, row, part, parts, GROUP);
+  load(q, r, r.v_begin);
+  long long y = LabelOf(a, row);
+  for (;;) {
+    const long long next_row = row + stride;
+    const bool more = next_row < a.rows;
+    const float head_v = r.first && tid < r.head ? ToFloat(r.s[tid]) : -INFINITY, tail_v = r.last_part && tid < r.K - r.tail ? ToFloat(r.s[r.tail + tid]) : -INFINITY;
+    const float given = tid == 0 && y >= 0 && y < r.K ? ToFloat(r.s[y]) : 0.f;
+    const RowShare<T> rn(a, more ? next_row : row, part, parts, GROUP);
+    const long long y_next = more ? LabelOf(a, next_row) : -1;
+    PairSums<T> pairs;
+    int at = r.v_begin;
+    do {                                         // a share without vectors takes one empty step
+      const int then = at + GROUP * kUnroll;
+      if (then < r.v_end) load(next, r, then); else if (more) load(next, rn, rn.v_begin);
+      float most = Max(q[0], type);
+#pragma unroll
+      for (int u = 1; u < kUnroll; ++u) most = MaxNan(most, Max(q[u], type));
+      if (most > pairs.m) pairs.Raise(most);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (u == 0 || at + u * GROUP + (tid & ~31) < r.v_end) pairs.Add16(q[u]);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) q[u] = next[u];
+      at = then;
+    } while (at < r.v_end);
+    Sums sums = pairs.Total();
+    if (head_v != -INFINITY) sums.AddOne(head_v);
+    if (tail_v != -INFINITY) sums.AddOne(tail_v);
+    const float most = sums.m;
+    sums.JoinLanes();
+    if constexpr (GROUP == 32) {
+      const RowResult res(sums);
+      if (tid == 0) res.Store(a, row, y, given);
+      if constexpr (TOP) {
+        Alternatives<GROUP, T> alt{sh, r, a.top_k, tid};
+        const int have = alt.Find(most, head_v, tail_v);
+        if (tid < a.top_k) { const Entry e = sh.list[tid]; res.StoreTop(a, row * a.top_k + tid, tid < have ? e.v : -INFINITY, e.cls); }
+        __syncwarp();
+      }
+    } else {
+      if ((tid & 31) == 0) { s_m[tid >> 5] = sums.m; s_s[tid >> 5] = sums.s; s_t[tid >> 5] = sums.t; }
+      int have = 0;
+      if constexpr (TOP) { Alternatives<GROUP, T> alt{sh, r, a.top_k, tid}; have = alt.Find(most, head_v, tail_v); } else __syncthreads();
+      if (tid < 32) {
+        sums = Sums();
+        if (tid < GROUP / 32) { sums.m = s_m[tid]; sums.s = s_s[tid]; sums.t = s_t[tid]; }
+        sums.JoinLanes();
+      }
+      if (parts > 1) {
+        // the cluster's first block joins the others' sums and lists, read from their shared memory
+        __syncthreads();
+        if (tid == 0) { s_m[0] = sums.m; s_s[0] = sums.s; s_t[0] = sums.t; if constexpr (TOP) sh.have = have; }
+        cg::this_cluster().sync();
+        if (part == 0) {
+          int count = have;
+          if (TOP && tid < have) sh.cand[tid] = sh.list[tid];
+          for (int p = 1; p < parts; ++p) {
+            if (tid < 32) sums.Join(*cg::this_cluster().map_shared_rank(&s_m[0], p), *cg::this_cluster().map_shared_rank(&s_s[0], p), *cg::this_cluster().map_shared_rank(&s_t[0], p));
+            if constexpr (TOP) {
+              const RowShared<GROUP>* o = cg::this_cluster().map_shared_rank(&sh, p);
+              const int n = o->have;
+              if (tid < n) sh.cand[count + tid] = o->list[tid];
+              count += n;
+            }
+          }
+          if constexpr (TOP) { __syncthreads(); Alternatives<GROUP, T> alt{sh, r, a.top_k, tid}; have = alt.Rank(count); }
+        }
+        cg::this_cluster().sync();         // no block goes on while its shared memory is read
+      }
+      if (part == 0 && tid < 32) {
+        const RowResult res(sums);
+        if (tid == 0) res.Store(a, row, y, given);
+        if constexpr (TOP) if (tid < a.top_k) { const Entry e = sh.list[tid]; res.StoreTop(a, row * a.top_k + tid, tid < have ? e.v : -INFINITY, e.cls); }
+      }
+      __syncthreads();                     // the next row writes the shared parts again
+    }
+    if (!more) return;
+    row = next_row; r = rn; y = y_next;
   }
 }
 
@@ -593,6 +727,8 @@ template <typename F> void DispatchType(int dtype, F&& f) {
   }
 }
 
+constexpr int kSms = 148;
+
 template <typename T, bool BY_CLASS>
 void LaunchFew(const ClassScoresArgs& a, cudaStream_t s) {
   const unsigned int blocks = static_cast<unsigned int>((a.rows + kFewThreads - 1) / kFewThreads);
@@ -605,22 +741,18 @@ void LaunchFew(const ClassScoresArgs& a, cudaStream_t s) {
 
 template <typename T, int GROUP, bool TOP>
 void LaunchRows(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
-  static PerDevice allowed;
-  constexpr int kGroups = 256 / GROUP, kMost = kGroups * RowSharedBytes<GROUP, T>(kMaxTopClasses);
-  if (kMost > 48 * 1024) AllowSharedMemory(ClassLogProbsRowKernel<T, GROUP, TOP>, kMost, &allowed);
+  // as many groups as are resident at once, each with several rows
+  const long long groups = GROUP == 32 ? (a.rows + 7) / 8 : a.rows, most = static_cast<long long>(kSms) * (TOP ? 3 : 4) * (GROUP == 32 ? 2 : 1) / cluster;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned int>(GROUP == 32 ? (a.rows + kGroups - 1) / kGroups : a.rows * cluster)); cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = kGroups * RowSharedBytes<GROUP, T>(a.top_k); cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cfg.gridDim = dim3(static_cast<unsigned int>(std::min(groups, most) * cluster)); cfg.blockDim = dim3(256); cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
   FB_CUDA(cudaLaunchKernelEx(&cfg, ClassLogProbsRowKernel<T, GROUP, TOP>, a));
 }
 template <typename T, int GROUP>
 void LaunchRows(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
   if (a.top_k > 0) LaunchRows<T, GROUP, true>(a, cluster, s); else LaunchRows<T, GROUP, false>(a, cluster, s);
 }
-
-constexpr int kSms = 148;
 
 }  // namespace
 
@@ -639,7 +771,6 @@ void LaunchClassLogProbs(const ClassScoresArgs& a, cudaStream_t s) {
       else {
         int cluster = 1;
         while (cluster < 8 && a.rows * cluster < 2 * kSms && a.classes >= 2 * cluster * chunk / kUnroll) cluster *= 2;
-        if (a.rows * cluster > 0x7fffffffLL) Log::Fatal("class scores: too many rows");
         LaunchRows<T, 256>(a, cluster, s);
       }
     } else {
