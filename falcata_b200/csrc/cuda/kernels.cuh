@@ -377,6 +377,10 @@ struct LeafProductsArgs {
 // out [leaves x a_cols x b_cols] dense, of the inputs' type or fp32.
 struct LeafGramArgs { LeafWindows leaves; const void* a; const void* b; void* out; int dtype, out_dtype; int a_cols, b_cols; long long a_stride, b_stride; };
 void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s);
-void LaunchLeafGram(const LeafGramArgs& a, cudaStream_t s);
+// Long leaves are summed in slices of rows: LeafGramWorkspace floats for their sums (0: none wanted).
+long long LeafGramWorkspace(const LeafGramArgs& a);
+int LeafGramSliceRows(const LeafGramArgs& a);
+long long LeafGramSlices(const LeafGramArgs& a);
+void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s);
 
 }  // namespace fb

@@ -262,15 +262,19 @@ int FB_OpLeafProducts(const void* x, long long x_stride, const void* weight, lon
   LaunchLeafProducts(a, static_cast<cudaStream_t>(stream));
   OPS_END();
 }
-// P_g = sum over the rows of leaf g of a_i b_i^T.
+// P_g = sum over the rows of leaf g of a_i b_i^T. With `workspace_floats` not null nothing runs: it takes the floats of workspace
+// that the call with the same sizes needs (possibly 0).
 int FB_OpLeafGram(const void* a_rows, long long a_stride, const void* b_rows, long long b_stride, const void* begin, int begin_bits, int leaves, long long rows, int a_cols, int b_cols,
-                  int dtype, int out_dtype, void* out, int device, void* stream) {
+                  int dtype, int out_dtype, void* out, void* workspace, long long* workspace_floats, int device, void* stream) {
   OPS_BEGIN();
   CheckLeafWindows(begin_bits, leaves, rows);
   if (a_cols < 1 || b_cols < 1) Log::Fatal("leaf Gram: at least one column on each side (got %d, %d)", a_cols, b_cols);
-  DeviceScope scope(device);
   LeafGramArgs a{{begin, begin_bits, leaves, rows}, a_rows, b_rows, out, dtype, out_dtype, a_cols, b_cols, a_stride, b_stride};
-  LaunchLeafGram(a, static_cast<cudaStream_t>(stream));
+  const long long floats = LeafGramWorkspace(a);
+  if (workspace_floats != nullptr) { *workspace_floats = floats; return 0; }
+  if (floats > 0 && workspace == nullptr) Log::Fatal("leaf Gram: a workspace of %lld floats is needed", floats);
+  DeviceScope scope(device);
+  LaunchLeafGram(a, static_cast<float*>(workspace), static_cast<cudaStream_t>(stream));
   OPS_END();
 }
 

@@ -98,8 +98,13 @@ def leaf_gram(a: torch.Tensor, b: torch.Tensor, leaf_begin: torch.Tensor, dtype:
     a, b, leaf_begin = _inner_contiguous(a), _inner_contiguous(b), leaf_begin.contiguous()
     leaves = leaf_begin.numel() - 1
     out = torch.empty((leaves, a.shape[1], b.shape[1]), dtype=dtype, device=a.device)
-    check(_gram()(ptr(a), a.stride(0), ptr(b), b.stride(0), ptr(leaf_begin), 8 * leaf_begin.element_size(), leaves, a.shape[0], a.shape[1], b.shape[1], type_code("a", a),
-                  type_code("dtype", out), ptr(out), *device_and_stream(a.device)))
+    args = (ptr(a), a.stride(0), ptr(b), b.stride(0), ptr(leaf_begin), 8 * leaf_begin.element_size(), leaves, a.shape[0], a.shape[1], b.shape[1], type_code("a", a),
+            type_code("dtype", out), ptr(out))
+    floats = ctypes.c_longlong(0)
+    where = device_and_stream(a.device)
+    check(_gram()(*args, None, ctypes.byref(floats), *where))
+    workspace = torch.empty(floats.value, dtype=torch.float32, device=a.device) if floats.value else None
+    check(_gram()(*args, ptr(workspace), None, *where))
     return out
 
 
@@ -111,4 +116,4 @@ def _fwd():
 
 
 def _gram():
-    return bind("FB_OpLeafGram", (_P, _L, _P, _L, _P, _I, _I, _L, _I, _I, _I, _I, _P, _I, _P))
+    return bind("FB_OpLeafGram", (_P, _L, _P, _L, _P, _I, _I, _L, _I, _I, _I, _I, _P, _P, ctypes.POINTER(_L), _I, _P))

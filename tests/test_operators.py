@@ -97,4 +97,4 @@ def test_native_entry_points_return_errors():
     assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(32), I(0), L(4), I(3), I(5), I(0), P(), I(0), P()) == -1 and b"leaves" in lib.FB_OpsLastError()
     assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(16), I(2), L(4), I(3), I(5), I(0), P(), I(0), P()) == -1 and b"boundaries" in lib.FB_OpsLastError()
     assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(32), I(2), L(4), I(0), I(5), I(0), P(), I(0), P()) == -1 and b"feature" in lib.FB_OpsLastError()
-    assert lib.FB_OpLeafGram(P(), L(3), P(), L(3), P(), I(32), I(2), L(4), I(0), I(3), I(0), I(0), P(), I(0), P()) == -1 and b"column" in lib.FB_OpsLastError()
+    assert lib.FB_OpLeafGram(P(), L(3), P(), L(3), P(), I(32), I(2), L(4), I(0), I(3), I(0), I(0), P(), P(), P(), I(0), P()) == -1 and b"column" in lib.FB_OpsLastError()
