@@ -303,52 +303,271 @@ __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int ro
   }
 }
 
-// ------------------------------------------------------------------------------------- 16-bit types, any shape ----
-constexpr int kTile = 16;
+// ---------------------------------------------------------------------------------------------- 16-bit types ----
+// D [128 x N] += A [128 x 64] B [64 x N] steps on the tensor cores, N <= 256, accumulators in tensor memory (two sets, so that
+// one tile is stored while the next is summed). Products: A = 128 rows of x, B = N outputs of the leaf's map, the steps walk the
+// features. Gram: A = 128 columns of one side, B = N of the other, the steps walk the slice's rows.
+// Operands lie in shared memory in the 128-byte-swizzled layout: lines of 64 values, the 16-byte piece c of line l at piece
+// c ^ (l % 8). A line is a row / output with 64 features (K-major), or a feature / row with 64 outputs / columns (MN-major), whatever
+// is contiguous in memory. Copies go in pieces of 16, 8 or 4 bytes as the operand's alignment allows, single values else; what lies
+// outside the operand is zero, which is what makes ragged leaves and odd sizes exact.
+// Warps: 0-3 store the accumulators, 4-11 copy, 12 issues the matrix instructions. Every wait is bounded; one that gives up
+// makes all roles leave, the tile's outputs NaN and the device's status word 1.
+constexpr int kDepthTc = 64, kTileM = 128, kMostN = 256;
+constexpr int kCopyWarps = 8, kCopyThreads = 32 * kCopyWarps, kTcThreads = 128 + kCopyThreads + 32;
+constexpr int kMostStages = 8, kLag = 2;           // a stage is handed over when kLag younger ones are on their way
+constexpr int kABytes = kTileM * 128;
 
-// Block (x: 16 outputs, y: slice of a leaf's rows, z: leaf): 16 x 16 outputs at a time through shared memory.
-template <typename T>
-__global__ void __launch_bounds__(kTile * kTile) LeafProductsKernel(LeafProductsArgs a) {
-  __shared__ float s_x[kTile][kTile + 1], s_w[kTile][kTile + 1];
-  const int tx = threadIdx.x % kTile, ty = threadIdx.x / kTile;
-  for (int g = blockIdx.z; g < a.leaves.leaves; g += gridDim.z) {
-    long long begin, end; LeafWindow(a.leaves, g, &begin, &end);
-    const T* w = static_cast<const T*>(a.weight) + g * a.weight_leaf_stride;
-    for (long long r0 = begin + static_cast<long long>(blockIdx.y) * kTile; r0 < end; r0 += static_cast<long long>(gridDim.y) * kTile) {
-      for (int p0 = blockIdx.x * kTile; p0 < a.outputs; p0 += gridDim.x * kTile) {
-        float acc = 0.f;
-        for (int f0 = 0; f0 < a.features; f0 += kTile) {
-          s_x[ty][tx] = (r0 + ty < end && f0 + tx < a.features) ? ToFloat(static_cast<const T*>(a.x)[(r0 + ty) * a.x_stride + f0 + tx]) : 0.f;
-          s_w[ty][tx] = (p0 + ty < a.outputs && f0 + tx < a.features) ? ToFloat(w[(p0 + ty) * a.weight_out_stride + (f0 + tx) * a.weight_in_stride]) : 0.f;
-          __syncthreads();
-          for (int f = 0; f < kTile; ++f) acc = fmaf(s_x[ty][f], s_w[tx][f], acc);
-          __syncthreads();
-        }
-        if (r0 + ty < end && p0 + tx < a.outputs) static_cast<T*>(a.y)[(r0 + ty) * a.outputs + p0 + tx] = FromFloat<T>(acc);
-      }
+__device__ unsigned int g_product_status;
+
+__device__ __forceinline__ void BarInit(unsigned long long* bar, unsigned int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(Smem32(bar)), "r"(count) : "memory"); }
+__device__ __forceinline__ void BarArrive(unsigned long long* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(Smem32(bar)) : "memory"); }
+__device__ __forceinline__ bool BarTry(unsigned long long* bar, unsigned int parity) {
+  unsigned int ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(Smem32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// false: the budget ran out, here or in another role
+__device__ __forceinline__ bool BarWait(unsigned long long* bar, unsigned int parity, volatile int* stop) {
+  for (int i = 0; i < (1 << 20); ++i) { if (BarTry(bar, parity)) return true; if (*stop != 0) return false; }
+  *stop = 1; atomicExch(&g_product_status, 1u);
+  return false;
+}
+__device__ __forceinline__ void MmaCommit(unsigned long long* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(Smem32(bar)) : "memory");
+}
+// 128-byte swizzle. K-major: 8-line groups `stride` = 1024 bytes apart. MN-major: 8-line groups 1024 bytes apart, blocks of 64 values
+// `lead` = 8192 bytes apart.
+__device__ __forceinline__ unsigned long long OperandDesc(unsigned int addr, unsigned int lead) {
+  return static_cast<unsigned long long>((addr & 0x3FFFFu) >> 4) | (static_cast<unsigned long long>(lead >> 4) << 16) | (static_cast<unsigned long long>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void Mma16(unsigned int d, unsigned long long da, unsigned long long db, unsigned int idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+               ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void TmemLoad16(unsigned int addr, unsigned int (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(addr) : "memory");
+}
+
+// One operand's part of a tile in memory: `lines` lines `stride` values apart, `along` values each.
+struct OperandView { const unsigned short* base; long long stride; int lines, along; };
+
+// `valid` of 8 values to a 16-byte piece of shared memory, the rest zero.
+__device__ __forceinline__ void CopyPiece(unsigned int dst, const unsigned short* src, int valid, int vec) {
+  if (vec == 8) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(2 * valid) : "memory");
+  } else if (vec == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int n = max(0, min(4, valid - 4 * h));
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + 8 * h), "l"(n > 0 ? src + 4 * h : src), "r"(2 * n) : "memory");
     }
+  } else if (vec == 2) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int n = max(0, min(2, valid - 2 * h));
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * h), "l"(n > 0 ? src + 2 * h : src), "r"(2 * n) : "memory");
+    }
+  } else {
+    unsigned int w[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const unsigned int lo = 2 * h < valid ? __ldg(src + 2 * h) : 0u, hi = 2 * h + 1 < valid ? __ldg(src + 2 * h + 1) : 0u;
+      w[h] = lo | (hi << 16);
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+  }
+}
+// Lines of `depth` (a multiple of 16) features from k0 on.
+__device__ __forceinline__ void CopyKMajor(unsigned int dst, const OperandView& o, int tile_lines, int k0, int depth, int vec, int tid) {
+  const int c = tid & 7;
+  if (c * 8 >= depth) return;
+  const int along = max(0, min(8, o.along - (k0 + 8 * c)));
+#pragma unroll 4
+  for (int l = tid >> 3; l < tile_lines; l += kCopyThreads / 8) {
+    const int valid = l < o.lines ? along : 0;
+    CopyPiece(dst + l * 128 + ((c ^ (l & 7)) << 4), valid > 0 ? o.base + l * o.stride + k0 + 8 * c : o.base, valid, vec);
+  }
+}
+// `depth` lines from k0 on, of `pieces` 16-byte pieces.
+__device__ __forceinline__ void CopyMnMajor(unsigned int dst, const OperandView& o, int pieces, int k0, int depth, int vec, int tid) {
+  const int bits = 32 - __clz(pieces - 1), c = tid & ((1 << bits) - 1);      // pieces 2..32
+  if (c >= pieces) return;
+  const int along = max(0, min(8, o.along - 8 * c));
+#pragma unroll 4
+  for (int l = tid >> bits; l < depth; l += kCopyThreads >> bits) {
+    const int valid = k0 + l < o.lines ? along : 0;
+    CopyPiece(dst + (c >> 3) * 8192 + l * 128 + (((c & 7) ^ (l & 7)) << 4), valid > 0 ? o.base + (k0 + l) * o.stride + 8 * c : o.base, valid, vec);
   }
 }
 
-template <typename T, typename O>
-__global__ void __launch_bounds__(kTile * kTile) LeafGramKernel(LeafGramArgs a) {
-  __shared__ float s_a[kTile][kTile + 1], s_b[kTile][kTile + 1];
-  const int tx = threadIdx.x % kTile, ty = threadIdx.x / kTile;
-  for (int g = blockIdx.z; g < a.leaves.leaves; g += gridDim.z) {
-    long long begin, end; LeafWindow(a.leaves, g, &begin, &end);
-    for (int p0 = blockIdx.y * kTile; p0 < a.a_cols; p0 += gridDim.y * kTile)
-      for (int q0 = blockIdx.x * kTile; q0 < a.b_cols; q0 += gridDim.x * kTile) {
-        float acc = 0.f;
-        for (long long r0 = begin; r0 < end; r0 += kTile) {
-          s_a[ty][tx] = (r0 + ty < end && p0 + tx < a.a_cols) ? ToFloat(static_cast<const T*>(a.a)[(r0 + ty) * a.a_stride + p0 + tx]) : 0.f;
-          s_b[ty][tx] = (r0 + ty < end && q0 + tx < a.b_cols) ? ToFloat(static_cast<const T*>(a.b)[(r0 + ty) * a.b_stride + q0 + tx]) : 0.f;
-          __syncthreads();
-          for (int r = 0; r < kTile; ++r) acc = fmaf(s_a[r][ty], s_b[r][tx], acc);
-          __syncthreads();
-        }
-        if (p0 + ty < a.a_cols && q0 + tx < a.b_cols) static_cast<O*>(a.out)[(static_cast<long long>(g) * a.a_cols + p0 + ty) * a.b_cols + q0 + tx] = FromFloat<O>(acc);
-      }
+// What a launch walks, for both products.
+struct TensorArgs {
+  LeafWindows leaves; int tile_rows, least;                     // rows per tile or slice; tiles of a leaf without rows
+  const unsigned short *a, *b; long long a_stride, b_stride, b_leaf_stride;
+  int a_vec, b_vec, a_size, b_size, depth;                      // columns of a Gram's sides; outputs (b_size) and features (depth) of products
+  int n, across_a, across_b, stages, stage_bytes, tmem_cols;
+  unsigned int idesc;
+  void* out; float* partial; long long out_row_stride, out_col_stride;
+};
+enum { kProductsK, kProductsMn, kGram };
+
+template <typename T, typename O, int MODE>
+__global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) {
+  extern __shared__ unsigned char s_raw[];
+  __shared__ TileMap map;
+  __shared__ unsigned long long s_full[kMostStages], s_empty[kMostStages], s_done[2], s_free[2];
+  __shared__ unsigned int s_tmem; __shared__ int s_stop;
+  unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Smem32(&s_tmem)), "r"(a.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) { BarInit(s_full + i, kCopyWarps); BarInit(s_empty + i, 1); }
+    for (int i = 0; i < 2; ++i) { BarInit(s_done + i, 1); BarInit(s_free + i, 4); }
+    s_stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  map.Build(a.leaves, a.tile_rows, a.least);
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned int tmem = *reinterpret_cast<volatile unsigned int*>(&s_tmem);
+  volatile int* stop = &s_stop;
+  const int across = a.across_a * a.across_b;
+  const long long tiles = static_cast<long long>(map.Total()) * across;
+  // Products: the row tiles of the leaves, `across_b` output tiles each. Gram: slices, across_a x across_b tiles each.
+  struct Tile { int leaf, which, m0, n0, depth; long long row0, end; };
+  auto tile_of = [&](long long t) {
+    Tile r;
+    r.which = static_cast<int>(t / across);
+    const int rest = static_cast<int>(t % across);
+    map.Find(a.leaves, r.which, a.tile_rows, a.least, &r.leaf, &r.row0, &r.end);
+    r.m0 = MODE == kGram ? rest / a.across_b * kTileM : 0; r.n0 = rest % a.across_b * a.n;
+    r.depth = MODE == kGram ? static_cast<int>(r.end - r.row0) : a.depth;
+    return r;
+  };
+
+  if (warp >= 4 && warp < 12) {
+    const int tid = threadIdx.x - 128;
+    int it = 0;
+    bool ok = true;
+    auto hand_over = [&](int step) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // this thread's copies -> visible to the tensor core's reads
+      __syncwarp();
+      if (lane == 0) BarArrive(s_full + step % a.stages);
+    };
+    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile tile = tile_of(t);
+      OperandView va, vb;
+      const int rows = static_cast<int>(tile.end - tile.row0);
+      va.stride = a.a_stride; vb.stride = a.b_stride;
+      if constexpr (MODE == kGram) {
+        va.base = a.a + tile.row0 * a.a_stride + tile.m0; va.lines = rows; va.along = a.a_size - tile.m0;
+        vb.base = a.b + tile.row0 * a.b_stride + tile.n0; vb.lines = rows; vb.along = a.b_size - tile.n0;
+      } else {
+        va.base = a.a + tile.row0 * a.a_stride; va.lines = rows; va.along = a.depth;
+        if constexpr (MODE == kProductsK) { vb.base = a.b + tile.leaf * a.b_leaf_stride + tile.n0 * a.b_stride; vb.lines = a.b_size - tile.n0; vb.along = a.depth; }
+        else { vb.base = a.b + tile.leaf * a.b_leaf_stride + tile.n0; vb.lines = a.depth; vb.along = a.b_size - tile.n0; }
+      }
+      for (int k0 = 0; k0 < tile.depth; k0 += kDepthTc, ++it) {
+        const int st = it % a.stages, depth = min(kDepthTc, (tile.depth - k0 + 15) & ~15);
+        if (it >= a.stages) ok = __all_sync(0xffffffffu, BarWait(s_empty + st, ((it / a.stages) - 1) & 1, stop)) != 0;      // one decision per warp
+        if (!ok) break;
+        const unsigned int sa = Smem32(stages + static_cast<size_t>(st) * a.stage_bytes), sb = sa + kABytes;
+        if constexpr (MODE == kGram) CopyMnMajor(sa, va, kTileM / 8, k0, depth, a.a_vec, tid); else CopyKMajor(sa, va, kTileM, k0, depth, a.a_vec, tid);
+        if constexpr (MODE == kProductsK) CopyKMajor(sb, vb, a.n, k0, depth, a.b_vec, tid); else CopyMnMajor(sb, vb, a.n / 8, k0, depth, a.b_vec, tid);
+        CopyCommit();
+        if (it >= kLag) { CopyWait<kLag>(); hand_over(it - kLag); }
+      }
+    }
+    CopyWait<0>();
+    if (ok) for (int step = max(0, it - kLag); step < it; ++step) hand_over(step);
+  } else if (warp == 12) {
+    if (lane == 0) {
+      int it = 0, set = 0;
+      bool ok = true;
+      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const Tile tile = tile_of(t);
+        if (tile.depth == 0) continue;
+        const int acc = set & 1;
+        if (set >= 2 && !BarWait(s_free + acc, ((set >> 1) - 1) & 1, stop)) break;
+        const unsigned int d = tmem + acc * (a.tmem_cols / 2);
+        for (int k0 = 0; k0 < tile.depth; k0 += kDepthTc, ++it) {
+          const int st = it % a.stages, depth = min(kDepthTc, (tile.depth - k0 + 15) & ~15);
+          if (!BarWait(s_full + st, (it / a.stages) & 1, stop)) { ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const unsigned int sa = Smem32(stages + static_cast<size_t>(st) * a.stage_bytes), sb = sa + kABytes;
+          // 16 deep at a time: 32 bytes on inside a K-major line, 16 lines on in MN-major order
+          for (int k = 0; k < depth; k += 16) {
+            const unsigned long long da = MODE == kGram ? OperandDesc(sa + k * 128, 8192) : OperandDesc(sa + k * 2, 16);
+            const unsigned long long db = MODE == kProductsK ? OperandDesc(sb + k * 2, 16) : OperandDesc(sb + k * 128, 8192);
+            Mma16(d, da, db, a.idesc, k0 + k > 0);
+          }
+          MmaCommit(s_empty + st);
+        }
+        if (ok) { MmaCommit(s_done + acc); ++set; }
+      }
+      if (!ok && it > 0) {      // the matrix instructions in flight still read shared memory
+        const int last = (it - 1) % a.stages;
+        for (int i = 0; i < (1 << 20) && !BarTry(s_empty + last, ((it - 1) / a.stages) & 1); ++i) {}
+      }
+    }
+    __syncwarp();
+  } else {
+    int set = 0;
+    for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const Tile tile = tile_of(t);
+      const int acc = set & 1;
+      bool ok = true;
+      if (tile.depth > 0) {
+        ok = BarWait(s_done + acc, (set >> 1) & 1, stop);
+        ok = __all_sync(0xffffffffu, ok);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        ++set;
+      }
+      const int m = warp * 32 + lane, m_end = MODE == kGram ? min(kTileM, a.a_size - tile.m0) : static_cast<int>(tile.end - tile.row0), n_end = min(a.n, a.b_size - tile.n0);
+      const long long at = MODE == kGram ? (a.partial != nullptr ? 0 : static_cast<long long>(tile.leaf) * a.a_size * a.b_size) + (tile.m0 + m) * a.out_row_stride + tile.n0 * a.out_col_stride
+                                         : (tile.row0 + m) * a.out_row_stride + tile.n0;
+      O* out = static_cast<O*>(a.out) + at;
+      float* part = MODE == kGram && a.partial != nullptr ? a.partial + static_cast<long long>(tile.which) * a.a_size * a.b_size + at : nullptr;
+      for (int n0 = 0; n0 < n_end; n0 += 16) {
+        unsigned int v[16];
+        if (tile.depth > 0 && ok) {
+          TmemLoad16(tmem + acc * (a.tmem_cols / 2) + (static_cast<unsigned int>(warp * 32) << 16) + n0, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = ok ? 0u : 0x7fc00000u;
+        }
+        if (m >= m_end) continue;
+        if (part != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) if (n0 + j < n_end) part[(n0 + j) * a.out_col_stride] = __uint_as_float(v[j]);
+        } else if (a.out_col_stride == 1 && sizeof(O) == 2 && n0 + 16 <= n_end && (reinterpret_cast<uintptr_t>(out + n0) & 15) == 0) {
+          union { O o[16]; uint4 q[2]; } u;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) u.o[j] = FromFloat<O>(__uint_as_float(v[j]));
+          reinterpret_cast<uint4*>(out + n0)[0] = u.q[0]; reinterpret_cast<uint4*>(out + n0)[1] = u.q[1];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) if (n0 + j < n_end) out[(n0 + j) * a.out_col_stride] = FromFloat<O>(__uint_as_float(v[j]));
+        }
+      }
+      if (tile.depth > 0 && ok) {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) BarArrive(s_free + acc);
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
 }
 
 // Rows that belong to no leaf: zero.
@@ -370,7 +589,29 @@ template <typename F> void DispatchHalf(int dtype, F&& f) {
   }
 }
 
-inline unsigned int Tiles(long long n, long long most) { return static_cast<unsigned int>(std::max(1LL, std::min(most, (n + kTile - 1) / kTile))); }
+// Widest pieces (in values) that an operand's start and strides allow.
+inline int PieceWidth(const void* p, long long stride0, long long stride1) {
+  for (int v = 8; v > 1; v /= 2) if (reinterpret_cast<uintptr_t>(p) % (2 * v) == 0 && stride0 % v == 0 && stride1 % v == 0) return v;
+  return 1;
+}
+// N of the tiles of `size` columns: as few tiles as 256 allows, evenly filled.
+inline int TileN(int size) { const int tiles = (size + kMostN - 1) / kMostN; return ((size + tiles - 1) / tiles + 15) / 16 * 16; }
+
+template <typename T, typename O, int MODE>
+void LaunchTensor(TensorArgs a, long long most_tiles, cudaStream_t s) {
+  const int most_bytes = 212 * 1024;
+  a.stage_bytes = kABytes + (a.n + 63) / 64 * 64 * 128;
+  a.stages = std::min(kMostStages, (most_bytes - 1024) / a.stage_bytes);
+  a.tmem_cols = 32; while (a.tmem_cols < a.n) a.tmem_cols *= 2;
+  a.tmem_cols *= 2;
+  // D fp32; A, B fp16 (0) or bf16 (1), their majors; N, M
+  const unsigned int type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  a.idesc = (1u << 4) | (type << 7) | (type << 10) | (MODE == kGram ? 1u << 15 : 0u) | (MODE != kProductsK ? 1u << 16 : 0u) | (static_cast<unsigned int>(a.n >> 3) << 17) | (static_cast<unsigned int>(kTileM >> 4) << 24);
+  const int bytes = a.stages * a.stage_bytes + 1024;
+  static PerDevice allowed;
+  AllowSharedMemory(LeafTensorKernel<T, O, MODE>, most_bytes, &allowed);
+  LeafTensorKernel<T, O, MODE><<<static_cast<unsigned int>(std::min<long long>(most_tiles, kSms)), kTcThreads, bytes, s>>>(a);
+}
 
 template <int TM, int TN, int WR, int WO>
 void LaunchFloatProducts(const LeafProductsArgs& a, int per_sm, cudaStream_t s) {
@@ -391,6 +632,9 @@ void LaunchFloatGram(const LeafGramArgs& a, int per_sm, float* workspace, cudaSt
   const long long tiles = (split ? LeafGramSlices(a) : a.leaves.leaves) * across;
   LeafGramFloatKernel<TA, TB, GA, GB, SLICES><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, Tile::kBytes, s>>>(a, rows, split ? workspace : nullptr);
 }
+// Gram tiles of 128 x N: the side in 128s is the one that leaves fewer columns of the last tiles empty.
+inline long long GramTiles(const LeafGramArgs& a, bool swap) { const int m = swap ? a.b_cols : a.a_cols, n = swap ? a.a_cols : a.b_cols; return (m + 127LL) / 128 * ((n + TileN(n) - 1) / TileN(n)); }
+inline bool GramSwap(const LeafGramArgs& a) { return GramTiles(a, true) * TileN(a.a_cols) < GramTiles(a, false) * TileN(a.b_cols); }
 // narrow sides: few outputs / both sides of a Gram matrix within one small tile
 constexpr int kNarrow = 16;
 
@@ -399,15 +643,14 @@ constexpr int kNarrow = 16;
 // Rows of a leaf that one block sums up: all of them where the output tiles and the leaves alone fill the machine, else shorter
 // slices, whose sums are added in a second step.
 int LeafGramSliceRows(const LeafGramArgs& a) {
-  const long long tile = a.dtype == kOpFloat32 ? (a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow ? kNarrow * 2 * kNarrow : 64 * 64) : 128 * 256;
-  const long long outputs = std::max(1LL, (static_cast<long long>(a.a_cols) * a.b_cols + tile - 1) / tile);
+  long long outputs = GramTiles(a, GramSwap(a));
+  if (a.dtype == kOpFloat32) { const bool narrow = a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow; outputs = narrow ? 1 : (a.a_cols + 63LL) / 64 * ((a.b_cols + 63) / 64); }
   const long long wanted = std::max(1LL, 4LL * kSms / outputs);        // slices, over all leaves
   const long long rows = std::max(256LL, ((a.leaves.rows + wanted - 1) / wanted + 63) / 64 * 64);
   return static_cast<int>(std::min<long long>(rows, std::max(1LL, a.leaves.rows)));
 }
 long long LeafGramSlices(const LeafGramArgs& a) { const int rows = LeafGramSliceRows(a); return (a.leaves.rows + rows - 1) / rows + a.leaves.leaves; }
 long long LeafGramWorkspace(const LeafGramArgs& a) {
-  if (a.dtype != kOpFloat32) return 0;
   return LeafGramSliceRows(a) < a.leaves.rows ? LeafGramSlices(a) * a.a_cols * a.b_cols : 0;
 }
 
@@ -423,7 +666,17 @@ void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s) {
     using T = std::remove_pointer_t<decltype(p)>;
     LeaflessRowsKernel<T><<<64, 256, 0, s>>>(a);
     FB_LAUNCHED(); FB_KERNEL_CHECK();
-    LeafProductsKernel<T><<<dim3(Tiles(a.outputs, 64), Tiles(a.leaves.rows, 64), std::min(a.leaves.leaves, 1024)), kTile * kTile, 0, s>>>(a);
+    TensorArgs t = TensorArgs();
+    const bool by_feature = a.weight_in_stride == 1 || a.features == 1;
+    if (!by_feature && a.weight_out_stride != 1 && a.outputs != 1) Log::Fatal("leaf products: the maps' features or outputs have to be contiguous");
+    t.leaves = a.leaves; t.tile_rows = kTileM; t.least = 0;
+    t.a = static_cast<const unsigned short*>(a.x); t.a_stride = a.x_stride; t.a_vec = PieceWidth(a.x, a.x_stride, 0);
+    t.b = static_cast<const unsigned short*>(a.weight); t.b_stride = by_feature ? a.weight_out_stride : a.weight_in_stride; t.b_leaf_stride = a.weight_leaf_stride;
+    t.b_vec = PieceWidth(a.weight, t.b_stride, t.b_leaf_stride);
+    t.b_size = a.outputs; t.depth = a.features; t.n = TileN(a.outputs); t.across_a = 1; t.across_b = (a.outputs + t.n - 1) / t.n;
+    t.out = a.y; t.out_row_stride = a.outputs; t.out_col_stride = 1;
+    const long long tiles = ((a.leaves.rows + kTileM - 1) / kTileM + a.leaves.leaves) * t.across_b;
+    if (by_feature) LaunchTensor<T, T, kProductsK>(t, tiles, s); else LaunchTensor<T, T, kProductsMn>(t, tiles, s);
   });
   FB_LAUNCHED(); FB_KERNEL_CHECK();
 }
@@ -441,12 +694,26 @@ void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
     }
     return;
   }
-  const dim3 grid(Tiles(a.b_cols, 64), Tiles(a.a_cols, 64), std::min(a.leaves.leaves, 1024));
   DispatchHalf(a.dtype, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    if (a.out_dtype == a.dtype) LeafGramKernel<T, T><<<grid, kTile * kTile, 0, s>>>(a);
-    else if (a.out_dtype == kOpFloat32) LeafGramKernel<T, float><<<grid, kTile * kTile, 0, s>>>(a);
-    else Log::Fatal("leaf Gram: sums of type code %d as type code %d", a.dtype, a.out_dtype);
+    if (a.out_dtype != a.dtype && a.out_dtype != kOpFloat32) Log::Fatal("leaf Gram: sums of type code %d as type code %d", a.dtype, a.out_dtype);
+    const int rows = LeafGramSliceRows(a);
+    const bool split = rows < a.leaves.rows, swap = GramSwap(a);
+    TensorArgs t = TensorArgs();
+    t.leaves = a.leaves; t.tile_rows = rows; t.least = 1;
+    t.a = static_cast<const unsigned short*>(swap ? a.b : a.a); t.b = static_cast<const unsigned short*>(swap ? a.a : a.b);
+    t.a_stride = swap ? a.b_stride : a.a_stride; t.b_stride = swap ? a.a_stride : a.b_stride;
+    t.a_vec = PieceWidth(t.a, t.a_stride, 0); t.b_vec = PieceWidth(t.b, t.b_stride, 0);
+    t.a_size = swap ? a.b_cols : a.a_cols; t.b_size = swap ? a.a_cols : a.b_cols;
+    t.n = TileN(t.b_size); t.across_a = (t.a_size + kTileM - 1) / kTileM; t.across_b = (t.b_size + t.n - 1) / t.n;
+    t.out = a.out; t.partial = split ? workspace : nullptr; t.out_row_stride = swap ? 1 : a.b_cols; t.out_col_stride = swap ? a.b_cols : 1;
+    const long long tiles = (split ? LeafGramSlices(a) : a.leaves.leaves) * t.across_a * t.across_b, size = static_cast<long long>(a.a_cols) * a.b_cols;
+    const dim3 join(static_cast<unsigned int>(std::min(64LL, (size + 255) / 256)), std::min(a.leaves.leaves, 1024));
+    if (a.out_dtype == a.dtype) LaunchTensor<T, T, kGram>(t, tiles, s); else LaunchTensor<T, float, kGram>(t, tiles, s);
+    if (split) {
+      FB_LAUNCHED(); FB_KERNEL_CHECK();
+      if (a.out_dtype == a.dtype) LeafGramJoinKernel<T><<<join, 256, 0, s>>>(a, rows, workspace); else LeafGramJoinKernel<float><<<join, 256, 0, s>>>(a, rows, workspace);
+    }
   });
   FB_LAUNCHED(); FB_KERNEL_CHECK();
 }

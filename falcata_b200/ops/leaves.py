@@ -34,6 +34,8 @@ def _inner_contiguous(t: torch.Tensor) -> torch.Tensor:
 
 def _products(x: torch.Tensor, weight: torch.Tensor, leaf_begin: torch.Tensor) -> torch.Tensor:
     x, leaf_begin = _inner_contiguous(x), leaf_begin.contiguous()
+    if weight.stride(2) != 1 and weight.stride(1) != 1:
+        weight = weight.contiguous()
     n, f = x.shape
     leaves, outputs = weight.shape[0], weight.shape[1]
     y = torch.empty((n, outputs), dtype=x.dtype, device=x.device)
