@@ -37,6 +37,18 @@ __device__ __forceinline__ void LeafWindow(const LeafWindows& w, int g, long lon
   *begin = min(max(b, 0LL), w.rows); *end = min(max(e, *begin), w.rows);
 }
 
+// Rows that belong to no leaf: zero. All threads of the grid.
+template <typename T>
+__device__ __forceinline__ void ZeroLeaflessRows(const LeafWindows& w, T* y, int outputs) {
+  long long first, last, unused;
+  LeafWindow(w, 0, &first, &unused); LeafWindow(w, w.leaves - 1, &unused, &last);
+  if (first == 0 && last == w.rows) return;
+  const long long head = first * outputs, tail = last * outputs, total = w.rows * outputs, stride = static_cast<long long>(gridDim.x) * blockDim.x;
+  const long long t = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (long long i = t; i < head; i += stride) y[i] = FromFloat<T>(0.f);
+  for (long long i = tail + t; i < total; i += stride) y[i] = FromFloat<T>(0.f);
+}
+
 // The tiles of all leaves one behind the other: `rows` rows each, a leaf's last one shorter. Up to kSpans leaves are looked up by
 // bisection; more are counted in spans of several leaves.
 constexpr int kSpans = 1024;
@@ -88,114 +100,173 @@ __device__ __forceinline__ F2 MakeF2(float x, float y) { F2 r; asm("mov.b64 %0, 
 __device__ __forceinline__ void Split(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
 __device__ __forceinline__ F2 Fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
 __device__ __forceinline__ unsigned int Smem32(const void* p) { return static_cast<unsigned int>(__cvta_generic_to_shared(p)); }
-// 4 bytes global -> shared, zero when !in; asynchronous
-__device__ __forceinline__ void Copy4(float* dst, const float* src, bool in) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(Smem32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
-}
 __device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING> __device__ __forceinline__ void CopyWait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
-// Tile: ROWS = 32 * TM * WR rows x OUTS = TN * WO outputs, kDepth features at a time, double-buffered. A lane has TM rows, 32 apart,
-// and TN neighbouring outputs, two to a 64-bit register; x lies [feature][row] (odd pitch: the transposing copies and the reads of
-// 32 neighbouring rows are both free of bank conflicts), w [feature][output], read by whole warps at once.
-constexpr int kDepth = 32;
+// Asynchronous copies of 16, 8 or 4 bytes, of which the first `valid` are read and the rest becomes zero.
+template <int BYTES>
+__device__ __forceinline__ void CopyFloats(float* dst, const float* src, int valid) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(Smem32(dst)), "l"(src), "r"(valid) : "memory");
+  else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(Smem32(dst)), "l"(src), "r"(valid) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(Smem32(dst)), "l"(src), "r"(valid) : "memory");
+}
+// `all` lines of `width` floats (a multiple of 4) to shared memory, lines `pitch` apart; the source has `lines` lines, `stride` apart,
+// of `along` floats, zero beyond. Neighbouring threads take neighbouring pieces.
+template <int BYTES, int THREADS>
+__device__ __forceinline__ void CopyBlockBy(float* dst, const float* src, int all, int lines, long long stride, int along, int width, int pitch) {
+  constexpr int V = BYTES / 4;
+  const int per = width / V, dl = THREADS / per, dp = THREADS - dl * per;
+  int l = threadIdx.x / per, p = threadIdx.x - l * per;
+  while (l < all) {
+    const int valid = l < lines ? max(0, min(V, along - p * V)) : 0;
+    CopyFloats<BYTES>(dst + l * pitch + p * V, valid > 0 ? src + l * stride + p * V : src, 4 * valid);
+    l += dl; p += dp;
+    if (p >= per) { p -= per; ++l; }
+  }
+}
+template <int THREADS>
+__device__ __forceinline__ void CopyBlock(int vec, float* dst, const float* src, int all, int lines, long long stride, int along, int width, int pitch) {
+  if (vec == 4) CopyBlockBy<16, THREADS>(dst, src, all, lines, stride, along, width, pitch);
+  else if (vec == 2) CopyBlockBy<8, THREADS>(dst, src, all, lines, stride, along, width, pitch);
+  else CopyBlockBy<4, THREADS>(dst, src, all, lines, stride, along, width, pitch);
+}
+
+// Products. Tile: ROWS = 32 * TM * WR rows x OUTS = TN * WO outputs, up to kDepth features a step. x and the maps lie in shared
+// memory as they do in memory, line by line, the pitch an odd number of 16-byte pieces: 32 lanes then read 4 features of 32 rows
+// without bank conflicts, the outputs' features are read by whole warps at once. A lane has TM rows, 32 apart, and TN outputs; a
+// 64-bit register holds the sums over even and over odd features, added at the end. Steps (of all the block's tiles, one behind the
+// other) go through a ring of kRing buffers.
+// `width` and `pitch` of the launch: features a step, in multiples of 4, and their pitch.
+constexpr int kDepth = 32, kRing = 3;
+struct FloatShape { int width, pitch, x_vec, w_vec; bool w_by_output; };
 template <int TM, int TN, int WR, int WO>
 struct FloatTile {
-  static constexpr int ROWS = 32 * TM * WR, OUTS = TN * WO, THREADS = 32 * WR * WO, XP = ROWS + 1, WP = OUTS + 4;
-  static constexpr int kBytes = 2 * kDepth * (XP + WP) * 4;
+  static constexpr int ROWS = 32 * TM * WR, OUTS = TN * WO, THREADS = 32 * WR * WO;
+  static int Bytes(int pitch) { return (kRing * (ROWS + OUTS) * pitch + (WO == 1 ? ROWS * OUTS : 0)) * 4; }
 };
 template <int TM, int TN, int WR, int WO>
-__global__ void __launch_bounds__(32 * WR * WO) LeafProductsFloatKernel(LeafProductsArgs a) {
+__global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProductsFloatKernel(LeafProductsArgs a, FloatShape shape) {
   using Tile = FloatTile<TM, TN, WR, WO>;
   extern __shared__ __align__(16) float s_float[];
   __shared__ TileMap map;
-  float* s_x = s_float + 2 * kDepth * Tile::WP;      // w first: its rows are read 16 bytes at a time
-  float* s_w = s_float;
+  const int pitch = shape.pitch, buffer = (Tile::ROWS + Tile::OUTS) * pitch;
+  ZeroLeaflessRows(a.leaves, static_cast<float*>(a.y), a.outputs);
   map.Build(a.leaves, Tile::ROWS, 0);
   const int across = (a.outputs + Tile::OUTS - 1) / Tile::OUTS;
   const long long tiles = static_cast<long long>(map.Total()) * across;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, wr = warp % WR, wo = warp / WR;
-  for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
-    int leaf; long long row0, end;
-    map.Find(a.leaves, static_cast<int>(t / across), Tile::ROWS, 0, &leaf, &row0, &end);
-    const int out0 = static_cast<int>(t % across) * Tile::OUTS, rows = static_cast<int>(end - row0), outs = min(Tile::OUTS, a.outputs - out0);
-    const float* x = static_cast<const float*>(a.x) + row0 * a.x_stride;
-    const float* w = static_cast<const float*>(a.weight) + leaf * a.weight_leaf_stride + out0 * a.weight_out_stride;
-    auto load = [&](int f0, int buf) {
-      float* to = s_x + buf * kDepth * Tile::XP;
-#pragma unroll 4
-      for (int e = threadIdx.x; e < Tile::ROWS * kDepth; e += Tile::THREADS) {      // lanes: neighbouring features of a row
-        const int r = e / kDepth, f = e % kDepth;
-        const bool in = r < rows && f0 + f < a.features;
-        Copy4(to + f * Tile::XP + r, in ? x + r * a.x_stride + f0 + f : x, in);
-      }
-      to = s_w + buf * kDepth * Tile::WP;
-      for (int e = threadIdx.x; e < Tile::OUTS * kDepth; e += Tile::THREADS) {
-        // lanes along whichever of the two is contiguous
-        const int o = a.weight_out_stride == 1 ? e % Tile::OUTS : e / kDepth, f = a.weight_out_stride == 1 ? e / Tile::OUTS : e % kDepth;
-        const bool in = o < outs && f0 + f < a.features;
-        Copy4(to + f * Tile::WP + o, in ? w + o * a.weight_out_stride + (f0 + f) * a.weight_in_stride : w, in);
-      }
-      CopyCommit();
-    };
-    F2 acc[TM][TN / 2];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN / 2; ++j) acc[i][j] = MakeF2(0.f, 0.f);
-    load(0, 0);
-    int buf = 0;
-    for (int f0 = 0; f0 < a.features; f0 += kDepth, buf ^= 1) {
-      if (f0 + kDepth < a.features) { load(f0 + kDepth, buf ^ 1); CopyWait<1>(); } else CopyWait<0>();
-      __syncthreads();
-      const float* xs = s_x + buf * kDepth * Tile::XP + wr * 32 * TM + lane;
-      const float* ws = s_w + buf * kDepth * Tile::WP + wo * TN;
-      const int depth = min(kDepth, a.features - f0);
-#pragma unroll 4
-      for (int f = 0; f < depth; ++f) {
-        F2 wv[TN / 2];
-#pragma unroll
-        for (int j = 0; j < TN / 4; ++j) { const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(ws + f * Tile::WP + 4 * j); wv[2 * j].v = q.x; wv[2 * j + 1].v = q.y; }
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const float v = xs[f * Tile::XP + 32 * i];
-          const F2 xv = MakeF2(v, v);
-#pragma unroll
-          for (int j = 0; j < TN / 2; ++j) acc[i][j] = Fma2(xv, wv[j], acc[i][j]);
+  struct At { long long t, row0; int leaf, rows, out0, f0; };
+  auto find = [&](At& at) {
+    long long end;
+    map.Find(a.leaves, static_cast<int>(at.t / across), Tile::ROWS, 0, &at.leaf, &at.row0, &end);
+    at.rows = static_cast<int>(end - at.row0); at.out0 = static_cast<int>(at.t % across) * Tile::OUTS; at.f0 = 0;
+  };
+  auto advance = [&](At& at) { at.f0 += shape.width; if (at.f0 >= a.features) { at.t += gridDim.x; if (at.t < tiles) find(at); } };
+  auto copy = [&](const At& at, int slot) {
+    if (at.t < tiles) {
+      float* to = s_float + slot * buffer;
+      CopyBlock<Tile::THREADS>(shape.x_vec, to, static_cast<const float*>(a.x) + at.row0 * a.x_stride + at.f0, Tile::ROWS, at.rows, a.x_stride, a.features - at.f0, shape.width, pitch);
+      to += Tile::ROWS * pitch;
+      const float* w = static_cast<const float*>(a.weight) + at.leaf * a.weight_leaf_stride + at.out0 * a.weight_out_stride + at.f0 * a.weight_in_stride;
+      const int outs = a.outputs - at.out0;
+      if (!shape.w_by_output) {
+        CopyBlock<Tile::THREADS>(shape.w_vec, to, w, Tile::OUTS, outs, a.weight_out_stride, a.features - at.f0, shape.width, pitch);
+      } else {      // the outputs are contiguous (or nothing is): value by value, neighbouring threads along the outputs
+        for (int e = threadIdx.x; e < Tile::OUTS * shape.width; e += Tile::THREADS) {
+          const int o = e % Tile::OUTS, f = e / Tile::OUTS;
+          const bool in = o < outs && at.f0 + f < a.features;
+          CopyFloats<4>(to + o * pitch + f, in ? w + o * a.weight_out_stride + f * a.weight_in_stride : w, in ? 4 : 0);
         }
       }
-      __syncthreads();
     }
+    CopyCommit();
+  };
+  At now, ahead;
+  now.t = blockIdx.x;
+  if (now.t < tiles) find(now);
+  ahead = now;
+  int slot = 0;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int r = wr * 32 * TM + lane + 32 * i;
-      if (r >= rows) continue;
-      float* y = static_cast<float*>(a.y) + (row0 + r) * a.outputs + out0 + wo * TN;
+  for (int i = 0; i < kRing - 1; ++i) { copy(ahead, i); if (ahead.t < tiles) advance(ahead); }
+  F2 acc[TM][TN];
+  while (now.t < tiles) {
+    if (now.f0 == 0) {
 #pragma unroll
-      for (int j = 0; j < TN / 2; ++j) {
-        float v0, v1; Split(acc[i][j], v0, v1);
-        if (wo * TN + 2 * j < outs) y[2 * j] = v0;
-        if (wo * TN + 2 * j + 1 < outs) y[2 * j + 1] = v1;
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = MakeF2(0.f, 0.f);
+    }
+    CopyWait<kRing - 2>();
+    __syncthreads();
+    copy(ahead, (slot + kRing - 1) % kRing);      // the buffer that everyone has left
+    if (ahead.t < tiles) advance(ahead);
+    const float* xs = s_float + slot * buffer + (wr * 32 * TM + lane) * pitch;
+    const float* ws = s_float + slot * buffer + (Tile::ROWS + wo * TN) * pitch;
+    const int depth = min(shape.width, a.features - now.f0);
+    for (int f = 0; f < depth; f += 4) {          // beyond the last feature both sides are zero
+      ulonglong2 xv[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) xv[i] = *reinterpret_cast<const ulonglong2*>(xs + 32 * i * pitch + f);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(ws + j * pitch + f);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) { acc[i][j] = Fma2(F2{xv[i].x}, F2{w.x}, acc[i][j]); acc[i][j] = Fma2(F2{xv[i].y}, F2{w.y}, acc[i][j]); }
       }
     }
+    if (now.f0 + shape.width >= a.features) {
+      const int outs = min(Tile::OUTS, a.outputs - now.out0);
+      float* y = static_cast<float*>(a.y) + now.row0 * a.outputs + now.out0;
+      if constexpr (WO == 1) {
+        // narrow outputs: a tile's rows are one piece of memory when the tile holds all outputs; a warp's rows go through shared memory
+        float* s_y = s_float + kRing * buffer + wr * 32 * TM * Tile::OUTS;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) if (j < outs) { float lo, hi; Split(acc[i][j], lo, hi); s_y[(lane + 32 * i) * outs + j] = lo + hi; }
+        __syncwarp();
+        const int first = wr * 32 * TM, rows = max(0, min(32 * TM, now.rows - first));
+        if (outs == a.outputs) for (int e = lane; e < rows * outs; e += 32) y[static_cast<long long>(first) * outs + e] = s_y[e];
+        else for (int e = lane; e < rows * outs; e += 32) y[static_cast<long long>(first + e / outs) * a.outputs + e % outs] = s_y[e];
+        __syncwarp();
+      } else {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const int r = wr * 32 * TM + lane + 32 * i;
+          if (r >= now.rows) continue;
+          float* to = y + static_cast<long long>(r) * a.outputs + wo * TN;
+          float v[TN];
+#pragma unroll
+          for (int j = 0; j < TN; ++j) { float lo, hi; Split(acc[i][j], lo, hi); v[j] = lo + hi; }
+          if (wo * TN + TN <= outs && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < TN; j += 4) *reinterpret_cast<float4*>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) if (wo * TN + j < outs) to[j] = v[j];
+          }
+        }
+      }
+    }
+    advance(now);
+    slot = (slot + 1) % kRing;
   }
+  CopyWait<0>();
 }
 
-// Tile: AC = TA * GA columns of a x BC = TB * GB columns of b, kRowsDeep rows at a time; SLICES groups of GA * GB threads take every
-// SLICES-th row each and are added up at the end, in order.
-constexpr int kRowsDeep = 32;
-template <int TA, int TB, int GA, int GB, int SLICES>
+// Gram matrices. Tile: AC = TA * GA columns of a x BC = TB * GB columns of b, RD rows a step through a ring of kRing buffers; SLICES
+// groups of GA * GB threads take every SLICES-th row each and are added up at the end, in order.
+template <int TA, int TB, int GA, int GB, int SLICES, int RD>
 struct FloatGramTile {
-  static constexpr int AC = TA * GA, BC = TB * GB, GROUP = GA * GB, THREADS = GROUP * SLICES, AP = AC + 4, BP = BC + 4;
-  static constexpr int kLoad = 2 * kRowsDeep * (AP + BP) * 4, kSum = SLICES > 1 ? SLICES * AC * BC * 4 : 0, kBytes = kLoad > kSum ? kLoad : kSum;
+  static constexpr int AC = TA * GA, BC = TB * GB, GROUP = GA * GB, THREADS = GROUP * SLICES;
+  static constexpr int kLoad = kRing * RD * (AC + BC) * 4, kSum = SLICES > 1 ? SLICES * AC * BC * 4 : 0, kBytes = kLoad > kSum ? kLoad : kSum;
 };
 // `partial` null: one slice of rows per leaf, written to out; else slice t's sums go to partial [slice][a_cols][b_cols].
-template <int TA, int TB, int GA, int GB, int SLICES>
-__global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGramArgs a, int rows_per_slice, float* partial) {
-  using Tile = FloatGramTile<TA, TB, GA, GB, SLICES>;
+template <int TA, int TB, int GA, int GB, int SLICES, int RD>
+__global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGramArgs a, int rows_per_slice, int a_vec, int b_vec, float* partial) {
+  using Tile = FloatGramTile<TA, TB, GA, GB, SLICES, RD>;
   extern __shared__ __align__(16) float s_float[];
   __shared__ TileMap map;
-  float* s_a = s_float; float* s_b = s_float + 2 * kRowsDeep * Tile::AP;
   map.Build(a.leaves, rows_per_slice, 1);
   const int across_a = (a.a_cols + Tile::AC - 1) / Tile::AC, across_b = (a.b_cols + Tile::BC - 1) / Tile::BC;
   const long long tiles = static_cast<long long>(map.Total()) * across_a * across_b;
@@ -205,19 +276,15 @@ __global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGram
     int leaf; long long row0, end;
     map.Find(a.leaves, which, rows_per_slice, 1, &leaf, &row0, &end);
     const int a0 = rest / across_b * Tile::AC, b0 = rest % across_b * Tile::BC, a_in = min(Tile::AC, a.a_cols - a0), b_in = min(Tile::BC, a.b_cols - b0);
-    const float* pa = static_cast<const float*>(a.a) + a0; const float* pb = static_cast<const float*>(a.b) + b0;
-    auto load = [&](long long r0, int buf) {
-#pragma unroll 2
-      for (int e = threadIdx.x; e < kRowsDeep * Tile::AC; e += Tile::THREADS) {
-        const int r = e / Tile::AC, c = e % Tile::AC;
-        const bool in = r0 + r < end && c < a_in;
-        Copy4(s_a + (buf * kRowsDeep + r) * Tile::AP + c, in ? pa + (r0 + r) * a.a_stride + c : static_cast<const float*>(a.a), in);
-      }
-#pragma unroll 2
-      for (int e = threadIdx.x; e < kRowsDeep * Tile::BC; e += Tile::THREADS) {
-        const int r = e / Tile::BC, c = e % Tile::BC;
-        const bool in = r0 + r < end && c < b_in;
-        Copy4(s_b + (buf * kRowsDeep + r) * Tile::BP + c, in ? pb + (r0 + r) * a.b_stride + c : static_cast<const float*>(a.b), in);
+    const int a_width = (a_in + 3) & ~3, b_width = (b_in + 3) & ~3;
+    const float* pa = static_cast<const float*>(a.a) + row0 * a.a_stride + a0; const float* pb = static_cast<const float*>(a.b) + row0 * a.b_stride + b0;
+    const int rows = static_cast<int>(end - row0), steps = (rows + RD - 1) / RD;
+    auto copy = [&](int step) {
+      if (step < steps) {
+        float* to = s_float + step % kRing * RD * (Tile::AC + Tile::BC);
+        const int r0 = step * RD;
+        CopyBlock<Tile::THREADS>(a_vec, to, pa + r0 * a.a_stride, RD, rows - r0, a.a_stride, a_in, a_width, Tile::AC);
+        CopyBlock<Tile::THREADS>(b_vec, to + RD * Tile::AC, pb + r0 * a.b_stride, RD, rows - r0, a.b_stride, b_in, b_width, Tile::BC);
       }
       CopyCommit();
     };
@@ -226,19 +293,21 @@ __global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGram
     for (int i = 0; i < TA; ++i)
 #pragma unroll
       for (int j = 0; j < TB / 2; ++j) acc[i][j] = MakeF2(0.f, 0.f);
-    if (row0 < end) load(row0, 0);
-    int buf = 0;
-    for (long long r0 = row0; r0 < end; r0 += kRowsDeep, buf ^= 1) {
-      if (r0 + kRowsDeep < end) { load(r0 + kRowsDeep, buf ^ 1); CopyWait<1>(); } else CopyWait<0>();
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) copy(i);
+    for (int step = 0; step < steps; ++step) {
+      CopyWait<kRing - 2>();
       __syncthreads();
-#pragma unroll 2
-      for (int r = slice; r < kRowsDeep; r += SLICES) {
-        const float* as = s_a + (buf * kRowsDeep + r) * Tile::AP + ga * TA; const float* bs = s_b + (buf * kRowsDeep + r) * Tile::BP + gb * TB;
+      copy(step + kRing - 1);                     // the buffer that everyone has left
+      // columns beyond the operands hold anything; they reach only sums that are not stored
+      const float* as = s_float + step % kRing * RD * (Tile::AC + Tile::BC) + ga * TA; const float* bs = s_float + (step % kRing * (Tile::AC + Tile::BC) + Tile::AC) * RD + gb * TB;
+#pragma unroll 4
+      for (int r = slice; r < RD; r += SLICES) {
         F2 bv[TB / 2]; float av[TA];
 #pragma unroll
-        for (int j = 0; j < TB / 4; ++j) { const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(bs + 4 * j); bv[2 * j].v = q.x; bv[2 * j + 1].v = q.y; }
+        for (int j = 0; j < TB / 4; ++j) { const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(bs + r * Tile::BC + 4 * j); bv[2 * j].v = q.x; bv[2 * j + 1].v = q.y; }
 #pragma unroll
-        for (int i = 0; i < TA / 4; ++i) { const float4 q = *reinterpret_cast<const float4*>(as + 4 * i); av[4 * i] = q.x; av[4 * i + 1] = q.y; av[4 * i + 2] = q.z; av[4 * i + 3] = q.w; }
+        for (int i = 0; i < TA / 4; ++i) { const float4 q = *reinterpret_cast<const float4*>(as + r * Tile::AC + 4 * i); av[4 * i] = q.x; av[4 * i + 1] = q.y; av[4 * i + 2] = q.z; av[4 * i + 3] = q.w; }
 #pragma unroll
         for (int i = 0; i < TA; ++i) {
           const F2 v = MakeF2(av[i], av[i]);
@@ -246,8 +315,9 @@ __global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGram
           for (int j = 0; j < TB / 2; ++j) acc[i][j] = Fma2(v, bv[j], acc[i][j]);
         }
       }
-      __syncthreads();
     }
+    CopyWait<0>();
+    __syncthreads();
     float* to = partial != nullptr ? partial + static_cast<long long>(which) * a.a_cols * a.b_cols : static_cast<float*>(a.out) + static_cast<long long>(leaf) * a.a_cols * a.b_cols;
     if constexpr (SLICES == 1) {
 #pragma unroll
@@ -434,6 +504,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) 
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  if constexpr (MODE != kGram) ZeroLeaflessRows(a.leaves, static_cast<O*>(a.out), a.b_size);
   map.Build(a.leaves, a.tile_rows, a.least);
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned int tmem = *reinterpret_cast<volatile unsigned int*>(&s_tmem);
@@ -570,17 +641,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) 
   if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
 }
 
-// Rows that belong to no leaf: zero.
-template <typename T>
-__global__ void __launch_bounds__(256) LeaflessRowsKernel(LeafProductsArgs a) {
-  long long first, last, unused;
-  LeafWindow(a.leaves, 0, &first, &unused); LeafWindow(a.leaves, a.leaves.leaves - 1, &unused, &last);
-  const long long head = first * a.outputs, tail = last * a.outputs, total = a.leaves.rows * a.outputs, stride = static_cast<long long>(gridDim.x) * blockDim.x;
-  const long long t = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  for (long long i = t; i < head; i += stride) static_cast<T*>(a.y)[i] = FromFloat<T>(0.f);
-  for (long long i = tail + t; i < total; i += stride) static_cast<T*>(a.y)[i] = FromFloat<T>(0.f);
-}
-
 template <typename F> void DispatchHalf(int dtype, F&& f) {
   switch (dtype) {
     case kOpFloat16: f(static_cast<__half*>(nullptr)); return;
@@ -613,24 +673,38 @@ void LaunchTensor(TensorArgs a, long long most_tiles, cudaStream_t s) {
   LeafTensorKernel<T, O, MODE><<<static_cast<unsigned int>(std::min<long long>(most_tiles, kSms)), kTcThreads, bytes, s>>>(a);
 }
 
-template <int TM, int TN, int WR, int WO>
-void LaunchFloatProducts(const LeafProductsArgs& a, int per_sm, cudaStream_t s) {
-  using Tile = FloatTile<TM, TN, WR, WO>;
-  static PerDevice allowed;
-  AllowSharedMemory(LeafProductsFloatKernel<TM, TN, WR, WO>, Tile::kBytes, &allowed);
-  const long long tiles = ((a.leaves.rows + Tile::ROWS - 1) / Tile::ROWS + a.leaves.leaves) * ((a.outputs + Tile::OUTS - 1) / Tile::OUTS);
-  LeafProductsFloatKernel<TM, TN, WR, WO><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, Tile::kBytes, s>>>(a);
+// Widest pieces (in floats) of a side whose lines start at p, `stride` apart.
+inline int FloatPieces(const void* p, long long stride) {
+  for (int v = 4; v > 1; v /= 2) if (reinterpret_cast<uintptr_t>(p) % (4 * v) == 0 && stride % v == 0) return v;
+  return 1;
 }
-template <int TA, int TB, int GA, int GB, int SLICES>
-void LaunchFloatGram(const LeafGramArgs& a, int per_sm, float* workspace, cudaStream_t s) {
-  using Tile = FloatGramTile<TA, TB, GA, GB, SLICES>;
+template <int TM, int TN, int WR, int WO>
+void LaunchFloatProducts(const LeafProductsArgs& a, cudaStream_t s) {
+  using Tile = FloatTile<TM, TN, WR, WO>;
+  FloatShape shape;
+  shape.width = std::min(kDepth, (a.features + 3) / 4 * 4); shape.pitch = shape.width / 4 % 2 == 0 ? shape.width + 4 : shape.width;
+  shape.x_vec = FloatPieces(a.x, a.x_stride); shape.w_by_output = a.weight_in_stride != 1 && a.features > 1;
+  shape.w_vec = std::min(FloatPieces(a.weight, a.weight_out_stride), FloatPieces(a.weight, a.weight_leaf_stride));
+  const int bytes = Tile::Bytes(shape.pitch);
   static PerDevice allowed;
-  AllowSharedMemory(LeafGramFloatKernel<TA, TB, GA, GB, SLICES>, Tile::kBytes, &allowed);
+  AllowSharedMemory(LeafProductsFloatKernel<TM, TN, WR, WO>, Tile::Bytes(kDepth + 4), &allowed);
+  // as many blocks as are resident, by shared memory (224 KB) and by threads (8 warps of 255 registers, 16 of 128)
+  const int per_sm = std::max(1, std::min(224 * 1024 / (bytes + 6 * 1024), 512 / Tile::THREADS));
+  const long long tiles = ((a.leaves.rows + Tile::ROWS - 1) / Tile::ROWS + a.leaves.leaves) * ((a.outputs + Tile::OUTS - 1) / Tile::OUTS);
+  LeafProductsFloatKernel<TM, TN, WR, WO><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, bytes, s>>>(a, shape);
+}
+template <int TA, int TB, int GA, int GB, int SLICES, int RD>
+void LaunchFloatGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
+  using Tile = FloatGramTile<TA, TB, GA, GB, SLICES, RD>;
+  static PerDevice allowed;
+  AllowSharedMemory(LeafGramFloatKernel<TA, TB, GA, GB, SLICES, RD>, Tile::kBytes, &allowed);
   const long long across = static_cast<long long>((a.a_cols + Tile::AC - 1) / Tile::AC) * ((a.b_cols + Tile::BC - 1) / Tile::BC);
   const int rows = LeafGramSliceRows(a);
   const bool split = rows < a.leaves.rows;
   const long long tiles = (split ? LeafGramSlices(a) : a.leaves.leaves) * across;
-  LeafGramFloatKernel<TA, TB, GA, GB, SLICES><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, Tile::kBytes, s>>>(a, rows, split ? workspace : nullptr);
+  const int per_sm = std::max(1, std::min(224 * 1024 / (Tile::kBytes + 6 * 1024), 1024 / Tile::THREADS));
+  LeafGramFloatKernel<TA, TB, GA, GB, SLICES, RD><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, Tile::kBytes, s>>>(
+      a, rows, FloatPieces(a.a, a.a_stride), FloatPieces(a.b, a.b_stride), split ? workspace : nullptr);
 }
 // Gram tiles of 128 x N: the side in 128s is the one that leaves fewer columns of the last tiles empty.
 inline long long GramTiles(const LeafGramArgs& a, bool swap) { const int m = swap ? a.b_cols : a.a_cols, n = swap ? a.a_cols : a.b_cols; return (m + 127LL) / 128 * ((n + TileN(n) - 1) / TileN(n)); }
@@ -657,15 +731,13 @@ long long LeafGramWorkspace(const LeafGramArgs& a) {
 void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s) {
   if (a.leaves.rows <= 0) return;
   if (a.dtype == kOpFloat32) {
-    LeaflessRowsKernel<float><<<64, 256, 0, s>>>(a);
-    FB_LAUNCHED(); FB_KERNEL_CHECK();
-    if (a.outputs <= kNarrow) LaunchFloatProducts<2, 16, 4, 1>(a, 3, s);
-    else if (a.outputs <= 64) LaunchFloatProducts<4, 8, 1, 8>(a, 3, s);
-    else LaunchFloatProducts<4, 16, 1, 8>(a, 2, s);
+    if (a.outputs <= 4) LaunchFloatProducts<2, 4, 4, 1>(a, s);
+    else if (a.outputs <= 12) LaunchFloatProducts<2, 12, 4, 1>(a, s);
+    else if (a.outputs <= 16) LaunchFloatProducts<2, 16, 4, 1>(a, s);
+    else if (a.outputs <= 32) LaunchFloatProducts<2, 16, 2, 2>(a, s);
+    else LaunchFloatProducts<4, 8, 1, 8>(a, s);
   } else DispatchHalf(a.dtype, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    LeaflessRowsKernel<T><<<64, 256, 0, s>>>(a);
-    FB_LAUNCHED(); FB_KERNEL_CHECK();
     TensorArgs t = TensorArgs();
     const bool by_feature = a.weight_in_stride == 1 || a.features == 1;
     if (!by_feature && a.weight_out_stride != 1 && a.outputs != 1) Log::Fatal("leaf products: the maps' features or outputs have to be contiguous");
@@ -684,8 +756,8 @@ void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s) {
 void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
   if (a.dtype == kOpFloat32) {
     if (a.out_dtype != kOpFloat32) Log::Fatal("leaf Gram: sums of type code %d as type code %d", a.dtype, a.out_dtype);
-    if (a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow) LaunchFloatGram<4, 4, 4, 8, 8>(a, 3, workspace, s);
-    else LaunchFloatGram<8, 8, 8, 8, 4>(a, 2, workspace, s);
+    if (a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow) LaunchFloatGram<4, 4, 4, 8, 8, 64>(a, workspace, s);
+    else LaunchFloatGram<8, 8, 8, 8, 4, 32>(a, workspace, s);
     FB_LAUNCHED(); FB_KERNEL_CHECK();
     if (LeafGramSliceRows(a) < a.leaves.rows) {
       const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
