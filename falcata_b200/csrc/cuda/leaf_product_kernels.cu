@@ -103,33 +103,46 @@ __device__ __forceinline__ unsigned int Smem32(const void* p) { return static_ca
 __device__ __forceinline__ void CopyCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING> __device__ __forceinline__ void CopyWait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
-// Asynchronous copies of 16, 8 or 4 bytes, of which the first `valid` are read and the rest becomes zero.
-template <int BYTES>
-__device__ __forceinline__ void CopyFloats(float* dst, const float* src, int valid) {
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(Smem32(dst)), "l"(src), "r"(valid) : "memory");
-  else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(Smem32(dst)), "l"(src), "r"(valid) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(Smem32(dst)), "l"(src), "r"(valid) : "memory");
+// 4 bytes global -> shared, zero when !in
+__device__ __forceinline__ void CopyFloat(float* dst, const float* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(Smem32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
-// `all` lines of `width` floats (a multiple of 4) to shared memory, lines `pitch` apart; the source has `lines` lines, `stride` apart,
-// of `along` floats, zero beyond. Neighbouring threads take neighbouring pieces.
-template <int BYTES, int THREADS>
-__device__ __forceinline__ void CopyBlockBy(float* dst, const float* src, int all, int lines, long long stride, int along, int width, int pitch) {
-  constexpr int V = BYTES / 4;
-  const int per = width / V, dl = THREADS / per, dp = THREADS - dl * per;
-  int l = threadIdx.x / per, p = threadIdx.x - l * per;
-  while (l < all) {
-    const int valid = l < lines ? max(0, min(V, along - p * V)) : 0;
-    CopyFloats<BYTES>(dst + l * pitch + p * V, valid > 0 ? src + l * stride + p * V : src, 4 * valid);
-    l += dl; p += dp;
-    if (p >= per) { p -= per; ++l; }
-  }
-}
+// Copies blocks of `all` lines of `width` floats (a multiple of 4), `pitch` apart in shared memory, in pieces of `vec` floats;
+// neighbouring threads take neighbouring pieces. What a thread copies where is worked out once and walked by adding.
 template <int THREADS>
-__device__ __forceinline__ void CopyBlock(int vec, float* dst, const float* src, int all, int lines, long long stride, int along, int width, int pitch) {
-  if (vec == 4) CopyBlockBy<16, THREADS>(dst, src, all, lines, stride, along, width, pitch);
-  else if (vec == 2) CopyBlockBy<8, THREADS>(dst, src, all, lines, stride, along, width, pitch);
-  else CopyBlockBy<4, THREADS>(dst, src, all, lines, stride, along, width, pitch);
-}
+struct CopyPlan {
+  int all, vec, per, line0, piece0, lines_on, pieces_on, pitch;
+  __device__ __forceinline__ CopyPlan(int all_, int width, int pitch_, int vec_) {
+    all = all_; vec = vec_; pitch = pitch_; per = width / vec;
+    lines_on = THREADS / per; pieces_on = THREADS - lines_on * per;
+    line0 = static_cast<int>(threadIdx.x) / per; piece0 = static_cast<int>(threadIdx.x) - line0 * per;
+  }
+  template <int BYTES, bool WHOLE>
+  __device__ __forceinline__ void Walk(float* dst, const float* src, int lines, long long stride, int along) const {
+    constexpr int V = BYTES / 4;
+    const float* from = src + line0 * stride + piece0 * V;
+    unsigned int to = Smem32(dst + line0 * pitch + piece0 * V);
+    const long long from_on = lines_on * stride + pieces_on * V, from_wrap = stride - per * V;
+    const unsigned int to_on = 4u * (lines_on * pitch + pieces_on * V), to_wrap = 4u * (pitch - per * V);
+    int piece = piece0;
+#pragma unroll 2
+    for (int line = line0; line < all;) {
+      int valid = line < lines ? (WHOLE ? BYTES : 4 * max(0, min(V, along - piece * V))) : 0;
+      const float* at = WHOLE ? (line < lines ? from : src) : (valid > 0 ? from : src);
+      if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(at), "r"(valid) : "memory");
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(to), "l"(at), "r"(valid), "n"(BYTES) : "memory");
+      line += lines_on; piece += pieces_on; from += from_on; to += to_on;
+      if (piece >= per) { piece -= per; ++line; from += from_wrap; to += to_wrap; }
+    }
+  }
+  // the source has `lines` lines, `stride` apart, of `along` floats; zero beyond
+  __device__ __forceinline__ void Copy(float* dst, const float* src, int lines, long long stride, int along) const {
+    const bool whole = along >= per * vec;
+    if (vec == 4) { if (whole) Walk<16, true>(dst, src, lines, stride, along); else Walk<16, false>(dst, src, lines, stride, along); }
+    else if (vec == 2) Walk<8, false>(dst, src, lines, stride, along);
+    else Walk<4, false>(dst, src, lines, stride, along);
+  }
+};
 
 // Products. Tile: ROWS = 32 * TM * WR rows x OUTS = TN * WO outputs, up to kDepth features a step. x and the maps lie in shared
 // memory as they do in memory, line by line, the pitch an odd number of 16-byte pieces: 32 lanes then read 4 features of 32 rows
@@ -153,29 +166,31 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
   ZeroLeaflessRows(a.leaves, static_cast<float*>(a.y), a.outputs);
   map.Build(a.leaves, Tile::ROWS, 0);
   const int across = (a.outputs + Tile::OUTS - 1) / Tile::OUTS;
-  const long long tiles = static_cast<long long>(map.Total()) * across;
+  const int tiles = map.Total() * across, grid = gridDim.x;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, wr = warp % WR, wo = warp / WR;
-  struct At { long long t, row0; int leaf, rows, out0, f0; };
+  const CopyPlan<Tile::THREADS> x_plan(Tile::ROWS, shape.width, pitch, shape.x_vec), w_plan(Tile::OUTS, shape.width, pitch, shape.w_vec);
+  struct At { long long row0; int t, leaf, rows, out0, f0; };
   auto find = [&](At& at) {
     long long end;
-    map.Find(a.leaves, static_cast<int>(at.t / across), Tile::ROWS, 0, &at.leaf, &at.row0, &end);
-    at.rows = static_cast<int>(end - at.row0); at.out0 = static_cast<int>(at.t % across) * Tile::OUTS; at.f0 = 0;
+    const int which = at.t / across;
+    map.Find(a.leaves, which, Tile::ROWS, 0, &at.leaf, &at.row0, &end);
+    at.rows = static_cast<int>(end - at.row0); at.out0 = (at.t - which * across) * Tile::OUTS; at.f0 = 0;
   };
-  auto advance = [&](At& at) { at.f0 += shape.width; if (at.f0 >= a.features) { at.t += gridDim.x; if (at.t < tiles) find(at); } };
+  auto advance = [&](At& at) { at.f0 += shape.width; if (at.f0 >= a.features) { at.t += grid; if (at.t < tiles) find(at); } };
   auto copy = [&](const At& at, int slot) {
     if (at.t < tiles) {
       float* to = s_float + slot * buffer;
-      CopyBlock<Tile::THREADS>(shape.x_vec, to, static_cast<const float*>(a.x) + at.row0 * a.x_stride + at.f0, Tile::ROWS, at.rows, a.x_stride, a.features - at.f0, shape.width, pitch);
+      x_plan.Copy(to, static_cast<const float*>(a.x) + at.row0 * a.x_stride + at.f0, at.rows, a.x_stride, a.features - at.f0);
       to += Tile::ROWS * pitch;
       const float* w = static_cast<const float*>(a.weight) + at.leaf * a.weight_leaf_stride + at.out0 * a.weight_out_stride + at.f0 * a.weight_in_stride;
       const int outs = a.outputs - at.out0;
       if (!shape.w_by_output) {
-        CopyBlock<Tile::THREADS>(shape.w_vec, to, w, Tile::OUTS, outs, a.weight_out_stride, a.features - at.f0, shape.width, pitch);
+        w_plan.Copy(to, w, outs, a.weight_out_stride, a.features - at.f0);
       } else {      // the outputs are contiguous (or nothing is): value by value, neighbouring threads along the outputs
         for (int e = threadIdx.x; e < Tile::OUTS * shape.width; e += Tile::THREADS) {
           const int o = e % Tile::OUTS, f = e / Tile::OUTS;
           const bool in = o < outs && at.f0 + f < a.features;
-          CopyFloats<4>(to + o * pitch + f, in ? w + o * a.weight_out_stride + f * a.weight_in_stride : w, in ? 4 : 0);
+          CopyFloat(to + o * pitch + f, in ? w + o * a.weight_out_stride + f * a.weight_in_stride : w, in);
         }
       }
     }
@@ -269,22 +284,22 @@ __global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGram
   __shared__ TileMap map;
   map.Build(a.leaves, rows_per_slice, 1);
   const int across_a = (a.a_cols + Tile::AC - 1) / Tile::AC, across_b = (a.b_cols + Tile::BC - 1) / Tile::BC;
-  const long long tiles = static_cast<long long>(map.Total()) * across_a * across_b;
+  const int across = across_a * across_b, tiles = map.Total() * across;
   const int slice = threadIdx.x / Tile::GROUP, member = threadIdx.x % Tile::GROUP, ga = member / GB, gb = member % GB;
-  for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int which = static_cast<int>(t / (across_a * across_b)), rest = static_cast<int>(t % (across_a * across_b));
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int which = t / across, rest = t - which * across;
     int leaf; long long row0, end;
     map.Find(a.leaves, which, rows_per_slice, 1, &leaf, &row0, &end);
     const int a0 = rest / across_b * Tile::AC, b0 = rest % across_b * Tile::BC, a_in = min(Tile::AC, a.a_cols - a0), b_in = min(Tile::BC, a.b_cols - b0);
-    const int a_width = (a_in + 3) & ~3, b_width = (b_in + 3) & ~3;
+    const CopyPlan<Tile::THREADS> a_plan(RD, (a_in + 3) & ~3, Tile::AC, a_vec), b_plan(RD, (b_in + 3) & ~3, Tile::BC, b_vec);
     const float* pa = static_cast<const float*>(a.a) + row0 * a.a_stride + a0; const float* pb = static_cast<const float*>(a.b) + row0 * a.b_stride + b0;
     const int rows = static_cast<int>(end - row0), steps = (rows + RD - 1) / RD;
     auto copy = [&](int step) {
       if (step < steps) {
         float* to = s_float + step % kRing * RD * (Tile::AC + Tile::BC);
         const int r0 = step * RD;
-        CopyBlock<Tile::THREADS>(a_vec, to, pa + r0 * a.a_stride, RD, rows - r0, a.a_stride, a_in, a_width, Tile::AC);
-        CopyBlock<Tile::THREADS>(b_vec, to + RD * Tile::AC, pb + r0 * a.b_stride, RD, rows - r0, a.b_stride, b_in, b_width, Tile::BC);
+        a_plan.Copy(to, pa + r0 * a.a_stride, rows - r0, a.a_stride, a_in);
+        b_plan.Copy(to + RD * Tile::AC, pb + r0 * a.b_stride, rows - r0, a.b_stride, b_in);
       }
       CopyCommit();
     };
@@ -510,13 +525,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) 
   const unsigned int tmem = *reinterpret_cast<volatile unsigned int*>(&s_tmem);
   volatile int* stop = &s_stop;
   const int across = a.across_a * a.across_b;
-  const long long tiles = static_cast<long long>(map.Total()) * across;
+  const int tiles = map.Total() * across;
   // Products: the row tiles of the leaves, `across_b` output tiles each. Gram: slices, across_a x across_b tiles each.
   struct Tile { int leaf, which, m0, n0, depth; long long row0, end; };
-  auto tile_of = [&](long long t) {
+  auto tile_of = [&](int t) {
     Tile r;
-    r.which = static_cast<int>(t / across);
-    const int rest = static_cast<int>(t % across);
+    r.which = t / across;
+    const int rest = t - r.which * across;
     map.Find(a.leaves, r.which, a.tile_rows, a.least, &r.leaf, &r.row0, &r.end);
     r.m0 = MODE == kGram ? rest / a.across_b * kTileM : 0; r.n0 = rest % a.across_b * a.n;
     r.depth = MODE == kGram ? static_cast<int>(r.end - r.row0) : a.depth;
@@ -532,7 +547,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) 
       __syncwarp();
       if (lane == 0) BarArrive(s_full + step % a.stages);
     };
-    for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile tile = tile_of(t);
       OperandView va, vb;
       const int rows = static_cast<int>(tile.end - tile.row0);
@@ -562,7 +577,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) 
     if (lane == 0) {
       int it = 0, set = 0;
       bool ok = true;
-      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const Tile tile = tile_of(t);
         if (tile.depth == 0) continue;
         const int acc = set & 1;
@@ -591,7 +606,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) 
     __syncwarp();
   } else {
     int set = 0;
-    for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
       const Tile tile = tile_of(t);
       const int acc = set & 1;
       bool ok = true;
@@ -649,6 +664,7 @@ template <typename F> void DispatchHalf(int dtype, F&& f) {
   }
 }
 
+inline void CheckTiles(long long tiles) { if (tiles > 0x7ff00000LL) Log::Fatal("leaf products: %lld tiles are not covered", tiles); }
 // Widest pieces (in values) that an operand's start and strides allow.
 inline int PieceWidth(const void* p, long long stride0, long long stride1) {
   for (int v = 8; v > 1; v /= 2) if (reinterpret_cast<uintptr_t>(p) % (2 * v) == 0 && stride0 % v == 0 && stride1 % v == 0) return v;
@@ -667,6 +683,7 @@ void LaunchTensor(TensorArgs a, long long most_tiles, cudaStream_t s) {
   // D fp32; A, B fp16 (0) or bf16 (1), their majors; N, M
   const unsigned int type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   a.idesc = (1u << 4) | (type << 7) | (type << 10) | (MODE == kGram ? 1u << 15 : 0u) | (MODE != kProductsK ? 1u << 16 : 0u) | (static_cast<unsigned int>(a.n >> 3) << 17) | (static_cast<unsigned int>(kTileM >> 4) << 24);
+  CheckTiles(most_tiles);
   const int bytes = a.stages * a.stage_bytes + 1024;
   static PerDevice allowed;
   AllowSharedMemory(LeafTensorKernel<T, O, MODE>, most_bytes, &allowed);
@@ -691,6 +708,7 @@ void LaunchFloatProducts(const LeafProductsArgs& a, cudaStream_t s) {
   // as many blocks as are resident, by shared memory (224 KB) and by threads (8 warps of 255 registers, 16 of 128)
   const int per_sm = std::max(1, std::min(224 * 1024 / (bytes + 6 * 1024), 512 / Tile::THREADS));
   const long long tiles = ((a.leaves.rows + Tile::ROWS - 1) / Tile::ROWS + a.leaves.leaves) * ((a.outputs + Tile::OUTS - 1) / Tile::OUTS);
+  CheckTiles(tiles);
   LeafProductsFloatKernel<TM, TN, WR, WO><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, bytes, s>>>(a, shape);
 }
 template <int TA, int TB, int GA, int GB, int SLICES, int RD>
@@ -703,6 +721,7 @@ void LaunchFloatGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
   const bool split = rows < a.leaves.rows;
   const long long tiles = (split ? LeafGramSlices(a) : a.leaves.leaves) * across;
   const int per_sm = std::max(1, std::min(224 * 1024 / (Tile::kBytes + 6 * 1024), 1024 / Tile::THREADS));
+  CheckTiles(tiles);
   LeafGramFloatKernel<TA, TB, GA, GB, SLICES, RD><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, Tile::kBytes, s>>>(
       a, rows, FloatPieces(a.a, a.a_stride), FloatPieces(a.b, a.b_stride), split ? workspace : nullptr);
 }
@@ -719,7 +738,7 @@ constexpr int kNarrow = 16;
 int LeafGramSliceRows(const LeafGramArgs& a) {
   long long outputs = GramTiles(a, GramSwap(a));
   if (a.dtype == kOpFloat32) { const bool narrow = a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow; outputs = narrow ? 1 : (a.a_cols + 63LL) / 64 * ((a.b_cols + 63) / 64); }
-  const long long wanted = std::max(1LL, 4LL * kSms / outputs);        // slices, over all leaves
+  const long long wanted = std::max(1LL, 16LL * kSms / outputs);       // slices, over all leaves: enough that uneven leaves even out
   const long long rows = std::max(256LL, ((a.leaves.rows + wanted - 1) / wanted + 63) / 64 * 64);
   return static_cast<int>(std::min<long long>(rows, std::max(1LL, a.leaves.rows)));
 }
