@@ -11,6 +11,8 @@
 //   fp32          fused multiply-adds, so that fp32 products stay exact   (LeafProductsFloatKernel, LeafGramFloatKernel)
 #include "kernels.cuh"
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -394,8 +396,10 @@ __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int ro
 // features. Gram: A = 128 columns of one side, B = N of the other, the steps walk the slice's rows.
 // Operands lie in shared memory in the 128-byte-swizzled layout: lines of 64 values, the 16-byte piece c of line l at piece
 // c ^ (l % 8). A line is a row / output with 64 features (K-major), or a feature / row with 64 outputs / columns (MN-major), whatever
-// is contiguous in memory. Copies go in pieces of 16, 8 or 4 bytes as the operand's alignment allows, single values else; what lies
-// outside the operand is zero, which is what makes ragged leaves and odd sizes exact.
+// is contiguous in memory. An operand whose lines start on 16-byte boundaries comes by tensor-map copies (TMA) issued by one thread;
+// others go through the copying warps in pieces of 8 or 4 bytes or single values. Rows of a neighbouring leaf in an x tile
+// reach only outputs that are not stored; in a Gram's last step, where they would be summed, the copying warps bring the rows
+// that belong to the slice and zeros (unless the slice ends at a multiple of 16 rows, the depth of an instruction).
 // Warps: 0-3 store the accumulators, 4-11 copy, 12 issues the matrix instructions. Every wait is bounded; one that gives up
 // makes all roles leave, the tile's outputs NaN and the device's status word 1.
 constexpr int kDepthTc = 64, kTileM = 128, kMostN = 256;
@@ -434,6 +438,16 @@ __device__ __forceinline__ void TmemLoad16(unsigned int addr, unsigned int (&v)[
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void BarExpect(unsigned long long* bar, unsigned int bytes) { asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(Smem32(bar)), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void TmaLoad2D(unsigned int dst, const CUtensorMap* map, int x, int y, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(Smem32(bar)) : "memory");
+}
+__device__ __forceinline__ void TmaLoad3D(unsigned int dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(z), "r"(Smem32(bar)) : "memory");
 }
 
 // One operand's part of a tile in memory: `lines` lines `stride` values apart, `along` values each.
@@ -492,6 +506,7 @@ __device__ __forceinline__ void CopyMnMajor(unsigned int dst, const OperandView&
 struct TensorArgs {
   LeafWindows leaves; int tile_rows, least;                     // rows per tile or slice; tiles of a leaf without rows
   const unsigned short *a, *b; long long a_stride, b_stride, b_leaf_stride;
+  int a_tma, b_tma, b_leaf_on;                                  // operand by tensor map; 1: its third coordinate is the leaf
   int a_vec, b_vec, a_size, b_size, depth;                      // columns of a Gram's sides; outputs (b_size) and features (depth) of products
   int n, across_a, across_b, stages, stage_bytes, tmem_cols;
   unsigned int idesc;
@@ -500,7 +515,7 @@ struct TensorArgs {
 enum { kProductsK, kProductsMn, kGram };
 
 template <typename T, typename O, int MODE>
-__global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) {
+__global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_constant__ TensorArgs a, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map) {
   extern __shared__ unsigned char s_raw[];
   __shared__ TileMap map;
   __shared__ unsigned long long s_full[kMostStages], s_empty[kMostStages], s_done[2], s_free[2];
@@ -540,6 +555,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) 
 
   if (warp >= 4 && warp < 12) {
     const int tid = threadIdx.x - 128;
+    const bool both = a.a_tma != 0 && a.b_tma != 0;
     int it = 0;
     bool ok = true;
     auto hand_over = [&](int step) {
@@ -565,14 +581,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(TensorArgs a) 
         if (it >= a.stages) ok = __all_sync(0xffffffffu, BarWait(s_empty + st, ((it / a.stages) - 1) & 1, stop)) != 0;      // one decision per warp
         if (!ok) break;
         const unsigned int sa = Smem32(stages + static_cast<size_t>(st) * a.stage_bytes), sb = sa + kABytes;
-        if constexpr (MODE == kGram) CopyMnMajor(sa, va, kTileM / 8, k0, depth, a.a_vec, tid); else CopyKMajor(sa, va, kTileM, k0, depth, a.a_vec, tid);
-        if constexpr (MODE == kProductsK) CopyKMajor(sb, vb, a.n, k0, depth, a.b_vec, tid); else CopyMnMajor(sb, vb, a.n / 8, k0, depth, a.b_vec, tid);
-        CopyCommit();
-        if (it >= kLag) { CopyWait<kLag>(); hand_over(it - kLag); }
+        const bool cut = MODE == kGram && ((tile.depth - k0) & 15) != 0 && tile.depth - k0 < kDepthTc;      // a Gram's ragged last step
+        const bool ta = a.a_tma != 0 && !cut, tb = a.b_tma != 0 && !cut;
+        if (tid == 0 && (ta || tb)) {
+          const int b_boxes = (a.n + 63) / 64;
+          BarExpect(s_full + st, (ta ? kABytes : 0) + (tb ? (MODE == kProductsK ? a.n * 128 : b_boxes * 8192) : 0));
+          if (ta) {
+            if constexpr (MODE == kGram) { for (int i = 0; i < 2; ++i) TmaLoad2D(sa + i * 8192, &a_map, tile.m0 + 64 * i, static_cast<int>(tile.row0) + k0, s_full + st); }
+            else TmaLoad2D(sa, &a_map, k0, static_cast<int>(tile.row0), s_full + st);
+          }
+          if (tb) {
+            if constexpr (MODE == kProductsK) TmaLoad3D(sb, &b_map, k0, tile.n0, tile.leaf * a.b_leaf_on, s_full + st);
+            else
+              for (int i = 0; i < b_boxes; ++i) {
+                if constexpr (MODE == kGram) TmaLoad2D(sb + i * 8192, &b_map, tile.n0 + 64 * i, static_cast<int>(tile.row0) + k0, s_full + st);
+                else TmaLoad3D(sb + i * 8192, &b_map, tile.n0 + 64 * i, k0, tile.leaf * a.b_leaf_on, s_full + st);
+              }
+          }
+        }
+        if (!ta) { if constexpr (MODE == kGram) CopyMnMajor(sa, va, kTileM / 8, k0, depth, a.a_vec, tid); else CopyKMajor(sa, va, kTileM, k0, depth, a.a_vec, tid); }
+        if (!tb) { if constexpr (MODE == kProductsK) CopyKMajor(sb, vb, a.n, k0, depth, a.b_vec, tid); else CopyMnMajor(sb, vb, a.n / 8, k0, depth, a.b_vec, tid); }
+        if (both) {                // nothing to wait for, but in a ragged step
+          if (cut) { CopyCommit(); CopyWait<0>(); }
+          hand_over(it);
+        } else {
+          CopyCommit();
+          if (it >= kLag) { CopyWait<kLag>(); hand_over(it - kLag); }
+        }
       }
     }
     CopyWait<0>();
-    if (ok) for (int step = max(0, it - kLag); step < it; ++step) hand_over(step);
+    if (ok && !both) for (int step = max(0, it - kLag); step < it; ++step) hand_over(step);
+    if (!ok && tid == 0 && (a.a_tma != 0 || a.b_tma != 0))      // the copies in flight still write shared memory
+      for (int step = max(0, it - a.stages); step < it; ++step)
+        for (int i = 0; i < (1 << 16) && !BarTry(s_full + step % a.stages, (step / a.stages) & 1); ++i) {}
   } else if (warp == 12) {
     if (lane == 0) {
       int it = 0, set = 0;
@@ -673,8 +715,42 @@ inline int PieceWidth(const void* p, long long stride0, long long stride1) {
 // N of the tiles of `size` columns: as few tiles as 256 allows, evenly filled.
 inline int TileN(int size) { const int tiles = (size + kMostN - 1) / kMostN; return ((size + tiles - 1) / tiles + 15) / 16 * 16; }
 
+PFN_cuTensorMapEncodeTiled_v12000 TensorMapEncoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr; cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+// Map of `along` x `lines` (x `leaves`) values, boxes of 64 x box_lines, 128-byte swizzle. false: such an operand is copied by the warps.
+template <typename T>
+bool EncodeMap(CUtensorMap* map, const void* p, int dims, long long along, long long lines, long long leaves, long long line_stride, long long leaf_stride, int box_lines) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = TensorMapEncoder();
+  if (encode == nullptr || PieceWidth(p, line_stride, leaf_stride) != 8 || line_stride < along || (dims == 3 && leaves > 1 && leaf_stride <= 0)) return false;
+  const cuuint64_t size[3] = {static_cast<cuuint64_t>(along), static_cast<cuuint64_t>(lines), static_cast<cuuint64_t>(leaves)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(line_stride) * 2, static_cast<cuuint64_t>(leaves > 1 ? leaf_stride : line_stride * lines) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_lines), 1}, step[3] = {1, 1, 1};
+  const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode(map, type, dims, const_cast<void*>(p), size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, typename O, int MODE>
 void LaunchTensor(TensorArgs a, long long most_tiles, cudaStream_t s) {
+  CUtensorMap a_map = CUtensorMap(), b_map = CUtensorMap();
+  const long long rows = a.leaves.rows;
+  // a map shared by all leaves (stride 0) is one leaf to the tensor map
+  const bool shared = a.b_leaf_stride == 0 || a.leaves.leaves == 1;
+  a.b_leaf_on = shared ? 0 : 1;
+  const long long leaves = shared ? 1 : a.leaves.leaves;
+  if (MODE == kGram) {
+    a.a_tma = EncodeMap<T>(&a_map, a.a, 2, a.a_size, rows, 1, a.a_stride, 0, kDepthTc); a.b_tma = EncodeMap<T>(&b_map, a.b, 2, a.b_size, rows, 1, a.b_stride, 0, kDepthTc);
+  } else {
+    a.a_tma = EncodeMap<T>(&a_map, a.a, 2, a.depth, rows, 1, a.a_stride, 0, kTileM);
+    if (MODE == kProductsK) a.b_tma = EncodeMap<T>(&b_map, a.b, 3, a.depth, a.b_size, leaves, a.b_stride, a.b_leaf_stride, a.n);
+    else a.b_tma = EncodeMap<T>(&b_map, a.b, 3, a.b_size, a.depth, leaves, a.b_stride, a.b_leaf_stride, kDepthTc);
+  }
   const int most_bytes = 212 * 1024;
   a.stage_bytes = kABytes + (a.n + 63) / 64 * 64 * 128;
   a.stages = std::min(kMostStages, (most_bytes - 1024) / a.stage_bytes);
@@ -687,7 +763,7 @@ void LaunchTensor(TensorArgs a, long long most_tiles, cudaStream_t s) {
   const int bytes = a.stages * a.stage_bytes + 1024;
   static PerDevice allowed;
   AllowSharedMemory(LeafTensorKernel<T, O, MODE>, most_bytes, &allowed);
-  LeafTensorKernel<T, O, MODE><<<static_cast<unsigned int>(std::min<long long>(most_tiles, kSms)), kTcThreads, bytes, s>>>(a);
+  LeafTensorKernel<T, O, MODE><<<static_cast<unsigned int>(std::min<long long>(most_tiles, kSms)), kTcThreads, bytes, s>>>(a, a_map, b_map);
 }
 
 // Widest pieces (in floats) of a side whose lines start at p, `stride` apart.

@@ -335,6 +335,25 @@ def test_leaf_products_strides_and_alignment(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("f,k,cut", [(24, 16, 100), (64, 40, 112), (20, 16, 90)])
+def test_leaf_products_neighbours_do_not_mix(dtype, f, k, cut):
+    """A leaf of NaN and infinite rows next to others: they reach no other leaf's rows or sums, wherever tiles and steps end."""
+    from falcata_b200 import ops
+    g = _gen(8)
+    x = torch.randn((400, f), generator=g, device="cuda").to(dtype); d = torch.randn((400, k), generator=g, device="cuda").to(dtype)
+    w = torch.randn((4, k, f), generator=g, device="cuda").to(dtype)
+    bad = slice(cut, cut + 37)
+    x[bad] = math.nan; x[cut + 3] = math.inf; d[bad] = -math.inf
+    begin = torch.tensor([0, cut, cut + 37, cut + 37, 400], device="cuda")
+    y, p = ops.leaf_products(x, w, begin), ops.leaf_gram(d, x, begin)
+    keep = [(0, 0, cut), (3, cut + 37, 400)]
+    for leaf, lo, hi in keep:
+        _near(y[lo:hi], x[lo:hi].double() @ w[leaf].double().t(), x[lo:hi].double().abs() @ w[leaf].double().abs().t(), f, dtype)
+        _near(p[leaf], d[lo:hi].double().t() @ x[lo:hi].double(), d[lo:hi].double().abs().t() @ x[lo:hi].double().abs(), hi - lo, dtype)
+    assert bool((p[2] == 0).all()) and bool(torch.isnan(p[1]).any()) and bool(torch.isnan(y[bad]).all(1).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_leaf_products_rows_outside_the_leaves(dtype):
     """Rows in no leaf: zero outputs, no share in the sums, whatever they hold; boundaries past the rows are clamped."""
     from falcata_b200 import ops
