@@ -380,7 +380,6 @@ void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s);
 // Long leaves are summed in slices of rows: LeafGramWorkspace floats for their sums (0: none wanted).
 long long LeafGramWorkspace(const LeafGramArgs& a);
 int LeafGramSliceRows(const LeafGramArgs& a);
-long long LeafGramSlices(const LeafGramArgs& a);
 void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s);
 
 }  // namespace fb

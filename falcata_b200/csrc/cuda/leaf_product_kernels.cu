@@ -56,6 +56,7 @@ __device__ __forceinline__ void ZeroLeaflessRows(const LeafWindows& w, T* y, int
 constexpr int kSpans = 1024;
 struct TileMap {
   int before[kSpans + 1];        // tiles before span i
+  int row[kSpans + 1];           // with a leaf per span: its first row
   int per, spans;
   __device__ __forceinline__ static int Count(const LeafWindows& w, int g, int rows, int least) {
     long long b, e; LeafWindow(w, g, &b, &e);
@@ -69,6 +70,9 @@ struct TileMap {
       int c = 0;
       for (int g = i * p; g < min(w.leaves, (i + 1) * p); ++g) c += Count(w, g, rows, least);
       before[i + 1] = c;
+      long long b, e; LeafWindow(w, min(w.leaves - 1, i * p), &b, &e);
+      row[i] = static_cast<int>(b);
+      if (i == n - 1) row[n] = static_cast<int>(e);
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -85,14 +89,27 @@ struct TileMap {
     __syncthreads();
   }
   __device__ __forceinline__ int Total() const { return before[spans]; }
-  // tile -> leaf, its first row and the end of the rows that it covers
-  __device__ __forceinline__ void Find(const LeafWindows& w, int tile, int rows, int least, int* leaf, long long* first, long long* end) const {
-    int lo = 0, hi = spans;
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (before[mid] <= tile) lo = mid; else hi = mid; }
-    int g = lo * per, left = tile - before[lo];
-    if (per > 1) for (int c = Count(w, g, rows, least); left >= c; c = Count(w, g, rows, least)) { left -= c; ++g; }
-    long long b, e; LeafWindow(w, g, &b, &e);
-    *leaf = g; *first = min(e, b + static_cast<long long>(left) * rows); *end = min(e, *first + rows);
+  // tile -> leaf, its first row and the end of the rows that it covers. `span`: where the last search of an earlier tile ended (0 at
+  // first); the next tile is mostly a few leaves on.
+  __device__ __forceinline__ void Find(const LeafWindows& w, int tile, int rows, int least, int* span, int* leaf, int* first, int* end) const {
+    int lo = *span, step = 0;
+    while (step < 8 && before[lo + 1] <= tile) { ++lo; ++step; }
+    if (before[lo + 1] <= tile) { int hi = spans; while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (before[mid] <= tile) lo = mid; else hi = mid; } }
+    *span = lo;
+    int g = lo * per, left = tile - before[lo], b = row[lo], e = row[lo + 1];
+    if (per > 1) {
+      for (int c = Count(w, g, rows, least); left >= c; c = Count(w, g, rows, least)) { left -= c; ++g; }
+      long long b64, e64; LeafWindow(w, g, &b64, &e64);
+      b = static_cast<int>(b64); e = static_cast<int>(e64);
+    }
+    e = max(e, b);
+    *leaf = g; *first = static_cast<int>(min(static_cast<long long>(e), b + static_cast<long long>(left) * rows)); *end = static_cast<int>(min(static_cast<long long>(e), static_cast<long long>(*first) + rows));
+  }
+  // tiles before leaf g
+  __device__ __forceinline__ int Before(const LeafWindows& w, int g, int rows, int least) const {
+    int first = before[g / per];
+    for (int o = g / per * per; o < g; ++o) first += Count(w, o, rows, least);
+    return first;
   }
 };
 
@@ -171,12 +188,12 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
   const int tiles = map.Total() * across, grid = gridDim.x;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, wr = warp % WR, wo = warp / WR;
   const CopyPlan<Tile::THREADS> x_plan(Tile::ROWS, shape.width, pitch, shape.x_vec), w_plan(Tile::OUTS, shape.width, pitch, shape.w_vec);
-  struct At { long long row0; int t, leaf, rows, out0, f0; };
+  struct At { int t, span, row0, leaf, rows, out0, f0; };
   auto find = [&](At& at) {
-    long long end;
+    int end;
     const int which = at.t / across;
-    map.Find(a.leaves, which, Tile::ROWS, 0, &at.leaf, &at.row0, &end);
-    at.rows = static_cast<int>(end - at.row0); at.out0 = (at.t - which * across) * Tile::OUTS; at.f0 = 0;
+    map.Find(a.leaves, which, Tile::ROWS, 0, &at.span, &at.leaf, &at.row0, &end);
+    at.rows = end - at.row0; at.out0 = (at.t - which * across) * Tile::OUTS; at.f0 = 0;
   };
   auto advance = [&](At& at) { at.f0 += shape.width; if (at.f0 >= a.features) { at.t += grid; if (at.t < tiles) find(at); } };
   auto copy = [&](const At& at, int slot) {
@@ -199,7 +216,7 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
     CopyCommit();
   };
   At now, ahead;
-  now.t = blockIdx.x;
+  now.t = blockIdx.x; now.span = 0;
   if (now.t < tiles) find(now);
   ahead = now;
   int slot = 0;
@@ -233,7 +250,7 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
     }
     if (now.f0 + shape.width >= a.features) {
       const int outs = min(Tile::OUTS, a.outputs - now.out0);
-      float* y = static_cast<float*>(a.y) + now.row0 * a.outputs + now.out0;
+      float* y = static_cast<float*>(a.y) + static_cast<long long>(now.row0) * a.outputs + now.out0;
       if constexpr (WO == 1) {
         // narrow outputs: a tile's rows are one piece of memory when the tile holds all outputs; a warp's rows go through shared memory
         float* s_y = s_float + kRing * buffer + wr * 32 * TM * Tile::OUTS;
@@ -271,6 +288,13 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
   CopyWait<0>();
 }
 
+// Where the sums of a slice go: -1 straight to the output (its leaf has no other), else a place of the workspace. Of the leaves with
+// several slices, first slices start more than a slice apart, and so do the others: 2 places per `rows` rows are enough.
+__device__ __forceinline__ int SliceSlot(const LeafWindows& w, int leaf, int row0, int rows) {
+  long long b, e; LeafWindow(w, leaf, &b, &e);
+  return e - b <= rows ? -1 : 2 * (row0 / rows) + (row0 == b ? 0 : 1);
+}
+
 // Gram matrices. Tile: AC = TA * GA columns of a x BC = TB * GB columns of b, RD rows a step through a ring of kRing buffers; SLICES
 // groups of GA * GB threads take every SLICES-th row each and are added up at the end, in order.
 template <int TA, int TB, int GA, int GB, int SLICES, int RD>
@@ -278,9 +302,9 @@ struct FloatGramTile {
   static constexpr int AC = TA * GA, BC = TB * GB, GROUP = GA * GB, THREADS = GROUP * SLICES;
   static constexpr int kLoad = kRing * RD * (AC + BC) * 4, kSum = SLICES > 1 ? SLICES * AC * BC * 4 : 0, kBytes = kLoad > kSum ? kLoad : kSum;
 };
-// `partial` null: one slice of rows per leaf, written to out; else slice t's sums go to partial [slice][a_cols][b_cols].
+// A leaf of one slice is written to out; the sums of the slices of longer leaves go to partial [slot][a_cols][b_cols].
 template <int TA, int TB, int GA, int GB, int SLICES, int RD>
-__global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGramArgs a, int rows_per_slice, int a_vec, int b_vec, float* partial) {
+__global__ void __launch_bounds__(GA * GB * SLICES, TA * TB <= 16 ? 3 : 2) LeafGramFloatKernel(LeafGramArgs a, int rows_per_slice, int a_vec, int b_vec, float* partial) {
   using Tile = FloatGramTile<TA, TB, GA, GB, SLICES, RD>;
   extern __shared__ __align__(16) float s_float[];
   __shared__ TileMap map;
@@ -288,14 +312,15 @@ __global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGram
   const int across_a = (a.a_cols + Tile::AC - 1) / Tile::AC, across_b = (a.b_cols + Tile::BC - 1) / Tile::BC;
   const int across = across_a * across_b, tiles = map.Total() * across;
   const int slice = threadIdx.x / Tile::GROUP, member = threadIdx.x % Tile::GROUP, ga = member / GB, gb = member % GB;
+  int span = 0;
   for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
     const int which = t / across, rest = t - which * across;
-    int leaf; long long row0, end;
-    map.Find(a.leaves, which, rows_per_slice, 1, &leaf, &row0, &end);
+    int leaf, row0, end;
+    map.Find(a.leaves, which, rows_per_slice, 1, &span, &leaf, &row0, &end);
     const int a0 = rest / across_b * Tile::AC, b0 = rest % across_b * Tile::BC, a_in = min(Tile::AC, a.a_cols - a0), b_in = min(Tile::BC, a.b_cols - b0);
     const CopyPlan<Tile::THREADS> a_plan(RD, (a_in + 3) & ~3, Tile::AC, a_vec), b_plan(RD, (b_in + 3) & ~3, Tile::BC, b_vec);
     const float* pa = static_cast<const float*>(a.a) + row0 * a.a_stride + a0; const float* pb = static_cast<const float*>(a.b) + row0 * a.b_stride + b0;
-    const int rows = static_cast<int>(end - row0), steps = (rows + RD - 1) / RD;
+    const int rows = end - row0, steps = (rows + RD - 1) / RD;
     auto copy = [&](int step) {
       if (step < steps) {
         float* to = s_float + step % kRing * RD * (Tile::AC + Tile::BC);
@@ -335,7 +360,8 @@ __global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGram
     }
     CopyWait<0>();
     __syncthreads();
-    float* to = partial != nullptr ? partial + static_cast<long long>(which) * a.a_cols * a.b_cols : static_cast<float*>(a.out) + static_cast<long long>(leaf) * a.a_cols * a.b_cols;
+    const int slot = SliceSlot(a.leaves, leaf, row0, rows_per_slice);
+    float* to = slot >= 0 ? partial + static_cast<long long>(slot) * a.a_cols * a.b_cols : static_cast<float*>(a.out) + static_cast<long long>(leaf) * a.a_cols * a.b_cols;
     if constexpr (SLICES == 1) {
 #pragma unroll
       for (int i = 0; i < TA; ++i)
@@ -372,20 +398,18 @@ __global__ void __launch_bounds__(GA * GB * SLICES) LeafGramFloatKernel(LeafGram
   }
 }
 
-// Adds the partial sums of each leaf's slices, in order.
+// Adds the sums of the slices of each leaf that has several, in order.
 template <typename O>
 __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int rows_per_slice, const float* __restrict__ partial) {
-  __shared__ TileMap map;
-  map.Build(a.leaves, rows_per_slice, 1);
   const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
   for (int g = blockIdx.y; g < a.leaves.leaves; g += gridDim.y) {
-    int first = map.before[g / map.per];
-    for (int o = g / map.per * map.per; o < g; ++o) first += TileMap::Count(a.leaves, o, rows_per_slice, 1);
-    const int slices = TileMap::Count(a.leaves, g, rows_per_slice, 1);
-    for (long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; e < size; e += static_cast<long long>(gridDim.x) * 256) {
+    long long b, e; LeafWindow(a.leaves, g, &b, &e);
+    if (e - b <= rows_per_slice) continue;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < size; i += static_cast<long long>(gridDim.x) * 256) {
       float v = 0.f;
-      for (int s = 0; s < slices; ++s) v += partial[(first + s) * size + e];
-      static_cast<O*>(a.out)[g * size + e] = FromFloat<O>(v);
+#pragma unroll 4
+      for (int r = static_cast<int>(b); r < e; r += rows_per_slice) v += __ldg(partial + (2 * (r / rows_per_slice) + (r == b ? 0 : 1)) * size + i);
+      static_cast<O*>(a.out)[g * size + i] = FromFloat<O>(v);
     }
   }
 }
@@ -404,7 +428,8 @@ __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int ro
 // makes all roles leave, the tile's outputs NaN and the device's status word 1.
 constexpr int kDepthTc = 64, kTileM = 128, kMostN = 256;
 constexpr int kCopyWarps = 8, kCopyThreads = 32 * kCopyWarps, kTcThreads = 128 + kCopyThreads + 32;
-constexpr int kMostStages = 8, kLag = 2;           // a stage is handed over when kLag younger ones are on their way
+constexpr int kMostStages = 8;
+constexpr int kLag = 5, kLagFew = 2;               // a stage is handed over when so many younger ones are on their way (of 8; of fewer stages)
 constexpr int kABytes = kTileM * 128;
 
 __device__ unsigned int g_product_status;
@@ -542,20 +567,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
   const int across = a.across_a * a.across_b;
   const int tiles = map.Total() * across;
   // Products: the row tiles of the leaves, `across_b` output tiles each. Gram: slices, across_a x across_b tiles each.
-  struct Tile { int leaf, which, m0, n0, depth; long long row0, end; };
+  struct Tile { int leaf, which, m0, n0, depth, row0, end; };
+  int span = 0;
   auto tile_of = [&](int t) {
     Tile r;
     r.which = t / across;
     const int rest = t - r.which * across;
-    map.Find(a.leaves, r.which, a.tile_rows, a.least, &r.leaf, &r.row0, &r.end);
+    map.Find(a.leaves, r.which, a.tile_rows, a.least, &span, &r.leaf, &r.row0, &r.end);
     r.m0 = MODE == kGram ? rest / a.across_b * kTileM : 0; r.n0 = rest % a.across_b * a.n;
-    r.depth = MODE == kGram ? static_cast<int>(r.end - r.row0) : a.depth;
+    r.depth = MODE == kGram ? r.end - r.row0 : a.depth;
     return r;
   };
 
   if (warp >= 4 && warp < 12) {
     const int tid = threadIdx.x - 128;
     const bool both = a.a_tma != 0 && a.b_tma != 0;
+    const int lag = a.stages > kLag + 1 ? kLag : kLagFew;
     int it = 0;
     bool ok = true;
     auto hand_over = [&](int step) {
@@ -566,13 +593,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile tile = tile_of(t);
       OperandView va, vb;
-      const int rows = static_cast<int>(tile.end - tile.row0);
+      const int rows = tile.end - tile.row0;
       va.stride = a.a_stride; vb.stride = a.b_stride;
       if constexpr (MODE == kGram) {
-        va.base = a.a + tile.row0 * a.a_stride + tile.m0; va.lines = rows; va.along = a.a_size - tile.m0;
-        vb.base = a.b + tile.row0 * a.b_stride + tile.n0; vb.lines = rows; vb.along = a.b_size - tile.n0;
+        va.base = a.a + static_cast<long long>(tile.row0) * a.a_stride + tile.m0; va.lines = rows; va.along = a.a_size - tile.m0;
+        vb.base = a.b + static_cast<long long>(tile.row0) * a.b_stride + tile.n0; vb.lines = rows; vb.along = a.b_size - tile.n0;
       } else {
-        va.base = a.a + tile.row0 * a.a_stride; va.lines = rows; va.along = a.depth;
+        va.base = a.a + static_cast<long long>(tile.row0) * a.a_stride; va.lines = rows; va.along = a.depth;
         if constexpr (MODE == kProductsK) { vb.base = a.b + tile.leaf * a.b_leaf_stride + tile.n0 * a.b_stride; vb.lines = a.b_size - tile.n0; vb.along = a.depth; }
         else { vb.base = a.b + tile.leaf * a.b_leaf_stride + tile.n0; vb.lines = a.depth; vb.along = a.b_size - tile.n0; }
       }
@@ -587,14 +614,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
           const int b_boxes = (a.n + 63) / 64;
           BarExpect(s_full + st, (ta ? kABytes : 0) + (tb ? (MODE == kProductsK ? a.n * 128 : b_boxes * 8192) : 0));
           if (ta) {
-            if constexpr (MODE == kGram) { for (int i = 0; i < 2; ++i) TmaLoad2D(sa + i * 8192, &a_map, tile.m0 + 64 * i, static_cast<int>(tile.row0) + k0, s_full + st); }
-            else TmaLoad2D(sa, &a_map, k0, static_cast<int>(tile.row0), s_full + st);
+            if constexpr (MODE == kGram) { for (int i = 0; i < 2; ++i) TmaLoad2D(sa + i * 8192, &a_map, tile.m0 + 64 * i, tile.row0 + k0, s_full + st); }
+            else TmaLoad2D(sa, &a_map, k0, tile.row0, s_full + st);
           }
           if (tb) {
             if constexpr (MODE == kProductsK) TmaLoad3D(sb, &b_map, k0, tile.n0, tile.leaf * a.b_leaf_on, s_full + st);
             else
               for (int i = 0; i < b_boxes; ++i) {
-                if constexpr (MODE == kGram) TmaLoad2D(sb + i * 8192, &b_map, tile.n0 + 64 * i, static_cast<int>(tile.row0) + k0, s_full + st);
+                if constexpr (MODE == kGram) TmaLoad2D(sb + i * 8192, &b_map, tile.n0 + 64 * i, tile.row0 + k0, s_full + st);
                 else TmaLoad3D(sb + i * 8192, &b_map, tile.n0 + 64 * i, k0, tile.leaf * a.b_leaf_on, s_full + st);
               }
           }
@@ -606,12 +633,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
           hand_over(it);
         } else {
           CopyCommit();
-          if (it >= kLag) { CopyWait<kLag>(); hand_over(it - kLag); }
+          if (it >= lag) { if (lag == kLag) CopyWait<kLag>(); else CopyWait<kLagFew>(); hand_over(it - lag); }
         }
       }
     }
     CopyWait<0>();
-    if (ok && !both) for (int step = max(0, it - kLag); step < it; ++step) hand_over(step);
+    if (ok && !both) for (int step = max(0, it - lag); step < it; ++step) hand_over(step);
     if (!ok && tid == 0 && (a.a_tma != 0 || a.b_tma != 0))      // the copies in flight still write shared memory
       for (int step = max(0, it - a.stages); step < it; ++step)
         for (int i = 0; i < (1 << 16) && !BarTry(s_full + step % a.stages, (step / a.stages) & 1); ++i) {}
@@ -658,11 +685,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         ++set;
       }
-      const int m = warp * 32 + lane, m_end = MODE == kGram ? min(kTileM, a.a_size - tile.m0) : static_cast<int>(tile.end - tile.row0), n_end = min(a.n, a.b_size - tile.n0);
-      const long long at = MODE == kGram ? (a.partial != nullptr ? 0 : static_cast<long long>(tile.leaf) * a.a_size * a.b_size) + (tile.m0 + m) * a.out_row_stride + tile.n0 * a.out_col_stride
-                                         : (tile.row0 + m) * a.out_row_stride + tile.n0;
-      O* out = static_cast<O*>(a.out) + at;
-      float* part = MODE == kGram && a.partial != nullptr ? a.partial + static_cast<long long>(tile.which) * a.a_size * a.b_size + at : nullptr;
+      const int m = warp * 32 + lane, m_end = MODE == kGram ? min(kTileM, a.a_size - tile.m0) : tile.end - tile.row0, n_end = min(a.n, a.b_size - tile.n0);
+      const long long at = MODE == kGram ? (tile.m0 + m) * a.out_row_stride + tile.n0 * a.out_col_stride : (tile.row0 + m) * a.out_row_stride + tile.n0;
+      const int slot = MODE == kGram ? SliceSlot(a.leaves, tile.leaf, tile.row0, a.tile_rows) : -1;
+      O* out = static_cast<O*>(a.out) + (MODE == kGram ? static_cast<long long>(tile.leaf) * a.a_size * a.b_size : 0) + at;
+      float* part = slot >= 0 ? a.partial + static_cast<long long>(slot) * a.a_size * a.b_size + at : nullptr;
       for (int n0 = 0; n0 < n_end; n0 += 16) {
         unsigned int v[16];
         if (tile.depth > 0 && ok) {
@@ -771,6 +798,8 @@ inline int FloatPieces(const void* p, long long stride) {
   for (int v = 4; v > 1; v /= 2) if (reinterpret_cast<uintptr_t>(p) % (4 * v) == 0 && stride % v == 0) return v;
   return 1;
 }
+// At most so many slices: whole ones, and every leaf's last.
+inline long long LeafGramTiles(const LeafGramArgs& a) { return a.leaves.rows / std::max(1, LeafGramSliceRows(a)) + a.leaves.leaves; }
 template <int TM, int TN, int WR, int WO>
 void LaunchFloatProducts(const LeafProductsArgs& a, cudaStream_t s) {
   using Tile = FloatTile<TM, TN, WR, WO>;
@@ -795,7 +824,7 @@ void LaunchFloatGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
   const long long across = static_cast<long long>((a.a_cols + Tile::AC - 1) / Tile::AC) * ((a.b_cols + Tile::BC - 1) / Tile::BC);
   const int rows = LeafGramSliceRows(a);
   const bool split = rows < a.leaves.rows;
-  const long long tiles = (split ? LeafGramSlices(a) : a.leaves.leaves) * across;
+  const long long tiles = LeafGramTiles(a) * across;
   const int per_sm = std::max(1, std::min(224 * 1024 / (Tile::kBytes + 6 * 1024), 1024 / Tile::THREADS));
   CheckTiles(tiles);
   LeafGramFloatKernel<TA, TB, GA, GB, SLICES, RD><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, Tile::kBytes, s>>>(
@@ -809,20 +838,23 @@ constexpr int kNarrow = 16;
 
 }  // namespace
 
-// Rows of a leaf that one block sums up: all of them where the output tiles and the leaves alone fill the machine, else shorter
-// slices, whose sums are added in a second step.
+// Rows of a leaf that one block sums up. Slices short enough that uneven leaves even out (4 of them per SM, 16 of small ones), long
+// enough that a slice's work outweighs its sums' way through the workspace, and that the workspace stays within 128 MB.
 int LeafGramSliceRows(const LeafGramArgs& a) {
-  long long outputs = GramTiles(a, GramSwap(a));
-  if (a.dtype == kOpFloat32) { const bool narrow = a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow; outputs = narrow ? 1 : (a.a_cols + 63LL) / 64 * ((a.b_cols + 63) / 64); }
-  const long long wanted = std::max(1LL, 16LL * kSms / outputs);       // slices, over all leaves: enough that uneven leaves even out
-  const long long rows = std::max(256LL, ((a.leaves.rows + wanted - 1) / wanted + 63) / 64 * 64);
+  long long outputs = GramTiles(a, GramSwap(a)), least = 1024, per_sm = 4;
+  const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
+  if (a.dtype == kOpFloat32) {
+    const bool narrow = a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow;
+    outputs = narrow ? 1 : (a.a_cols + 63LL) / 64 * ((a.b_cols + 63) / 64); least = 256; if (narrow) per_sm = 16;
+  }
+  const long long wanted = std::max(1LL, std::min(per_sm * kSms / outputs, (16LL << 20) / size));
+  const long long rows = std::max(least, ((a.leaves.rows + wanted - 1) / wanted + 63) / 64 * 64);
   return static_cast<int>(std::min<long long>(rows, std::max(1LL, a.leaves.rows)));
 }
-long long LeafGramSlices(const LeafGramArgs& a) { const int rows = LeafGramSliceRows(a); return (a.leaves.rows + rows - 1) / rows + a.leaves.leaves; }
 long long LeafGramWorkspace(const LeafGramArgs& a) {
-  return LeafGramSliceRows(a) < a.leaves.rows ? LeafGramSlices(a) * a.a_cols * a.b_cols : 0;
+  const long long rows = LeafGramSliceRows(a);
+  return rows < a.leaves.rows ? 2 * ((a.leaves.rows - 1) / rows + 1) * a.a_cols * a.b_cols : 0;
 }
-
 void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s) {
   if (a.leaves.rows <= 0) return;
   if (a.dtype == kOpFloat32) {
@@ -874,7 +906,7 @@ void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
     t.a_size = swap ? a.b_cols : a.a_cols; t.b_size = swap ? a.a_cols : a.b_cols;
     t.n = TileN(t.b_size); t.across_a = (t.a_size + kTileM - 1) / kTileM; t.across_b = (t.b_size + t.n - 1) / t.n;
     t.out = a.out; t.partial = split ? workspace : nullptr; t.out_row_stride = swap ? 1 : a.b_cols; t.out_col_stride = swap ? a.b_cols : 1;
-    const long long tiles = (split ? LeafGramSlices(a) : a.leaves.leaves) * t.across_a * t.across_b, size = static_cast<long long>(a.a_cols) * a.b_cols;
+    const long long tiles = LeafGramTiles(a) * t.across_a * t.across_b, size = static_cast<long long>(a.a_cols) * a.b_cols;
     const dim3 join(static_cast<unsigned int>(std::min(64LL, (size + 255) / 256)), std::min(a.leaves.leaves, 1024));
     if (a.out_dtype == a.dtype) LaunchTensor<T, T, kGram>(t, tiles, s); else LaunchTensor<T, float, kGram>(t, tiles, s);
     if (split) {
