@@ -376,8 +376,10 @@ struct LeafProductsArgs {
 };
 // out [leaves x a_cols x b_cols] dense, of the inputs' type or fp32.
 struct LeafGramArgs { LeafWindows leaves; const void* a; const void* b; void* out; int dtype, out_dtype; int a_cols, b_cols; long long a_stride, b_stride; };
-void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s);
-// Long leaves are summed in slices of rows: LeafGramWorkspace floats for their sums (0: none wanted).
+// The workspaces hold (in floats, possibly none) aligned copies of 16-bit operands and the sums of long leaves' slices; they start on
+// 16-byte boundaries.
+long long LeafProductsWorkspace(const LeafProductsArgs& a);
+void LaunchLeafProducts(const LeafProductsArgs& a, float* workspace, cudaStream_t s);
 long long LeafGramWorkspace(const LeafGramArgs& a);
 int LeafGramSliceRows(const LeafGramArgs& a);
 void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s);

@@ -415,6 +415,36 @@ __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int ro
 }
 
 // ---------------------------------------------------------------------------------------------- 16-bit types ----
+// Lines that do not start on 16-byte boundaries, copied to lines that do: tensor-map copies need it, and the tensor cores read an
+// operand many times. A thread writes 8 values; it reads whole words and shifts where the line starts between two.
+__global__ void __launch_bounds__(256) PackLinesKernel(const unsigned short* __restrict__ from, long long stride, long long lines, int along, unsigned short* __restrict__ to, int to_stride) {
+  const int pieces = to_stride / 8;
+  const long long total = lines * pieces;
+  for (long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; e < total; e += static_cast<long long>(gridDim.x) * 256) {
+    const long long line = e / pieces;
+    const int c = static_cast<int>(e - line * pieces) * 8;
+    const unsigned short* src = from + line * stride + c;
+    unsigned int w[4];
+    const bool odd = (reinterpret_cast<uintptr_t>(src) & 2) != 0;
+    if (c + 8 <= along && (!odd || (c > 0 && c + 9 <= along))) {       // the words read lie within the line
+      const unsigned int* words = reinterpret_cast<const unsigned int*>(odd ? src - 1 : src);
+      unsigned int v[5];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __ldg(words + i);
+      v[4] = odd ? __ldg(words + 4) : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = odd ? __funnelshift_r(v[i], v[i + 1], 16) : v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned int lo = c + 2 * i < along ? __ldg(src + 2 * i) : 0u, hi = c + 2 * i + 1 < along ? __ldg(src + 2 * i + 1) : 0u;
+        w[i] = lo | (hi << 16);
+      }
+    }
+    reinterpret_cast<uint4*>(to + line * to_stride)[c / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // D [128 x N] += A [128 x 64] B [64 x N] steps on the tensor cores, N <= 256, accumulators in tensor memory (two sets, so that
 // one tile is stored while the next is summed). Products: A = 128 rows of x, B = N outputs of the leaf's map, the steps walk the
 // features. Gram: A = 128 columns of one side, B = N of the other, the steps walk the slice's rows.
@@ -431,6 +461,9 @@ constexpr int kCopyWarps = 8, kCopyThreads = 32 * kCopyWarps, kTcThreads = 128 +
 constexpr int kMostStages = 8;
 constexpr int kLag = 5, kLagFew = 2;               // a stage is handed over when so many younger ones are on their way (of 8; of fewer stages)
 constexpr int kABytes = kTileM * 128;
+// Outputs whose rows do not start on 16-byte boundaries go through shared memory, 64 columns of a warp's 32 rows at a time, so that a
+// row is stored by neighbouring lanes (stored by its own lane, value by value, 200000 x 100 -> 100 took 130 us, of it 100 for the stores).
+constexpr int kStorePitch = 33, kStoreBytes = 4 * 32 * kStorePitch * 4;      // words: a row's 64 values and one to spare
 
 __device__ unsigned int g_product_status;
 
@@ -690,6 +723,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
       const int slot = MODE == kGram ? SliceSlot(a.leaves, tile.leaf, tile.row0, a.tile_rows) : -1;
       O* out = static_cast<O*>(a.out) + (MODE == kGram ? static_cast<long long>(tile.leaf) * a.a_size * a.b_size : 0) + at;
       float* part = slot >= 0 ? a.partial + static_cast<long long>(slot) * a.a_size * a.b_size + at : nullptr;
+      if (MODE != kGram && !(reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row_stride % 8 == 0) && tile.depth > 0 && ok) {
+        unsigned int* s_words = reinterpret_cast<unsigned int*>(stages + static_cast<size_t>(a.stages) * a.stage_bytes) + warp * 32 * kStorePitch;
+        O* rows_out = static_cast<O*>(a.out) + (tile.row0 + warp * 32) * a.out_row_stride + tile.n0;
+        const int rows = max(0, min(32, m_end - warp * 32));
+        for (int c0 = 0; c0 < n_end; c0 += 64) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            if (c0 + 16 * h >= a.n) break;
+            unsigned int v[16];
+            TmemLoad16(tmem + acc * (a.tmem_cols / 2) + (static_cast<unsigned int>(warp * 32) << 16) + c0 + 16 * h, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              union { O o[2]; unsigned int w; } u;
+              u.o[0] = FromFloat<O>(__uint_as_float(v[2 * j])); u.o[1] = FromFloat<O>(__uint_as_float(v[2 * j + 1]));
+              s_words[lane * kStorePitch + 8 * h + j] = u.w;
+            }
+          }
+          __syncwarp();
+          const int cols = min(64, n_end - c0);
+          const O* s_row = reinterpret_cast<const O*>(s_words);
+          if (cols > 32) {
+            for (int r = 0; r < rows; ++r) {
+              O* to = rows_out + static_cast<long long>(r) * a.out_row_stride + c0; const O* from = s_row + r * 2 * kStorePitch;
+              to[lane] = from[lane];
+              if (32 + lane < cols) to[32 + lane] = from[32 + lane];
+            }
+          } else {      // several rows at a time
+            const int at_once = 32 / cols, r_on = lane / cols, c = lane - r_on * cols;
+            if (r_on < at_once)
+              for (int r = r_on; r < rows; r += at_once) rows_out[static_cast<long long>(r) * a.out_row_stride + c0 + c] = s_row[r * 2 * kStorePitch + c];
+          }
+          __syncwarp();
+        }
+      } else
       for (int n0 = 0; n0 < n_end; n0 += 16) {
         unsigned int v[16];
         if (tile.depth > 0 && ok) {
@@ -734,6 +802,12 @@ template <typename F> void DispatchHalf(int dtype, F&& f) {
 }
 
 inline void CheckTiles(long long tiles) { if (tiles > 0x7ff00000LL) Log::Fatal("leaf products: %lld tiles are not covered", tiles); }
+inline int PackedStride(int along) { return (along + 7) / 8 * 8; }
+void LaunchPack(const unsigned short* from, long long stride, long long lines, int along, unsigned short* to, cudaStream_t s) {
+  const long long pieces = lines * (PackedStride(along) / 8);
+  PackLinesKernel<<<static_cast<unsigned int>(std::max(1LL, std::min<long long>(kSms * 16, (pieces + 255) / 256))), 256, 0, s>>>(from, stride, lines, along, to, PackedStride(along));
+  FB_LAUNCHED(); FB_KERNEL_CHECK();
+}
 // Widest pieces (in values) that an operand's start and strides allow.
 inline int PieceWidth(const void* p, long long stride0, long long stride1) {
   for (int v = 8; v > 1; v /= 2) if (reinterpret_cast<uintptr_t>(p) % (2 * v) == 0 && stride0 % v == 0 && stride1 % v == 0) return v;
@@ -778,16 +852,16 @@ void LaunchTensor(TensorArgs a, long long most_tiles, cudaStream_t s) {
     if (MODE == kProductsK) a.b_tma = EncodeMap<T>(&b_map, a.b, 3, a.depth, a.b_size, leaves, a.b_stride, a.b_leaf_stride, a.n);
     else a.b_tma = EncodeMap<T>(&b_map, a.b, 3, a.b_size, a.depth, leaves, a.b_stride, a.b_leaf_stride, kDepthTc);
   }
-  const int most_bytes = 212 * 1024;
+  const int store_bytes = MODE == kGram ? 0 : kStoreBytes, most_bytes = 216 * 1024;
   a.stage_bytes = kABytes + (a.n + 63) / 64 * 64 * 128;
-  a.stages = std::min(kMostStages, (most_bytes - 1024) / a.stage_bytes);
+  a.stages = std::min(kMostStages, (most_bytes - 1024 - store_bytes) / a.stage_bytes);
   a.tmem_cols = 32; while (a.tmem_cols < a.n) a.tmem_cols *= 2;
   a.tmem_cols *= 2;
   // D fp32; A, B fp16 (0) or bf16 (1), their majors; N, M
   const unsigned int type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   a.idesc = (1u << 4) | (type << 7) | (type << 10) | (MODE == kGram ? 1u << 15 : 0u) | (MODE != kProductsK ? 1u << 16 : 0u) | (static_cast<unsigned int>(a.n >> 3) << 17) | (static_cast<unsigned int>(kTileM >> 4) << 24);
   CheckTiles(most_tiles);
-  const int bytes = a.stages * a.stage_bytes + 1024;
+  const int bytes = a.stages * a.stage_bytes + 1024 + store_bytes;
   static PerDevice allowed;
   AllowSharedMemory(LeafTensorKernel<T, O, MODE>, most_bytes, &allowed);
   LeafTensorKernel<T, O, MODE><<<static_cast<unsigned int>(std::min<long long>(most_tiles, kSms)), kTcThreads, bytes, s>>>(a, a_map, b_map);
@@ -830,9 +904,32 @@ void LaunchFloatGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
   LeafGramFloatKernel<TA, TB, GA, GB, SLICES, RD><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, Tile::kBytes, s>>>(
       a, rows, FloatPieces(a.a, a.a_stride), FloatPieces(a.b, a.b_stride), split ? workspace : nullptr);
 }
-// Gram tiles of 128 x N: the side in 128s is the one that leaves fewer columns of the last tiles empty.
-inline long long GramTiles(const LeafGramArgs& a, bool swap) { const int m = swap ? a.b_cols : a.a_cols, n = swap ? a.a_cols : a.b_cols; return (m + 127LL) / 128 * ((n + TileN(n) - 1) / TileN(n)); }
-inline bool GramSwap(const LeafGramArgs& a) { return GramTiles(a, true) * TileN(a.a_cols) < GramTiles(a, false) * TileN(a.b_cols); }
+// Gram tiles: 128 columns of b x N columns of a, so that the lanes of a store have neighbouring columns of an output row.
+inline long long GramTiles(const LeafGramArgs& a) { const int n = TileN(a.a_cols); return (a.b_cols + 127LL) / 128 * ((a.a_cols + n - 1) / n); }
+// Operands that are packed first (see PackLinesKernel). An operand that is read once only, because the other side fits one tile, is
+// not worth two more passes over it.
+inline bool Unaligned(const void* p, long long stride, long long along) { return PieceWidth(p, stride, 0) != 8 && stride >= along; }
+struct GramPacking {
+  bool a, b;
+  explicit GramPacking(const LeafGramArgs& g) {
+    const bool half = g.dtype != kOpFloat32;
+    a = half && g.b_cols > kTileM && Unaligned(g.a, g.a_stride, g.a_cols);
+    b = half && g.a_cols > kTileM && Unaligned(g.b, g.b_stride, g.b_cols);
+  }
+};
+// Products: x is read once per tile of outputs, a map once per tile of its leaf's rows.
+struct ProductsPacking {
+  bool x, w; long long w_lines; int w_along;
+  explicit ProductsPacking(const LeafProductsArgs& p) {
+    const bool half = p.dtype != kOpFloat32, by_feature = p.weight_in_stride == 1 || p.features == 1;
+    w_lines = by_feature ? p.outputs : p.features; w_along = by_feature ? p.features : p.outputs;
+    const long long line_stride = by_feature ? p.weight_out_stride : p.weight_in_stride;
+    x = half && p.outputs > kTileM && Unaligned(p.x, p.x_stride, p.features);
+    // whole dense maps only: one run of lines for all leaves
+    w = half && p.leaves.rows > 2LL * kTileM * p.leaves.leaves && p.leaves.leaves > 1 && line_stride == w_along && p.weight_leaf_stride == w_lines * line_stride &&
+        PieceWidth(p.weight, line_stride, p.weight_leaf_stride) != 8;
+  }
+};
 // narrow sides: few outputs / both sides of a Gram matrix within one small tile
 constexpr int kNarrow = 16;
 
@@ -841,7 +938,7 @@ constexpr int kNarrow = 16;
 // Rows of a leaf that one block sums up. Slices short enough that uneven leaves even out (4 of them per SM, 16 of small ones), long
 // enough that a slice's work outweighs its sums' way through the workspace, and that the workspace stays within 128 MB.
 int LeafGramSliceRows(const LeafGramArgs& a) {
-  long long outputs = GramTiles(a, GramSwap(a)), least = 1024, per_sm = 4;
+  long long outputs = GramTiles(a), least = 1024, per_sm = 4;
   const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
   if (a.dtype == kOpFloat32) {
     const bool narrow = a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow;
@@ -851,11 +948,20 @@ int LeafGramSliceRows(const LeafGramArgs& a) {
   const long long rows = std::max(least, ((a.leaves.rows + wanted - 1) / wanted + 63) / 64 * 64);
   return static_cast<int>(std::min<long long>(rows, std::max(1LL, a.leaves.rows)));
 }
-long long LeafGramWorkspace(const LeafGramArgs& a) {
+// floats of the slices' sums, in whole 16-byte pieces
+static long long GramSumFloats(const LeafGramArgs& a) {
   const long long rows = LeafGramSliceRows(a);
-  return rows < a.leaves.rows ? 2 * ((a.leaves.rows - 1) / rows + 1) * a.a_cols * a.b_cols : 0;
+  return rows < a.leaves.rows ? (2 * ((a.leaves.rows - 1) / rows + 1) * a.a_cols * a.b_cols + 3) / 4 * 4 : 0;
 }
-void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s) {
+long long LeafGramWorkspace(const LeafGramArgs& a) {
+  const GramPacking packing(a);
+  return GramSumFloats(a) + a.leaves.rows * ((packing.a ? PackedStride(a.a_cols) : 0) + (packing.b ? PackedStride(a.b_cols) : 0)) / 2;
+}
+long long LeafProductsWorkspace(const LeafProductsArgs& a) {
+  const ProductsPacking packing(a);
+  return (packing.x ? a.leaves.rows * PackedStride(a.features) / 2 : 0) + (packing.w ? a.leaves.leaves * packing.w_lines * PackedStride(packing.w_along) / 2 : 0);
+}
+void LaunchLeafProducts(const LeafProductsArgs& a, float* workspace, cudaStream_t s) {
   if (a.leaves.rows <= 0) return;
   if (a.dtype == kOpFloat32) {
     if (a.outputs <= 4) LaunchFloatProducts<2, 4, 4, 1>(a, s);
@@ -869,9 +975,16 @@ void LaunchLeafProducts(const LeafProductsArgs& a, cudaStream_t s) {
     const bool by_feature = a.weight_in_stride == 1 || a.features == 1;
     if (!by_feature && a.weight_out_stride != 1 && a.outputs != 1) Log::Fatal("leaf products: the maps' features or outputs have to be contiguous");
     t.leaves = a.leaves; t.tile_rows = kTileM; t.least = 0;
-    t.a = static_cast<const unsigned short*>(a.x); t.a_stride = a.x_stride; t.a_vec = PieceWidth(a.x, a.x_stride, 0);
+    t.a = static_cast<const unsigned short*>(a.x); t.a_stride = a.x_stride;
     t.b = static_cast<const unsigned short*>(a.weight); t.b_stride = by_feature ? a.weight_out_stride : a.weight_in_stride; t.b_leaf_stride = a.weight_leaf_stride;
-    t.b_vec = PieceWidth(a.weight, t.b_stride, t.b_leaf_stride);
+    unsigned short* packed = reinterpret_cast<unsigned short*>(workspace);
+    const ProductsPacking packing(a);
+    if (packing.x) { t.a_stride = PackedStride(a.features); LaunchPack(t.a, a.x_stride, a.leaves.rows, a.features, packed, s); t.a = packed; packed += a.leaves.rows * t.a_stride; }
+    if (packing.w) {
+      t.b_stride = PackedStride(packing.w_along); t.b_leaf_stride = packing.w_lines * t.b_stride;
+      LaunchPack(t.b, packing.w_along, a.leaves.leaves * packing.w_lines, packing.w_along, packed, s); t.b = packed;
+    }
+    t.a_vec = PieceWidth(t.a, t.a_stride, 0); t.b_vec = PieceWidth(t.b, t.b_stride, t.b_leaf_stride);
     t.b_size = a.outputs; t.depth = a.features; t.n = TileN(a.outputs); t.across_a = 1; t.across_b = (a.outputs + t.n - 1) / t.n;
     t.out = a.y; t.out_row_stride = a.outputs; t.out_col_stride = 1;
     const long long tiles = ((a.leaves.rows + kTileM - 1) / kTileM + a.leaves.leaves) * t.across_b;
@@ -897,15 +1010,18 @@ void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
     using T = std::remove_pointer_t<decltype(p)>;
     if (a.out_dtype != a.dtype && a.out_dtype != kOpFloat32) Log::Fatal("leaf Gram: sums of type code %d as type code %d", a.dtype, a.out_dtype);
     const int rows = LeafGramSliceRows(a);
-    const bool split = rows < a.leaves.rows, swap = GramSwap(a);
+    const bool split = rows < a.leaves.rows;
     TensorArgs t = TensorArgs();
     t.leaves = a.leaves; t.tile_rows = rows; t.least = 1;
-    t.a = static_cast<const unsigned short*>(swap ? a.b : a.a); t.b = static_cast<const unsigned short*>(swap ? a.a : a.b);
-    t.a_stride = swap ? a.b_stride : a.a_stride; t.b_stride = swap ? a.a_stride : a.b_stride;
+    t.a = static_cast<const unsigned short*>(a.b); t.a_stride = a.b_stride; t.a_size = a.b_cols;
+    t.b = static_cast<const unsigned short*>(a.a); t.b_stride = a.a_stride; t.b_size = a.a_cols;
+    unsigned short* packed = reinterpret_cast<unsigned short*>(workspace + (split ? GramSumFloats(a) : 0));
+    const GramPacking packing(a);
+    if (packing.b) { t.a_stride = PackedStride(a.b_cols); LaunchPack(t.a, a.b_stride, a.leaves.rows, a.b_cols, packed, s); t.a = packed; packed += a.leaves.rows * t.a_stride; }
+    if (packing.a) { t.b_stride = PackedStride(a.a_cols); LaunchPack(t.b, a.a_stride, a.leaves.rows, a.a_cols, packed, s); t.b = packed; }
     t.a_vec = PieceWidth(t.a, t.a_stride, 0); t.b_vec = PieceWidth(t.b, t.b_stride, 0);
-    t.a_size = swap ? a.b_cols : a.a_cols; t.b_size = swap ? a.a_cols : a.b_cols;
     t.n = TileN(t.b_size); t.across_a = (t.a_size + kTileM - 1) / kTileM; t.across_b = (t.b_size + t.n - 1) / t.n;
-    t.out = a.out; t.partial = split ? workspace : nullptr; t.out_row_stride = swap ? 1 : a.b_cols; t.out_col_stride = swap ? a.b_cols : 1;
+    t.out = a.out; t.partial = split ? workspace : nullptr; t.out_row_stride = 1; t.out_col_stride = a.b_cols;
     const long long tiles = LeafGramTiles(a) * t.across_a * t.across_b, size = static_cast<long long>(a.a_cols) * a.b_cols;
     const dim3 join(static_cast<unsigned int>(std::min(64LL, (size + 255) / 256)), std::min(a.leaves.leaves, 1024));
     if (a.out_dtype == a.dtype) LaunchTensor<T, T, kGram>(t, tiles, s); else LaunchTensor<T, float, kGram>(t, tiles, s);

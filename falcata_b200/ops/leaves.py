@@ -40,9 +40,18 @@ def _products(x: torch.Tensor, weight: torch.Tensor, leaf_begin: torch.Tensor) -
     leaves, outputs = weight.shape[0], weight.shape[1]
     y = torch.empty((n, outputs), dtype=x.dtype, device=x.device)
     if n:
-        check(_fwd()(ptr(x), x.stride(0), ptr(weight), weight.stride(0), weight.stride(1), weight.stride(2), ptr(leaf_begin), 8 * leaf_begin.element_size(), leaves, n, f, outputs,
-                     type_code("x", x), ptr(y), *device_and_stream(x.device)))
+        _run(_fwd(), (ptr(x), x.stride(0), ptr(weight), weight.stride(0), weight.stride(1), weight.stride(2), ptr(leaf_begin), 8 * leaf_begin.element_size(), leaves, n, f, outputs,
+                      type_code("x", x), ptr(y)), x.device)
     return y
+
+
+def _run(entry, args: tuple, device: torch.device) -> None:
+    """The native call with the workspace that it asks for; the workspace belongs to the current stream, as every tensor made here."""
+    floats = ctypes.c_longlong(0)
+    where = device_and_stream(device)
+    check(entry(*args, None, ctypes.byref(floats), *where))
+    workspace = torch.empty(floats.value, dtype=torch.float32, device=device) if floats.value else None
+    check(entry(*args, ptr(workspace), None, *where))
 
 
 class _LeafProducts(torch.autograd.Function):
@@ -100,13 +109,8 @@ def leaf_gram(a: torch.Tensor, b: torch.Tensor, leaf_begin: torch.Tensor, dtype:
     a, b, leaf_begin = _inner_contiguous(a), _inner_contiguous(b), leaf_begin.contiguous()
     leaves = leaf_begin.numel() - 1
     out = torch.empty((leaves, a.shape[1], b.shape[1]), dtype=dtype, device=a.device)
-    args = (ptr(a), a.stride(0), ptr(b), b.stride(0), ptr(leaf_begin), 8 * leaf_begin.element_size(), leaves, a.shape[0], a.shape[1], b.shape[1], type_code("a", a),
-            type_code("dtype", out), ptr(out))
-    floats = ctypes.c_longlong(0)
-    where = device_and_stream(a.device)
-    check(_gram()(*args, None, ctypes.byref(floats), *where))
-    workspace = torch.empty(floats.value, dtype=torch.float32, device=a.device) if floats.value else None
-    check(_gram()(*args, ptr(workspace), None, *where))
+    _run(_gram(), (ptr(a), a.stride(0), ptr(b), b.stride(0), ptr(leaf_begin), 8 * leaf_begin.element_size(), leaves, a.shape[0], a.shape[1], b.shape[1], type_code("a", a),
+                   type_code("dtype", out), ptr(out)), a.device)
     return out
 
 
@@ -114,7 +118,7 @@ _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 
 
 def _fwd():
-    return bind("FB_OpLeafProducts", (_P, _L, _P, _L, _L, _L, _P, _I, _I, _L, _I, _I, _I, _P, _I, _P))
+    return bind("FB_OpLeafProducts", (_P, _L, _P, _L, _L, _L, _P, _I, _I, _L, _I, _I, _I, _P, _P, ctypes.POINTER(_L), _I, _P))
 
 
 def _gram():

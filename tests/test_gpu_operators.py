@@ -286,7 +286,7 @@ def _near(got, want, size, terms, dtype):
 
 
 SHAPES = [(1, 1, 1, 1), (3, 5, 2, 4), (100, 28, 10, 7), (257, 33, 17, 3), (1000, 136, 1, 31), (513, 100, 100, 5), (64, 130, 257, 2), (2000, 8, 64, 255), (300, 257, 129, 4), (40, 2000, 30, 40),
-          (1200, 64, 256, 3), (700, 200, 520, 2)]
+          (1200, 64, 256, 3), (700, 200, 520, 2), (1500, 135, 259, 3), (5000, 40, 70, 4)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

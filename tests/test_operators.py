@@ -94,7 +94,7 @@ def test_native_entry_points_return_errors():
     for bad, word in ((dict(rows=-1), b"rows"), (dict(rows=1 << 31), b"rows"), (dict(classes=0), b"classes"), (dict(classes=1 << 31), b"classes"),
                       (dict(label_bits=16), b"labels"), (dict(top_k=33, classes=100), b"alternatives"), (dict(top_k=7), b"alternatives"), (dict(top_k=-1), b"alternatives")):
         assert scores(**bad) == -1 and word in lib.FB_OpsLastError()
-    assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(32), I(0), L(4), I(3), I(5), I(0), P(), I(0), P()) == -1 and b"leaves" in lib.FB_OpsLastError()
-    assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(16), I(2), L(4), I(3), I(5), I(0), P(), I(0), P()) == -1 and b"boundaries" in lib.FB_OpsLastError()
-    assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(32), I(2), L(4), I(0), I(5), I(0), P(), I(0), P()) == -1 and b"feature" in lib.FB_OpsLastError()
+    assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(32), I(0), L(4), I(3), I(5), I(0), P(), P(), P(), I(0), P()) == -1 and b"leaves" in lib.FB_OpsLastError()
+    assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(16), I(2), L(4), I(3), I(5), I(0), P(), P(), P(), I(0), P()) == -1 and b"boundaries" in lib.FB_OpsLastError()
+    assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(32), I(2), L(4), I(0), I(5), I(0), P(), P(), P(), I(0), P()) == -1 and b"feature" in lib.FB_OpsLastError()
     assert lib.FB_OpLeafGram(P(), L(3), P(), L(3), P(), I(32), I(2), L(4), I(0), I(3), I(0), I(0), P(), P(), P(), I(0), P()) == -1 and b"column" in lib.FB_OpsLastError()
