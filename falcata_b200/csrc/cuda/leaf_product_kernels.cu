@@ -499,6 +499,7 @@ __device__ __forceinline__ void TmemLoad16(unsigned int addr, unsigned int (&v)[
 }
 
 __device__ __forceinline__ void BarExpect(unsigned long long* bar, unsigned int bytes) { asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(Smem32(bar)), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void BarArriveExpect(unsigned long long* bar, unsigned int bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(Smem32(bar)), "r"(bytes) : "memory"); }
 __device__ __forceinline__ void TmaLoad2D(unsigned int dst, const CUtensorMap* map, int x, int y, unsigned long long* bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                ::"r"(dst), "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(Smem32(bar)) : "memory");
@@ -576,7 +577,7 @@ template <typename T, typename O, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_constant__ TensorArgs a, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map) {
   extern __shared__ unsigned char s_raw[];
   __shared__ TileMap map;
-  __shared__ unsigned long long s_full[kMostStages], s_empty[kMostStages], s_done[2], s_free[2];
+  __shared__ unsigned long long s_full[kMostStages], s_empty[kMostStages], s_done[2], s_free[2], s_cut, s_go;
   __shared__ unsigned int s_tmem; __shared__ int s_stop;
   unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -585,8 +586,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < a.stages; ++i) { BarInit(s_full + i, kCopyWarps); BarInit(s_empty + i, 1); }
+    for (int i = 0; i < a.stages; ++i) { BarInit(s_full + i, a.a_tma != 0 && a.b_tma != 0 ? 1 : kCopyWarps); BarInit(s_empty + i, 1); }
     for (int i = 0; i < 2; ++i) { BarInit(s_done + i, 1); BarInit(s_free + i, 4); }
+    BarInit(&s_cut, kCopyWarps); BarInit(&s_go, 1);
     s_stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -616,7 +618,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
     const int tid = threadIdx.x - 128;
     const bool both = a.a_tma != 0 && a.b_tma != 0;
     const int lag = a.stages > kLag + 1 ? kLag : kLagFew;
-    int it = 0;
+    int it = 0, cuts = 0;
     bool ok = true;
     auto hand_over = [&](int step) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // this thread's copies -> visible to the tensor core's reads
@@ -636,36 +638,67 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
         if constexpr (MODE == kProductsK) { vb.base = a.b + tile.leaf * a.b_leaf_stride + tile.n0 * a.b_stride; vb.lines = a.b_size - tile.n0; vb.along = a.depth; }
         else { vb.base = a.b + tile.leaf * a.b_leaf_stride + tile.n0; vb.lines = a.depth; vb.along = a.b_size - tile.n0; }
       }
-      for (int k0 = 0; k0 < tile.depth; k0 += kDepthTc, ++it) {
-        const int st = it % a.stages, depth = min(kDepthTc, (tile.depth - k0 + 15) & ~15);
-        if (it >= a.stages) ok = __all_sync(0xffffffffu, BarWait(s_empty + st, ((it / a.stages) - 1) & 1, stop)) != 0;      // one decision per warp
-        if (!ok) break;
+      auto load = [&](bool ta, bool tb, int st, int k0) {      // one thread
         const unsigned int sa = Smem32(stages + static_cast<size_t>(st) * a.stage_bytes), sb = sa + kABytes;
-        const bool cut = MODE == kGram && ((tile.depth - k0) & 15) != 0 && tile.depth - k0 < kDepthTc;      // a Gram's ragged last step
-        const bool ta = a.a_tma != 0 && !cut, tb = a.b_tma != 0 && !cut;
-        if (tid == 0 && (ta || tb)) {
-          const int b_boxes = (a.n + 63) / 64;
-          BarExpect(s_full + st, (ta ? kABytes : 0) + (tb ? (MODE == kProductsK ? a.n * 128 : b_boxes * 8192) : 0));
-          if (ta) {
-            if constexpr (MODE == kGram) { for (int i = 0; i < 2; ++i) TmaLoad2D(sa + i * 8192, &a_map, tile.m0 + 64 * i, tile.row0 + k0, s_full + st); }
-            else TmaLoad2D(sa, &a_map, k0, tile.row0, s_full + st);
-          }
-          if (tb) {
-            if constexpr (MODE == kProductsK) TmaLoad3D(sb, &b_map, k0, tile.n0, tile.leaf * a.b_leaf_on, s_full + st);
-            else
-              for (int i = 0; i < b_boxes; ++i) {
-                if constexpr (MODE == kGram) TmaLoad2D(sb + i * 8192, &b_map, tile.n0 + 64 * i, tile.row0 + k0, s_full + st);
-                else TmaLoad3D(sb + i * 8192, &b_map, tile.n0 + 64 * i, k0, tile.leaf * a.b_leaf_on, s_full + st);
-              }
+        const int b_boxes = (a.n + 63) / 64;
+        if (ta) {
+          if constexpr (MODE == kGram) { for (int i = 0; i < 2; ++i) TmaLoad2D(sa + i * 8192, &a_map, tile.m0 + 64 * i, tile.row0 + k0, s_full + st); }
+          else TmaLoad2D(sa, &a_map, k0, tile.row0, s_full + st);
+        }
+        if (tb) {
+          if constexpr (MODE == kProductsK) { TmaLoad3D(sb, &b_map, k0, tile.n0, tile.leaf * a.b_leaf_on, s_full + st); }
+          else if constexpr (MODE == kGram) { for (int i = 0; i < b_boxes; ++i) TmaLoad2D(sb + i * 8192, &b_map, tile.n0 + 64 * i, tile.row0 + k0, s_full + st); }
+          else { for (int i = 0; i < b_boxes; ++i) TmaLoad3D(sb + i * 8192, &b_map, tile.n0 + 64 * i, k0, tile.leaf * a.b_leaf_on, s_full + st); }
+        }
+      };
+      auto copy = [&](bool ca, bool cb, int st, int k0) {      // all copying warps
+        const unsigned int sa = Smem32(stages + static_cast<size_t>(st) * a.stage_bytes), sb = sa + kABytes;
+        const int depth = min(kDepthTc, (tile.depth - k0 + 15) & ~15);
+        if (ca) { if constexpr (MODE == kGram) CopyMnMajor(sa, va, kTileM / 8, k0, depth, a.a_vec, tid); else CopyKMajor(sa, va, kTileM, k0, depth, a.a_vec, tid); }
+        if (cb) { if constexpr (MODE == kProductsK) CopyKMajor(sb, vb, a.n, k0, depth, a.b_vec, tid); else CopyMnMajor(sb, vb, a.n / 8, k0, depth, a.b_vec, tid); }
+        CopyCommit();
+      };
+      const unsigned int a_bytes = kABytes, b_bytes = MODE == kProductsK ? a.n * 128 : (a.n + 63) / 64 * 8192;
+      if (both) {
+        // One thread fills the stages; all warps come together only for a Gram's ragged last step.
+        const int steps = (tile.depth + kDepthTc - 1) / kDepthTc, cut = MODE == kGram && (tile.depth & 15) != 0 ? 1 : 0, first = it;
+        it += steps;
+        if (tid == 0) {
+          for (int i = 0; i < steps - cut && ok; ++i) {
+            const int step = first + i, st = step % a.stages;
+            if (step >= a.stages) ok = BarWait(s_empty + st, ((step / a.stages) - 1) & 1, stop);
+            if (!ok) { it = step; break; }
+            BarArriveExpect(s_full + st, a_bytes + b_bytes);
+            load(true, true, st, i * kDepthTc);
           }
         }
-        if (!ta) { if constexpr (MODE == kGram) CopyMnMajor(sa, va, kTileM / 8, k0, depth, a.a_vec, tid); else CopyKMajor(sa, va, kTileM, k0, depth, a.a_vec, tid); }
-        if (!tb) { if constexpr (MODE == kProductsK) CopyKMajor(sb, vb, a.n, k0, depth, a.b_vec, tid); else CopyMnMajor(sb, vb, a.n / 8, k0, depth, a.b_vec, tid); }
-        if (both) {                // nothing to wait for, but in a ragged step
-          if (cut) { CopyCommit(); CopyWait<0>(); }
-          hand_over(it);
-        } else {
-          CopyCommit();
+        if (cut != 0) {
+          const int step = it - 1, st = step % a.stages;
+          // the filling thread alone knows when the stage is free: the others skip steps, and a parity tells neighbouring uses apart only
+          if (tid == 0 && ok) { if (step >= a.stages) ok = BarWait(s_empty + st, ((step / a.stages) - 1) & 1, stop); if (ok) BarArrive(&s_go); }
+          __syncwarp();
+          ok = ok && BarWait(&s_go, cuts & 1, stop);
+          ok = __all_sync(0xffffffffu, ok) != 0;
+          if (ok) {
+            copy(true, true, st, (steps - 1) * kDepthTc);
+            CopyWait<0>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) BarArrive(&s_cut);
+            if (tid == 0) { ok = BarWait(&s_cut, cuts & 1, stop); if (ok) BarArrive(s_full + st); }
+            ok = __all_sync(0xffffffffu, ok) != 0;
+          }
+          ++cuts;
+        }
+      } else {
+        for (int k0 = 0; k0 < tile.depth; k0 += kDepthTc, ++it) {
+          const int st = it % a.stages;
+          if (it >= a.stages) ok = __all_sync(0xffffffffu, BarWait(s_empty + st, ((it / a.stages) - 1) & 1, stop)) != 0;      // one decision per warp
+          if (!ok) break;
+          const bool cut = MODE == kGram && ((tile.depth - k0) & 15) != 0 && tile.depth - k0 < kDepthTc;
+          const bool ta = a.a_tma != 0 && !cut, tb = a.b_tma != 0 && !cut;
+          if (tid == 0 && (ta || tb)) { BarExpect(s_full + st, (ta ? a_bytes : 0) + (tb ? b_bytes : 0)); load(ta, tb, st, k0); }
+          copy(!ta, !tb, st, k0);
           if (it >= lag) { if (lag == kLag) CopyWait<kLag>(); else CopyWait<kLagFew>(); hand_over(it - lag); }
         }
       }
