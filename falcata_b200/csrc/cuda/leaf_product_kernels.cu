@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
   extern __shared__ unsigned char s_raw[];
   __shared__ TileMap map;
   __shared__ unsigned long long s_full[kMostStages], s_empty[kMostStages], s_done[2], s_free[2], s_cut, s_go;
-  __shared__ unsigned int s_tmem; __shared__ int s_stop;
+  __shared__ unsigned int s_tmem; __shared__ int s_stop, s_go_stage;
   unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (warp == 12) {
@@ -618,7 +618,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
     const int tid = threadIdx.x - 128;
     const bool both = a.a_tma != 0 && a.b_tma != 0;
     const int lag = a.stages > kLag + 1 ? kLag : kLagFew;
-    int it = 0, cuts = 0;
+    int it = 0, cuts = 0, fill = 0;
+    unsigned int fill_parity = 1;            // of the stage's use before: flips when the ring starts over (the first use waits for nothing)
     bool ok = true;
     auto hand_over = [&](int step) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // this thread's copies -> visible to the tensor core's reads
@@ -661,31 +662,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
       const unsigned int a_bytes = kABytes, b_bytes = MODE == kProductsK ? a.n * 128 : (a.n + 63) / 64 * 8192;
       if (both) {
         // One thread fills the stages; all warps come together only for a Gram's ragged last step.
-        const int steps = (tile.depth + kDepthTc - 1) / kDepthTc, cut = MODE == kGram && (tile.depth & 15) != 0 ? 1 : 0, first = it;
-        it += steps;
+        const int steps = (tile.depth + kDepthTc - 1) / kDepthTc, cut = MODE == kGram && (tile.depth & 15) != 0 ? 1 : 0;
         if (tid == 0) {
-          for (int i = 0; i < steps - cut && ok; ++i) {
-            const int step = first + i, st = step % a.stages;
-            if (step >= a.stages) ok = BarWait(s_empty + st, ((step / a.stages) - 1) & 1, stop);
-            if (!ok) { it = step; break; }
-            BarArriveExpect(s_full + st, a_bytes + b_bytes);
-            load(true, true, st, i * kDepthTc);
+          for (int i = 0; i < steps - cut; ++i) {
+            if (it >= a.stages && !BarWait(s_empty + fill, fill_parity, stop)) { ok = false; break; }
+            BarArriveExpect(s_full + fill, a_bytes + b_bytes);
+            load(true, true, fill, i * kDepthTc);
+            ++it;
+            if (++fill == a.stages) { fill = 0; fill_parity ^= 1u; }
           }
         }
         if (cut != 0) {
-          const int step = it - 1, st = step % a.stages;
           // the filling thread alone knows when the stage is free: the others skip steps, and a parity tells neighbouring uses apart only
-          if (tid == 0 && ok) { if (step >= a.stages) ok = BarWait(s_empty + st, ((step / a.stages) - 1) & 1, stop); if (ok) BarArrive(&s_go); }
+          if (tid == 0 && ok) { if (it >= a.stages) ok = BarWait(s_empty + fill, fill_parity, stop); if (ok) { s_go_stage = fill; BarArrive(&s_go); } }
           __syncwarp();
           ok = ok && BarWait(&s_go, cuts & 1, stop);
           ok = __all_sync(0xffffffffu, ok) != 0;
           if (ok) {
+            const int st = *const_cast<volatile int*>(&s_go_stage);
             copy(true, true, st, (steps - 1) * kDepthTc);
             CopyWait<0>();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) BarArrive(&s_cut);
-            if (tid == 0) { ok = BarWait(&s_cut, cuts & 1, stop); if (ok) BarArrive(s_full + st); }
+            if (tid == 0) {
+              ok = BarWait(&s_cut, cuts & 1, stop);
+              if (ok) { BarArrive(s_full + st); ++it; if (++fill == a.stages) { fill = 0; fill_parity ^= 1u; } }
+            }
             ok = __all_sync(0xffffffffu, ok) != 0;
           }
           ++cuts;
@@ -710,32 +713,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
         for (int i = 0; i < (1 << 16) && !BarTry(s_full + step % a.stages, (step / a.stages) & 1); ++i) {}
   } else if (warp == 12) {
     if (lane == 0) {
-      int it = 0, set = 0;
+      // One thread feeds the tensor cores: its own instructions must take less time than the matrix instructions that they issue (512
+      // cycles a step), so stages, parities and descriptors are carried along by adding (worked out anew: 1000 cycles a step).
+      int set = 0, st = 0, steps = 0;
+      unsigned int parity = 0;
       bool ok = true;
+      const unsigned long long a_desc0 = OperandDesc(Smem32(stages), MODE == kGram ? 8192 : 16), b_desc0 = OperandDesc(Smem32(stages) + kABytes, MODE == kProductsK ? 16 : 8192);
+      const unsigned int stage_on = static_cast<unsigned int>(a.stage_bytes) >> 4;
+      // 16 deep at a time: 32 bytes on inside a K-major line, 16 lines on in MN-major order
+      constexpr unsigned int kAOn = MODE == kGram ? 2048 >> 4 : 32 >> 4, kBOn = MODE == kProductsK ? 32 >> 4 : 2048 >> 4;
       for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const Tile tile = tile_of(t);
         if (tile.depth == 0) continue;
         const int acc = set & 1;
-        if (set >= 2 && !BarWait(s_free + acc, ((set >> 1) - 1) & 1, stop)) break;
+        if (set >= 2 && !BarWait(s_free + acc, ((set >> 1) - 1) & 1, stop)) { ok = false; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const unsigned int d = tmem + acc * (a.tmem_cols / 2);
-        for (int k0 = 0; k0 < tile.depth; k0 += kDepthTc, ++it) {
-          const int st = it % a.stages, depth = min(kDepthTc, (tile.depth - k0 + 15) & ~15);
-          if (!BarWait(s_full + st, (it / a.stages) & 1, stop)) { ok = false; break; }
+        bool fresh = true;
+        for (int left = tile.depth; left > 0; left -= kDepthTc) {
+          if (!BarWait(s_full + st, parity, stop)) { ok = false; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const unsigned int sa = Smem32(stages + static_cast<size_t>(st) * a.stage_bytes), sb = sa + kABytes;
-          // 16 deep at a time: 32 bytes on inside a K-major line, 16 lines on in MN-major order
-          for (int k = 0; k < depth; k += 16) {
-            const unsigned long long da = MODE == kGram ? OperandDesc(sa + k * 128, 8192) : OperandDesc(sa + k * 2, 16);
-            const unsigned long long db = MODE == kProductsK ? OperandDesc(sb + k * 2, 16) : OperandDesc(sb + k * 128, 8192);
-            Mma16(d, da, db, a.idesc, k0 + k > 0);
-          }
+          const unsigned long long da = a_desc0 + static_cast<unsigned long long>(st * stage_on), db = b_desc0 + static_cast<unsigned long long>(st * stage_on);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (16 * k < left) { Mma16(d, da + k * kAOn, db + k * kBOn, a.idesc, !fresh); fresh = false; }
           MmaCommit(s_empty + st);
+          ++steps;
+          if (++st == a.stages) { st = 0; parity ^= 1u; }
         }
         if (ok) { MmaCommit(s_done + acc); ++set; }
       }
-      if (!ok && it > 0) {      // the matrix instructions in flight still read shared memory
-        const int last = (it - 1) % a.stages;
-        for (int i = 0; i < (1 << 20) && !BarTry(s_empty + last, ((it - 1) / a.stages) & 1); ++i) {}
+      if (!ok && steps > 0) {      // the matrix instructions in flight still read shared memory
+        const int last = st == 0 ? a.stages - 1 : st - 1;
+        const unsigned int last_parity = st == 0 ? parity ^ 1u : parity;
+        for (int i = 0; i < (1 << 20) && !BarTry(s_empty + last, last_parity); ++i) {}
       }
     }
     __syncwarp();
