@@ -179,21 +179,28 @@ struct RowResult {
 };
 
 // ------------------------------------------------------------------------------------------------ few classes ----
-// A thread per row, the row's scores in MOST registers. Class-major scores are read straight into them, 32 rows per instruction;
-// rows go through shared memory (an odd row pitch there, so that neither side meets bank conflicts).
+// A thread has ROWS rows, each row's scores in MOST registers. Class-major scores are read straight into them, 32 rows per instruction,
+// all rows' loads before the first use; rows go through shared memory (an odd row pitch there, so that neither side meets bank
+// conflicts).
 constexpr int kFewThreads = 128, kFewClasses = 64;
-template <typename T, int MOST, bool BY_CLASS>
+template <typename T, int MOST, bool BY_CLASS, int ROWS>
 __global__ void __launch_bounds__(kFewThreads) ClassLogProbsFewKernel(ClassScoresArgs a) {
   __shared__ float s_rows[BY_CLASS ? 1 : kFewThreads * (MOST + 1)];
   const int K = static_cast<int>(a.classes);
-  const long long row0 = static_cast<long long>(blockIdx.x) * kFewThreads, row = row0 + threadIdx.x;
+  const long long row0 = static_cast<long long>(blockIdx.x) * (kFewThreads * ROWS);
   const T* base = static_cast<const T*>(a.scores);
-  float v[MOST];
-  if constexpr (BY_CLASS) {
-    if (row >= a.rows) return;
+  float v[ROWS][MOST]; long long y[ROWS];
 #pragma unroll
-    for (int j = 0; j < MOST; ++j) v[j] = j < K ? ToFloat(base[row * a.row_stride + j * a.class_stride]) : -INFINITY;
+  for (int i = 0; i < ROWS; ++i) { const long long row = row0 + i * kFewThreads + threadIdx.x; y[i] = row < a.rows ? LabelOf(a, row) : -1; }
+  if constexpr (BY_CLASS) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const long long row = row0 + i * kFewThreads + threadIdx.x;
+#pragma unroll
+      for (int j = 0; j < MOST; ++j) v[i][j] = j < K && row < a.rows ? ToFloat(base[row * a.row_stride + j * a.class_stride]) : -INFINITY;
+    }
   } else {
+    static_assert(ROWS == 1, "rows in shared memory: one per thread");
     const int rows = static_cast<int>(min(static_cast<long long>(kFewThreads), a.rows - row0)), pitch = K | 1;
     for (int e = threadIdx.x, r = e / K, j = e - r * K; e < rows * K; e += kFewThreads) {
       s_rows[r * pitch + j] = ToFloat(base[(row0 + r) * a.row_stride + j * a.class_stride]);
@@ -201,31 +208,34 @@ __global__ void __launch_bounds__(kFewThreads) ClassLogProbsFewKernel(ClassScore
       if (j >= K) { j -= K; ++r; }
     }
     __syncthreads();
-    if (row >= a.rows) return;
 #pragma unroll
-    for (int j = 0; j < MOST; ++j) v[j] = j < K ? s_rows[threadIdx.x * pitch + j] : -INFINITY;
+    for (int j = 0; j < MOST; ++j) v[0][j] = j < K ? s_rows[threadIdx.x * pitch + j] : -INFINITY;
   }
-  Sums sums;
-  float m = v[0];
 #pragma unroll
-  for (int j = 1; j < MOST; ++j) m = MaxNan(m, v[j]);
-  sums.m = m;
-  const float b = sums.Base();
+  for (int i = 0; i < ROWS; ++i) {
+    const long long row = row0 + i * kFewThreads + threadIdx.x;
+    if (row >= a.rows) return;
+    Sums sums;
+    float m = v[i][0];
 #pragma unroll
-  for (int j = 0; j < MOST; ++j) sums.Add(v[j], b);
-  const RowResult res(sums);
-  const long long y = LabelOf(a, row);
-  float given = 0.f;
+    for (int j = 1; j < MOST; ++j) m = MaxNan(m, v[i][j]);
+    sums.m = m;
+    const float b = sums.Base();
 #pragma unroll
-  for (int j = 0; j < MOST; ++j) if (j == y) given = v[j];
-  res.Store(a, row, y, given);
-  for (int t = 0; t < a.top_k; ++t) {
-    float best = -INFINITY; int cls = -1;
+    for (int j = 0; j < MOST; ++j) sums.Add(v[i][j], b);
+    const RowResult res(sums);
+    float given = 0.f;
 #pragma unroll
-    for (int j = 0; j < MOST; ++j) if (v[j] > best) { best = v[j]; cls = j; }
+    for (int j = 0; j < MOST; ++j) if (j == y[i]) given = v[i][j];
+    res.Store(a, row, y[i], given);
+    for (int t = 0; t < a.top_k; ++t) {
+      float best = -INFINITY; int cls = -1;
 #pragma unroll
-    for (int j = 0; j < MOST; ++j) if (j == cls) v[j] = -INFINITY;
-    res.StoreTop(a, row * a.top_k + t, best, cls);
+      for (int j = 0; j < MOST; ++j) if (v[i][j] > best) { best = v[i][j]; cls = j; }
+#pragma unroll
+      for (int j = 0; j < MOST; ++j) if (j == cls) v[i][j] = -INFINITY;
+      res.StoreTop(a, row * a.top_k + t, best, cls);
+    }
   }
 }
 
@@ -328,8 +338,8 @@ struct Alternatives {
     GroupSync<GROUP>();
     return min(count, top_k);
   }
-  // most: this thread's maximum. All threads; the list is complete on return.
-  __device__ __forceinline__ int Find(float most, float head_v, float tail_v) {
+  // most: this thread's maximum. All threads; the list is complete on return. Not inlined: once per row, and the walk keeps its registers.
+  __device__ __noinline__ int Find(float most, float head_v, float tail_v) {
     constexpr int PER = GROUP / 32;
     sh.key[tid] = OrderKey<T>(most);
     GroupSync<GROUP>();
@@ -423,7 +433,7 @@ struct Alternatives {
 
 // TOP: alternatives are wanted. Groups walk the rows with the grid's stride; a row belongs to a warp, a block or a cluster.
 template <typename T, int GROUP, bool TOP>
-__global__ void __launch_bounds__(256, TOP ? 3 : 4) ClassLogProbsRowKernel(ClassScoresArgs a) {
+__global__ void __launch_bounds__(256, 4) ClassLogProbsRowKernel(ClassScoresArgs a) {
   constexpr int kGroups = 256 / GROUP;
   __shared__ RowShared<GROUP> s_all[TOP ? kGroups : 1];
   __shared__ float s_m[8], s_s[8], s_t[8];
@@ -447,13 +457,12 @@ __global__ void __launch_bounds__(256, TOP ? 3 : 4) ClassLogProbsRowKernel(Class
     const bool more = next_row < a.rows;
     const float head_v = r.first && tid < r.head ? ToFloat(r.s[tid]) : -INFINITY, tail_v = r.last_part && tid < r.K - r.tail ? ToFloat(r.s[r.tail + tid]) : -INFINITY;
     const float given = tid == 0 && y >= 0 && y < r.K ? ToFloat(r.s[y]) : 0.f;
-    const RowShare<T> rn(a, more ? next_row : row, part, parts, GROUP);
     const long long y_next = more ? LabelOf(a, next_row) : -1;
     PairSums<T> pairs;
     int at = r.v_begin;
     do {                                         // a share without vectors takes one empty step
       const int then = at + GROUP * kUnroll;
-      if (then < r.v_end) load(next, r, then); else if (more) load(next, rn, rn.v_begin);
+      if (then < r.v_end) load(next, r, then); else if (more) { const RowShare<T> rn(a, next_row, part, parts, GROUP); load(next, rn, rn.v_begin); }
       float most = Max(q[0], type);
 #pragma unroll
       for (int u = 1; u < kUnroll; ++u) most = MaxNan(most, Max(q[u], type));
@@ -495,7 +504,7 @@ __global__ void __launch_bounds__(256, TOP ? 3 : 4) ClassLogProbsRowKernel(Class
         cg::this_cluster().sync();
         if (part == 0) {
           int count = have;
-          if (TOP && tid < have) sh.cand[tid] = sh.list[tid];
+          if constexpr (TOP) { if (tid < have) sh.cand[tid] = sh.list[tid]; if (tid == 0) { sh.flagged[0] = 0; sh.flagged[1] = have; } }
           for (int p = 1; p < parts; ++p) {
             if (tid < 32) sums.Join(*cg::this_cluster().map_shared_rank(&s_m[0], p), *cg::this_cluster().map_shared_rank(&s_s[0], p), *cg::this_cluster().map_shared_rank(&s_t[0], p));
             if constexpr (TOP) {
@@ -503,9 +512,26 @@ __global__ void __launch_bounds__(256, TOP ? 3 : 4) ClassLogProbsRowKernel(Class
               const int n = o->have;
               if (tid < n) sh.cand[count + tid] = o->list[tid];
               count += n;
+              if (tid == 0) sh.flagged[p + 1] = count;
             }
           }
-          if constexpr (TOP) { __syncthreads(); Alternatives<GROUP, T> alt{sh, r, a.top_k, tid}; have = alt.Rank(count); }
+          if constexpr (TOP) {
+            // the lists are sorted: an entry's rank is its place in its own list and, by bisection, how many of each other come before it
+            __syncthreads();
+            if (tid < count) {
+              const Entry e = sh.cand[tid];
+              int rank = 0;
+              for (int p = 0; p < parts; ++p) {
+                const int begin = sh.flagged[p];
+                int lo = begin, hi = sh.flagged[p + 1];
+                while (lo < hi) { const int mid = (lo + hi) >> 1; if (Before(sh.cand[mid], e)) lo = mid + 1; else hi = mid; }
+                rank += lo - begin;
+              }
+              if (rank < a.top_k) sh.list[rank] = e;
+            }
+            __syncthreads();
+            have = min(count, a.top_k);
+          }
         }
         cg::this_cluster().sync();         // no block goes on while its shared memory is read
       }
@@ -517,7 +543,7 @@ __global__ void __launch_bounds__(256, TOP ? 3 : 4) ClassLogProbsRowKernel(Class
       __syncthreads();                     // the next row writes the shared parts again
     }
     if (!more) return;
-    row = next_row; r = rn; y = y_next;
+    row = next_row; r = RowShare<T>(a, row, part, parts, GROUP); y = y_next;
   }
 }
 
@@ -581,15 +607,26 @@ struct RowGrad {
   float m, log_sum, a, h, g_label; int label; bool none, bad, again;
   __device__ __forceinline__ RowGrad() {}
   __device__ __forceinline__ RowGrad(const ClassScoresArgs& s, const ClassGradArgs& g, long long row) {
+    float top = 0.f;
+    for (int t = 0; t < s.top_k; ++t) top += Top(s, g, row, t);
+    Set(s, g, row, top);
+  }
+  __device__ __forceinline__ static float Top(const ClassScoresArgs& s, const ClassGradArgs& g, long long row, int t) {
+    const int c = s.top_class[row * s.top_k + t]; const float v = g.g_top[row * s.top_k + t];
+    return c >= 0 && c < s.classes ? v : 0.f;
+  }
+  // top: the sum of the gradients of the alternatives' log probabilities
+  __device__ __forceinline__ void Set(const ClassScoresArgs& s, const ClassGradArgs& g, long long row, float top) {
     const float log_norm = s.log_norm[row];
     const long long y = LabelOf(s, row);
+    const float g_norm = g.g_log_norm ? g.g_log_norm[row] : 0.f, g_prob = g.g_log_prob ? g.g_log_prob[row] : 0.f, entropy = s.entropy[row];
+    h = g.g_entropy ? g.g_entropy[row] : 0.f;
     none = log_norm == -INFINITY; bad = (!none && !(fabsf(log_norm) < InfF())) || y >= s.classes;
     again = !none && !bad && fabsf(log_norm) > kTrustedLogNorm;
     m = none ? 0.f : log_norm; log_sum = 0.f;
     label = y >= 0 && y < s.classes ? static_cast<int>(y) : -1;
-    h = g.g_entropy ? g.g_entropy[row] : 0.f; g_label = g.g_log_prob && label >= 0 ? g.g_log_prob[row] : 0.f;
-    a = (g.g_log_norm ? g.g_log_norm[row] : 0.f) - g_label - h * s.entropy[row];
-    for (int t = 0; t < s.top_k; ++t) { const int c = s.top_class[row * s.top_k + t]; if (c >= 0 && c < s.classes) a -= g.g_top[row * s.top_k + t]; }
+    g_label = label >= 0 ? g_prob : 0.f;
+    a = g_norm - g_label - h * entropy - top;
     if (none) { a = h = g_label = 0.f; }
     if (bad) a = NanF();
   }
@@ -616,7 +653,7 @@ __device__ __forceinline__ void PatchTop(const ClassScoresArgs& a, const ClassGr
 }
 
 // Rows of few classes: the block's rows are one after the other in memory, its threads walk their elements.
-constexpr int kGradThreads = 256, kGradRows = 64;
+constexpr int kGradThreads = 256, kGradRows = 64, kGradVectors = 4;      // kGradVectors: 16-byte loads of a thread and chunk
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) ClassGradFewKernel(ClassScoresArgs a, ClassGradArgs g) {
   __shared__ RowGrad s_row[kGradRows];
@@ -654,7 +691,22 @@ __global__ void __launch_bounds__(kGradThreads) ClassGradRowKernel(ClassScoresAr
   const T* in = static_cast<const T*>(a.scores) + row * a.row_stride;
   T* out = static_cast<T*>(g.grad) + row * g.grad_row_stride;
   const T* type = nullptr;
-  if (threadIdx.x == 0) s_row = RowGrad(a, g, row);
+  // chunk c: the classes from head + c * chunk (chunk 0: from 0) to the next one's start. Its scores are asked for before the row's
+  // values, on which everything else waits.
+  const int c = blockIdx.x % chunks;
+  const int lo = c == 0 ? 0 : min(K, head + c * chunk), hi = c == chunks - 1 ? K : min(K, head + (c + 1) * chunk);
+  const int first = min(K, head + c * chunk), vectors = ALIGNED ? (hi - first) / N : 0, rest = first + vectors * N;
+  const uint4* from = reinterpret_cast<const uint4*>(in + first); uint4* to = reinterpret_cast<uint4*>(out + first);
+  uint4 q[kGradVectors];
+#pragma unroll
+  for (int u = 0; u < kGradVectors; ++u) { const int i = threadIdx.x + u * kGradThreads; if (i < vectors) q[u] = __ldg(from + i); }
+  if (threadIdx.x < 32) {
+    float top = threadIdx.x < a.top_k ? RowGrad::Top(a, g, row, threadIdx.x) : 0.f;
+    for (int o = 16; o > 0; o >>= 1) top += __shfl_xor_sync(0xffffffffu, top, o);
+    RowGrad r;
+    r.Set(a, g, row, top);
+    if (threadIdx.x == 0) s_row = r;
+  }
   __syncthreads();
   if (s_row.again) {
     Sums r;
@@ -666,36 +718,27 @@ __global__ void __launch_bounds__(kGradThreads) ClassGradRowKernel(ClassScoresAr
     __syncthreads();
   }
   const RowGrad r = s_row;
-  // chunk c: the classes from head + c * chunk (chunk 0: from 0) to the next one's start
-  const int c = blockIdx.x % chunks;
-  const int lo = c == 0 ? 0 : min(K, head + c * chunk), hi = c == chunks - 1 ? K : min(K, head + (c + 1) * chunk);
   if constexpr (ALIGNED) {
-    const int first = min(K, head + c * chunk), vectors = (hi - first) / N, rest = first + vectors * N;
     for (int j = lo + threadIdx.x; j < first; j += kGradThreads) out[j] = FromFloat<T>(r.At(ToFloat(in[j]), j));
-    const uint4* from = reinterpret_cast<const uint4*>(in + first); uint4* to = reinterpret_cast<uint4*>(out + first);
-    for (int i = threadIdx.x; i < vectors; i += 2 * kGradThreads) {
-      const bool two = i + kGradThreads < vectors;
-      const uint4 q0 = __ldg(from + i), q1 = two ? __ldg(from + i + kGradThreads) : q0;
-      auto one = [&](const uint4& q, int at) {
-        float v[N]; Unpack(q, v, type);
-        union { uint4 q; T t[N]; } o;
 #pragma unroll
-        for (int k = 0; k < N; ++k) o.t[k] = FromFloat<T>(r.At(v[k], first + at * N + k));
-        to[at] = o.q;
-      };
-      one(q0, i);
-      if (two) one(q1, i + kGradThreads);
+    for (int u = 0; u < kGradVectors; ++u) {
+      const int i = threadIdx.x + u * kGradThreads;
+      if (i >= vectors) break;
+      float v[N]; Unpack(q[u], v, type);
+      union { uint4 q; T t[N]; } o;
+#pragma unroll
+      for (int k = 0; k < N; ++k) o.t[k] = FromFloat<T>(r.At(v[k], first + i * N + k));
+      to[i] = o.q;
     }
-    for (int j = rest + threadIdx.x; j < hi; j += kGradThreads) out[j] = FromFloat<T>(r.At(ToFloat(in[j]), j));
-  } else {
-    for (int j = lo + threadIdx.x; j < hi; j += kGradThreads) out[j] = FromFloat<T>(r.At(ToFloat(in[j]), j));
   }
+  for (int j = rest + threadIdx.x; j < hi; j += kGradThreads) out[j] = FromFloat<T>(r.At(ToFloat(in[j]), j));
   if (a.top_k > 0) {
     __syncthreads();
     if (threadIdx.x < a.top_k) PatchTop<T>(a, g, r, row, threadIdx.x, lo, hi);
   }
 }
 
+constexpr int kGradClasses = 12;      // scores of a thread in flight
 // A thread per row (class-major scores, or any strides); the classes in slices over the grid's second dimension.
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) ClassGradColumnKernel(ClassScoresArgs a, ClassGradArgs g, int slice) {
@@ -704,17 +747,19 @@ __global__ void __launch_bounds__(kGradThreads) ClassGradColumnKernel(ClassScore
   const int K = static_cast<int>(a.classes), lo = blockIdx.y * slice, hi = min(K, lo + slice);
   const T* in = static_cast<const T*>(a.scores) + row * a.row_stride;
   T* out = static_cast<T*>(g.grad) + row * g.grad_row_stride;
+  float v[kGradClasses];
+#pragma unroll
+  for (int u = 0; u < kGradClasses; ++u) v[u] = lo + u < hi ? ToFloat(in[(lo + u) * a.class_stride]) : 0.f;      // before the row's values
   RowGrad r(a, g, row);
   if (r.again) r.TakeAgain(a, in);
-  int j = lo;
-  for (; j + 8 <= hi; j += 8) {
-    float v[8];
+  for (int j = lo; j < hi; j += kGradClasses) {
+    if (j > lo) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = ToFloat(in[(j + u) * a.class_stride]);
+      for (int u = 0; u < kGradClasses; ++u) v[u] = j + u < hi ? ToFloat(in[(j + u) * a.class_stride]) : 0.f;
+    }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) out[(j + u) * g.grad_class_stride] = FromFloat<T>(r.At(v[u], j + u));
+    for (int u = 0; u < kGradClasses; ++u) if (j + u < hi) out[(j + u) * g.grad_class_stride] = FromFloat<T>(r.At(v[u], j + u));
   }
-  for (; j < hi; ++j) out[j * g.grad_class_stride] = FromFloat<T>(r.At(ToFloat(in[j * a.class_stride]), j));
   for (int t = 0; t < a.top_k; ++t) PatchTop<T>(a, g, r, row, t, lo, hi);
 }
 
@@ -729,20 +774,28 @@ template <typename F> void DispatchType(int dtype, F&& f) {
 
 constexpr int kSms = 148;
 
-template <typename T, bool BY_CLASS>
+template <typename T, int MOST>
+void LaunchFew(const ClassScoresArgs& a, bool by_class, cudaStream_t s) {
+  constexpr int kRows = MOST <= 16 ? 2 : 1;      // two rows' scores in flight per thread while they fit the registers
+  if (by_class) ClassLogProbsFewKernel<T, MOST, true, kRows><<<static_cast<unsigned int>((a.rows + kFewThreads * kRows - 1) / (kFewThreads * kRows)), kFewThreads, 0, s>>>(a);
+  else ClassLogProbsFewKernel<T, MOST, false, 1><<<static_cast<unsigned int>((a.rows + kFewThreads - 1) / kFewThreads), kFewThreads, 0, s>>>(a);
+}
+template <typename T>
 void LaunchFew(const ClassScoresArgs& a, cudaStream_t s) {
-  const unsigned int blocks = static_cast<unsigned int>((a.rows + kFewThreads - 1) / kFewThreads);
-  if (a.classes <= 4) ClassLogProbsFewKernel<T, 4, BY_CLASS><<<blocks, kFewThreads, 0, s>>>(a);
-  else if (a.classes <= 8) ClassLogProbsFewKernel<T, 8, BY_CLASS><<<blocks, kFewThreads, 0, s>>>(a);
-  else if (a.classes <= 16) ClassLogProbsFewKernel<T, 16, BY_CLASS><<<blocks, kFewThreads, 0, s>>>(a);
-  else if (a.classes <= 32) ClassLogProbsFewKernel<T, 32, BY_CLASS><<<blocks, kFewThreads, 0, s>>>(a);
-  else ClassLogProbsFewKernel<T, kFewClasses, BY_CLASS><<<blocks, kFewThreads, 0, s>>>(a);
+  // lanes walk rows: right where neighbouring rows are nearer to each other than neighbouring classes
+  const bool by_class = a.row_stride < a.class_stride;
+  if (a.classes <= 4) LaunchFew<T, 4>(a, by_class, s);
+  else if (a.classes <= 8) LaunchFew<T, 8>(a, by_class, s);
+  else if (a.classes <= 12) LaunchFew<T, 12>(a, by_class, s);
+  else if (a.classes <= 16) LaunchFew<T, 16>(a, by_class, s);
+  else if (a.classes <= 32) LaunchFew<T, 32>(a, by_class, s);
+  else LaunchFew<T, kFewClasses>(a, by_class, s);
 }
 
 template <typename T, int GROUP, bool TOP>
 void LaunchRows(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
   // as many groups as are resident at once, each with several rows
-  const long long groups = GROUP == 32 ? (a.rows + 7) / 8 : a.rows, most = static_cast<long long>(kSms) * (TOP ? 3 : 4) * (GROUP == 32 ? 2 : 1) / cluster;
+  const long long groups = GROUP == 32 ? (a.rows + 7) / 8 : a.rows, most = static_cast<long long>(kSms) * 4 * (GROUP == 32 ? 2 : 1) / cluster;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
@@ -761,8 +814,7 @@ void LaunchClassLogProbs(const ClassScoresArgs& a, cudaStream_t s) {
   DispatchType(a.dtype, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
     if (a.classes <= kFewClasses) {
-      // lanes walk rows: right where neighbouring rows are nearer to each other than neighbouring classes
-      if (a.row_stride < a.class_stride) LaunchFew<T, true>(a, s); else LaunchFew<T, false>(a, s);
+      LaunchFew<T>(a, s);
     } else if (a.class_stride == 1) {
       // A warp per row as long as that fills the machine and a warp's walk stays short; else a block, and a cluster of blocks while
       // there are fewer blocks than two per SM and every block has a full chunk.
@@ -802,7 +854,7 @@ void LaunchClassLogProbsGrad(const ClassScoresArgs& a, const ClassGradArgs& g, c
     } else if (a.classes < 2 * kGradThreads) {
       ClassGradFewKernel<T><<<static_cast<unsigned int>((a.rows + kGradRows - 1) / kGradRows), kGradThreads, 0, s>>>(a, g);
     } else {
-      const int chunk = kGradThreads * N * 4;
+      const int chunk = kGradThreads * N * kGradVectors;
       const long long chunks = (a.classes + chunk - 1) / chunk;
       if (a.rows * chunks > 0x7fffffffLL) Log::Fatal("class scores: %lld rows x %lld classes are not covered", a.rows, a.classes);
       const bool aligned = (reinterpret_cast<uintptr_t>(a.scores) & 15) == (reinterpret_cast<uintptr_t>(g.grad) & 15) && ((a.row_stride - g.grad_row_stride) * sizeof(T)) % 16 == 0;

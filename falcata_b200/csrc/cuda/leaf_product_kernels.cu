@@ -144,17 +144,18 @@ struct CopyPlan {
     const long long from_on = lines_on * stride + pieces_on * V, from_wrap = stride - per * V;
     const unsigned int to_on = 4u * (lines_on * pitch + pieces_on * V), to_wrap = 4u * (pitch - per * V);
     int piece = piece0;
+    const int end = min(all, lines);
 #pragma unroll 2
-    for (int line = line0; line < all;) {
-      int valid = line < lines ? (WHOLE ? BYTES : 4 * max(0, min(V, along - piece * V))) : 0;
-      const float* at = WHOLE ? (line < lines ? from : src) : (valid > 0 ? from : src);
+    for (int line = line0; line < end;) {
+      const int valid = WHOLE ? BYTES : 4 * max(0, min(V, along - piece * V));
+      const float* at = WHOLE || valid > 0 ? from : src;
       if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(at), "r"(valid) : "memory");
       else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(to), "l"(at), "r"(valid), "n"(BYTES) : "memory");
       line += lines_on; piece += pieces_on; from += from_on; to += to_on;
       if (piece >= per) { piece -= per; ++line; from += from_wrap; to += to_wrap; }
     }
   }
-  // the source has `lines` lines, `stride` apart, of `along` floats; zero beyond
+  // the source has `lines` lines, `stride` apart, of `along` floats (zero beyond); lines that it does not have are left as they are
   __device__ __forceinline__ void Copy(float* dst, const float* src, int lines, long long stride, int along) const {
     const bool whole = along >= per * vec;
     if (vec == 4) { if (whole) Walk<16, true>(dst, src, lines, stride, along); else Walk<16, false>(dst, src, lines, stride, along); }
@@ -236,8 +237,9 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
     if (ahead.t < tiles) advance(ahead);
     const float* xs = s_float + slot * buffer + (wr * 32 * TM + lane) * pitch;
     const float* ws = s_float + slot * buffer + (Tile::ROWS + wo * TN) * pitch;
-    const int depth = min(shape.width, a.features - now.f0);
-    for (int f = 0; f < depth; f += 4) {          // beyond the last feature both sides are zero
+    // beyond the last feature both sides are zero; rows and outputs that do not exist hold anything, and are not stored
+    const int depth = wr * 32 * TM < now.rows ? min(shape.width, a.features - now.f0) : 0;
+    for (int f = 0; f < depth; f += 4) {
       ulonglong2 xv[TM];
 #pragma unroll
       for (int i = 0; i < TM; ++i) xv[i] = *reinterpret_cast<const ulonglong2*>(xs + 32 * i * pitch + f);
@@ -343,8 +345,9 @@ __global__ void __launch_bounds__(GA * GB * SLICES, TA * TB <= 16 ? 3 : 2) LeafG
       copy(step + kRing - 1);                     // the buffer that everyone has left
       // columns beyond the operands hold anything; they reach only sums that are not stored
       const float* as = s_float + step % kRing * RD * (Tile::AC + Tile::BC) + ga * TA; const float* bs = s_float + (step % kRing * (Tile::AC + Tile::BC) + Tile::AC) * RD + gb * TB;
+      const int here = min(RD, rows - step * RD);
 #pragma unroll 4
-      for (int r = slice; r < RD; r += SLICES) {
+      for (int r = slice; r < here; r += SLICES) {
         F2 bv[TB / 2]; float av[TA];
 #pragma unroll
         for (int j = 0; j < TB / 4; ++j) { const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(bs + r * Tile::BC + 4 * j); bv[2 * j].v = q.x; bv[2 * j + 1].v = q.y; }

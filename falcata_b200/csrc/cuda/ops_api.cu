@@ -251,8 +251,8 @@ int FB_OpClassLogProbsGrad(const void* scores, int dtype, long long rows, long l
   LaunchClassLogProbsGrad(a, g, static_cast<cudaStream_t>(stream));
   OPS_END();
 }
-// The two products take a workspace. With `workspace_floats` not null nothing runs: it receives the floats of workspace that the
-// call with the same arguments needs (possibly 0; the workspace starts on a 16-byte boundary).
+// The two products may need a workspace (on a 16-byte boundary). With `workspace_floats` not null it receives the floats wanted, and
+// the call runs only if that is none; else the same call follows with the workspace and a null `workspace_floats`.
 // y_i = W_leaf(i) x_i for rows grouped by leaf.
 int FB_OpLeafProducts(const void* x, long long x_stride, const void* weight, long long weight_leaf_stride, long long weight_out_stride, long long weight_in_stride, const void* begin,
                       int begin_bits, int leaves, long long rows, int features, int outputs, int dtype, void* y, void* workspace, long long* workspace_floats, int device, void* stream) {
@@ -261,7 +261,7 @@ int FB_OpLeafProducts(const void* x, long long x_stride, const void* weight, lon
   if (features < 1 || outputs < 1) Log::Fatal("leaf products: at least one feature and one output (got %d, %d)", features, outputs);
   LeafProductsArgs a{{begin, begin_bits, leaves, rows}, x, weight, y, dtype, features, outputs, x_stride, weight_leaf_stride, weight_out_stride, weight_in_stride};
   const long long floats = LeafProductsWorkspace(a);
-  if (workspace_floats != nullptr) { *workspace_floats = floats; return 0; }
+  if (workspace_floats != nullptr) { *workspace_floats = floats; if (floats > 0) return 0; }
   if (floats > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) Log::Fatal("leaf products: a workspace of %lld floats is needed, on a 16-byte boundary", floats);
   DeviceScope scope(device);
   LaunchLeafProducts(a, static_cast<float*>(workspace), static_cast<cudaStream_t>(stream));
@@ -275,7 +275,7 @@ int FB_OpLeafGram(const void* a_rows, long long a_stride, const void* b_rows, lo
   if (a_cols < 1 || b_cols < 1) Log::Fatal("leaf Gram: at least one column on each side (got %d, %d)", a_cols, b_cols);
   LeafGramArgs a{{begin, begin_bits, leaves, rows}, a_rows, b_rows, out, dtype, out_dtype, a_cols, b_cols, a_stride, b_stride};
   const long long floats = LeafGramWorkspace(a);
-  if (workspace_floats != nullptr) { *workspace_floats = floats; return 0; }
+  if (workspace_floats != nullptr) { *workspace_floats = floats; if (floats > 0) return 0; }
   if (floats > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)) Log::Fatal("leaf Gram: a workspace of %lld floats is needed, on a 16-byte boundary", floats);
   DeviceScope scope(device);
   LaunchLeafGram(a, static_cast<float*>(workspace), static_cast<cudaStream_t>(stream));

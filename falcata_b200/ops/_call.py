@@ -47,16 +47,23 @@ def require_tensor(name: str, t: torch.Tensor) -> None:
 
 def one_device(**tensors: Optional[torch.Tensor]) -> None:
     """All of them on one CUDA device (that of the first)."""
-    first = None
+    device = None
     for name, t in tensors.items():
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError(f"{name}: a CUDA tensor is wanted, got one on {t.device}")
-        if first is not None and t.device != first.device:
-            raise ValueError(f"{name}: on {t.device}, the other tensors are on {first.device}")
-        first = first if first is not None else t
+        where = t.device
+        if where != device:
+            if where.type != "cuda":
+                raise ValueError(f"{name}: a CUDA tensor is wanted, got one on {where}")
+            if device is not None:
+                raise ValueError(f"{name}: on {where}, the other tensors are on {device}")
+            device = where
+
+
+# The stream's handle without the Python object around it, where torch offers that (1 us less per call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def device_and_stream(device: torch.device) -> Tuple[int, int]:
-    return device.index, torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return index, _raw_stream(index)

@@ -38,7 +38,7 @@ def _products(x: torch.Tensor, weight: torch.Tensor, leaf_begin: torch.Tensor) -
         weight = weight.contiguous()
     n, f = x.shape
     leaves, outputs = weight.shape[0], weight.shape[1]
-    y = torch.empty((n, outputs), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, outputs))
     if n:
         _run(_fwd(), (ptr(x), x.stride(0), ptr(weight), weight.stride(0), weight.stride(1), weight.stride(2), ptr(leaf_begin), 8 * leaf_begin.element_size(), leaves, n, f, outputs,
                       type_code("x", x), ptr(y)), x.device)
@@ -47,11 +47,12 @@ def _products(x: torch.Tensor, weight: torch.Tensor, leaf_begin: torch.Tensor) -
 
 def _run(entry, args: tuple, device: torch.device) -> None:
     """The native call with the workspace that it asks for; the workspace belongs to the current stream, as every tensor made here."""
-    floats = ctypes.c_longlong(0)
+    floats = ctypes.c_longlong(0)      # in: no workspace yet; out: the floats that are wanted, 0 when the call has run
     where = device_and_stream(device)
     check(entry(*args, None, ctypes.byref(floats), *where))
-    workspace = torch.empty(floats.value, dtype=torch.float32, device=device) if floats.value else None
-    check(entry(*args, ptr(workspace), None, *where))
+    if floats.value:
+        workspace = torch.empty(floats.value, dtype=torch.float32, device=device)
+        check(entry(*args, workspace.data_ptr(), None, *where))
 
 
 class _LeafProducts(torch.autograd.Function):
@@ -108,7 +109,7 @@ def leaf_gram(a: torch.Tensor, b: torch.Tensor, leaf_begin: torch.Tensor, dtype:
     one_device(a=a, b=b, leaf_begin=leaf_begin)
     a, b, leaf_begin = _inner_contiguous(a), _inner_contiguous(b), leaf_begin.contiguous()
     leaves = leaf_begin.numel() - 1
-    out = torch.empty((leaves, a.shape[1], b.shape[1]), dtype=dtype, device=a.device)
+    out = a.new_empty((leaves, a.shape[1], b.shape[1]), dtype=dtype)
     _run(_gram(), (ptr(a), a.stride(0), ptr(b), b.stride(0), ptr(leaf_begin), 8 * leaf_begin.element_size(), leaves, a.shape[0], a.shape[1], b.shape[1], type_code("a", a),
                    type_code("dtype", out), ptr(out)), a.device)
     return out

@@ -65,13 +65,14 @@ def _row_values(name: str, t: Optional[torch.Tensor], shape) -> Optional[torch.T
 def _forward(scores: torch.Tensor, labels: Optional[torch.Tensor], top_k: int) -> ClassLogProbs:
     n, k = scores.shape
     labels = None if labels is None else labels.contiguous()
-    new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=scores.device)  # noqa: E731
-    log_prob = None if labels is None else new(n)
-    log_norm, entropy = new(n), new(n)
-    top_log_prob, top_class = (new(n, top_k), new(n, top_k, dtype=torch.int32)) if top_k else (None, None)
+    new = scores.new_empty
+    log_prob = None if labels is None else new(n, dtype=torch.float32)
+    log_norm, entropy = new(n, dtype=torch.float32), new(n, dtype=torch.float32)
+    top_log_prob, top_class = (new((n, top_k), dtype=torch.float32), new((n, top_k), dtype=torch.int32)) if top_k else (None, None)
     if n:
-        check(_fwd()(ptr(scores), type_code("scores", scores), n, k, scores.stride(0), scores.stride(1), ptr(labels), 0 if labels is None else 8 * labels.element_size(), top_k,
-                     ptr(log_prob), ptr(log_norm), ptr(entropy), ptr(top_log_prob), ptr(top_class), *device_and_stream(scores.device)))
+        row_stride, class_stride = scores.stride()
+        check(_fwd()(scores.data_ptr(), type_code("scores", scores), n, k, row_stride, class_stride, ptr(labels), 0 if labels is None else 8 * labels.element_size(), top_k,
+                     ptr(log_prob), log_norm.data_ptr(), entropy.data_ptr(), ptr(top_log_prob), ptr(top_class), *device_and_stream(scores.device)))
     return ClassLogProbs(log_prob, log_norm, entropy, top_log_prob, top_class)
 
 
@@ -144,11 +145,10 @@ def class_log_probs_grad(scores: torch.Tensor, log_norm: torch.Tensor, entropy: 
     grads = [_row_values(name, t, (n,)) for name, t in (("grad_log_prob", grad_log_prob), ("grad_log_norm", grad_log_norm), ("grad_entropy", grad_entropy))]
     one_device(scores=scores, labels=labels, log_norm=log_norm, entropy=entropy, top_class=top_class, grad_log_prob=grads[0], grad_log_norm=grads[1], grad_entropy=grads[2],
                grad_top_log_prob=grad_top_log_prob)
-    log_norm, entropy, grad_top_log_prob, *grads = (None if t is None else t.to(torch.float32).contiguous() for t in (log_norm, entropy, grad_top_log_prob, *grads))
+    log_norm, entropy, grad_top_log_prob, *grads = (None if t is None else (t if t.dtype is torch.float32 else t.float()).contiguous() for t in (log_norm, entropy, grad_top_log_prob, *grads))
     labels, top_class = (None if t is None else t.contiguous() for t in (labels, top_class))
     by_class = scores.stride(0) < scores.stride(1)
-    out = torch.empty((k, n) if by_class else (n, k), dtype=scores.dtype, device=scores.device)
-    out = out.t() if by_class else out
+    out = scores.new_empty((k, n)).t() if by_class else scores.new_empty((n, k))
     if n:
         check(_bwd()(ptr(scores), type_code("scores", scores), n, k, scores.stride(0), scores.stride(1), ptr(labels), 0 if labels is None else 8 * labels.element_size(), top_k,
                      ptr(log_norm), ptr(entropy), ptr(top_class), *map(ptr, grads), ptr(grad_top_log_prob), ptr(out), out.stride(0), out.stride(1), *device_and_stream(scores.device)))
