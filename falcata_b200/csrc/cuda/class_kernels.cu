@@ -240,14 +240,15 @@ __global__ void __launch_bounds__(kFewThreads) ClassLogProbsFewKernel(ClassScore
 }
 
 // -------------------------------------------------------------------------------------------- contiguous rows ----
-// GROUP threads (a warp or a block) walk a row, or a block cluster's share of one, kUnroll 16-byte loads per thread at a time, the
-// next loads (at a row's end: the next row's) in flight while these are worked on. Scores before the first 16-byte boundary and
-// behind the last come one by one.
+// GROUP threads (a warp or a block) walk a row, or a block cluster's share of one, kUnroll 16-byte pieces per thread at a time. The
+// pieces come by asynchronous copies through a ring of kWalkRing chunks, every thread its own pieces, so that a thread waits only for
+// itself; the copies run ahead into the group's next row, which covers the end of a row (sums joined, alternatives found).
+// Scores before the first 16-byte boundary and behind the last come one by one.
 // Alternatives: every thread knows the maximum of the scores that it has seen. With V the top_k-th largest of these maxima, only
 // the threads whose maximum reaches V can hold one of the top_k best scores: about top_k of them, so the group reads only
 // those threads' share of the row again (from L2, 1 / 12 of it for 20 alternatives and 256 threads), lists the scores that
 // reach V and ranks that short list by counting. Nothing is done for the alternatives during the walk itself.
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 4, kWalkRing = 3, kWalkBytes = kWalkRing * kUnroll * 256 * 16;
 struct Entry { float v; int cls; };
 __device__ __forceinline__ bool Before(const Entry& a, const Entry& b) { return a.v > b.v || (a.v == b.v && a.cls < b.cls); }
 // Order of scores as unsigned numbers, -inf 0, zeros of both signs alike; types of 16 bits need fewer.
@@ -338,8 +339,8 @@ struct Alternatives {
     GroupSync<GROUP>();
     return min(count, top_k);
   }
-  // most: this thread's maximum. All threads; the list is complete on return. Not inlined: once per row, and the walk keeps its registers.
-  __device__ __noinline__ int Find(float most, float head_v, float tail_v) {
+  // most: this thread's maximum. All threads; the list is complete on return.
+  __device__ __forceinline__ int Find(float most, float head_v, float tail_v) {
     constexpr int PER = GROUP / 32;
     sh.key[tid] = OrderKey<T>(most);
     GroupSync<GROUP>();
@@ -347,7 +348,16 @@ struct Alternatives {
       unsigned int mine[PER];
 #pragma unroll
       for (int i = 0; i < PER; ++i) mine[i] = sh.key[tid + 32 * i];
-      const unsigned int limit = max(1u, KthLargest<PER>(mine, top_k, KeyBits<T>::kBits));      // key 0: a thread without a score
+      unsigned int limit;
+      if (top_k == 1) {
+        unsigned int best = mine[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) best = max(best, mine[i]);
+        limit = __reduce_max_sync(0xffffffffu, best);
+      } else {
+        limit = KthLargest<PER>(mine, top_k, KeyBits<T>::kBits);
+      }
+      limit = max(1u, limit);      // key 0: a thread without a score
       int n = 0;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -444,13 +454,31 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsRowKernel(ClassScoresArgs
   const long long stride = GROUP == 32 ? static_cast<long long>(gridDim.x) * kGroups : gridDim.x / parts;
   long long row = GROUP == 32 ? static_cast<long long>(blockIdx.x) * kGroups + threadIdx.x / 32 : blockIdx.x / parts;
   if (row >= a.rows) return;                     // whole groups
-  uint4 q[kUnroll], next[kUnroll];
-  auto load = [&](uint4 (&to)[kUnroll], const RowShare<T>& r, int at) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) { const int i = at + u * GROUP + tid; to[u] = i < r.v_end ? __ldg(r.body + i) : AllRuledOut(type); }
-  };
+  extern __shared__ __align__(16) uint4 s_ring[];      // [kWalkRing][kUnroll][256]
+  uint4* mine = s_ring + threadIdx.x;
   RowShare<T> r(a, row, part, parts, GROUP);
-  load(q, r, r.v_begin);
+  // what is copied next
+  long long ahead_row = row;
+  const uint4* ahead_body = r.body; int ahead_at = r.v_begin, ahead_end = r.v_end, ahead_slot = 0;
+  auto copy_ahead = [&]() {
+    if (ahead_row < a.rows) {
+      const unsigned int to = static_cast<unsigned int>(__cvta_generic_to_shared(mine + ahead_slot * (kUnroll * 256)));
+      const uint4* from = ahead_body + ahead_at + tid;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (ahead_at + u * GROUP + tid < ahead_end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * (256 * 16)), "l"(from + u * GROUP) : "memory");
+      ahead_at += GROUP * kUnroll;
+      if (ahead_at >= ahead_end) {
+        ahead_row += stride;
+        if (ahead_row < a.rows) { const RowShare<T> n(a, ahead_row, part, parts, GROUP); ahead_body = n.body; ahead_at = n.v_begin; ahead_end = n.v_end; }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ahead_slot = ahead_slot == kWalkRing - 1 ? 0 : ahead_slot + 1;
+  };
+#pragma unroll
+  for (int i = 0; i < kWalkRing - 1; ++i) copy_ahead();
+  int slot = 0;
   long long y = LabelOf(a, row);
   for (;;) {
     const long long next_row = row + stride;
@@ -460,9 +488,12 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsRowKernel(ClassScoresArgs
     const long long y_next = more ? LabelOf(a, next_row) : -1;
     PairSums<T> pairs;
     int at = r.v_begin;
-    do {                                         // a share without vectors takes one empty step
-      const int then = at + GROUP * kUnroll;
-      if (then < r.v_end) load(next, r, then); else if (more) { const RowShare<T> rn(a, next_row, part, parts, GROUP); load(next, rn, rn.v_begin); }
+    do {                                         // a share without pieces takes one empty step
+      copy_ahead();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kWalkRing - 1) : "memory");
+      uint4 q[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) q[u] = at + u * GROUP + tid < r.v_end ? mine[slot * (kUnroll * 256) + u * 256] : AllRuledOut(type);
       float most = Max(q[0], type);
 #pragma unroll
       for (int u = 1; u < kUnroll; ++u) most = MaxNan(most, Max(q[u], type));
@@ -470,9 +501,8 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsRowKernel(ClassScoresArgs
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
         if (u == 0 || at + u * GROUP + (tid & ~31) < r.v_end) pairs.Add16(q[u]);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) q[u] = next[u];
-      at = then;
+      at += GROUP * kUnroll;
+      slot = slot == kWalkRing - 1 ? 0 : slot + 1;
     } while (at < r.v_end);
     Sums sums = pairs.Total();
     if (head_v != -INFINITY) sums.AddOne(head_v);
@@ -795,11 +825,14 @@ void LaunchFew(const ClassScoresArgs& a, cudaStream_t s) {
 template <typename T, int GROUP, bool TOP>
 void LaunchRows(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
   // as many groups as are resident at once, each with several rows
+  static PerDevice allowed;
+  AllowSharedMemory(ClassLogProbsRowKernel<T, GROUP, TOP>, kWalkBytes, &allowed);
   const long long groups = GROUP == 32 ? (a.rows + 7) / 8 : a.rows, most = static_cast<long long>(kSms) * 4 * (GROUP == 32 ? 2 : 1) / cluster;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned int>(std::min(groups, most) * cluster)); cfg.blockDim = dim3(256); cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cfg.gridDim = dim3(static_cast<unsigned int>(std::min(groups, most) * cluster)); cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = kWalkBytes; cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
   FB_CUDA(cudaLaunchKernelEx(&cfg, ClassLogProbsRowKernel<T, GROUP, TOP>, a));
 }
 template <typename T, int GROUP>
