@@ -33,7 +33,8 @@ namespace {
 
 // log_norm in fp32 gives p to a relative 2^-24 |log_norm|: beyond this size the gradient takes the row's maximum and sum again.
 constexpr float kTrustedLogNorm = 64.f;
-constexpr float kLowestExponent = -200.f;     // e^x is 0 in fp32 from here on; keeps 0 * (-inf) out of T
+constexpr float kLowestExponent = -200.f;     // 2^x is 0 in fp32 from here on; keeps 0 * (-inf) out of T
+constexpr float kLn2 = 0.69314718055994530942f;
 
 __device__ __forceinline__ float ToFloat(float v) { return v; }
 __device__ __forceinline__ float ToFloat(__half v) { return __half2float(v); }
@@ -82,20 +83,29 @@ __device__ __forceinline__ F2 Fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %
 __device__ __forceinline__ float Exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }   // 2 ulp; e^x below is 2^(x log2 e)
 constexpr float kLog2E = 1.44269504088896340736f;
 
-// The running sums of a part of a row, relative to its maximum m (-inf: nothing yet; a NaN or +inf among the scores makes s NaN).
+// Exponents are taken to base 2 against the rounded product B = m log2 e: x_j = s_j log2 e - B is one fused multiply-add. The rounding
+// of B shifts all x alike, and the results are put together from the same x and B, so it drops out (scores far from 0 lose
+// nothing). Where B overflows (|m| > kHugeScore: scores that differ at all differ by more than e^x can hold) x = (s_j - m) log2 e.
+constexpr float kHugeScore = 1e36f;
+__device__ __forceinline__ bool Huge(float m) { return !(fabsf(m) <= kHugeScore); }
+__device__ __forceinline__ float Exponent(float v, float m) { return Huge(m) ? (v - m) * kLog2E : fmaf(v, kLog2E, -(m * kLog2E)); }
+// how much lower the exponents are when the maximum goes from m to `to` (> m)
+__device__ __forceinline__ float Lower(float m, float to) { return fmaxf(Huge(m) || Huge(to) ? (m - to) * kLog2E : __fsub_rn(__fmul_rn(m, kLog2E), __fmul_rn(to, kLog2E)), kLowestExponent); }
+
+// The running sums of a part of a row, relative to its maximum m (-inf: nothing yet; a NaN or +inf among the scores makes s NaN):
+// s = sum 2^x, t = sum 2^x x.
 struct Sums {
   float m = -INFINITY, s = 0.f, t = 0.f;
-  __device__ __forceinline__ static float Down(float by) { return Exp2(by * kLog2E); }
   __device__ __forceinline__ void Raise(float to) {     // to > m
-    const float d = fmaxf(m - to, kLowestExponent), f = Down(d);
+    const float d = Lower(m, to), f = Exp2(d);
     t = (t + s * d) * f; s *= f; m = to;
   }
   __device__ __forceinline__ float Base() const { return m == -INFINITY ? 0.f : m; }
-  __device__ __forceinline__ void Add(float v, float base) { const float x = MaxNan(v - base, kLowestExponent), e = Down(x); s += e; t = fmaf(e, x, t); }
+  __device__ __forceinline__ void Add(float v, float base) { const float x = MaxNan(Exponent(v, base), kLowestExponent), e = Exp2(x); s += e; t = fmaf(e, x, t); }
   __device__ __forceinline__ void AddOne(float v) { if (v > m) Raise(v); Add(v, Base()); }
   __device__ __forceinline__ void Join(float m2, float s2, float t2) {
     if (m2 > m) { const float m1 = m, s1 = s, t1 = t; m = m2; s = s2; t = t2; m2 = m1; s2 = s1; t2 = t1; }
-    const float d = m2 == -INFINITY ? kLowestExponent : fmaxf(m2 - m, kLowestExponent), f = Down(d);
+    const float d = m2 == -INFINITY ? kLowestExponent : m2 == m ? 0.f : Lower(m2, m), f = Exp2(d);
     t += (t2 + s2 * d) * f; s += s2 * f;
   }
   // Over LANES neighbouring lanes: one maximum, one rescaling, then plain sums.
@@ -111,63 +121,83 @@ struct Sums {
   }
 };
 // The same for 16 bytes of scores at a time, two sums side by side.
-// In a pair's product e^x * x a ruled-out score must not give 0 * (-inf): 16-bit scores are lifted to a finite low value first, two
-// per instruction. That is exact as long as the maximum is far above that value; near it (kFar) every score is clamped by itself.
+// In a pair's product 2^x * x a ruled-out score must not give 0 * (-inf): 16-bit scores are lifted to a finite low value first, two
+// per instruction. That is exact as long as the maximum is far above that value; elsewhere every exponent is clamped by itself.
 template <typename T> struct FarBelow;
 template <> struct FarBelow<float> { static constexpr float kFar = INFINITY; };
 template <> struct FarBelow<__half> { static constexpr unsigned int kLow = 0xfbfffbffu; static constexpr float kFar = -60000.f; };               // -65504
-template <> struct FarBelow<__nv_bfloat16> { static constexpr unsigned int kLow = 0xf14af14au; static constexpr float kFar = -1e29f; };          // -1.0e30: the distance to any score stays finite
+template <> struct FarBelow<__nv_bfloat16> { static constexpr unsigned int kLow = 0xf14af14au; static constexpr float kFar = -1e29f; };          // -1.0e30
 template <typename T>
 struct PairSums {
   float m = -INFINITY; F2 s = MakeF2(0.f, 0.f), t = MakeF2(0.f, 0.f);
   __device__ __forceinline__ void Raise(float to) {
-    const float d = fmaxf(m - to, kLowestExponent), f = Sums::Down(d);
+    const float d = Lower(m, to), f = Exp2(d);
     const F2 d2 = MakeF2(d, d), f2 = MakeF2(f, f);
     t = Mul2(Fma2(s, d2, t), f2); s = Mul2(s, f2); m = to;
   }
-  __device__ __forceinline__ void AddPair(float v0, float v1, F2 minus_base) {
-    const F2 x = Add2(MakeF2(v0, v1), minus_base), u = Mul2(x, MakeF2(kLog2E, kLog2E));
-    float u0, u1; Split(u, u0, u1);
-    const F2 e = MakeF2(Exp2(u0), Exp2(u1));
+  __device__ __forceinline__ void AddExponents(F2 x) {
+    float x0, x1; Split(x, x0, x1);
+    const F2 e = MakeF2(Exp2(x0), Exp2(x1));
     s = Add2(s, e); t = Fma2(e, x, t);
   }
-  __device__ __forceinline__ void AddPairClamped(float v0, float v1, float base) {
-    const float x0 = MaxNan(v0 - base, kLowestExponent), x1 = MaxNan(v1 - base, kLowestExponent);
-    const F2 e = MakeF2(Sums::Down(x0), Sums::Down(x1));
-    s = Add2(s, e); t = Fma2(e, MakeF2(x0, x1), t);
-  }
-  __device__ __forceinline__ void Add16(uint4 q) {
+  // COUNT pieces of 16 bytes
+  template <int COUNT>
+  __device__ __forceinline__ void Add16(const uint4 (&all)[COUNT]) {
     constexpr int N = Pack<T>::N;
     const float base = m == -INFINITY ? 0.f : m;
     const T* type = nullptr;
-    float v[N];
     if constexpr (sizeof(T) == 2) {
-      if (base > FarBelow<T>::kFar) {
+      if (base > FarBelow<T>::kFar && base <= kHugeScore) {
         const unsigned int low = FarBelow<T>::kLow;
-        q.x = Max2(q.x, low, type); q.y = Max2(q.y, low, type); q.z = Max2(q.z, low, type); q.w = Max2(q.w, low, type);
-        Unpack(q, v, type);
-        const F2 minus_base = MakeF2(-base, -base);
+        const float minus_b = -(base * kLog2E);
+        const F2 minus_base = MakeF2(minus_b, minus_b), scale = MakeF2(kLog2E, kLog2E);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) AddPair(v[i], v[i + 1], minus_base);
+        for (int u = 0; u < COUNT; ++u) {
+          uint4 q = all[u];
+          q.x = Max2(q.x, low, type); q.y = Max2(q.y, low, type); q.z = Max2(q.z, low, type); q.w = Max2(q.w, low, type);
+          float v[N]; Unpack(q, v, type);
+#pragma unroll
+          for (int i = 0; i < N; i += 2) AddExponents(Fma2(MakeF2(v[i], v[i + 1]), scale, minus_base));
+        }
         return;
       }
     }
-    Unpack(q, v, type);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) AddPairClamped(v[i], v[i + 1], base);
+    for (int u = 0; u < COUNT; ++u) {
+      float v[N]; Unpack(all[u], v, type);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) AddExponents(MakeF2(MaxNan(Exponent(v[i], base), kLowestExponent), MaxNan(Exponent(v[i + 1], base), kLowestExponent)));
+    }
   }
   __device__ __forceinline__ Sums Total() const { Sums r; float a, b; Split(s, a, b); r.s = a + b; Split(t, a, b); r.t = a + b; r.m = m; return r; }
 };
+// The largest of COUNT pieces.
+template <int COUNT, typename T>
+__device__ __forceinline__ float MaxOf(const uint4 (&q)[COUNT], const T* t) {
+  if constexpr (sizeof(T) == 2) {
+    unsigned int w = Max2(Max2(q[0].x, q[0].y, t), Max2(q[0].z, q[0].w, t), t);
+#pragma unroll
+    for (int u = 1; u < COUNT; ++u) w = Max2(w, Max2(Max2(q[u].x, q[u].y, t), Max2(q[u].z, q[u].w, t), t), t);
+    float lo, hi; Unpack2(w, lo, hi, t);
+    return MaxNan(lo, hi);
+  } else {
+    float r = Max(q[0], t);
+#pragma unroll
+    for (int u = 1; u < COUNT; ++u) r = MaxNan(r, Max(q[u], t));
+    return r;
+  }
+}
 
 // The results of a row from its sums.
 struct RowResult {
-  float m, log_sum, entropy; bool none, bad;
+  float m, log_sum, entropy; bool none, bad;      // log_sum: to base 2
   __device__ explicit RowResult(const Sums& r) {
     none = r.m == -INFINITY && !(r.s != r.s); bad = !none && !(fabsf(r.m) < InfF() && r.s < InfF());   // a NaN sum fails the comparison
-    m = r.m; log_sum = logf(r.s); entropy = none ? 0.f : bad ? NanF() : log_sum - r.t / r.s;
+    m = r.m; log_sum = log2f(r.s); entropy = none ? 0.f : bad ? NanF() : fmaxf((log_sum - r.t / r.s) * kLn2, 0.f);
   }
-  __device__ __forceinline__ float LogProb(float v) const { return none ? -INFINITY : bad ? NanF() : (v - m) - log_sum; }
-  __device__ __forceinline__ float LogNorm() const { return none ? -INFINITY : bad ? NanF() : m + log_sum; }
+  __device__ __forceinline__ float LogProb(float v) const { return none || v == -INFINITY ? (bad ? NanF() : -INFINITY) : bad ? NanF() : Huge(m) || Huge(v) ? (v - m) - log_sum * kLn2 : fminf((Exponent(v, m) - log_sum) * kLn2, 0.f); }
+  // m + the rest: what B lacks of m log2 e is put back
+  __device__ __forceinline__ float LogNorm() const { return none ? -INFINITY : bad ? NanF() : m + (log_sum + (Huge(m) ? 0.f : fmaf(-m, kLog2E, __fmul_rn(m, kLog2E)))) * kLn2; }
   __device__ __forceinline__ void Store(const ClassScoresArgs& a, long long row, long long y, float label_score) const {
     a.log_norm[row] = LogNorm(); a.entropy[row] = entropy;
     if (a.log_prob != nullptr) a.log_prob[row] = y < 0 ? 0.f : y >= a.classes ? NanF() : LogProb(label_score);
@@ -464,9 +494,14 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsRowKernel(ClassScoresArgs
     if (ahead_row < a.rows) {
       const unsigned int to = static_cast<unsigned int>(__cvta_generic_to_shared(mine + ahead_slot * (kUnroll * 256)));
       const uint4* from = ahead_body + ahead_at + tid;
+      if (ahead_at + GROUP * kUnroll <= ahead_end) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (ahead_at + u * GROUP + tid < ahead_end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * (256 * 16)), "l"(from + u * GROUP) : "memory");
+        for (int u = 0; u < kUnroll; ++u) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * (256 * 16)), "l"(from + u * GROUP) : "memory");
+      } else {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (ahead_at + u * GROUP + tid < ahead_end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + u * (256 * 16)), "l"(from + u * GROUP) : "memory");
+      }
       ahead_at += GROUP * kUnroll;
       if (ahead_at >= ahead_end) {
         ahead_row += stride;
@@ -492,15 +527,21 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsRowKernel(ClassScoresArgs
       copy_ahead();
       asm volatile("cp.async.wait_group %0;" ::"n"(kWalkRing - 1) : "memory");
       uint4 q[kUnroll];
+      if (at + GROUP * kUnroll <= r.v_end) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) q[u] = at + u * GROUP + tid < r.v_end ? mine[slot * (kUnroll * 256) + u * 256] : AllRuledOut(type);
-      float most = Max(q[0], type);
-#pragma unroll
-      for (int u = 1; u < kUnroll; ++u) most = MaxNan(most, Max(q[u], type));
-      if (most > pairs.m) pairs.Raise(most);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (u == 0 || at + u * GROUP + (tid & ~31) < r.v_end) pairs.Add16(q[u]);
+        for (int u = 0; u < kUnroll; ++u) q[u] = mine[slot * (kUnroll * 256) + u * 256];
+        const float most = MaxOf(q, type);
+        if (most > pairs.m) pairs.Raise(most);
+        pairs.Add16(q);
+      } else {                                   // the last chunk, piece by piece
+#pragma unroll 1
+        for (int u = 0; u < kUnroll && (u == 0 || at + u * GROUP + (tid & ~31) < r.v_end); ++u) {
+          const uint4 one[1] = {at + u * GROUP + tid < r.v_end ? mine[slot * (kUnroll * 256) + u * 256] : AllRuledOut(type)};
+          const float most = MaxOf(one, type);
+          if (most > pairs.m) pairs.Raise(most);
+          pairs.Add16(one);
+        }
+      }
       at += GROUP * kUnroll;
       slot = slot == kWalkRing - 1 ? 0 : slot + 1;
     } while (at < r.v_end);
@@ -660,15 +701,17 @@ struct RowGrad {
     if (none) { a = h = g_label = 0.f; }
     if (bad) a = NanF();
   }
-  __device__ __forceinline__ float Soft(float v) const { const float lp = MaxNan((v - m) - log_sum, kLowestExponent); return __expf(lp) * fmaf(-h, lp, a); }
+  __device__ __forceinline__ float Soft(float v) const { const float lp = MaxNan((v - m) - log_sum, kLowestExponent); return Exp2(lp * kLog2E) * fmaf(-h, lp, a); }
   // with the label's own gradient
   __device__ __forceinline__ float At(float v, int j) const { const float d = Soft(v); return none ? 0.f : j == label ? d + g_label : d; }
+  // log sum e^(s - m), with what B lacks of m log2 e
+  __device__ __forceinline__ static float AgainLog(const Sums& r) { return (log2f(r.s) + (Huge(r.m) ? 0.f : fmaf(-r.m, kLog2E, __fmul_rn(r.m, kLog2E)))) * kLn2; }
   // one thread walks the row
   template <typename T>
   __device__ __forceinline__ void TakeAgain(const ClassScoresArgs& s, const T* row) {
     Sums r;
     for (long long j = 0; j < s.classes; ++j) r.AddOne(ToFloat(row[j * s.class_stride]));
-    m = r.m; log_sum = logf(r.s);
+    m = r.m; log_sum = AgainLog(r);
   }
 };
 // The whole gradient of an alternative's class: an index that is named several times gets all its gradients.
@@ -744,7 +787,7 @@ __global__ void __launch_bounds__(kGradThreads) ClassGradRowKernel(ClassScoresAr
     r.JoinLanes();
     if ((threadIdx.x & 31) == 0) { s_m[threadIdx.x >> 5] = r.m; s_s[threadIdx.x >> 5] = r.s; s_t[threadIdx.x >> 5] = r.t; }
     __syncthreads();
-    if (threadIdx.x == 0) { Sums all; for (int w = 0; w < kGradThreads / 32; ++w) all.Join(s_m[w], s_s[w], s_t[w]); s_row.m = all.m; s_row.log_sum = logf(all.s); }
+    if (threadIdx.x == 0) { Sums all; for (int w = 0; w < kGradThreads / 32; ++w) all.Join(s_m[w], s_s[w], s_t[w]); s_row.m = all.m; s_row.log_sum = RowGrad::AgainLog(all); }
     __syncthreads();
   }
   const RowGrad r = s_row;
