@@ -15,7 +15,8 @@
 // (S, T) are kept relative to a running maximum and rescaled when it grows, so partial results of any split of a row can be
 // joined. Which threads share a row goes by the number of classes and by what is contiguous:
 //   few classes                 a thread per row, the row in registers           (ClassLogProbsFewKernel)
-//   contiguous rows             a warp per row, or a block or cluster per row    (ClassLogProbsRowKernel)
+//   some, contiguous rows       8 lanes per row, the row in their registers      (ClassLogProbsSomeKernel)
+//   contiguous rows             a warp, or a block or cluster of blocks, per row  (ClassLogProbsWarpKernel, ClassLogProbsBlockKernel)
 //   contiguous columns, others  32 rows per block, the classes over its warps    (ClassLogProbsColumnKernel)
 #include "kernels.cuh"
 
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kFewThreads) ClassLogProbsFewKernel(ClassScore
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const long long row = row0 + i * kFewThreads + threadIdx.x;
-    if (row >= a.rows) return;
+    if (row >= a.rows) continue;
     Sums sums;
     float m = v[i][0];
 #pragma unroll
@@ -269,16 +270,58 @@ __global__ void __launch_bounds__(kFewThreads) ClassLogProbsFewKernel(ClassScore
   }
 }
 
+// Rows of up to kSomeClasses contiguous classes: 8 lanes per row, PER scores each in registers. An alternative at a time: the best of a
+// lane's scores, of the 8 lanes', and out of the registers.
+constexpr int kSomeClasses = 256;
+template <typename T, int PER>
+__global__ void __launch_bounds__(128) ClassLogProbsSomeKernel(ClassScoresArgs a) {
+  const int lane8 = threadIdx.x & 7, K = static_cast<int>(a.classes);
+  const long long row = static_cast<long long>(blockIdx.x) * 16 + threadIdx.x / 8;
+  const bool is_row = row < a.rows;               // a warp's lanes stay together
+  const T* s = static_cast<const T*>(a.scores) + (is_row ? row : 0) * a.row_stride;
+  const long long y = is_row ? LabelOf(a, row) : -1;
+  float v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) v[i] = is_row && lane8 + 8 * i < K ? ToFloat(s[lane8 + 8 * i]) : -INFINITY;
+  const float given = lane8 == 0 && y >= 0 && y < K ? ToFloat(s[y]) : 0.f;
+  Sums sums;
+  sums.m = v[0];
+#pragma unroll
+  for (int i = 1; i < PER; ++i) sums.m = MaxNan(sums.m, v[i]);
+  const float b = sums.Base();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sums.Add(v[i], b);
+  sums.JoinLanes<8>();
+  const RowResult res(sums);
+  if (is_row && lane8 == 0) res.Store(a, row, y, given);
+  for (int t = 0; t < a.top_k; ++t) {
+    float best = -INFINITY; int cls = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) if (v[i] > best) { best = v[i]; cls = lane8 + 8 * i; }
+    const int mine = cls;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      const float bo = __shfl_xor_sync(0xffffffffu, best, o); const int co = __shfl_xor_sync(0xffffffffu, cls, o);
+      if (bo > best || (bo == best && co < cls)) { best = bo; cls = co; }
+    }
+    if (mine == cls) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) if (lane8 + 8 * i == cls) v[i] = -INFINITY;
+    }
+    if (is_row && lane8 == 0) res.StoreTop(a, row * a.top_k + t, best, cls);
+  }
+}
+
 // -------------------------------------------------------------------------------------------- contiguous rows ----
-// GROUP threads (a warp or a block) walk a row, or a block cluster's share of one, kUnroll 16-byte pieces per thread at a time. The
-// pieces come by asynchronous copies through a ring of kWalkRing chunks, every thread its own pieces, so that a thread waits only for
-// itself; the copies run ahead into the group's next row, which covers the end of a row (sums joined, alternatives found).
-// Scores before the first 16-byte boundary and behind the last come one by one.
-// Alternatives: every thread knows the maximum of the scores that it has seen. With V the top_k-th largest of these maxima, only
-// the threads whose maximum reaches V can hold one of the top_k best scores: about top_k of them, so the group reads only
-// those threads' share of the row again (from L2, 1 / 12 of it for 20 alternatives and 256 threads), lists the scores that
-// reach V and ranks that short list by counting. Nothing is done for the alternatives during the walk itself.
-constexpr int kUnroll = 4, kWalkRing = 3, kWalkBytes = kWalkRing * kUnroll * 256 * 16;
+// A warp, or 8 warps of a block, walk a row (or a block cluster's share of one), kUnroll 16-byte pieces per thread at a time. The
+// pieces come by asynchronous copies through a ring of chunks, every thread its own pieces, so that a thread waits only for itself;
+// the copies run ahead into the next row, which covers the end of a row. Scores before the first 16-byte boundary and behind
+// the last come one by one.
+// Alternatives: every thread notes the maximum of its pieces, the chunk that held it, and the best that any other of its chunks held.
+// With V the top_k-th largest of these maxima, only the threads whose maximum reaches V can hold one of the top_k best
+// scores: about top_k of them, each mostly with that one score, so little more than one chunk of each is read again (from
+// L2; the whole share where another chunk reaches V too). The scores that reach V are listed and the short list is ranked by counting.
+constexpr int kUnroll = 4;
 struct Entry { float v; int cls; };
 __device__ __forceinline__ bool Before(const Entry& a, const Entry& b) { return a.v > b.v || (a.v == b.v && a.cls < b.cls); }
 // Order of scores as unsigned numbers, -inf 0, zeros of both signs alike; types of 16 bits need fewer.
@@ -291,22 +334,25 @@ __device__ __forceinline__ unsigned int OrderKey(float v) {
   return v == -INFINITY ? 0u : ((u & 0x80000000u) != 0 ? ~u : u | 0x80000000u) >> KeyBits<T>::kShift;
 }
 
-template <int GROUP>
-struct RowShared {
-  static constexpr int kFlagged = 64, kCandidates = GROUP == 32 ? 128 : 512;
-  Entry list[kMaxTopClasses], cand[kCandidates];
-  unsigned int key[GROUP];
-  float part_m[GROUP / 32], part_s[GROUP / 32], part_t[GROUP / 32];
-  int flagged[kFlagged];
-  int num_flagged, num_cand, last, have; unsigned int limit;
-};
+// The score of a key; below the finite scores (key 1: anything but -inf) the lowest finite one.
+template <typename T>
+__device__ __forceinline__ float KeyScore(unsigned int k) {
+  constexpr int kShift = KeyBits<T>::kShift;
+  const bool positive = (k & (1u << (31 - kShift))) != 0;
+  const unsigned int low = kShift > 0 ? (1u << kShift) - 1u : 0u;
+  return fmaxf(__uint_as_float(positive ? (k << kShift) & 0x7fffffffu : ~((k << kShift) | low)), -3.402823466e38f);      // a NaN pattern gives way
+}
 
-template <int GROUP> __device__ __forceinline__ void GroupSync() { if constexpr (GROUP == 32) __syncwarp(); else __syncthreads(); }
-
-// The `rank`-th largest (1-based) of GROUP numbers of `bits` bits, GROUP / 32 per lane: bit by bit, the largest value that at least
-// `rank` numbers reach (0: there are fewer). Run by one warp.
+// The `rank`-th largest (1-based) of PER numbers per lane, of `bits` bits: bit by bit, the largest value that at least `rank` numbers
+// reach (0: there are fewer). Run by one warp.
 template <int PER>
 __device__ __forceinline__ unsigned int KthLargest(const unsigned int (&mine)[PER], int rank, int bits) {
+  if (rank == 1) {
+    unsigned int best = mine[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) best = max(best, mine[i]);
+    return __reduce_max_sync(0xffffffffu, best);
+  }
   unsigned int found = 0u;
   for (int bit = bits - 1; bit >= 0; --bit) {
     const unsigned int probe = found | (1u << bit);
@@ -322,7 +368,7 @@ __device__ __forceinline__ unsigned int KthLargest(const unsigned int (&mine)[PE
   return found;
 }
 
-// A group's share of a row.
+// A share of a row: part `part` of `parts`, of whole rounds of `group` threads.
 template <typename T>
 struct RowShare {
   const T* s; const uint4* body; int K, head, tail, v_begin, v_end; bool first, last_part;
@@ -332,165 +378,27 @@ struct RowShare {
     head = min(K, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(s) & 15)) & 15) / static_cast<int>(sizeof(T)));
     const int vectors = (K - head) / N;
     tail = head + vectors * N; body = reinterpret_cast<const uint4*>(s + head);
-    const int each = ((vectors + parts - 1) / parts + group - 1) / group * group;      // whole rounds of the group
+    const int each = ((vectors + parts - 1) / parts + group - 1) / group * group;
     v_begin = min(vectors, part * each); v_end = min(vectors, v_begin + each);
     first = part == 0; last_part = part == parts - 1;
   }
+  // the scores outside the 16-byte pieces, one per thread (-inf: none)
+  __device__ __forceinline__ float Head(int tid) const { return first && tid < head ? ToFloat(s[tid]) : -INFINITY; }
+  __device__ __forceinline__ float Tail(int tid) const { return last_part && tid < K - tail ? ToFloat(s[tail + tid]) : -INFINITY; }
 };
 
-template <int GROUP, typename T>
-struct Alternatives {
-  static constexpr int N = Pack<T>::N;
-  RowShared<GROUP>& sh; const RowShare<T>& r; int top_k, tid;
-  // f(score, class) for the scores of the flagged threads and the ends of the row, dealt out over the group
-  template <typename F>
-  __device__ __forceinline__ void Scores(int num_flagged, float head_v, float tail_v, F&& f) const {
-    if (r.first && tid < r.head) f(head_v, tid);
-    if (r.last_part && tid < r.K - r.tail) f(tail_v, r.tail + tid);
-    const int rounds = (r.v_end - r.v_begin + GROUP - 1) / GROUP;
-    for (int e = tid; e < num_flagged * rounds; e += GROUP) {
-      const int i = r.v_begin + (e / num_flagged) * GROUP + sh.flagged[e % num_flagged];
-      if (i >= r.v_end) continue;
-      const uint4 q = __ldg(r.body + i);
-      float v[N];
-      Unpack(q, v, static_cast<const T*>(nullptr));
+// The walk of GROUP threads through the rows row, row + stride, ... with RING chunks of shared memory per thread.
+template <typename T, int GROUP, int RING>
+struct Walk {
+  const ClassScoresArgs& a; uint4* mine; long long stride; int tid, part, parts, slot, ahead_slot, ahead_at, ahead_end; long long ahead_row; const uint4* ahead_body;
+  __device__ __forceinline__ Walk(const ClassScoresArgs& args, uint4* ring, long long row, long long stride_, int tid_, int part_, int parts_) : a(args) {
+    mine = ring + threadIdx.x; stride = stride_; tid = tid_; part = part_; parts = parts_; slot = ahead_slot = 0; ahead_row = row;
+    const RowShare<T> r(a, row, part, parts, GROUP);
+    ahead_body = r.body; ahead_at = r.v_begin; ahead_end = r.v_end;
 #pragma unroll
-      for (int k = 0; k < N; ++k) f(v[k], r.head + i * N + k);
-    }
+    for (int i = 0; i < RING - 1; ++i) CopyAhead();
   }
-  // Ranks the first `count` candidates into the list; returns how many that leaves.
-  __device__ __forceinline__ int Rank(int count) {
-    for (int i = tid; i < count; i += GROUP) {
-      const Entry e = sh.cand[i];
-      int rank = 0;
-      for (int j = 0; j < count; ++j) rank += Before(sh.cand[j], e) ? 1 : 0;
-      if (rank < top_k) sh.list[rank] = e;
-    }
-    GroupSync<GROUP>();
-    return min(count, top_k);
-  }
-  // most: this thread's maximum. All threads; the list is complete on return.
-  __device__ __forceinline__ int Find(float most, float head_v, float tail_v) {
-    constexpr int PER = GROUP / 32;
-    sh.key[tid] = OrderKey<T>(most);
-    GroupSync<GROUP>();
-    if (tid < 32) {
-      unsigned int mine[PER];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) mine[i] = sh.key[tid + 32 * i];
-      unsigned int limit;
-      if (top_k == 1) {
-        unsigned int best = mine[0];
-#pragma unroll
-        for (int i = 1; i < PER; ++i) best = max(best, mine[i]);
-        limit = __reduce_max_sync(0xffffffffu, best);
-      } else {
-        limit = KthLargest<PER>(mine, top_k, KeyBits<T>::kBits);
-      }
-      limit = max(1u, limit);      // key 0: a thread without a score
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const unsigned int in = __ballot_sync(0xffffffffu, mine[i] >= limit);
-        const int at = n + __popc(in & ((1u << tid) - 1u));
-        if (mine[i] >= limit && at < RowShared<GROUP>::kFlagged) sh.flagged[at] = tid + 32 * i;
-        n += __popc(in);
-      }
-      if (tid == 0) { sh.limit = limit; sh.num_flagged = n; sh.num_cand = 0; sh.last = 0x7fffffff; }
-    }
-    GroupSync<GROUP>();
-    const unsigned int limit = sh.limit;
-    if (GROUP > 32 && sh.num_flagged > RowShared<GROUP>::kFlagged) Ties(limit);
-    const int last = sh.last, num_flagged = sh.num_flagged;
-    Scores(num_flagged, head_v, tail_v, [&](float v, int cls) {
-      const unsigned int k = OrderKey<T>(v);
-      if (k > limit || (k == limit && cls <= last)) { const int at = atomicAdd(&sh.num_cand, 1); if (at < RowShared<GROUP>::kCandidates) { sh.cand[at].v = v; sh.cand[at].cls = cls; } }
-    });
-    GroupSync<GROUP>();
-    const int count = sh.num_cand;
-    if (count <= RowShared<GROUP>::kCandidates) return Rank(count);
-    return OneByOne(num_flagged, head_v, tail_v);
-  }
-  // Very many equal maxima: of the threads with maximum `limit` only those count that reach it at the lowest classes.
-  __device__ void Ties(unsigned int limit) {
-    constexpr int PER = GROUP / 32;
-    unsigned int order = 0u;
-    const unsigned int mine = sh.key[tid];
-    if (mine == limit) {
-      int at = 0x7fffffff;
-      if (r.first && tid < r.head && OrderKey<T>(ToFloat(r.s[tid])) == limit) at = tid;
-      for (int i = r.v_begin + tid; i < r.v_end && at == 0x7fffffff; i += GROUP) {
-        float v[N];
-        Unpack(__ldg(r.body + i), v, static_cast<const T*>(nullptr));
-#pragma unroll
-        for (int k = N - 1; k >= 0; --k) if (OrderKey<T>(v[k]) == limit) at = r.head + i * N + k;
-      }
-      if (at == 0x7fffffff) at = r.tail + tid;      // its last score
-      order = 0x80000000u - static_cast<unsigned int>(at);
-    }
-    const int higher = __syncthreads_count(mine > limit);
-    sh.key[tid] = order;
-    const bool above = mine > limit;
-    if (tid == 0) sh.num_flagged = 0;
-    __syncthreads();
-    if (tid < 32) {
-      unsigned int all[PER];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) all[i] = sh.key[tid + 32 * i];
-      const unsigned int kth = KthLargest<PER>(all, top_k - higher, 32);
-      if (tid == 0) sh.last = static_cast<int>(0x80000000u - kth);
-    }
-    __syncthreads();
-    if (above || (mine == limit && order >= 0x80000000u - static_cast<unsigned int>(sh.last))) sh.flagged[atomicAdd(&sh.num_flagged, 1)] = tid;
-    __syncthreads();
-  }
-  // More candidates than the list holds (few threads own very many of the best scores): one alternative per pass.
-  __device__ int OneByOne(int num_flagged, float head_v, float tail_v) {
-    Entry before; before.v = INFINITY; before.cls = -1;
-    int t = 0;
-    for (; t < top_k; ++t) {
-      Entry best; best.v = -INFINITY; best.cls = 0x7fffffff;
-      Scores(num_flagged, head_v, tail_v, [&](float v, int cls) { Entry e; e.v = v; e.cls = cls; if (v > -INFINITY && Before(before, e) && Before(e, best)) best = e; });
-      for (int o = 16; o > 0; o >>= 1) {
-        Entry e; e.v = __shfl_xor_sync(0xffffffffu, best.v, o); e.cls = __shfl_xor_sync(0xffffffffu, best.cls, o);
-        if (Before(e, best)) best = e;
-      }
-      if constexpr (GROUP > 32) {
-        if ((tid & 31) == 0) sh.cand[tid >> 5] = best;
-        __syncthreads();
-        best = sh.cand[0];
-        for (int w = 1; w < GROUP / 32; ++w) if (Before(sh.cand[w], best)) best = sh.cand[w];
-        __syncthreads();
-      }
-      if (best.cls == 0x7fffffff) break;
-      if (tid == 0) sh.list[t] = best;
-      before = best;
-    }
-    GroupSync<GROUP>();
-    return t;
-  }
-};
-
-// TOP: alternatives are wanted. Groups walk the rows with the grid's stride; a row belongs to a warp, a block or a cluster.
-template <typename T, int GROUP, bool TOP>
-__global__ void __launch_bounds__(256, 4) ClassLogProbsRowKernel(ClassScoresArgs a) {
-  constexpr int kGroups = 256 / GROUP;
-  __shared__ RowShared<GROUP> s_all[TOP ? kGroups : 1];
-  __shared__ float s_m[8], s_s[8], s_t[8];
-  RowShared<GROUP>& sh = s_all[TOP && GROUP == 32 ? threadIdx.x / 32 : 0];
-  const int tid = threadIdx.x % GROUP;
-  const T* type = nullptr;
-  const int parts = GROUP == 32 ? 1 : static_cast<int>(cg::this_cluster().num_blocks()), part = GROUP == 32 ? 0 : static_cast<int>(cg::this_cluster().block_rank());
-  const long long stride = GROUP == 32 ? static_cast<long long>(gridDim.x) * kGroups : gridDim.x / parts;
-  long long row = GROUP == 32 ? static_cast<long long>(blockIdx.x) * kGroups + threadIdx.x / 32 : blockIdx.x / parts;
-  if (row >= a.rows) return;                     // whole groups
-  extern __shared__ __align__(16) uint4 s_ring[];      // [kWalkRing][kUnroll][256]
-  uint4* mine = s_ring + threadIdx.x;
-  RowShare<T> r(a, row, part, parts, GROUP);
-  // what is copied next
-  long long ahead_row = row;
-  const uint4* ahead_body = r.body; int ahead_at = r.v_begin, ahead_end = r.v_end, ahead_slot = 0;
-  auto copy_ahead = [&]() {
+  __device__ __forceinline__ void CopyAhead() {
     if (ahead_row < a.rows) {
       const unsigned int to = static_cast<unsigned int>(__cvta_generic_to_shared(mine + ahead_slot * (kUnroll * 256)));
       const uint4* from = ahead_body + ahead_at + tid;
@@ -509,112 +417,323 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsRowKernel(ClassScoresArgs
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    ahead_slot = ahead_slot == kWalkRing - 1 ? 0 : ahead_slot + 1;
-  };
-#pragma unroll
-  for (int i = 0; i < kWalkRing - 1; ++i) copy_ahead();
-  int slot = 0;
-  long long y = LabelOf(a, row);
-  for (;;) {
-    const long long next_row = row + stride;
-    const bool more = next_row < a.rows;
-    const float head_v = r.first && tid < r.head ? ToFloat(r.s[tid]) : -INFINITY, tail_v = r.last_part && tid < r.K - r.tail ? ToFloat(r.s[r.tail + tid]) : -INFINITY;
-    const float given = tid == 0 && y >= 0 && y < r.K ? ToFloat(r.s[y]) : 0.f;
-    const long long y_next = more ? LabelOf(a, next_row) : -1;
+    ahead_slot = ahead_slot == RING - 1 ? 0 : ahead_slot + 1;
+  }
+  // the chunk (its first piece) that held this thread's maximum, and the best of the others
+  int best_at; float second;
+  // This thread's sums of the pieces of the next row's share; m is its maximum.
+  __device__ __forceinline__ Sums Row(const RowShare<T>& r) {
+    const T* type = nullptr;
     PairSums<T> pairs;
     int at = r.v_begin;
+    best_at = at; second = -INFINITY;
     do {                                         // a share without pieces takes one empty step
-      copy_ahead();
-      asm volatile("cp.async.wait_group %0;" ::"n"(kWalkRing - 1) : "memory");
-      uint4 q[kUnroll];
-      if (at + GROUP * kUnroll <= r.v_end) {
+      CopyAhead();
+      asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+      const uint4* from = mine + slot * (kUnroll * 256);
+      if (GROUP == 32 || at + GROUP * kUnroll <= r.v_end) {
+        uint4 q[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) q[u] = mine[slot * (kUnroll * 256) + u * 256];
+        for (int u = 0; u < kUnroll; ++u) q[u] = GROUP > 32 || at + u * GROUP + tid < r.v_end ? from[u * 256] : AllRuledOut(type);
         const float most = MaxOf(q, type);
-        if (most > pairs.m) pairs.Raise(most);
+        if (most > pairs.m) { second = pairs.m; best_at = at; pairs.Raise(most); } else second = fmaxf(second, most);
         pairs.Add16(q);
       } else {                                   // the last chunk, piece by piece
+        const float before = pairs.m;
+        float most = -INFINITY;
 #pragma unroll 1
         for (int u = 0; u < kUnroll && (u == 0 || at + u * GROUP + (tid & ~31) < r.v_end); ++u) {
-          const uint4 one[1] = {at + u * GROUP + tid < r.v_end ? mine[slot * (kUnroll * 256) + u * 256] : AllRuledOut(type)};
-          const float most = MaxOf(one, type);
-          if (most > pairs.m) pairs.Raise(most);
+          const uint4 one[1] = {at + u * GROUP + tid < r.v_end ? from[u * 256] : AllRuledOut(type)};
+          const float here = MaxOf(one, type);
+          most = fmaxf(most, here);
+          if (here > pairs.m) pairs.Raise(here);
           pairs.Add16(one);
         }
+        if (most > before) { second = before; best_at = at; } else second = fmaxf(second, most);
       }
       at += GROUP * kUnroll;
-      slot = slot == kWalkRing - 1 ? 0 : slot + 1;
+      slot = slot == RING - 1 ? 0 : slot + 1;
     } while (at < r.v_end);
-    Sums sums = pairs.Total();
+    return pairs.Total();
+  }
+};
+
+// One warp finds the alternatives of a share that GROUP threads have walked.
+template <int GROUP>
+struct TopShared {
+  static constexpr int kFlagged = 64, kCandidates = GROUP == 32 ? 128 : 512;
+  Entry list[kMaxTopClasses], cand[kCandidates];
+  int flagged[kFlagged], flagged_at[kFlagged], num_flagged, num_cand;      // threads; the chunk to look at (-1: all of the thread's share)
+};
+template <int GROUP, typename T>
+struct Alternatives {
+  static constexpr int N = Pack<T>::N, PER = GROUP / 32;
+  TopShared<GROUP>& sh; const RowShare<T>& r; int top_k, lane;
+  // f(score, class) for the scores that reach `limit` among piece `at` of the share (each lane its own; at >= v_end: none)
+  template <int COUNT, typename F>
+  __device__ __forceinline__ void Pieces(const int (&at)[COUNT], float limit, F&& f) const {
+    uint4 q[COUNT];
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u) q[u] = at[u] < r.v_end ? __ldg(r.body + at[u]) : AllRuledOut(static_cast<const T*>(nullptr));
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u) {
+      const uint4 one[1] = {q[u]};
+      if (!(MaxOf(one, static_cast<const T*>(nullptr)) >= limit)) continue;
+      float v[N];
+      Unpack(q[u], v, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int k = 0; k < N; ++k) if (v[k] >= limit) f(v[k], r.head + at[u] * N + k);
+    }
+  }
+  // the same for what the flagged threads have to look at, and for the ends of the row
+  template <typename F>
+  __device__ __forceinline__ void Scores(int num_flagged, float limit, F&& f) const {
+    const float head_v = r.Head(lane), tail_v = r.Tail(lane);
+    if (head_v >= limit) f(head_v, lane);
+    if (tail_v >= limit) f(tail_v, r.tail + lane);
+    static_assert(kUnroll == 4, "a chunk is 4 pieces of a thread");
+    for (int e0 = lane; e0 < 4 * num_flagged; e0 += 128) {
+      int at[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = e0 + 32 * u, which = e >> 2;
+        const int chunk = which < num_flagged ? sh.flagged_at[which] : -1;
+        at[u] = chunk >= 0 ? chunk + (e & 3) * GROUP + sh.flagged[which] : 0x7fffffff;
+      }
+      Pieces(at, limit, f);
+    }
+    for (int which = 0; which < num_flagged; ++which) {
+      if (sh.flagged_at[which] >= 0) continue;
+      for (int p = r.v_begin + sh.flagged[which] + lane * GROUP; p < r.v_end; p += 32 * GROUP * 2) {
+        const int at[2] = {p, p + 32 * GROUP};
+        Pieces(at, limit, f);
+      }
+    }
+  }
+  // Ranks the first `count` candidates into the list; returns how many that leaves.
+  __device__ __forceinline__ int Rank(int count) {
+    for (int i = lane; i < count; i += 32) {
+      const Entry e = sh.cand[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += Before(sh.cand[j], e) ? 1 : 0;
+      if (rank < top_k) sh.list[rank] = e;
+    }
+    __syncwarp();
+    return min(count, top_k);
+  }
+  // Of the threads lane, lane + 32, ...: OrderKeys of their maxima and of the best of their other chunks, and the chunk of the maximum.
+  // Returns the number of alternatives found, in the list.
+  __device__ __forceinline__ int Find(const unsigned int (&keys)[PER], const unsigned int (&second)[PER], const int (&chunk)[PER]) {
+    const unsigned int limit = max(1u, KthLargest<PER>(keys, top_k, KeyBits<T>::kBits));      // key 0: a thread without a score
+    int flagged = 0, last = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const unsigned int in = __ballot_sync(0xffffffffu, keys[i] >= limit);
+      const int at = flagged + __popc(in & ((1u << lane) - 1u));
+      if (keys[i] >= limit && at < TopShared<GROUP>::kFlagged) { sh.flagged[at] = lane + 32 * i; sh.flagged_at[at] = second[i] >= limit ? -1 : chunk[i]; }
+      flagged += __popc(in);
+    }
+    if (lane == 0) sh.num_cand = 0;
+    __syncwarp();
+    if (GROUP > 32 && flagged > TopShared<GROUP>::kFlagged) flagged = Ties(keys, limit, &last);
+    const float limit_score = KeyScore<T>(limit);
+    Scores(flagged, limit_score, [&](float v, int cls) {
+      if (v > limit_score || cls <= last) { const int at = atomicAdd(&sh.num_cand, 1); if (at < TopShared<GROUP>::kCandidates) { sh.cand[at].v = v; sh.cand[at].cls = cls; } }
+    });
+    __syncwarp();
+    const int count = sh.num_cand;
+    return count <= TopShared<GROUP>::kCandidates ? Rank(count) : OneByOne(flagged, limit_score);
+  }
+  // Very many equal maxima: of the threads with maximum `limit` only those count that reach it at the lowest classes. *last: the
+  // highest of these classes.
+  __device__ __noinline__ int Ties(const unsigned int (&keys)[PER], unsigned int limit, int* last) {
+    unsigned int order[PER];
+    int higher = 0;
+    for (int i = 0; i < PER; ++i) {
+      order[i] = 0u;
+      higher += keys[i] > limit ? 1 : 0;
+      if (keys[i] != limit) continue;
+      const int thread = lane + 32 * i;
+      int at = 0x7fffffff;
+      for (int p = r.v_begin + thread; p < r.v_end && at == 0x7fffffff; p += GROUP) {
+        float v[N];
+        Unpack(__ldg(r.body + p), v, static_cast<const T*>(nullptr));
+#pragma unroll
+        for (int k = N - 1; k >= 0; --k) if (OrderKey<T>(v[k]) == limit) at = r.head + p * N + k;
+      }
+      order[i] = 0x80000000u - static_cast<unsigned int>(at);
+    }
+    higher = __reduce_add_sync(0xffffffffu, higher);
+    const unsigned int kth = KthLargest<PER>(order, top_k - higher, 32);
+    *last = static_cast<int>(0x80000000u - kth);
+    if (lane == 0) sh.num_flagged = 0;
+    __syncwarp();
+    for (int i = 0; i < PER; ++i) if (keys[i] > limit || order[i] >= kth) { const int at = atomicAdd(&sh.num_flagged, 1); sh.flagged[at] = lane + 32 * i; sh.flagged_at[at] = -1; }
+    __syncwarp();
+    return sh.num_flagged;
+  }
+  // More candidates than the list holds (few threads own very many of the best scores): one alternative per pass.
+  __device__ __noinline__ int OneByOne(int num_flagged, float limit) {
+    Entry before; before.v = INFINITY; before.cls = -1;
+    int t = 0;
+    for (; t < top_k; ++t) {
+      Entry best; best.v = -INFINITY; best.cls = 0x7fffffff;
+      Scores(num_flagged, limit, [&](float v, int cls) { Entry e; e.v = v; e.cls = cls; if (v > -INFINITY && Before(before, e) && Before(e, best)) best = e; });
+      for (int o = 16; o > 0; o >>= 1) {
+        Entry e; e.v = __shfl_xor_sync(0xffffffffu, best.v, o); e.cls = __shfl_xor_sync(0xffffffffu, best.cls, o);
+        if (Before(e, best)) best = e;
+      }
+      if (best.cls == 0x7fffffff) break;
+      if (lane == 0) sh.list[t] = best;
+      before = best;
+    }
+    __syncwarp();
+    return t;
+  }
+};
+
+// A warp per row, 8 warps per block, each walking rows with the grid's stride. TOP: alternatives are wanted.
+constexpr int kWarpRing = 3;
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(256, 4) ClassLogProbsWarpKernel(ClassScoresArgs a) {
+  extern __shared__ __align__(16) uint4 s_ring[];      // [kWarpRing][kUnroll][256]
+  __shared__ TopShared<32> s_top[TOP ? 8 : 1];
+  const int lane = threadIdx.x % 32;
+  const long long stride = static_cast<long long>(gridDim.x) * 8;
+  long long row = static_cast<long long>(blockIdx.x) * 8 + threadIdx.x / 32;
+  if (row >= a.rows) return;                     // whole warps
+  Walk<T, 32, kWarpRing> walk(a, s_ring, row, stride, lane, 0, 1);
+  long long y = LabelOf(a, row);
+  for (; row < a.rows; row += stride) {
+    const RowShare<T> r(a, row, 0, 1, 32);
+    const float head_v = r.Head(lane), tail_v = r.Tail(lane), given = lane == 0 && y >= 0 && y < r.K ? ToFloat(r.s[y]) : 0.f;
+    const long long y_next = row + stride < a.rows ? LabelOf(a, row + stride) : -1;
+    Sums sums = walk.Row(r);
+    const float most = sums.m;
     if (head_v != -INFINITY) sums.AddOne(head_v);
     if (tail_v != -INFINITY) sums.AddOne(tail_v);
-    const float most = sums.m;
     sums.JoinLanes();
-    if constexpr (GROUP == 32) {
-      const RowResult res(sums);
-      if (tid == 0) res.Store(a, row, y, given);
-      if constexpr (TOP) {
-        Alternatives<GROUP, T> alt{sh, r, a.top_k, tid};
-        const int have = alt.Find(most, head_v, tail_v);
-        if (tid < a.top_k) { const Entry e = sh.list[tid]; res.StoreTop(a, row * a.top_k + tid, tid < have ? e.v : -INFINITY, e.cls); }
-        __syncwarp();
-      }
-    } else {
-      if ((tid & 31) == 0) { s_m[tid >> 5] = sums.m; s_s[tid >> 5] = sums.s; s_t[tid >> 5] = sums.t; }
-      int have = 0;
-      if constexpr (TOP) { Alternatives<GROUP, T> alt{sh, r, a.top_k, tid}; have = alt.Find(most, head_v, tail_v); } else __syncthreads();
-      if (tid < 32) {
-        sums = Sums();
-        if (tid < GROUP / 32) { sums.m = s_m[tid]; sums.s = s_s[tid]; sums.t = s_t[tid]; }
-        sums.JoinLanes();
-      }
-      if (parts > 1) {
-        // the cluster's first block joins the others' sums and lists, read from their shared memory
-        __syncthreads();
-        if (tid == 0) { s_m[0] = sums.m; s_s[0] = sums.s; s_t[0] = sums.t; if constexpr (TOP) sh.have = have; }
-        cg::this_cluster().sync();
-        if (part == 0) {
-          int count = have;
-          if constexpr (TOP) { if (tid < have) sh.cand[tid] = sh.list[tid]; if (tid == 0) { sh.flagged[0] = 0; sh.flagged[1] = have; } }
-          for (int p = 1; p < parts; ++p) {
-            if (tid < 32) sums.Join(*cg::this_cluster().map_shared_rank(&s_m[0], p), *cg::this_cluster().map_shared_rank(&s_s[0], p), *cg::this_cluster().map_shared_rank(&s_t[0], p));
-            if constexpr (TOP) {
-              const RowShared<GROUP>* o = cg::this_cluster().map_shared_rank(&sh, p);
-              const int n = o->have;
-              if (tid < n) sh.cand[count + tid] = o->list[tid];
-              count += n;
-              if (tid == 0) sh.flagged[p + 1] = count;
-            }
-          }
-          if constexpr (TOP) {
-            // the lists are sorted: an entry's rank is its place in its own list and, by bisection, how many of each other come before it
-            __syncthreads();
-            if (tid < count) {
-              const Entry e = sh.cand[tid];
-              int rank = 0;
-              for (int p = 0; p < parts; ++p) {
-                const int begin = sh.flagged[p];
-                int lo = begin, hi = sh.flagged[p + 1];
-                while (lo < hi) { const int mid = (lo + hi) >> 1; if (Before(sh.cand[mid], e)) lo = mid + 1; else hi = mid; }
-                rank += lo - begin;
-              }
-              if (rank < a.top_k) sh.list[rank] = e;
-            }
-            __syncthreads();
-            have = min(count, a.top_k);
-          }
-        }
-        cg::this_cluster().sync();         // no block goes on while its shared memory is read
-      }
-      if (part == 0 && tid < 32) {
-        const RowResult res(sums);
-        if (tid == 0) res.Store(a, row, y, given);
-        if constexpr (TOP) if (tid < a.top_k) { const Entry e = sh.list[tid]; res.StoreTop(a, row * a.top_k + tid, tid < have ? e.v : -INFINITY, e.cls); }
-      }
-      __syncthreads();                     // the next row writes the shared parts again
+    const RowResult res(sums);
+    if (lane == 0) res.Store(a, row, y, given);
+    if constexpr (TOP) {
+      Alternatives<32, T> alt{s_top[threadIdx.x / 32], r, a.top_k, lane};
+      const unsigned int keys[1] = {OrderKey<T>(most)}, second[1] = {OrderKey<T>(walk.second)};
+      const int chunk[1] = {walk.best_at}, have = alt.Find(keys, second, chunk);
+      if (lane < a.top_k) { const Entry e = alt.sh.list[lane]; res.StoreTop(a, row * a.top_k + lane, lane < have ? e.v : -INFINITY, e.cls); }
+      __syncwarp();
     }
-    if (!more) return;
-    row = next_row; r = RowShare<T>(a, row, part, parts, GROUP); y = y_next;
+    y = y_next;
+  }
+}
+
+// 8 warps walk a row (with a cluster of blocks: a share of it), a ninth joins their sums, finds the alternatives and writes the results
+// while they are in the next row. Two sets
+// of hand-over buffers; named barriers kFull + set (walkers arrive, the ninth waits) and kFree + set (the other way round).
+constexpr int kBlockRing = 4, kBlockThreads = 288;
+enum { kFull = 1, kFree = 3 };
+template <int ID0> __device__ __forceinline__ void BarrierSync(int set) { asm volatile("bar.sync %0, %1;" ::"r"(ID0 + set), "n"(kBlockThreads) : "memory"); }
+template <int ID0> __device__ __forceinline__ void BarrierArrive(int set) { asm volatile("bar.arrive %0, %1;" ::"r"(ID0 + set), "n"(kBlockThreads) : "memory"); }
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kBlockThreads, 3) ClassLogProbsBlockKernel(ClassScoresArgs a) {
+  extern __shared__ __align__(16) uint4 s_ring[];      // [kBlockRing][kUnroll][256]
+  __shared__ TopShared<256> s_top[1];
+  __shared__ unsigned int s_key[2][256], s_second[2][256]; __shared__ int s_chunk[2][256];
+  __shared__ float s_m[2][8], s_s[2][8], s_t[2][8];
+  __shared__ float s_share[3]; __shared__ int s_have;                  // of a cluster's block: its share's sums and number of alternatives
+  __shared__ Entry s_join[8][kMaxTopClasses], s_joined[kMaxTopClasses]; __shared__ int s_count[8];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int parts = static_cast<int>(cg::this_cluster().num_blocks()), part = static_cast<int>(cg::this_cluster().block_rank());
+  const long long stride = gridDim.x / parts, row0 = blockIdx.x / parts;      // the grid has no more clusters than rows
+  int set = 0;
+  if (warp < 8) {
+    Walk<T, 256, kBlockRing> walk(a, s_ring, row0, stride, threadIdx.x, part, parts);
+    for (long long row = row0; row < a.rows; row += stride, set ^= 1) {
+      const RowShare<T> r(a, row, part, parts, 256);
+      const float head_v = r.Head(threadIdx.x), tail_v = r.Tail(threadIdx.x);
+      Sums sums = walk.Row(r);
+      const float most = sums.m;
+      if (head_v != -INFINITY) sums.AddOne(head_v);
+      if (tail_v != -INFINITY) sums.AddOne(tail_v);
+      sums.JoinLanes();
+      if (row >= row0 + 2 * stride) BarrierSync<kFree>(set);
+      if constexpr (TOP) { s_key[set][threadIdx.x] = OrderKey<T>(most); s_second[set][threadIdx.x] = OrderKey<T>(walk.second); s_chunk[set][threadIdx.x] = walk.best_at; }
+      if (lane == 0) { s_m[set][warp] = sums.m; s_s[set][warp] = sums.s; s_t[set][warp] = sums.t; }
+      BarrierArrive<kFull>(set);
+      if (parts > 1) {
+        // the first block joins the lists of all, read from their shared memory: warp w has block w's list, lane i its entry i. The lists
+        // are sorted, so an entry's rank is, list by list and by bisection, how many come before it.
+        cg::this_cluster().sync();
+        if (TOP && part == 0) {
+          int n = 0;
+          Entry e; e.v = -INFINITY; e.cls = 0x7fffffff;
+          if (warp < parts) {
+            n = *cg::this_cluster().map_shared_rank(&s_have, warp);
+            e = cg::this_cluster().map_shared_rank(&s_top[0], warp)->list[lane];      // beyond n: not an entry
+            s_join[warp][lane] = e;
+          }
+          if (lane == 0) s_count[warp] = n;
+          asm volatile("bar.sync 5, 256;" ::: "memory");
+          if (lane < n) {
+            int rank = 0;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+              const int m = s_count[p];
+              int before = 0;
+#pragma unroll
+              for (int step = 32; step > 0; step >>= 1) if (before + step <= m && Before(s_join[p][before + step - 1], e)) before += step;
+              rank += before;
+            }
+            if (rank < a.top_k) s_joined[rank] = e;
+          }
+          asm volatile("bar.sync 6, 288;" ::: "memory");
+        }
+        cg::this_cluster().sync();
+      }
+    }
+    return;
+  }
+  long long y = LabelOf(a, row0);
+  for (long long row = row0; row < a.rows; row += stride, set ^= 1) {
+    const RowShare<T> r(a, row, part, parts, 256);
+    const float given = lane == 0 && y >= 0 && y < r.K ? ToFloat(r.s[y]) : 0.f;
+    const long long y_next = row + stride < a.rows ? LabelOf(a, row + stride) : -1;
+    Alternatives<256, T> alt{s_top[0], r, a.top_k, lane};
+    BarrierSync<kFull>(set);
+    Sums sums;
+    if (lane < 8) { sums.m = s_m[set][lane]; sums.s = s_s[set][lane]; sums.t = s_t[set][lane]; }
+    sums.JoinLanes();
+    int have = 0;
+    if constexpr (TOP) {
+      unsigned int keys[8], second[8]; int chunk[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { keys[i] = s_key[set][lane + 32 * i]; second[i] = s_second[set][lane + 32 * i]; chunk[i] = s_chunk[set][lane + 32 * i]; }
+      have = alt.Find(keys, second, chunk);
+    }
+    if (row + 2 * stride < a.rows) BarrierArrive<kFree>(set);
+    if (parts > 1) {
+      if (lane == 0) { s_share[0] = sums.m; s_share[1] = sums.s; s_share[2] = sums.t; s_have = have; }
+      cg::this_cluster().sync();
+      if (part == 0) {
+        Sums other;
+        if (lane < parts) { const float* o = cg::this_cluster().map_shared_rank(&s_share[0], lane); other.m = o[0]; other.s = o[1]; other.t = o[2]; }
+        other.JoinLanes();
+        sums = other;
+        if constexpr (TOP) {
+          asm volatile("bar.sync 6, 288;" ::: "memory");      // the walkers have joined the lists
+          have = 0;
+          for (int p = 0; p < 8; ++p) have += s_count[p];
+          have = min(have, a.top_k);
+        }
+      }
+      cg::this_cluster().sync();           // no block goes on while its shared memory is read
+    }
+    if (part == 0) {
+      const RowResult res(sums);
+      if (lane == 0) res.Store(a, row, y, given);
+      if constexpr (TOP) if (lane < a.top_k) { const Entry e = parts > 1 ? s_joined[lane] : alt.sh.list[lane]; res.StoreTop(a, row * a.top_k + lane, lane < have ? e.v : -INFINITY, e.cls); }
+    }
+    __syncwarp();
+    y = y_next;
   }
 }
 
@@ -865,22 +984,25 @@ void LaunchFew(const ClassScoresArgs& a, cudaStream_t s) {
   else LaunchFew<T, kFewClasses>(a, by_class, s);
 }
 
-template <typename T, int GROUP, bool TOP>
-void LaunchRows(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
-  // as many groups as are resident at once, each with several rows
+// as many blocks as are resident at once, each with several rows
+template <typename T, bool TOP>
+void LaunchWarps(const ClassScoresArgs& a, cudaStream_t s) {
+  constexpr int kBytes = kWarpRing * kUnroll * 256 * 16;
   static PerDevice allowed;
-  AllowSharedMemory(ClassLogProbsRowKernel<T, GROUP, TOP>, kWalkBytes, &allowed);
-  const long long groups = GROUP == 32 ? (a.rows + 7) / 8 : a.rows, most = static_cast<long long>(kSms) * 4 * (GROUP == 32 ? 2 : 1) / cluster;
+  AllowSharedMemory(ClassLogProbsWarpKernel<T, TOP>, kBytes, &allowed);
+  ClassLogProbsWarpKernel<T, TOP><<<static_cast<unsigned int>(std::min<long long>((a.rows + 7) / 8, kSms * 4)), 256, kBytes, s>>>(a);
+}
+template <typename T, bool TOP>
+void LaunchBlocks(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
+  constexpr int kBytes = kBlockRing * kUnroll * 256 * 16;
+  static PerDevice allowed;
+  AllowSharedMemory(ClassLogProbsBlockKernel<T, TOP>, kBytes, &allowed);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned int>(std::min(groups, most) * cluster)); cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = kWalkBytes; cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
-  FB_CUDA(cudaLaunchKernelEx(&cfg, ClassLogProbsRowKernel<T, GROUP, TOP>, a));
-}
-template <typename T, int GROUP>
-void LaunchRows(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
-  if (a.top_k > 0) LaunchRows<T, GROUP, true>(a, cluster, s); else LaunchRows<T, GROUP, false>(a, cluster, s);
+  cfg.gridDim = dim3(static_cast<unsigned int>(std::min<long long>(a.rows, kSms * 3 / cluster) * cluster)); cfg.blockDim = dim3(kBlockThreads);
+  cfg.dynamicSmemBytes = kBytes; cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
+  FB_CUDA(cudaLaunchKernelEx(&cfg, ClassLogProbsBlockKernel<T, TOP>, a));
 }
 
 }  // namespace
@@ -889,17 +1011,23 @@ void LaunchClassLogProbs(const ClassScoresArgs& a, cudaStream_t s) {
   if (a.rows <= 0) return;
   DispatchType(a.dtype, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    if (a.classes <= kFewClasses) {
+    if (a.class_stride == 1 && a.classes > 32 && a.classes <= kSomeClasses) {
+      const unsigned int blocks = static_cast<unsigned int>((a.rows + 15) / 16);
+      if (a.classes <= 64) ClassLogProbsSomeKernel<T, 8><<<blocks, 128, 0, s>>>(a);
+      else if (a.classes <= 128) ClassLogProbsSomeKernel<T, 16><<<blocks, 128, 0, s>>>(a);
+      else ClassLogProbsSomeKernel<T, 32><<<blocks, 128, 0, s>>>(a);
+    } else if (a.classes <= kFewClasses) {
       LaunchFew<T>(a, s);
     } else if (a.class_stride == 1) {
       // A warp per row as long as that fills the machine and a warp's walk stays short; else a block, and a cluster of blocks while
       // there are fewer blocks than two per SM and every block has a full chunk.
       const long long chunk = 256LL * kUnroll * Pack<T>::N;
-      if (a.classes <= chunk / 8 || (a.classes <= chunk && a.rows >= kSms * 16)) { LaunchRows<T, 32>(a, 1, s); }
-      else {
+      if (a.classes <= chunk / 8 || (a.classes <= chunk && a.rows >= kSms * 16)) {
+        if (a.top_k > 0) LaunchWarps<T, true>(a, s); else LaunchWarps<T, false>(a, s);
+      } else {
         int cluster = 1;
         while (cluster < 8 && a.rows * cluster < 2 * kSms && a.classes >= 2 * cluster * chunk / kUnroll) cluster *= 2;
-        LaunchRows<T, 256>(a, cluster, s);
+        if (a.top_k > 0) LaunchBlocks<T, true>(a, cluster, s); else LaunchBlocks<T, false>(a, cluster, s);
       }
     } else {
       int warps = 8;
