@@ -390,8 +390,8 @@ struct RowShare {
 // The walk of GROUP threads through the rows row, row + stride, ... with RING chunks of shared memory per thread.
 template <typename T, int GROUP, int RING>
 struct Walk {
-  const ClassScoresArgs& a; uint4* mine; long long stride; int tid, part, parts, slot, ahead_slot, ahead_at, ahead_end; long long ahead_row; const uint4* ahead_body;
-  __device__ __forceinline__ Walk(const ClassScoresArgs& args, uint4* ring, long long row, long long stride_, int tid_, int part_, int parts_) : a(args) {
+  const ClassScoresArgs& a; uint4* mine; unsigned int stride; int tid, part, parts, slot, ahead_slot, ahead_at, ahead_end; unsigned int ahead_row; const uint4* ahead_body;
+  __device__ __forceinline__ Walk(const ClassScoresArgs& args, uint4* ring, unsigned int row, unsigned int stride_, int tid_, int part_, int parts_) : a(args) {
     mine = ring + threadIdx.x; stride = stride_; tid = tid_; part = part_; parts = parts_; slot = ahead_slot = 0; ahead_row = row;
     const RowShare<T> r(a, row, part, parts, GROUP);
     ahead_body = r.body; ahead_at = r.v_begin; ahead_end = r.v_end;
@@ -461,7 +461,7 @@ struct Walk {
 // One warp finds the alternatives of a share that GROUP threads have walked.
 template <int GROUP>
 struct TopShared {
-  static constexpr int kFlagged = 64, kCandidates = GROUP == 32 ? 128 : 512;
+  static constexpr int kFlagged = 64, kCandidates = GROUP == 32 ? 128 : 256;
   Entry list[kMaxTopClasses], cand[kCandidates];
   int flagged[kFlagged], flagged_at[kFlagged], num_flagged, num_cand;      // threads; the chunk to look at (-1: all of the thread's share)
 };
@@ -599,8 +599,8 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsWarpKernel(ClassScoresArg
   extern __shared__ __align__(16) uint4 s_ring[];      // [kWarpRing][kUnroll][256]
   __shared__ TopShared<32> s_top[TOP ? 8 : 1];
   const int lane = threadIdx.x % 32;
-  const long long stride = static_cast<long long>(gridDim.x) * 8;
-  long long row = static_cast<long long>(blockIdx.x) * 8 + threadIdx.x / 32;
+  const unsigned int stride = gridDim.x * 8;      // unsigned: row + stride may pass 2^31
+  unsigned int row = blockIdx.x * 8 + threadIdx.x / 32;
   if (row >= a.rows) return;                     // whole warps
   Walk<T, 32, kWarpRing> walk(a, s_ring, row, stride, lane, 0, 1);
   long long y = LabelOf(a, row);
@@ -627,27 +627,28 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsWarpKernel(ClassScoresArg
 }
 
 // 8 warps walk a row (with a cluster of blocks: a share of it), a ninth joins their sums, finds the alternatives and writes the results
-// while they are in the next row. Two sets
-// of hand-over buffers; named barriers kFull + set (walkers arrive, the ninth waits) and kFree + set (the other way round).
-constexpr int kBlockRing = 4, kBlockThreads = 288;
-enum { kFull = 1, kFree = 3 };
-template <int ID0> __device__ __forceinline__ void BarrierSync(int set) { asm volatile("bar.sync %0, %1;" ::"r"(ID0 + set), "n"(kBlockThreads) : "memory"); }
-template <int ID0> __device__ __forceinline__ void BarrierArrive(int set) { asm volatile("bar.arrive %0, %1;" ::"r"(ID0 + set), "n"(kBlockThreads) : "memory"); }
+// while they are in the next row. Named barriers: kFull (walkers arrive, the ninth waits), kFree (the other way round, as soon as it has
+// the maxima in registers). 56 registers a thread: 4 blocks, 32 walking warps on an SM; with 24 of them the walk takes a fifth longer.
+constexpr int kBlockRing = 3, kBlockThreads = 288;
+enum { kFull = 1, kFree = 2, kWalkers = 3, kJoined = 4 };
+template <int ID, int THREADS = kBlockThreads> __device__ __forceinline__ void BarrierSync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(THREADS) : "memory"); }
+template <int ID> __device__ __forceinline__ void BarrierArrive() { asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(kBlockThreads) : "memory"); }
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kBlockThreads, 3) ClassLogProbsBlockKernel(ClassScoresArgs a) {
+__global__ void __launch_bounds__(kBlockThreads, 4) ClassLogProbsBlockKernel(ClassScoresArgs a) {
   extern __shared__ __align__(16) uint4 s_ring[];      // [kBlockRing][kUnroll][256]
   __shared__ TopShared<256> s_top[1];
-  __shared__ unsigned int s_key[2][256], s_second[2][256]; __shared__ int s_chunk[2][256];
-  __shared__ float s_m[2][8], s_s[2][8], s_t[2][8];
+  __shared__ unsigned int s_key[256], s_second[256]; __shared__ int s_chunk[256];
+  __shared__ float s_m[8], s_s[8], s_t[8];
   __shared__ float s_share[3]; __shared__ int s_have;                  // of a cluster's block: its share's sums and number of alternatives
-  __shared__ Entry s_join[8][kMaxTopClasses], s_joined[kMaxTopClasses]; __shared__ int s_count[8];
+  __shared__ Entry s_joined[kMaxTopClasses]; __shared__ int s_count[8];
+  Entry (*s_join)[kMaxTopClasses] = reinterpret_cast<Entry (*)[kMaxTopClasses]>(s_top[0].cand);      // 8 lists, when the candidates are done with
+  static_assert(TopShared<256>::kCandidates >= 8 * kMaxTopClasses, "the lists of a cluster's blocks");
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int parts = static_cast<int>(cg::this_cluster().num_blocks()), part = static_cast<int>(cg::this_cluster().block_rank());
-  const long long stride = gridDim.x / parts, row0 = blockIdx.x / parts;      // the grid has no more clusters than rows
-  int set = 0;
+  const unsigned int stride = gridDim.x / parts, row0 = blockIdx.x / parts;      // the grid has no more clusters than rows
   if (warp < 8) {
     Walk<T, 256, kBlockRing> walk(a, s_ring, row0, stride, threadIdx.x, part, parts);
-    for (long long row = row0; row < a.rows; row += stride, set ^= 1) {
+    for (unsigned int row = row0; row < a.rows; row += stride) {
       const RowShare<T> r(a, row, part, parts, 256);
       const float head_v = r.Head(threadIdx.x), tail_v = r.Tail(threadIdx.x);
       Sums sums = walk.Row(r);
@@ -655,10 +656,10 @@ __global__ void __launch_bounds__(kBlockThreads, 3) ClassLogProbsBlockKernel(Cla
       if (head_v != -INFINITY) sums.AddOne(head_v);
       if (tail_v != -INFINITY) sums.AddOne(tail_v);
       sums.JoinLanes();
-      if (row >= row0 + 2 * stride) BarrierSync<kFree>(set);
-      if constexpr (TOP) { s_key[set][threadIdx.x] = OrderKey<T>(most); s_second[set][threadIdx.x] = OrderKey<T>(walk.second); s_chunk[set][threadIdx.x] = walk.best_at; }
-      if (lane == 0) { s_m[set][warp] = sums.m; s_s[set][warp] = sums.s; s_t[set][warp] = sums.t; }
-      BarrierArrive<kFull>(set);
+      if (row != row0) BarrierSync<kFree>();
+      if constexpr (TOP) { s_key[threadIdx.x] = OrderKey<T>(most); s_second[threadIdx.x] = OrderKey<T>(walk.second); s_chunk[threadIdx.x] = walk.best_at; }
+      if (lane == 0) { s_m[warp] = sums.m; s_s[warp] = sums.s; s_t[warp] = sums.t; }
+      BarrierArrive<kFull>();
       if (parts > 1) {
         // the first block joins the lists of all, read from their shared memory: warp w has block w's list, lane i its entry i. The lists
         // are sorted, so an entry's rank is, list by list and by bisection, how many come before it.
@@ -672,7 +673,7 @@ __global__ void __launch_bounds__(kBlockThreads, 3) ClassLogProbsBlockKernel(Cla
             s_join[warp][lane] = e;
           }
           if (lane == 0) s_count[warp] = n;
-          asm volatile("bar.sync 5, 256;" ::: "memory");
+          BarrierSync<kWalkers, 256>();
           if (lane < n) {
             int rank = 0;
 #pragma unroll
@@ -685,7 +686,7 @@ __global__ void __launch_bounds__(kBlockThreads, 3) ClassLogProbsBlockKernel(Cla
             }
             if (rank < a.top_k) s_joined[rank] = e;
           }
-          asm volatile("bar.sync 6, 288;" ::: "memory");
+          BarrierSync<kJoined>();
         }
         cg::this_cluster().sync();
       }
@@ -693,23 +694,26 @@ __global__ void __launch_bounds__(kBlockThreads, 3) ClassLogProbsBlockKernel(Cla
     return;
   }
   long long y = LabelOf(a, row0);
-  for (long long row = row0; row < a.rows; row += stride, set ^= 1) {
+  for (unsigned int row = row0; row < a.rows; row += stride) {
     const RowShare<T> r(a, row, part, parts, 256);
     const float given = lane == 0 && y >= 0 && y < r.K ? ToFloat(r.s[y]) : 0.f;
     const long long y_next = row + stride < a.rows ? LabelOf(a, row + stride) : -1;
     Alternatives<256, T> alt{s_top[0], r, a.top_k, lane};
-    BarrierSync<kFull>(set);
+    BarrierSync<kFull>();
     Sums sums;
-    if (lane < 8) { sums.m = s_m[set][lane]; sums.s = s_s[set][lane]; sums.t = s_t[set][lane]; }
-    sums.JoinLanes();
+    if (lane < 8) { sums.m = s_m[lane]; sums.s = s_s[lane]; sums.t = s_t[lane]; }
     int have = 0;
     if constexpr (TOP) {
       unsigned int keys[8], second[8]; int chunk[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { keys[i] = s_key[set][lane + 32 * i]; second[i] = s_second[set][lane + 32 * i]; chunk[i] = s_chunk[set][lane + 32 * i]; }
+      for (int i = 0; i < 8; ++i) { keys[i] = s_key[lane + 32 * i]; second[i] = s_second[lane + 32 * i]; chunk[i] = s_chunk[lane + 32 * i]; }
+      if (row + stride < a.rows) BarrierArrive<kFree>();
+      sums.JoinLanes();
       have = alt.Find(keys, second, chunk);
+    } else {
+      if (row + stride < a.rows) BarrierArrive<kFree>();
+      sums.JoinLanes();
     }
-    if (row + 2 * stride < a.rows) BarrierArrive<kFree>(set);
     if (parts > 1) {
       if (lane == 0) { s_share[0] = sums.m; s_share[1] = sums.s; s_share[2] = sums.t; s_have = have; }
       cg::this_cluster().sync();
@@ -719,7 +723,7 @@ __global__ void __launch_bounds__(kBlockThreads, 3) ClassLogProbsBlockKernel(Cla
         other.JoinLanes();
         sums = other;
         if constexpr (TOP) {
-          asm volatile("bar.sync 6, 288;" ::: "memory");      // the walkers have joined the lists
+          BarrierSync<kJoined>();      // the walkers have joined the lists
           have = 0;
           for (int p = 0; p < 8; ++p) have += s_count[p];
           have = min(have, a.top_k);
@@ -1000,7 +1004,7 @@ void LaunchBlocks(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned int>(std::min<long long>(a.rows, kSms * 3 / cluster) * cluster)); cfg.blockDim = dim3(kBlockThreads);
+  cfg.gridDim = dim3(static_cast<unsigned int>(std::min<long long>(a.rows, kSms * 4 / cluster) * cluster)); cfg.blockDim = dim3(kBlockThreads);
   cfg.dynamicSmemBytes = kBytes; cfg.stream = s; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
   FB_CUDA(cudaLaunchKernelEx(&cfg, ClassLogProbsBlockKernel<T, TOP>, a));
 }
