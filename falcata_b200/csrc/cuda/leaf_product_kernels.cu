@@ -306,7 +306,7 @@ struct FloatGramTile {
 };
 // A leaf of one slice is written to out; the sums of the slices of longer leaves go to partial [slot][a_cols][b_cols].
 template <int TA, int TB, int GA, int GB, int SLICES, int RD>
-__global__ void __launch_bounds__(GA * GB * SLICES, TA * TB <= 16 ? 3 : 2) LeafGramFloatKernel(LeafGramArgs a, int rows_per_slice, int a_vec, int b_vec, float* partial) {
+__global__ void __launch_bounds__(GA * GB * SLICES, 2) LeafGramFloatKernel(LeafGramArgs a, int rows_per_slice, int a_vec, int b_vec, float* partial) {
   using Tile = FloatGramTile<TA, TB, GA, GB, SLICES, RD>;
   extern __shared__ __align__(16) float s_float[];
   __shared__ TileMap map;
@@ -401,6 +401,222 @@ __global__ void __launch_bounds__(GA * GB * SLICES, TA * TB <= 16 ? 3 : 2) LeafG
   }
 }
 
+// --------------------------------------------------------------------------------------- few columns, any type ----
+// With at most 32 outputs and short rows the products are a matter of bandwidth: 14 warps per SM, each by itself, walk through tiles of
+// rows that come by asynchronous copies into the warp's own ring, so that about 100 KB per SM are on their way and no warp waits
+// for another. A warp's tiles are neighbours, so a leaf's map is loaded (as fp32) when the leaf changes. fp32 sums over even and
+// over odd features in one 64-bit register.
+constexpr int kNarrowWarps = 14, kNarrowThreads = 32 * kNarrowWarps, kNarrowRing = 2, kNarrowRowBytes = 256;
+// Copies rows to lines `pitch` bytes apart, in pieces of `piece` bytes; by one warp. What is worked out once: where a lane starts.
+struct WarpCopy {
+  int piece, per, pitch, row_bytes, line0, piece0, lines_on, pieces_on;
+  __device__ __forceinline__ WarpCopy(int row_bytes_, int pitch_, int piece_, int lane) {
+    piece = piece_; pitch = pitch_; row_bytes = row_bytes_; per = (row_bytes + piece - 1) / piece;
+    lines_on = 32 / per; pieces_on = 32 - lines_on * per; line0 = lane / per; piece0 = lane - line0 * per;
+  }
+  template <int BYTES>
+  __device__ __forceinline__ void Walk(unsigned int to, const char* from, long long stride, int rows) const {
+    from += line0 * stride + piece0 * BYTES; to += line0 * pitch + piece0 * BYTES;
+    const long long from_on = lines_on * stride + pieces_on * BYTES, from_wrap = stride - per * BYTES;
+    const int to_on = lines_on * pitch + pieces_on * BYTES, to_wrap = pitch - per * BYTES;
+    int p = piece0;
+#pragma unroll 2
+    for (int line = line0; line < rows;) {
+      const int valid = min(BYTES, row_bytes - p * BYTES);
+      if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid) : "memory");
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(to), "l"(from), "r"(valid), "n"(BYTES) : "memory");
+      line += lines_on; p += pieces_on; from += from_on; to += to_on;
+      if (p >= per) { p -= per; ++line; from += from_wrap; to += to_wrap; }
+    }
+  }
+  __device__ __forceinline__ void Copy(void* to, const void* from, long long stride_bytes, int rows) const {
+    const unsigned int dst = Smem32(to); const char* src = static_cast<const char*>(from);
+    if (piece == 16) Walk<16>(dst, src, stride_bytes, rows); else if (piece == 8) Walk<8>(dst, src, stride_bytes, rows); else Walk<4>(dst, src, stride_bytes, rows);
+  }
+};
+// 16 bytes of a row as pairs of fp32
+__device__ __forceinline__ void Pairs(const uint4& q, F2 (&p)[2], const float*) { p[0] = MakeF2(__uint_as_float(q.x), __uint_as_float(q.y)); p[1] = MakeF2(__uint_as_float(q.z), __uint_as_float(q.w)); }
+__device__ __forceinline__ F2 Pair(unsigned int w, const __nv_bfloat16*) { return MakeF2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ F2 Pair(unsigned int w, const __half*) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w)); return MakeF2(f.x, f.y); }
+template <typename T> __device__ __forceinline__ void Pairs(const uint4& q, F2 (&p)[4], const T* t) { p[0] = Pair(q.x, t); p[1] = Pair(q.y, t); p[2] = Pair(q.z, t); p[3] = Pair(q.w, t); }
+
+// A warp's share of the tiles of `rows` rows, one behind the other: [first, last) of them.
+struct WarpTiles {
+  int left, span, leaf, row, leaf_end, least;
+  __device__ __forceinline__ WarpTiles(const TileMap& map, const LeafWindows& w, int rows, int least_) {
+    least = least_;
+    const long long total = map.Total(), warps = static_cast<long long>(gridDim.x) * kNarrowWarps, me = static_cast<long long>(blockIdx.x) * kNarrowWarps + threadIdx.x / 32;
+    const int first = static_cast<int>(total * me / warps), last = static_cast<int>(total * (me + 1) / warps);
+    left = last - first; span = 0; leaf = row = leaf_end = 0;
+    if (left > 0) { int end; map.Find(w, first, rows, least, &span, &leaf, &row, &end); long long b, e; LeafWindow(w, leaf, &b, &e); leaf_end = static_cast<int>(e); }
+  }
+  __device__ __forceinline__ void Next(const LeafWindows& w, int rows) {
+    if (--left <= 0) return;
+    if (leaf_end - row > rows) row += rows;
+    else {
+      do { ++leaf; long long b, e; LeafWindow(w, leaf, &b, &e); row = static_cast<int>(b); leaf_end = static_cast<int>(e); } while (least == 0 && row >= leaf_end && leaf + 1 < w.leaves);
+    }
+  }
+};
+
+template <typename T, int TM, int TN>
+__global__ void __launch_bounds__(kNarrowThreads, 1) LeafProductsNarrowKernel(LeafProductsArgs a, int pitch, int piece) {
+  constexpr int ROWS = 32 * TM, V = 16 / sizeof(T);
+  extern __shared__ __align__(16) unsigned char s_bytes[];
+  __shared__ TileMap map;
+  ZeroLeaflessRows(a.leaves, static_cast<T*>(a.y), a.outputs);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, w_pitch = (a.features + V - 1) / V * V;      // features of a map's line in shared memory
+  const int stage = ROWS * pitch, of_warp = kNarrowRing * stage + TN * w_pitch * 4;
+  unsigned char* s_x = s_bytes + warp * of_warp;
+  float* s_w = reinterpret_cast<float*>(s_x + kNarrowRing * stage);
+  for (int i = lane; i < of_warp / 4; i += 32) reinterpret_cast<unsigned int*>(s_x)[i] = 0u;                // what no copy writes stays zero
+  map.Build(a.leaves, ROWS, 0);
+  WarpTiles now(map, a.leaves, ROWS, 0);
+  WarpTiles ahead = now;
+  const WarpCopy plan(a.features * static_cast<int>(sizeof(T)), pitch, piece, lane);
+  auto copy = [&](int slot) {
+    if (ahead.left > 0) {
+      plan.Copy(s_x + slot * stage, static_cast<const T*>(a.x) + static_cast<long long>(ahead.row) * a.x_stride, a.x_stride * static_cast<long long>(sizeof(T)), min(ROWS, ahead.leaf_end - ahead.row));
+      ahead.Next(a.leaves, ROWS);
+    }
+    CopyCommit();
+  };
+  copy(0);
+  int slot = 0, loaded = -1;
+  for (; now.left > 0; now.Next(a.leaves, ROWS), slot ^= 1) {
+    const int rows = min(ROWS, now.leaf_end - now.row);
+    if (now.leaf != loaded) {
+      loaded = now.leaf;
+      const T* w = static_cast<const T*>(a.weight) + loaded * a.weight_leaf_stride;
+      const bool by_feature = a.weight_in_stride == 1;
+      for (int e = lane; e < a.outputs * a.features; e += 32) {
+        const int o = by_feature ? e / a.features : e % a.outputs, f = by_feature ? e - o * a.features : e / a.outputs;
+        s_w[o * w_pitch + f] = ToFloat(w[o * a.weight_out_stride + f * a.weight_in_stride]);
+      }
+    }
+    copy(slot ^ 1);
+    CopyWait<1>();
+    __syncwarp();
+    F2 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = MakeF2(0.f, 0.f);
+    const unsigned char* xs = s_x + slot * stage + lane * pitch;
+    for (int f = 0; f < a.features; f += V) {
+      F2 xv[TM][V / 2];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) Pairs(*reinterpret_cast<const uint4*>(xs + 32 * i * pitch + f * static_cast<int>(sizeof(T))), xv[i], static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int h = 0; h < V / 4; ++h) {
+          const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(s_w + j * w_pitch + f + 4 * h);
+#pragma unroll
+          for (int i = 0; i < TM; ++i) { acc[i][j] = Fma2(xv[i][2 * h], F2{w.x}, acc[i][j]); acc[i][j] = Fma2(xv[i][2 * h + 1], F2{w.y}, acc[i][j]); }
+        }
+      }
+    }
+    // the tile's outputs are one piece of memory; they go there through the place of its rows, which only this warp has read
+    __syncwarp();
+    T* s_y = reinterpret_cast<T*>(s_x + slot * stage);
+    const int count = rows * a.outputs;
+    const bool fits = ROWS * a.outputs * static_cast<int>(sizeof(T)) <= stage;
+    T* y = static_cast<T*>(a.y) + static_cast<long long>(now.row) * a.outputs;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        if (j < a.outputs) {
+          float lo, hi; Split(acc[i][j], lo, hi);
+          const int at = (lane + 32 * i) * a.outputs + j;
+          if (fits) s_y[at] = FromFloat<T>(lo + hi); else if (lane + 32 * i < rows) y[at] = FromFloat<T>(lo + hi);
+        }
+    if (fits) {
+      __syncwarp();
+      if (sizeof(T) == 4 || (reinterpret_cast<uintptr_t>(y) & 3) != 0) { for (int e = lane; e < count; e += 32) y[e] = s_y[e]; }
+      else {
+        for (int e = lane; e < count / 2; e += 32) reinterpret_cast<unsigned int*>(y)[e] = reinterpret_cast<const unsigned int*>(s_y)[e];
+        if ((count & 1) != 0 && lane == 0) y[count - 1] = s_y[count - 1];
+      }
+      __syncwarp();
+      // the features' padding has to be zero again
+      const int row_bytes = a.features * static_cast<int>(sizeof(T)), pad = (row_bytes + 15) / 16 * 16 - row_bytes;
+      if (pad > 0) for (int l = lane; l < ROWS; l += 32) for (int b = 0; b < pad; b += static_cast<int>(sizeof(T))) *reinterpret_cast<T*>(s_x + slot * stage + l * pitch + row_bytes + b) = FromFloat<T>(0.f);
+      __syncwarp();
+    }
+  }
+  CopyWait<0>();
+}
+
+// Gram matrices of at most 4 GA columns of a and 4 GB of b (GA GB = 32): a lane has 4 x 4 of the sums, a warp a slice of a leaf's rows.
+constexpr int kGramRows = 32;
+constexpr int GramRing(int size) { return size == 4 ? 2 : 4; }      // of all warps: 172 KB
+template <typename T> __device__ __forceinline__ void Four(const void* p, float (&v)[4]);
+template <> __device__ __forceinline__ void Four<float>(const void* p, float (&v)[4]) { const float4 q = *static_cast<const float4*>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
+template <> __device__ __forceinline__ void Four<__nv_bfloat16>(const void* p, float (&v)[4]) { const uint2 q = *static_cast<const uint2*>(p); Split(Pair(q.x, static_cast<const __nv_bfloat16*>(nullptr)), v[0], v[1]); Split(Pair(q.y, static_cast<const __nv_bfloat16*>(nullptr)), v[2], v[3]); }
+template <> __device__ __forceinline__ void Four<__half>(const void* p, float (&v)[4]) { const uint2 q = *static_cast<const uint2*>(p); Split(Pair(q.x, static_cast<const __half*>(nullptr)), v[0], v[1]); Split(Pair(q.y, static_cast<const __half*>(nullptr)), v[2], v[3]); }
+template <typename T, typename O, int GA, int GB>
+__global__ void __launch_bounds__(kNarrowThreads, 1) LeafGramNarrowKernel(LeafGramArgs a, int rows_per_slice, int a_piece, int b_piece, float* partial) {
+  constexpr int A_PITCH = 4 * GA * static_cast<int>(sizeof(T)), B_PITCH = 4 * GB * static_cast<int>(sizeof(T)), STAGE = kGramRows * (A_PITCH + B_PITCH), RING = GramRing(static_cast<int>(sizeof(T)));
+  extern __shared__ __align__(16) unsigned char s_bytes[];
+  __shared__ TileMap map;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, ga = lane / GB, gb = lane % GB;
+  unsigned char* mine = s_bytes + warp * RING * STAGE;
+  map.Build(a.leaves, rows_per_slice, 1);
+  const WarpCopy a_plan(a.a_cols * static_cast<int>(sizeof(T)), A_PITCH, a_piece, lane), b_plan(a.b_cols * static_cast<int>(sizeof(T)), B_PITCH, b_piece, lane);
+  for (WarpTiles slice(map, a.leaves, rows_per_slice, 1); slice.left > 0; slice.Next(a.leaves, rows_per_slice)) {
+    const int rows = max(0, min(rows_per_slice, slice.leaf_end - slice.row));
+    const T* pa = static_cast<const T*>(a.a) + static_cast<long long>(slice.row) * a.a_stride; const T* pb = static_cast<const T*>(a.b) + static_cast<long long>(slice.row) * a.b_stride;
+    auto copy = [&](int r0) {
+      if (r0 < rows) {
+        unsigned char* to = mine + r0 / kGramRows % RING * STAGE;
+        const int n = min(kGramRows, rows - r0);
+        a_plan.Copy(to, pa + r0 * a.a_stride, a.a_stride * static_cast<long long>(sizeof(T)), n);
+        b_plan.Copy(to + kGramRows * A_PITCH, pb + r0 * a.b_stride, a.b_stride * static_cast<long long>(sizeof(T)), n);
+      }
+      CopyCommit();
+    };
+    F2 acc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = MakeF2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) copy(i * kGramRows);
+    for (int r0 = 0; r0 < rows; r0 += kGramRows) {
+      __syncwarp();                                 // every lane has left the buffer that is filled now
+      copy(r0 + (RING - 1) * kGramRows);
+      CopyWait<RING - 1>();
+      __syncwarp();
+      const unsigned char* as = mine + r0 / kGramRows % RING * STAGE + ga * 4 * sizeof(T); const unsigned char* bs = mine + r0 / kGramRows % RING * STAGE + kGramRows * A_PITCH + gb * 4 * sizeof(T);
+      const int here = min(kGramRows, rows - r0);
+#pragma unroll 8
+      for (int r = 0; r < here; ++r) {              // columns beyond the operands hold anything; they reach only sums that are not stored
+        float av[4], bv[4];
+        Four<T>(as + r * A_PITCH, av); Four<T>(bs + r * B_PITCH, bv);
+        const F2 b0 = MakeF2(bv[0], bv[1]), b1 = MakeF2(bv[2], bv[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const F2 v = MakeF2(av[i], av[i]); acc[i][0] = Fma2(v, b0, acc[i][0]); acc[i][1] = Fma2(v, b1, acc[i][1]); }
+      }
+    }
+    CopyWait<0>();
+    __syncwarp();
+    const int slot = SliceSlot(a.leaves, slice.leaf, slice.row, rows_per_slice);
+    const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float v[2]; Split(acc[i][j], v[0], v[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int ca = ga * 4 + i, cb = gb * 4 + 2 * j + h;
+          if (ca >= a.a_cols || cb >= a.b_cols) continue;
+          if (slot >= 0) partial[slot * size + ca * a.b_cols + cb] = v[h]; else static_cast<O*>(a.out)[slice.leaf * size + ca * a.b_cols + cb] = FromFloat<O>(v[h]);
+        }
+      }
+  }
+}
+
 // Adds the sums of the slices of each leaf that has several, in order.
 template <typename O>
 __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int rows_per_slice, const float* __restrict__ partial) {
@@ -411,7 +627,7 @@ __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int ro
     for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < size; i += static_cast<long long>(gridDim.x) * 256) {
       float v = 0.f;
 #pragma unroll 4
-      for (int r = static_cast<int>(b); r < e; r += rows_per_slice) v += __ldg(partial + (2 * (r / rows_per_slice) + (r == b ? 0 : 1)) * size + i);
+      for (long long r = b; r < e; r += rows_per_slice) v += __ldg(partial + (2 * (r / rows_per_slice) + (r == b ? 0 : 1)) * size + i);
       static_cast<O*>(a.out)[g * size + i] = FromFloat<O>(v);
     }
   }
@@ -937,6 +1153,58 @@ void LaunchFloatProducts(const LeafProductsArgs& a, cudaStream_t s) {
   CheckTiles(tiles);
   LeafProductsFloatKernel<TM, TN, WR, WO><<<static_cast<unsigned int>(std::min<long long>(tiles, kSms * per_sm)), Tile::THREADS, bytes, s>>>(a, shape);
 }
+// Pieces (in bytes) of rows that start at p, `stride` bytes apart; 2: not for asynchronous copies
+inline int BytePieces(const void* p, long long stride) {
+  for (int v = 16; v > 2; v /= 2) if (reinterpret_cast<uintptr_t>(p) % v == 0 && stride % v == 0) return v;
+  return 2;
+}
+// Shared memory of a warp: its ring of rows (an odd number of 16-byte pieces apart) and its leaf's map.
+inline int NarrowPitch(int row_bytes) { const int pieces = (row_bytes + 15) / 16; return 16 * (pieces | 1); }
+inline int NarrowBytes(int tm, int tn, int size, int features) { const int v = 16 / size; return kNarrowRing * 32 * tm * NarrowPitch(features * size) + tn * ((features + v - 1) / v * v) * 4; }
+constexpr int kNarrowMostBytes = 216 * 1024;
+inline int NarrowOutputs(int outputs) { return outputs <= 4 ? 4 : outputs <= 8 ? 8 : outputs <= 12 ? 12 : outputs <= 16 ? 16 : 32; }
+// Rows short enough for the warps' rings, on 4-byte boundaries; outputs that fit a lane's registers.
+inline bool NarrowProducts(const LeafProductsArgs& a) {
+  const int size = a.dtype == kOpFloat32 ? 4 : 2, tn = NarrowOutputs(a.outputs);
+  return a.outputs <= 32 && a.features * size <= kNarrowRowBytes && BytePieces(a.x, a.x_stride * size) >= 4 && kNarrowWarps * NarrowBytes(tn <= 16 ? 2 : 1, tn, size, a.features) <= kNarrowMostBytes;
+}
+template <typename T, int TM, int TN>
+void LaunchNarrowProducts(const LeafProductsArgs& a, cudaStream_t s) {
+  constexpr int kSize = static_cast<int>(sizeof(T));
+  const int bytes = kNarrowWarps * NarrowBytes(TM, TN, kSize, a.features);
+  static PerDevice allowed;
+  AllowSharedMemory(LeafProductsNarrowKernel<T, TM, TN>, kNarrowMostBytes, &allowed);
+  const long long tiles = (a.leaves.rows + 32 * TM - 1) / (32 * TM) + a.leaves.leaves;
+  LeafProductsNarrowKernel<T, TM, TN><<<static_cast<unsigned int>(std::max(1LL, std::min<long long>((tiles + kNarrowWarps - 1) / kNarrowWarps, kSms))), kNarrowThreads, bytes, s>>>(
+      a, NarrowPitch(a.features * kSize), BytePieces(a.x, a.x_stride * kSize));
+}
+template <typename T>
+void LaunchNarrowProducts(const LeafProductsArgs& a, cudaStream_t s) {
+  switch (NarrowOutputs(a.outputs)) {
+    case 4: LaunchNarrowProducts<T, 2, 4>(a, s); return;
+    case 8: LaunchNarrowProducts<T, 2, 8>(a, s); return;
+    case 12: LaunchNarrowProducts<T, 2, 12>(a, s); return;
+    case 16: LaunchNarrowProducts<T, 2, 16>(a, s); return;
+    default: LaunchNarrowProducts<T, 1, 32>(a, s);
+  }
+}
+inline bool NarrowGram(const LeafGramArgs& a) {
+  const int size = a.dtype == kOpFloat32 ? 4 : 2;
+  return ((a.a_cols <= 16 && a.b_cols <= 32) || (a.a_cols <= 32 && a.b_cols <= 16)) && BytePieces(a.a, a.a_stride * size) >= 4 && BytePieces(a.b, a.b_stride * size) >= 4;
+}
+template <typename T, typename O, int GA, int GB>
+void LaunchNarrowGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
+  constexpr int kSize = static_cast<int>(sizeof(T)), kBytes = kNarrowWarps * GramRing(kSize) * kGramRows * 4 * (GA + GB) * kSize;
+  static PerDevice allowed;
+  AllowSharedMemory(LeafGramNarrowKernel<T, O, GA, GB>, kBytes, &allowed);
+  const int rows = LeafGramSliceRows(a);
+  LeafGramNarrowKernel<T, O, GA, GB><<<static_cast<unsigned int>(std::max(1LL, std::min<long long>((LeafGramTiles(a) + kNarrowWarps - 1) / kNarrowWarps, kSms))), kNarrowThreads, kBytes, s>>>(
+      a, rows, BytePieces(a.a, a.a_stride * kSize), BytePieces(a.b, a.b_stride * kSize), rows < a.leaves.rows ? workspace : nullptr);
+}
+template <typename T, typename O>
+void LaunchNarrowGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
+  if (a.a_cols <= 16 && a.b_cols <= 32) LaunchNarrowGram<T, O, 4, 8>(a, workspace, s); else LaunchNarrowGram<T, O, 8, 4>(a, workspace, s);
+}
 template <int TA, int TB, int GA, int GB, int SLICES, int RD>
 void LaunchFloatGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
   using Tile = FloatGramTile<TA, TB, GA, GB, SLICES, RD>;
@@ -959,7 +1227,7 @@ inline bool Unaligned(const void* p, long long stride, long long along) { return
 struct GramPacking {
   bool a, b;
   explicit GramPacking(const LeafGramArgs& g) {
-    const bool half = g.dtype != kOpFloat32;
+    const bool half = g.dtype != kOpFloat32 && !NarrowGram(g);
     a = half && g.b_cols > kTileM && Unaligned(g.a, g.a_stride, g.a_cols);
     b = half && g.a_cols > kTileM && Unaligned(g.b, g.b_stride, g.b_cols);
   }
@@ -968,7 +1236,7 @@ struct GramPacking {
 struct ProductsPacking {
   bool x, w; long long w_lines; int w_along;
   explicit ProductsPacking(const LeafProductsArgs& p) {
-    const bool half = p.dtype != kOpFloat32, by_feature = p.weight_in_stride == 1 || p.features == 1;
+    const bool half = p.dtype != kOpFloat32 && !NarrowProducts(p), by_feature = p.weight_in_stride == 1 || p.features == 1;
     w_lines = by_feature ? p.outputs : p.features; w_along = by_feature ? p.features : p.outputs;
     const long long line_stride = by_feature ? p.weight_out_stride : p.weight_in_stride;
     x = half && p.outputs > kTileM && Unaligned(p.x, p.x_stride, p.features);
@@ -977,20 +1245,16 @@ struct ProductsPacking {
         PieceWidth(p.weight, line_stride, p.weight_leaf_stride) != 8;
   }
 };
-// narrow sides: few outputs / both sides of a Gram matrix within one small tile
-constexpr int kNarrow = 16;
 
 }  // namespace
 
-// Rows of a leaf that one block sums up. Slices short enough that uneven leaves even out (4 of them per SM, 16 of small ones), long
+// Rows of a leaf that one block (narrow: one warp) sums up. Slices short enough that uneven leaves even out (4 per SM, 2 per warp), long
 // enough that a slice's work outweighs its sums' way through the workspace, and that the workspace stays within 128 MB.
 int LeafGramSliceRows(const LeafGramArgs& a) {
   long long outputs = GramTiles(a), least = 1024, per_sm = 4;
   const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
-  if (a.dtype == kOpFloat32) {
-    const bool narrow = a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow;
-    outputs = narrow ? 1 : (a.a_cols + 63LL) / 64 * ((a.b_cols + 63) / 64); least = 256; if (narrow) per_sm = 16;
-  }
+  if (NarrowGram(a)) { outputs = 1; least = 128; per_sm = 2 * kNarrowWarps; }
+  else if (a.dtype == kOpFloat32) { outputs = (a.a_cols + 63LL) / 64 * ((a.b_cols + 63) / 64); least = 256; }
   const long long wanted = std::max(1LL, std::min(per_sm * kSms / outputs, (16LL << 20) / size));
   const long long rows = std::max(least, ((a.leaves.rows + wanted - 1) / wanted + 63) / 64 * 64);
   return static_cast<int>(std::min<long long>(rows, std::max(1LL, a.leaves.rows)));
@@ -1008,12 +1272,31 @@ long long LeafProductsWorkspace(const LeafProductsArgs& a) {
   const ProductsPacking packing(a);
   return (packing.x ? a.leaves.rows * PackedStride(a.features) / 2 : 0) + (packing.w ? a.leaves.leaves * packing.w_lines * PackedStride(packing.w_along) / 2 : 0);
 }
+template <typename T, typename O>
+static void LaunchTensorGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
+  const int rows = LeafGramSliceRows(a);
+  const bool split = rows < a.leaves.rows;
+  TensorArgs t = TensorArgs();
+  t.leaves = a.leaves; t.tile_rows = rows; t.least = 1;
+  t.a = static_cast<const unsigned short*>(a.b); t.a_stride = a.b_stride; t.a_size = a.b_cols;
+  t.b = static_cast<const unsigned short*>(a.a); t.b_stride = a.a_stride; t.b_size = a.a_cols;
+  unsigned short* packed = reinterpret_cast<unsigned short*>(workspace + (split ? GramSumFloats(a) : 0));
+  const GramPacking packing(a);
+  if (packing.b) { t.a_stride = PackedStride(a.b_cols); LaunchPack(t.a, a.b_stride, a.leaves.rows, a.b_cols, packed, s); t.a = packed; packed += a.leaves.rows * t.a_stride; }
+  if (packing.a) { t.b_stride = PackedStride(a.a_cols); LaunchPack(t.b, a.a_stride, a.leaves.rows, a.a_cols, packed, s); t.b = packed; }
+  t.a_vec = PieceWidth(t.a, t.a_stride, 0); t.b_vec = PieceWidth(t.b, t.b_stride, 0);
+  t.n = TileN(t.b_size); t.across_a = (t.a_size + kTileM - 1) / kTileM; t.across_b = (t.b_size + t.n - 1) / t.n;
+  t.out = a.out; t.partial = split ? workspace : nullptr; t.out_row_stride = 1; t.out_col_stride = a.b_cols;
+  LaunchTensor<T, O, kGram>(t, LeafGramTiles(a) * t.across_a * t.across_b, s);
+}
+
 void LaunchLeafProducts(const LeafProductsArgs& a, float* workspace, cudaStream_t s) {
   if (a.leaves.rows <= 0) return;
-  if (a.dtype == kOpFloat32) {
-    if (a.outputs <= 4) LaunchFloatProducts<2, 4, 4, 1>(a, s);
-    else if (a.outputs <= 12) LaunchFloatProducts<2, 12, 4, 1>(a, s);
-    else if (a.outputs <= 16) LaunchFloatProducts<2, 16, 4, 1>(a, s);
+  if (NarrowProducts(a)) {
+    if (a.dtype == kOpFloat32) LaunchNarrowProducts<float>(a, s);
+    else DispatchHalf(a.dtype, [&](auto* p) { LaunchNarrowProducts<std::remove_pointer_t<decltype(p)>>(a, s); });
+  } else if (a.dtype == kOpFloat32) {
+    if (a.outputs <= 16) LaunchFloatProducts<2, 16, 4, 1>(a, s);
     else if (a.outputs <= 32) LaunchFloatProducts<2, 16, 2, 2>(a, s);
     else LaunchFloatProducts<4, 8, 1, 8>(a, s);
   } else DispatchHalf(a.dtype, [&](auto* p) {
@@ -1041,42 +1324,23 @@ void LaunchLeafProducts(const LeafProductsArgs& a, float* workspace, cudaStream_
 }
 
 void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
-  if (a.dtype == kOpFloat32) {
-    if (a.out_dtype != kOpFloat32) Log::Fatal("leaf Gram: sums of type code %d as type code %d", a.dtype, a.out_dtype);
-    if (a.a_cols <= kNarrow && a.b_cols <= 2 * kNarrow) LaunchFloatGram<4, 4, 4, 8, 8, 64>(a, workspace, s);
-    else LaunchFloatGram<8, 8, 8, 8, 4, 32>(a, workspace, s);
-    FB_LAUNCHED(); FB_KERNEL_CHECK();
-    if (LeafGramSliceRows(a) < a.leaves.rows) {
-      const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
-      LeafGramJoinKernel<float><<<dim3(static_cast<unsigned int>(std::min(64LL, (size + 255) / 256)), std::min(a.leaves.leaves, 1024)), 256, 0, s>>>(a, LeafGramSliceRows(a), workspace);
-      FB_LAUNCHED(); FB_KERNEL_CHECK();
-    }
-    return;
+  const int rows = LeafGramSliceRows(a);
+  const bool split = rows < a.leaves.rows, same = a.out_dtype == a.dtype;
+  if (!same && a.out_dtype != kOpFloat32) Log::Fatal("leaf Gram: sums of type code %d as type code %d", a.dtype, a.out_dtype);
+  if (NarrowGram(a)) {
+    if (a.dtype == kOpFloat32) LaunchNarrowGram<float, float>(a, workspace, s);
+    else DispatchHalf(a.dtype, [&](auto* p) { using T = std::remove_pointer_t<decltype(p)>; if (same) LaunchNarrowGram<T, T>(a, workspace, s); else LaunchNarrowGram<T, float>(a, workspace, s); });
+  } else if (a.dtype == kOpFloat32) {
+    LaunchFloatGram<8, 8, 8, 8, 4, 32>(a, workspace, s);
+  } else {
+    DispatchHalf(a.dtype, [&](auto* p) { using T = std::remove_pointer_t<decltype(p)>; if (same) LaunchTensorGram<T, T>(a, workspace, s); else LaunchTensorGram<T, float>(a, workspace, s); });
   }
-  DispatchHalf(a.dtype, [&](auto* p) {
-    using T = std::remove_pointer_t<decltype(p)>;
-    if (a.out_dtype != a.dtype && a.out_dtype != kOpFloat32) Log::Fatal("leaf Gram: sums of type code %d as type code %d", a.dtype, a.out_dtype);
-    const int rows = LeafGramSliceRows(a);
-    const bool split = rows < a.leaves.rows;
-    TensorArgs t = TensorArgs();
-    t.leaves = a.leaves; t.tile_rows = rows; t.least = 1;
-    t.a = static_cast<const unsigned short*>(a.b); t.a_stride = a.b_stride; t.a_size = a.b_cols;
-    t.b = static_cast<const unsigned short*>(a.a); t.b_stride = a.a_stride; t.b_size = a.a_cols;
-    unsigned short* packed = reinterpret_cast<unsigned short*>(workspace + (split ? GramSumFloats(a) : 0));
-    const GramPacking packing(a);
-    if (packing.b) { t.a_stride = PackedStride(a.b_cols); LaunchPack(t.a, a.b_stride, a.leaves.rows, a.b_cols, packed, s); t.a = packed; packed += a.leaves.rows * t.a_stride; }
-    if (packing.a) { t.b_stride = PackedStride(a.a_cols); LaunchPack(t.b, a.a_stride, a.leaves.rows, a.a_cols, packed, s); t.b = packed; }
-    t.a_vec = PieceWidth(t.a, t.a_stride, 0); t.b_vec = PieceWidth(t.b, t.b_stride, 0);
-    t.n = TileN(t.b_size); t.across_a = (t.a_size + kTileM - 1) / kTileM; t.across_b = (t.b_size + t.n - 1) / t.n;
-    t.out = a.out; t.partial = split ? workspace : nullptr; t.out_row_stride = 1; t.out_col_stride = a.b_cols;
-    const long long tiles = LeafGramTiles(a) * t.across_a * t.across_b, size = static_cast<long long>(a.a_cols) * a.b_cols;
-    const dim3 join(static_cast<unsigned int>(std::min(64LL, (size + 255) / 256)), std::min(a.leaves.leaves, 1024));
-    if (a.out_dtype == a.dtype) LaunchTensor<T, T, kGram>(t, tiles, s); else LaunchTensor<T, float, kGram>(t, tiles, s);
-    if (split) {
-      FB_LAUNCHED(); FB_KERNEL_CHECK();
-      if (a.out_dtype == a.dtype) LeafGramJoinKernel<T><<<join, 256, 0, s>>>(a, rows, workspace); else LeafGramJoinKernel<float><<<join, 256, 0, s>>>(a, rows, workspace);
-    }
-  });
+  FB_LAUNCHED(); FB_KERNEL_CHECK();
+  if (!split) return;
+  const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
+  const dim3 grid(static_cast<unsigned int>(std::min(64LL, (size + 255) / 256)), std::min(a.leaves.leaves, 1024));
+  if (a.out_dtype == kOpFloat32) LeafGramJoinKernel<float><<<grid, 256, 0, s>>>(a, rows, workspace);
+  else DispatchHalf(a.out_dtype, [&](auto* p) { LeafGramJoinKernel<std::remove_pointer_t<decltype(p)>><<<grid, 256, 0, s>>>(a, rows, workspace); });
   FB_LAUNCHED(); FB_KERNEL_CHECK();
 }
 
