@@ -459,6 +459,8 @@ struct WarpTiles {
   }
 };
 
+// Shared memory for a tile's outputs, 0 where the place of its rows (`stage` bytes) is enough.
+__host__ __device__ constexpr int NarrowOutputBytes(int tm, int outputs, int size, int stage) { const int bytes = (32 * tm * outputs * size + 15) / 16 * 16; return bytes <= stage ? 0 : bytes; }
 template <typename T, int TM, int TN>
 __global__ void __launch_bounds__(kNarrowThreads, 1) LeafProductsNarrowKernel(LeafProductsArgs a, int pitch, int piece) {
   constexpr int ROWS = 32 * TM, V = 16 / sizeof(T);
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafProductsNarrowKernel(Le
   __shared__ TileMap map;
   ZeroLeaflessRows(a.leaves, static_cast<T*>(a.y), a.outputs);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, w_pitch = (a.features + V - 1) / V * V;      // features of a map's line in shared memory
-  const int stage = ROWS * pitch, of_warp = kNarrowRing * stage + TN * w_pitch * 4;
+  const int stage = ROWS * pitch, y_bytes = NarrowOutputBytes(TM, a.outputs, static_cast<int>(sizeof(T)), stage), of_warp = kNarrowRing * stage + TN * w_pitch * 4 + y_bytes;
   unsigned char* s_x = s_bytes + warp * of_warp;
   float* s_w = reinterpret_cast<float*>(s_x + kNarrowRing * stage);
   for (int i = lane; i < of_warp / 4; i += 32) reinterpret_cast<unsigned int*>(s_x)[i] = 0u;                // what no copy writes stays zero
@@ -517,11 +519,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafProductsNarrowKernel(Le
         }
       }
     }
-    // the tile's outputs are one piece of memory; they go there through the place of its rows, which only this warp has read
+    // the tile's outputs are one piece of memory; they go there through the place of its rows, which only this warp has read, or, where
+    // that is too small, through a place of their own
     __syncwarp();
-    T* s_y = reinterpret_cast<T*>(s_x + slot * stage);
+    T* s_y = reinterpret_cast<T*>(y_bytes > 0 ? reinterpret_cast<unsigned char*>(s_w + TN * w_pitch) : s_x + slot * stage);
     const int count = rows * a.outputs;
-    const bool fits = ROWS * a.outputs * static_cast<int>(sizeof(T)) <= stage;
     T* y = static_cast<T*>(a.y) + static_cast<long long>(now.row) * a.outputs;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -529,11 +531,10 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafProductsNarrowKernel(Le
       for (int j = 0; j < TN; ++j)
         if (j < a.outputs) {
           float lo, hi; Split(acc[i][j], lo, hi);
-          const int at = (lane + 32 * i) * a.outputs + j;
-          if (fits) s_y[at] = FromFloat<T>(lo + hi); else if (lane + 32 * i < rows) y[at] = FromFloat<T>(lo + hi);
+          s_y[(lane + 32 * i) * a.outputs + j] = FromFloat<T>(lo + hi);
         }
-    if (fits) {
-      __syncwarp();
+    __syncwarp();
+    {
       if (sizeof(T) == 4 || (reinterpret_cast<uintptr_t>(y) & 3) != 0) { for (int e = lane; e < count; e += 32) y[e] = s_y[e]; }
       else {
         for (int e = lane; e < count / 2; e += 32) reinterpret_cast<unsigned int*>(y)[e] = reinterpret_cast<const unsigned int*>(s_y)[e];
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafProductsNarrowKernel(Le
       __syncwarp();
       // the features' padding has to be zero again
       const int row_bytes = a.features * static_cast<int>(sizeof(T)), pad = (row_bytes + 15) / 16 * 16 - row_bytes;
-      if (pad > 0) for (int l = lane; l < ROWS; l += 32) for (int b = 0; b < pad; b += static_cast<int>(sizeof(T))) *reinterpret_cast<T*>(s_x + slot * stage + l * pitch + row_bytes + b) = FromFloat<T>(0.f);
+      if (pad > 0 && y_bytes == 0) for (int l = lane; l < ROWS; l += 32) for (int b = 0; b < pad; b += static_cast<int>(sizeof(T))) *reinterpret_cast<T*>(s_x + slot * stage + l * pitch + row_bytes + b) = FromFloat<T>(0.f);
       __syncwarp();
     }
   }
@@ -617,18 +618,33 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafGramNarrowKernel(LeafGr
   }
 }
 
-// Adds the sums of the slices of each leaf that has several, in order.
+// Adds the sums of the slices of each leaf that has several, always in the same order: a warp has 32 neighbouring sums and an eighth of
+// the slices, the eighths are added up at the end.
 template <typename O>
 __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int rows_per_slice, const float* __restrict__ partial) {
+  __shared__ float s_part[8][32];
   const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   for (int g = blockIdx.y; g < a.leaves.leaves; g += gridDim.y) {
     long long b, e; LeafWindow(a.leaves, g, &b, &e);
     if (e - b <= rows_per_slice) continue;
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < size; i += static_cast<long long>(gridDim.x) * 256) {
+    const int slices = static_cast<int>((e - b + rows_per_slice - 1) / rows_per_slice), each = (slices + 7) / 8, first = warp * each, last = min(slices, first + each);
+    for (long long i0 = static_cast<long long>(blockIdx.x) * 32; i0 < size; i0 += static_cast<long long>(gridDim.x) * 32) {
+      const long long i = i0 + lane;
       float v = 0.f;
-#pragma unroll 4
-      for (long long r = b; r < e; r += rows_per_slice) v += __ldg(partial + (2 * (r / rows_per_slice) + (r == b ? 0 : 1)) * size + i);
-      static_cast<O*>(a.out)[g * size + i] = FromFloat<O>(v);
+      if (i < size) {
+#pragma unroll 8
+        for (int s = first; s < last; ++s) v += __ldg(partial + (2 * (b / rows_per_slice + s) + (s == 0 ? 0 : 1)) * size + i);
+      }
+      s_part[warp][lane] = v;
+      __syncthreads();
+      if (warp == 0 && i < size) {
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += s_part[w][lane];
+        static_cast<O*>(a.out)[g * size + i] = FromFloat<O>(v);
+      }
+      __syncthreads();
     }
   }
 }
@@ -1160,18 +1176,21 @@ inline int BytePieces(const void* p, long long stride) {
 }
 // Shared memory of a warp: its ring of rows (an odd number of 16-byte pieces apart) and its leaf's map.
 inline int NarrowPitch(int row_bytes) { const int pieces = (row_bytes + 15) / 16; return 16 * (pieces | 1); }
-inline int NarrowBytes(int tm, int tn, int size, int features) { const int v = 16 / size; return kNarrowRing * 32 * tm * NarrowPitch(features * size) + tn * ((features + v - 1) / v * v) * 4; }
+inline int NarrowBytes(int tm, int tn, int size, int features, int outputs) {
+  const int v = 16 / size, stage = 32 * tm * NarrowPitch(features * size);
+  return kNarrowRing * stage + tn * ((features + v - 1) / v * v) * 4 + NarrowOutputBytes(tm, outputs, size, stage);
+}
 constexpr int kNarrowMostBytes = 216 * 1024;
-inline int NarrowOutputs(int outputs) { return outputs <= 4 ? 4 : outputs <= 8 ? 8 : outputs <= 12 ? 12 : outputs <= 16 ? 16 : 32; }
+inline int NarrowOutputs(int outputs) { return outputs <= 16 ? (outputs + 1) / 2 * 2 : (outputs + 3) / 4 * 4; }      // sums that a lane holds per row
 // Rows short enough for the warps' rings, on 4-byte boundaries; outputs that fit a lane's registers.
 inline bool NarrowProducts(const LeafProductsArgs& a) {
   const int size = a.dtype == kOpFloat32 ? 4 : 2, tn = NarrowOutputs(a.outputs);
-  return a.outputs <= 32 && a.features * size <= kNarrowRowBytes && BytePieces(a.x, a.x_stride * size) >= 4 && kNarrowWarps * NarrowBytes(tn <= 16 ? 2 : 1, tn, size, a.features) <= kNarrowMostBytes;
+  return a.outputs <= 32 && a.features * size <= kNarrowRowBytes && BytePieces(a.x, a.x_stride * size) >= 4 && kNarrowWarps * NarrowBytes(tn <= 16 ? 2 : 1, tn, size, a.features, a.outputs) <= kNarrowMostBytes;
 }
 template <typename T, int TM, int TN>
 void LaunchNarrowProducts(const LeafProductsArgs& a, cudaStream_t s) {
   constexpr int kSize = static_cast<int>(sizeof(T));
-  const int bytes = kNarrowWarps * NarrowBytes(TM, TN, kSize, a.features);
+  const int bytes = kNarrowWarps * NarrowBytes(TM, TN, kSize, a.features, a.outputs);
   static PerDevice allowed;
   AllowSharedMemory(LeafProductsNarrowKernel<T, TM, TN>, kNarrowMostBytes, &allowed);
   const long long tiles = (a.leaves.rows + 32 * TM - 1) / (32 * TM) + a.leaves.leaves;
@@ -1181,10 +1200,17 @@ void LaunchNarrowProducts(const LeafProductsArgs& a, cudaStream_t s) {
 template <typename T>
 void LaunchNarrowProducts(const LeafProductsArgs& a, cudaStream_t s) {
   switch (NarrowOutputs(a.outputs)) {
+    case 2: LaunchNarrowProducts<T, 2, 2>(a, s); return;
     case 4: LaunchNarrowProducts<T, 2, 4>(a, s); return;
+    case 6: LaunchNarrowProducts<T, 2, 6>(a, s); return;
     case 8: LaunchNarrowProducts<T, 2, 8>(a, s); return;
+    case 10: LaunchNarrowProducts<T, 2, 10>(a, s); return;
     case 12: LaunchNarrowProducts<T, 2, 12>(a, s); return;
+    case 14: LaunchNarrowProducts<T, 2, 14>(a, s); return;
     case 16: LaunchNarrowProducts<T, 2, 16>(a, s); return;
+    case 20: LaunchNarrowProducts<T, 1, 20>(a, s); return;
+    case 24: LaunchNarrowProducts<T, 1, 24>(a, s); return;
+    case 28: LaunchNarrowProducts<T, 1, 28>(a, s); return;
     default: LaunchNarrowProducts<T, 1, 32>(a, s);
   }
 }
@@ -1338,7 +1364,7 @@ void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s) {
   FB_LAUNCHED(); FB_KERNEL_CHECK();
   if (!split) return;
   const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
-  const dim3 grid(static_cast<unsigned int>(std::min(64LL, (size + 255) / 256)), std::min(a.leaves.leaves, 1024));
+  const dim3 grid(static_cast<unsigned int>(std::min(256LL, (size + 31) / 32)), std::min(a.leaves.leaves, 1024));
   if (a.out_dtype == kOpFloat32) LeafGramJoinKernel<float><<<grid, 256, 0, s>>>(a, rows, workspace);
   else DispatchHalf(a.out_dtype, [&](auto* p) { LeafGramJoinKernel<std::remove_pointer_t<decltype(p)>><<<grid, 256, 0, s>>>(a, rows, workspace); });
   FB_LAUNCHED(); FB_KERNEL_CHECK();
