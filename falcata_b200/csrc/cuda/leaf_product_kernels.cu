@@ -39,25 +39,13 @@ __device__ __forceinline__ void LeafWindow(const LeafWindows& w, int g, long lon
   *begin = min(max(b, 0LL), w.rows); *end = min(max(e, *begin), w.rows);
 }
 
-// Rows that belong to no leaf: zero. All threads of the grid.
-template <typename T>
-__device__ __forceinline__ void ZeroLeaflessRows(const LeafWindows& w, T* y, int outputs) {
-  long long first, last, unused;
-  LeafWindow(w, 0, &first, &unused); LeafWindow(w, w.leaves - 1, &unused, &last);
-  if (first == 0 && last == w.rows) return;
-  const long long head = first * outputs, tail = last * outputs, total = w.rows * outputs, stride = static_cast<long long>(gridDim.x) * blockDim.x;
-  const long long t = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  for (long long i = t; i < head; i += stride) y[i] = FromFloat<T>(0.f);
-  for (long long i = tail + t; i < total; i += stride) y[i] = FromFloat<T>(0.f);
-}
-
 // The tiles of all leaves one behind the other: `rows` rows each, a leaf's last one shorter. Up to kSpans leaves are looked up by
 // bisection; more are counted in spans of several leaves.
 constexpr int kSpans = 1024;
 struct TileMap {
   int before[kSpans + 1];        // tiles before span i
   int row[kSpans + 1];           // with a leaf per span: its first row
-  int per, spans;
+  int per, spans, first_row, last_row;      // rows of all leaves: [first_row, last_row)
   __device__ __forceinline__ static int Count(const LeafWindows& w, int g, int rows, int least) {
     long long b, e; LeafWindow(w, g, &b, &e);
     return max(least, static_cast<int>((e - b + rows - 1) / rows));
@@ -68,11 +56,15 @@ struct TileMap {
     if (threadIdx.x == 0) { per = p; spans = n; }
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
       int c = 0;
-      for (int g = i * p; g < min(w.leaves, (i + 1) * p); ++g) c += Count(w, g, rows, least);
+      long long b = 0, e = 0;
+      for (int g = i * p; g < min(w.leaves, (i + 1) * p); ++g) {
+        LeafWindow(w, g, &b, &e);
+        if (g == i * p) row[i] = static_cast<int>(b);
+        c += max(least, static_cast<int>((e - b + rows - 1) / rows));
+      }
       before[i + 1] = c;
-      long long b, e; LeafWindow(w, min(w.leaves - 1, i * p), &b, &e);
-      row[i] = static_cast<int>(b);
-      if (i == n - 1) row[n] = static_cast<int>(e);
+      if (i == 0) first_row = row[0];
+      if (i == n - 1) row[n] = last_row = static_cast<int>(e);      // with several leaves per span only the last use of row[] is this one
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -92,8 +84,8 @@ struct TileMap {
   // tile -> leaf, its first row and the end of the rows that it covers. `span`: where the last search of an earlier tile ended (0 at
   // first); the next tile is mostly a few leaves on.
   __device__ __forceinline__ void Find(const LeafWindows& w, int tile, int rows, int least, int* span, int* leaf, int* first, int* end) const {
-    int lo = *span, step = 0;
-    while (step < 8 && before[lo + 1] <= tile) { ++lo; ++step; }
+    int lo = *span;
+    if (before[lo + 1] <= tile && lo + 1 < spans) ++lo;
     if (before[lo + 1] <= tile) { int hi = spans; while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (before[mid] <= tile) lo = mid; else hi = mid; } }
     *span = lo;
     int g = lo * per, left = tile - before[lo], b = row[lo], e = row[lo + 1];
@@ -105,13 +97,23 @@ struct TileMap {
     e = max(e, b);
     *leaf = g; *first = static_cast<int>(min(static_cast<long long>(e), b + static_cast<long long>(left) * rows)); *end = static_cast<int>(min(static_cast<long long>(e), static_cast<long long>(*first) + rows));
   }
-  // tiles before leaf g
-  __device__ __forceinline__ int Before(const LeafWindows& w, int g, int rows, int least) const {
-    int first = before[g / per];
-    for (int o = g / per * per; o < g; ++o) first += Count(w, o, rows, least);
-    return first;
+  // the rows of leaf g
+  __device__ __forceinline__ void Rows(const LeafWindows& w, int g, int* b, int* e) const {
+    if (per == 1) { *b = row[g]; *e = max(row[g], row[g + 1]); return; }
+    long long b64, e64; LeafWindow(w, g, &b64, &e64);
+    *b = static_cast<int>(b64); *e = static_cast<int>(e64);
   }
 };
+
+// Rows that belong to no leaf: zero. All threads of the grid, when the map is built.
+template <typename T>
+__device__ __forceinline__ void ZeroLeaflessRows(const TileMap& map, const LeafWindows& w, T* y, int outputs) {
+  if (map.first_row == 0 && map.last_row == w.rows) return;
+  const long long head = static_cast<long long>(map.first_row) * outputs, tail = static_cast<long long>(map.last_row) * outputs, total = w.rows * outputs;
+  const long long t = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x, stride = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = t; i < head; i += stride) y[i] = FromFloat<T>(0.f);
+  for (long long i = tail + t; i < total; i += stride) y[i] = FromFloat<T>(0.f);
+}
 
 // ------------------------------------------------------------------------------------------------------- fp32 ----
 struct F2 { unsigned long long v; };
@@ -183,8 +185,8 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
   extern __shared__ __align__(16) float s_float[];
   __shared__ TileMap map;
   const int pitch = shape.pitch, buffer = (Tile::ROWS + Tile::OUTS) * pitch;
-  ZeroLeaflessRows(a.leaves, static_cast<float*>(a.y), a.outputs);
   map.Build(a.leaves, Tile::ROWS, 0);
+  ZeroLeaflessRows(map, a.leaves, static_cast<float*>(a.y), a.outputs);
   const int across = (a.outputs + Tile::OUTS - 1) / Tile::OUTS;
   const int tiles = map.Total() * across, grid = gridDim.x;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, wr = warp % WR, wo = warp / WR;
@@ -402,11 +404,11 @@ __global__ void __launch_bounds__(GA * GB * SLICES, 2) LeafGramFloatKernel(LeafG
 }
 
 // --------------------------------------------------------------------------------------- few columns, any type ----
-// With at most 32 outputs and short rows the products are a matter of bandwidth: 14 warps per SM, each by itself, walk through tiles of
-// rows that come by asynchronous copies into the warp's own ring, so that about 100 KB per SM are on their way and no warp waits
+// With at most 32 outputs and short rows the products are a matter of bandwidth: 12 warps per SM, each by itself, walk through tiles of
+// rows that come by asynchronous copies into the warp's own ring, so that about 90 KB per SM are on their way and no warp waits
 // for another. A warp's tiles are neighbours, so a leaf's map is loaded (as fp32) when the leaf changes. fp32 sums over even and
 // over odd features in one 64-bit register.
-constexpr int kNarrowWarps = 14, kNarrowThreads = 32 * kNarrowWarps, kNarrowRing = 2, kNarrowRowBytes = 256;
+constexpr int kNarrowWarps = 12, kNarrowThreads = 32 * kNarrowWarps, kNarrowRing = 2, kNarrowRowBytes = 256;
 // Copies rows to lines `pitch` bytes apart, in pieces of `piece` bytes; by one warp. What is worked out once: where a lane starts.
 struct WarpCopy {
   int piece, per, pitch, row_bytes, line0, piece0, lines_on, pieces_on;
@@ -442,19 +444,19 @@ template <typename T> __device__ __forceinline__ void Pairs(const uint4& q, F2 (
 
 // A warp's share of the tiles of `rows` rows, one behind the other: [first, last) of them.
 struct WarpTiles {
-  int left, span, leaf, row, leaf_end, least;
+  int left, leaf, row, leaf_end, least;
   __device__ __forceinline__ WarpTiles(const TileMap& map, const LeafWindows& w, int rows, int least_) {
     least = least_;
-    const long long total = map.Total(), warps = static_cast<long long>(gridDim.x) * kNarrowWarps, me = static_cast<long long>(blockIdx.x) * kNarrowWarps + threadIdx.x / 32;
-    const int first = static_cast<int>(total * me / warps), last = static_cast<int>(total * (me + 1) / warps);
-    left = last - first; span = 0; leaf = row = leaf_end = 0;
-    if (left > 0) { int end; map.Find(w, first, rows, least, &span, &leaf, &row, &end); long long b, e; LeafWindow(w, leaf, &b, &e); leaf_end = static_cast<int>(e); }
+    const int total = map.Total(), warps = gridDim.x * kNarrowWarps, me = blockIdx.x * kNarrowWarps + threadIdx.x / 32;
+    const int each = total / warps, more = total - each * warps, first = me * each + min(me, more);
+    left = each + (me < more ? 1 : 0); leaf = row = leaf_end = 0;
+    if (left > 0) { int span = 0, end, begin; map.Find(w, first, rows, least, &span, &leaf, &row, &end); map.Rows(w, leaf, &begin, &leaf_end); }
   }
-  __device__ __forceinline__ void Next(const LeafWindows& w, int rows) {
+  __device__ __forceinline__ void Next(const TileMap& map, const LeafWindows& w, int rows) {
     if (--left <= 0) return;
     if (leaf_end - row > rows) row += rows;
     else {
-      do { ++leaf; long long b, e; LeafWindow(w, leaf, &b, &e); row = static_cast<int>(b); leaf_end = static_cast<int>(e); } while (least == 0 && row >= leaf_end && leaf + 1 < w.leaves);
+      do { ++leaf; map.Rows(w, leaf, &row, &leaf_end); } while (least == 0 && row >= leaf_end && leaf + 1 < w.leaves);
     }
   }
 };
@@ -466,37 +468,39 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafProductsNarrowKernel(Le
   constexpr int ROWS = 32 * TM, V = 16 / sizeof(T);
   extern __shared__ __align__(16) unsigned char s_bytes[];
   __shared__ TileMap map;
-  ZeroLeaflessRows(a.leaves, static_cast<T*>(a.y), a.outputs);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, w_pitch = (a.features + V - 1) / V * V;      // features of a map's line in shared memory
   const int stage = ROWS * pitch, y_bytes = NarrowOutputBytes(TM, a.outputs, static_cast<int>(sizeof(T)), stage), of_warp = kNarrowRing * stage + TN * w_pitch * 4 + y_bytes;
   unsigned char* s_x = s_bytes + warp * of_warp;
   float* s_w = reinterpret_cast<float*>(s_x + kNarrowRing * stage);
-  for (int i = lane; i < of_warp / 4; i += 32) reinterpret_cast<unsigned int*>(s_x)[i] = 0u;                // what no copy writes stays zero
+  for (int i = lane; i < of_warp / 16; i += 32) reinterpret_cast<uint4*>(s_x)[i] = make_uint4(0u, 0u, 0u, 0u);      // what no copy writes stays zero
   map.Build(a.leaves, ROWS, 0);
+  ZeroLeaflessRows(map, a.leaves, static_cast<T*>(a.y), a.outputs);
   WarpTiles now(map, a.leaves, ROWS, 0);
   WarpTiles ahead = now;
   const WarpCopy plan(a.features * static_cast<int>(sizeof(T)), pitch, piece, lane);
   auto copy = [&](int slot) {
     if (ahead.left > 0) {
       plan.Copy(s_x + slot * stage, static_cast<const T*>(a.x) + static_cast<long long>(ahead.row) * a.x_stride, a.x_stride * static_cast<long long>(sizeof(T)), min(ROWS, ahead.leaf_end - ahead.row));
-      ahead.Next(a.leaves, ROWS);
+      ahead.Next(map, a.leaves, ROWS);
     }
     CopyCommit();
   };
   copy(0);
   int slot = 0, loaded = -1;
-  for (; now.left > 0; now.Next(a.leaves, ROWS), slot ^= 1) {
+  for (; now.left > 0; now.Next(map, a.leaves, ROWS), slot ^= 1) {
     const int rows = min(ROWS, now.leaf_end - now.row);
+    copy(slot ^ 1);
     if (now.leaf != loaded) {
       loaded = now.leaf;
       const T* w = static_cast<const T*>(a.weight) + loaded * a.weight_leaf_stride;
       const bool by_feature = a.weight_in_stride == 1;
-      for (int e = lane; e < a.outputs * a.features; e += 32) {
-        const int o = by_feature ? e / a.features : e % a.outputs, f = by_feature ? e - o * a.features : e / a.outputs;
-        s_w[o * w_pitch + f] = ToFloat(w[o * a.weight_out_stride + f * a.weight_in_stride]);
-      }
+      const int along = by_feature ? a.features : a.outputs, lines = by_feature ? a.outputs : a.features;
+      const long long along_on = by_feature ? a.weight_in_stride : a.weight_out_stride, line_on = by_feature ? a.weight_out_stride : a.weight_in_stride;
+      const int s_along = by_feature ? 1 : w_pitch, s_line = by_feature ? w_pitch : 1;
+#pragma unroll 8
+      for (int line = 0; line < lines; ++line)
+        for (int c = lane; c < along; c += 32) s_w[line * s_line + c * s_along] = ToFloat(w[line * line_on + c * along_on]);
     }
-    copy(slot ^ 1);
     CopyWait<1>();
     __syncwarp();
     F2 acc[TM][TN];
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafProductsNarrowKernel(Le
 
 // Gram matrices of at most 4 GA columns of a and 4 GB of b (GA GB = 32): a lane has 4 x 4 of the sums, a warp a slice of a leaf's rows.
 constexpr int kGramRows = 32;
-constexpr int GramRing(int size) { return size == 4 ? 2 : 4; }      // of all warps: 172 KB
+constexpr int GramRing(int size) { return size == 4 ? 2 : 4; }      // of all warps: 147 KB
 template <typename T> __device__ __forceinline__ void Four(const void* p, float (&v)[4]);
 template <> __device__ __forceinline__ void Four<float>(const void* p, float (&v)[4]) { const float4 q = *static_cast<const float4*>(p); v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w; }
 template <> __device__ __forceinline__ void Four<__nv_bfloat16>(const void* p, float (&v)[4]) { const uint2 q = *static_cast<const uint2*>(p); Split(Pair(q.x, static_cast<const __nv_bfloat16*>(nullptr)), v[0], v[1]); Split(Pair(q.y, static_cast<const __nv_bfloat16*>(nullptr)), v[2], v[3]); }
@@ -566,7 +570,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafGramNarrowKernel(LeafGr
   unsigned char* mine = s_bytes + warp * RING * STAGE;
   map.Build(a.leaves, rows_per_slice, 1);
   const WarpCopy a_plan(a.a_cols * static_cast<int>(sizeof(T)), A_PITCH, a_piece, lane), b_plan(a.b_cols * static_cast<int>(sizeof(T)), B_PITCH, b_piece, lane);
-  for (WarpTiles slice(map, a.leaves, rows_per_slice, 1); slice.left > 0; slice.Next(a.leaves, rows_per_slice)) {
+  for (WarpTiles slice(map, a.leaves, rows_per_slice, 1); slice.left > 0; slice.Next(map, a.leaves, rows_per_slice)) {
     const int rows = max(0, min(rows_per_slice, slice.leaf_end - slice.row));
     const T* pa = static_cast<const T*>(a.a) + static_cast<long long>(slice.row) * a.a_stride; const T* pb = static_cast<const T*>(a.b) + static_cast<long long>(slice.row) * a.b_stride;
     auto copy = [&](int r0) {
@@ -829,8 +833,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  if constexpr (MODE != kGram) ZeroLeaflessRows(a.leaves, static_cast<O*>(a.out), a.b_size);
   map.Build(a.leaves, a.tile_rows, a.least);
+  if constexpr (MODE != kGram) ZeroLeaflessRows(map, a.leaves, static_cast<O*>(a.out), a.b_size);
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned int tmem = *reinterpret_cast<volatile unsigned int*>(&s_tmem);
   volatile int* stop = &s_stop;
