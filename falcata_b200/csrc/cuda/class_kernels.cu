@@ -210,6 +210,32 @@ struct RowResult {
 };
 
 // ------------------------------------------------------------------------------------------------ few classes ----
+// The results of a row whose scores are in registers.
+template <int MOST>
+__device__ __forceinline__ void FinishRow(const ClassScoresArgs& a, long long row, long long y, float (&v)[MOST]) {
+  if (row >= a.rows) return;
+  Sums sums;
+  float m = v[0];
+#pragma unroll
+  for (int j = 1; j < MOST; ++j) m = MaxNan(m, v[j]);
+  sums.m = m;
+  const float b = sums.Base();
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) sums.Add(v[j], b);
+  const RowResult res(sums);
+  float given = 0.f;
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) if (j == y) given = v[j];
+  res.Store(a, row, y, given);
+  for (int t = 0; t < a.top_k; ++t) {
+    float best = -INFINITY; int cls = -1;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) if (v[j] > best) { best = v[j]; cls = j; }
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) if (j == cls) v[j] = -INFINITY;
+    res.StoreTop(a, row * a.top_k + t, best, cls);
+  }
+}
 // A thread has ROWS rows, each row's scores in MOST registers. Class-major scores are read straight into them, 32 rows per instruction,
 // all rows' loads before the first use; rows go through shared memory (an odd row pitch there, so that neither side meets bank
 // conflicts).
@@ -242,32 +268,8 @@ __global__ void __launch_bounds__(kFewThreads) ClassLogProbsFewKernel(ClassScore
 #pragma unroll
     for (int j = 0; j < MOST; ++j) v[0][j] = j < K ? s_rows[threadIdx.x * pitch + j] : -INFINITY;
   }
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const long long row = row0 + i * kFewThreads + threadIdx.x;
-    if (row >= a.rows) continue;
-    Sums sums;
-    float m = v[i][0];
-#pragma unroll
-    for (int j = 1; j < MOST; ++j) m = MaxNan(m, v[i][j]);
-    sums.m = m;
-    const float b = sums.Base();
-#pragma unroll
-    for (int j = 0; j < MOST; ++j) sums.Add(v[i][j], b);
-    const RowResult res(sums);
-    float given = 0.f;
-#pragma unroll
-    for (int j = 0; j < MOST; ++j) if (j == y[i]) given = v[i][j];
-    res.Store(a, row, y[i], given);
-    for (int t = 0; t < a.top_k; ++t) {
-      float best = -INFINITY; int cls = -1;
-#pragma unroll
-      for (int j = 0; j < MOST; ++j) if (v[i][j] > best) { best = v[i][j]; cls = j; }
-#pragma unroll
-      for (int j = 0; j < MOST; ++j) if (j == cls) v[i][j] = -INFINITY;
-      res.StoreTop(a, row * a.top_k + t, best, cls);
-    }
-  }
+  FinishRow<MOST>(a, row0 + threadIdx.x, y[0], v[0]);
+  if constexpr (ROWS == 2) FinishRow<MOST>(a, row0 + kFewThreads + threadIdx.x, y[1], v[1]);
 }
 
 // Rows of up to kSomeClasses contiguous classes: 8 lanes per row, PER scores each in registers. An alternative at a time: the best of a
