@@ -17,7 +17,8 @@
 //   few classes                 a thread per row, the row in registers           (ClassLogProbsFewKernel)
 //   some, contiguous rows       8 lanes per row, the row in their registers      (ClassLogProbsSomeKernel)
 //   contiguous rows             a warp, or a block or cluster of blocks, per row  (ClassLogProbsWarpKernel, ClassLogProbsBlockKernel)
-//   contiguous columns, others  32 rows per block, the classes over its warps    (ClassLogProbsColumnKernel)
+//   contiguous columns, others  rows gathered in shared memory, a warp per row    (ClassLogProbsTileKernel); very many classes: 32
+//                               rows per block, the classes over its warps          (ClassLogProbsColumnKernel)
 #include "kernels.cuh"
 
 #include <cooperative_groups.h>
@@ -275,12 +276,10 @@ __global__ void __launch_bounds__(kFewThreads) ClassLogProbsFewKernel(ClassScore
 // Rows of up to kSomeClasses contiguous classes: 8 lanes per row, PER scores each in registers. An alternative at a time: the best of a
 // lane's scores, of the 8 lanes', and out of the registers.
 constexpr int kSomeClasses = 256;
+// s: the row (any row where !is_row; a warp's lanes stay together)
 template <typename T, int PER>
-__global__ void __launch_bounds__(128) ClassLogProbsSomeKernel(ClassScoresArgs a) {
-  const int lane8 = threadIdx.x & 7, K = static_cast<int>(a.classes);
-  const long long row = static_cast<long long>(blockIdx.x) * 16 + threadIdx.x / 8;
-  const bool is_row = row < a.rows;               // a warp's lanes stay together
-  const T* s = static_cast<const T*>(a.scores) + (is_row ? row : 0) * a.row_stride;
+__device__ __forceinline__ void SomeRow(const ClassScoresArgs& a, long long row, bool is_row, const T* s, int lane8) {
+  const int K = static_cast<int>(a.classes);
   const long long y = is_row ? LabelOf(a, row) : -1;
   float v[PER];
 #pragma unroll
@@ -312,6 +311,12 @@ __global__ void __launch_bounds__(128) ClassLogProbsSomeKernel(ClassScoresArgs a
     }
     if (is_row && lane8 == 0) res.StoreTop(a, row * a.top_k + t, best, cls);
   }
+}
+template <typename T, int PER>
+__global__ void __launch_bounds__(128) ClassLogProbsSomeKernel(ClassScoresArgs a) {
+  const long long row = static_cast<long long>(blockIdx.x) * 16 + threadIdx.x / 8;
+  const bool is_row = row < a.rows;
+  SomeRow<T, PER>(a, row, is_row, static_cast<const T*>(a.scores) + (is_row ? row : 0) * a.row_stride, threadIdx.x & 7);
 }
 
 // -------------------------------------------------------------------------------------------- contiguous rows ----
@@ -384,6 +389,10 @@ struct RowShare {
     v_begin = min(vectors, part * each); v_end = min(vectors, v_begin + each);
     first = part == 0; last_part = part == parts - 1;
   }
+  // a whole row in shared memory, padded with -inf to 16-byte pieces
+  __device__ __forceinline__ RowShare(const T* row, int classes) {
+    s = row; K = classes; head = 0; v_begin = 0; v_end = (classes + Pack<T>::N - 1) / Pack<T>::N; tail = v_end * Pack<T>::N; body = reinterpret_cast<const uint4*>(row); first = last_part = true;
+  }
   // the scores outside the 16-byte pieces, one per thread (-inf: none)
   __device__ __forceinline__ float Head(int tid) const { return first && tid < head ? ToFloat(s[tid]) : -INFINITY; }
   __device__ __forceinline__ float Tail(int tid) const { return last_part && tid < K - tail ? ToFloat(s[tail + tid]) : -INFINITY; }
@@ -421,14 +430,24 @@ struct Walk {
     asm volatile("cp.async.commit_group;" ::: "memory");
     ahead_slot = ahead_slot == RING - 1 ? 0 : ahead_slot + 1;
   }
-  // the chunk (its first piece) that held this thread's maximum, and the best of the others
-  int best_at; float second;
+  // of this thread (a lone warp: of each of a lane's 4 pieces by itself): the maximum, the chunk (its first piece) that held it, and
+  // the best of the other chunks
+  static constexpr int kOf = GROUP == 32 ? kUnroll : 1;
+  float best[kOf], second[kOf]; int best_at[kOf];
+  __device__ __forceinline__ void Note(int u, float most, int at) { if (most > best[u]) { second[u] = best[u]; best[u] = most; best_at[u] = at; } else second[u] = fmaxf(second[u], most); }
+  __device__ __forceinline__ float NotePieces(const uint4 (&q)[kUnroll], int at) {
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kOf; ++u) { const uint4 one[1] = {q[u]}; const float m = MaxOf(one, static_cast<const T*>(nullptr)); Note(u, m, at); most = MaxNan(most, m); }
+    return most;
+  }
   // This thread's sums of the pieces of the next row's share; m is its maximum.
   __device__ __forceinline__ Sums Row(const RowShare<T>& r) {
     const T* type = nullptr;
     PairSums<T> pairs;
     int at = r.v_begin;
-    best_at = at; second = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kOf; ++u) { best[u] = second[u] = -INFINITY; best_at[u] = at; }
     do {                                         // a share without pieces takes one empty step
       CopyAhead();
       asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
@@ -437,11 +456,11 @@ struct Walk {
         uint4 q[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) q[u] = GROUP > 32 || at + u * GROUP + tid < r.v_end ? from[u * 256] : AllRuledOut(type);
-        const float most = MaxOf(q, type);
-        if (most > pairs.m) { second = pairs.m; best_at = at; pairs.Raise(most); } else second = fmaxf(second, most);
+        float most;
+        if constexpr (kOf == 1) { most = MaxOf(q, type); Note(0, most, at); } else most = NotePieces(q, at);
+        if (most > pairs.m) pairs.Raise(most);
         pairs.Add16(q);
       } else {                                   // the last chunk, piece by piece
-        const float before = pairs.m;
         float most = -INFINITY;
 #pragma unroll 1
         for (int u = 0; u < kUnroll && (u == 0 || at + u * GROUP + (tid & ~31) < r.v_end); ++u) {
@@ -451,7 +470,7 @@ struct Walk {
           if (here > pairs.m) pairs.Raise(here);
           pairs.Add16(one);
         }
-        if (most > before) { second = before; best_at = at; } else second = fmaxf(second, most);
+        Note(0, most, at);
       }
       at += GROUP * kUnroll;
       slot = slot == RING - 1 ? 0 : slot + 1;
@@ -460,23 +479,25 @@ struct Walk {
   }
 };
 
-// One warp finds the alternatives of a share that GROUP threads have walked.
+// One warp finds the alternatives of a share that GROUP walkers have walked, in chunks of CHUNK pieces of each. The walkers are a block's
+// threads (256, chunks of 4), or, where a warp walks alone, the 4 pieces of a lane's chunk taken by themselves (128, of 1), so
+// that there are enough walkers for 32 alternatives.
 template <int GROUP>
 struct TopShared {
-  static constexpr int kFlagged = 64, kCandidates = GROUP == 32 ? 128 : 256;
+  static constexpr int kFlagged = 64, kCandidates = GROUP == 128 ? 128 : 256;
   Entry list[kMaxTopClasses], cand[kCandidates];
   int flagged[kFlagged], flagged_at[kFlagged], num_flagged, num_cand;      // threads; the chunk to look at (-1: all of the thread's share)
 };
 template <int GROUP, typename T>
 struct Alternatives {
-  static constexpr int N = Pack<T>::N, PER = GROUP / 32;
+  static constexpr int N = Pack<T>::N, PER = GROUP / 32, CHUNK = GROUP == 128 ? 1 : kUnroll;
   TopShared<GROUP>& sh; const RowShare<T>& r; int top_k, lane;
   // f(score, class) for the scores that reach `limit` among piece `at` of the share (each lane its own; at >= v_end: none)
   template <int COUNT, typename F>
   __device__ __forceinline__ void Pieces(const int (&at)[COUNT], float limit, F&& f) const {
     uint4 q[COUNT];
 #pragma unroll
-    for (int u = 0; u < COUNT; ++u) q[u] = at[u] < r.v_end ? __ldg(r.body + at[u]) : AllRuledOut(static_cast<const T*>(nullptr));
+    for (int u = 0; u < COUNT; ++u) q[u] = at[u] < r.v_end ? r.body[at[u]] : AllRuledOut(static_cast<const T*>(nullptr));
 #pragma unroll
     for (int u = 0; u < COUNT; ++u) {
       const uint4 one[1] = {q[u]};
@@ -493,14 +514,14 @@ struct Alternatives {
     const float head_v = r.Head(lane), tail_v = r.Tail(lane);
     if (head_v >= limit) f(head_v, lane);
     if (tail_v >= limit) f(tail_v, r.tail + lane);
-    static_assert(kUnroll == 4, "a chunk is 4 pieces of a thread");
-    for (int e0 = lane; e0 < 4 * num_flagged; e0 += 128) {
-      int at[4];
+    constexpr int kAtOnce = CHUNK == 1 ? 2 : 4;
+    for (int e0 = lane; e0 < CHUNK * num_flagged; e0 += 32 * kAtOnce) {
+      int at[kAtOnce];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int e = e0 + 32 * u, which = e >> 2;
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int e = e0 + 32 * u, which = e / CHUNK;
         const int chunk = which < num_flagged ? sh.flagged_at[which] : -1;
-        at[u] = chunk >= 0 ? chunk + (e & 3) * GROUP + sh.flagged[which] : 0x7fffffff;
+        at[u] = chunk >= 0 ? chunk + (e % CHUNK) * GROUP + sh.flagged[which] : 0x7fffffff;
       }
       Pieces(at, limit, f);
     }
@@ -537,7 +558,7 @@ struct Alternatives {
     }
     if (lane == 0) sh.num_cand = 0;
     __syncwarp();
-    if (GROUP > 32 && flagged > TopShared<GROUP>::kFlagged) flagged = Ties(keys, limit, &last);
+    if (flagged > TopShared<GROUP>::kFlagged) flagged = Ties(keys, limit, &last);
     const float limit_score = KeyScore<T>(limit);
     Scores(flagged, limit_score, [&](float v, int cls) {
       if (v > limit_score || cls <= last) { const int at = atomicAdd(&sh.num_cand, 1); if (at < TopShared<GROUP>::kCandidates) { sh.cand[at].v = v; sh.cand[at].cls = cls; } }
@@ -559,7 +580,7 @@ struct Alternatives {
       int at = 0x7fffffff;
       for (int p = r.v_begin + thread; p < r.v_end && at == 0x7fffffff; p += GROUP) {
         float v[N];
-        Unpack(__ldg(r.body + p), v, static_cast<const T*>(nullptr));
+        Unpack(r.body[p], v, static_cast<const T*>(nullptr));
 #pragma unroll
         for (int k = N - 1; k >= 0; --k) if (OrderKey<T>(v[k]) == limit) at = r.head + p * N + k;
       }
@@ -599,7 +620,7 @@ constexpr int kWarpRing = 3;
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(256, 4) ClassLogProbsWarpKernel(ClassScoresArgs a) {
   extern __shared__ __align__(16) uint4 s_ring[];      // [kWarpRing][kUnroll][256]
-  __shared__ TopShared<32> s_top[TOP ? 8 : 1];
+  __shared__ TopShared<128> s_top[TOP ? 8 : 1];
   const int lane = threadIdx.x % 32;
   const unsigned int stride = gridDim.x * 8;      // unsigned: row + stride may pass 2^31
   unsigned int row = blockIdx.x * 8 + threadIdx.x / 32;
@@ -611,16 +632,17 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsWarpKernel(ClassScoresArg
     const float head_v = r.Head(lane), tail_v = r.Tail(lane), given = lane == 0 && y >= 0 && y < r.K ? ToFloat(r.s[y]) : 0.f;
     const long long y_next = row + stride < a.rows ? LabelOf(a, row + stride) : -1;
     Sums sums = walk.Row(r);
-    const float most = sums.m;
     if (head_v != -INFINITY) sums.AddOne(head_v);
     if (tail_v != -INFINITY) sums.AddOne(tail_v);
     sums.JoinLanes();
     const RowResult res(sums);
     if (lane == 0) res.Store(a, row, y, given);
     if constexpr (TOP) {
-      Alternatives<32, T> alt{s_top[threadIdx.x / 32], r, a.top_k, lane};
-      const unsigned int keys[1] = {OrderKey<T>(most)}, second[1] = {OrderKey<T>(walk.second)};
-      const int chunk[1] = {walk.best_at}, have = alt.Find(keys, second, chunk);
+      Alternatives<128, T> alt{s_top[threadIdx.x / 32], r, a.top_k, lane};
+      unsigned int keys[kUnroll], second[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) { keys[u] = OrderKey<T>(walk.best[u]); second[u] = OrderKey<T>(walk.second[u]); }
+      const int have = alt.Find(keys, second, walk.best_at);
       if (lane < a.top_k) { const Entry e = alt.sh.list[lane]; res.StoreTop(a, row * a.top_k + lane, lane < have ? e.v : -INFINITY, e.cls); }
       __syncwarp();
     }
@@ -654,12 +676,11 @@ __global__ void __launch_bounds__(kBlockThreads, 4) ClassLogProbsBlockKernel(Cla
       const RowShare<T> r(a, row, part, parts, 256);
       const float head_v = r.Head(threadIdx.x), tail_v = r.Tail(threadIdx.x);
       Sums sums = walk.Row(r);
-      const float most = sums.m;
       if (head_v != -INFINITY) sums.AddOne(head_v);
       if (tail_v != -INFINITY) sums.AddOne(tail_v);
       sums.JoinLanes();
       if (row != row0) BarrierSync<kFree>();
-      if constexpr (TOP) { s_key[threadIdx.x] = OrderKey<T>(most); s_second[threadIdx.x] = OrderKey<T>(walk.second); s_chunk[threadIdx.x] = walk.best_at; }
+      if constexpr (TOP) { s_key[threadIdx.x] = OrderKey<T>(walk.best[0]); s_second[threadIdx.x] = OrderKey<T>(walk.second[0]); s_chunk[threadIdx.x] = walk.best_at[0]; }
       if (lane == 0) { s_m[warp] = sums.m; s_s[warp] = sums.s; s_t[warp] = sums.t; }
       BarrierArrive<kFull>();
       if (parts > 1) {
@@ -744,6 +765,81 @@ __global__ void __launch_bounds__(kBlockThreads, 4) ClassLogProbsBlockKernel(Cla
 }
 
 // ----------------------------------------------------------------------------------------- contiguous columns ----
+// A block turns tile_rows rows of class-major scores (or of any strides) into rows in shared memory, read as they lie: neighbouring
+// lanes have neighbouring rows. Then a warp per row, as above. Rows up to kTileBytes / 8 classes' worth of bytes long.
+// (Against the kernel below, which keeps a list per thread: 2479 x 2000 fp32 with 32 alternatives 230 -> 34 us.)
+constexpr int kTileBytes = 72 * 1024, kTileMostBytes = 200 * 1024;
+// PER > 0: at most 8 PER classes, 8 lanes per row.
+template <typename T, bool TOP, int PER>
+__global__ void __launch_bounds__(256) ClassLogProbsTileKernel(ClassScoresArgs a, int tile_rows, int pitch) {
+  constexpr int N = Pack<T>::N;
+  extern __shared__ __align__(16) unsigned char s_tile[];
+  __shared__ TopShared<128> s_top[TOP ? 8 : 1];
+  const int K = static_cast<int>(a.classes), warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const long long row0 = static_cast<long long>(blockIdx.x) * tile_rows;
+  const int rows = static_cast<int>(min(static_cast<long long>(tile_rows), a.rows - row0));
+  {
+    const int r = threadIdx.x % tile_rows, step = 256 / tile_rows;
+    if (r < rows) {
+      const T* from = static_cast<const T*>(a.scores) + (row0 + r) * a.row_stride;
+      T* to = reinterpret_cast<T*>(s_tile + r * pitch);
+      int c = threadIdx.x / tile_rows;
+      for (; c + 7 * step < K; c += 8 * step) {
+        T v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = from[(c + u * step) * a.class_stride];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) to[c + u * step] = v[u];
+      }
+      for (; c < (K + N - 1) / N * N; c += step) to[c] = c < K ? from[c * a.class_stride] : FromFloat<T>(-INFINITY);
+    }
+  }
+  __syncthreads();
+  if constexpr (PER > 0) {
+    for (int i0 = 0; i0 < rows; i0 += 32) {
+      const int i = i0 + threadIdx.x / 8;
+      SomeRow<T, PER>(a, row0 + i, i < rows, reinterpret_cast<const T*>(s_tile + min(i, rows - 1) * pitch), threadIdx.x & 7);
+    }
+    return;
+  }
+  for (int i = warp; i < rows; i += 8) {
+    const long long row = row0 + i;
+    const RowShare<T> r(reinterpret_cast<const T*>(s_tile + i * pitch), K);
+    const long long y = LabelOf(a, row);
+    PairSums<T> pairs;
+    float best[kUnroll], second[kUnroll]; int best_at[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) { best[u] = second[u] = -INFINITY; best_at[u] = 0; }
+    for (int at = 0; at < r.v_end; at += 32 * kUnroll) {
+      uint4 q[kUnroll];
+      float most = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        q[u] = at + 32 * u + lane < r.v_end ? r.body[at + 32 * u + lane] : AllRuledOut(static_cast<const T*>(nullptr));
+        const uint4 one[1] = {q[u]};
+        const float m = MaxOf(one, static_cast<const T*>(nullptr));
+        if (m > best[u]) { second[u] = best[u]; best[u] = m; best_at[u] = at; } else second[u] = fmaxf(second[u], m);
+        most = MaxNan(most, m);
+      }
+      if (most > pairs.m) pairs.Raise(most);
+      pairs.Add16(q);
+    }
+    Sums sums = pairs.Total();
+    sums.JoinLanes();
+    const RowResult res(sums);
+    if (lane == 0) res.Store(a, row, y, y >= 0 && y < K ? ToFloat(r.s[y]) : 0.f);
+    if constexpr (TOP) {
+      Alternatives<128, T> alt{s_top[warp], r, a.top_k, lane};
+      unsigned int keys[kUnroll], seconds[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) { keys[u] = OrderKey<T>(best[u]); seconds[u] = OrderKey<T>(second[u]); }
+      const int have = alt.Find(keys, seconds, best_at);
+      if (lane < a.top_k) { const Entry e = alt.sh.list[lane]; res.StoreTop(a, row * a.top_k + lane, lane < have ? e.v : -INFINITY, e.cls); }
+      __syncwarp();
+    }
+  }
+}
+
 // 32 rows per block (lane = row, so class-major scores are read 32 rows at a time), the classes dealt out over the warps; every
 // thread keeps its own sums and its own sorted list, joined per row at the end.
 constexpr int kColumnUnroll = 8;
@@ -1011,6 +1107,15 @@ void LaunchBlocks(const ClassScoresArgs& a, int cluster, cudaStream_t s) {
   FB_CUDA(cudaLaunchKernelEx(&cfg, ClassLogProbsBlockKernel<T, TOP>, a));
 }
 
+// an odd number of 16-byte pieces: rows of a tile start in different banks
+template <typename T> long long TilePitch(long long classes) { return 16 * (((classes * static_cast<long long>(sizeof(T)) + 15) / 16) | 1); }
+template <typename T, bool TOP, int PER>
+void LaunchTiles(const ClassScoresArgs& a, int rows, int pitch, cudaStream_t s) {
+  static PerDevice allowed;
+  AllowSharedMemory(ClassLogProbsTileKernel<T, TOP, PER>, kTileMostBytes, &allowed);
+  ClassLogProbsTileKernel<T, TOP, PER><<<static_cast<unsigned int>((a.rows + rows - 1) / rows), 256, static_cast<size_t>(rows) * pitch, s>>>(a, rows, pitch);
+}
+
 }  // namespace
 
 void LaunchClassLogProbs(const ClassScoresArgs& a, cudaStream_t s) {
@@ -1035,6 +1140,15 @@ void LaunchClassLogProbs(const ClassScoresArgs& a, cudaStream_t s) {
         while (cluster < 8 && a.rows * cluster < 2 * kSms && a.classes >= 2 * cluster * chunk / kUnroll) cluster *= 2;
         if (a.top_k > 0) LaunchBlocks<T, true>(a, cluster, s); else LaunchBlocks<T, false>(a, cluster, s);
       }
+    } else if (TilePitch<T>(a.classes) * 8 <= kTileMostBytes) {
+      const int pitch = static_cast<int>(TilePitch<T>(a.classes));
+      int rows = 32;      // per tile: as many as leave room for three blocks on an SM, and no fewer than fill a 32-byte sector
+      while (rows > 32 / static_cast<int>(sizeof(T)) && rows * pitch > kTileBytes) rows /= 2;
+      while (rows > 8 && rows * pitch > kTileMostBytes) rows /= 2;
+      if (a.classes <= 128) LaunchTiles<T, false, 16>(a, rows, pitch, s);
+      else if (a.classes <= kSomeClasses) LaunchTiles<T, false, 32>(a, rows, pitch, s);
+      else if (a.top_k > 0) LaunchTiles<T, true, 0>(a, rows, pitch, s);
+      else LaunchTiles<T, false, 0>(a, rows, pitch, s);
     } else {
       int warps = 8;
       while (warps < 32 && (a.rows + 31) / 32 * warps < kSms * 32 && a.classes > 2LL * warps * kColumnUnroll) warps *= 2;

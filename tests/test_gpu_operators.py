@@ -86,7 +86,7 @@ def _check_forward(scores, labels, top):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("layout", ["row", "class", "padded", "strided"])
-@pytest.mark.parametrize("n,k,top", [(1, 1, 1), (5, 2, 2), (1000, 3, 0), (257, 10, 3), (33, 31, 31), (64, 64, 5), (65, 65, 32), (7, 127, 4), (130, 1000, 20), (3, 1025, 1), (9, 4099, 32), (2, 50021, 20)])
+@pytest.mark.parametrize("n,k,top", [(1, 1, 1), (5, 2, 2), (1000, 3, 0), (257, 10, 3), (33, 31, 31), (64, 64, 5), (65, 65, 32), (7, 127, 4), (130, 1000, 20), (3, 1025, 1), (9, 4099, 32), (41, 6401, 3), (2, 50021, 20)])
 def test_class_log_probs(dtype, layout, n, k, top):
     scores = _scores(n, k, dtype, layout, seed=n + k)
     labels = torch.randint(-1, k, (n,), generator=_gen(1), device="cuda")
