@@ -1267,6 +1267,19 @@ class Booster:
             return out.reshape(nrow, -1)
         return out
 
+    def predict_log_probs(self, data: Any, label: Any = None, top_k: int = 0, start_iteration: int = 0, num_iteration: Optional[int] = None) -> Any:
+        """Log probabilities of a multiclass model on the device: per row of a CUDA matrix the log probability of ``label`` (int32 /
+        int64 CUDA tensor, negative: none), the log of the softmax's normaliser, the entropy of the class distribution and
+        the ``top_k`` best classes (``falcata_b200.ops.ClassLogProbs``), without the probabilities being written out."""
+        from .ops import class_log_probs
+
+        if not _is_cuda_array(data):
+            raise TypeError("predict_log_probs needs the rows as a CUDA tensor")
+        if self.num_model_per_iteration() < 2 or self._objective_from_model() != "multiclass":
+            raise FalcataError("predict_log_probs needs a multiclass (softmax) model")
+        scores = self.predict(data, start_iteration=start_iteration, num_iteration=num_iteration, raw_score=True)
+        return class_log_probs(scores, label, top_k=top_k)
+
     def _predict_csr(self, csr: Any, ptype: int, start_iteration: int, num_iteration: int, pred_leaf: bool, pred_contrib: bool, kwargs: Dict[str, Any]) -> Any:
         lib = _lib()
         nrow, ncol = csr.shape

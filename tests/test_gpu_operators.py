@@ -423,6 +423,24 @@ def test_forest_leaves_with_class_heads():
     assert torch.allclose(gx.double(), rx, rtol=1e-4, atol=1e-9 + 256 * U / 3000) and torch.allclose(gw.double(), rw, rtol=1e-4, atol=4096 * U / 15)
 
 
+def test_booster_log_probs():
+    """The log probabilities of a model's answers agree with its probabilities."""
+    import falcata_b200 as fb
+    from util import make_multiclass
+    X, y = make_multiclass(n=1500, f=8, k=5)
+    bst = fb.train({"objective": "multiclass", "num_class": 5, "num_leaves": 15, "device_type": "cuda", "verbosity": -1}, fb.Dataset(X, y), 5)
+    Xd, labels = torch.from_numpy(X).cuda(), torch.from_numpy(y).cuda().long()
+    r, p = bst.predict_log_probs(Xd, labels, top_k=2), bst.predict(Xd).double()
+    # the probabilities are fp32 with a few roundings each, relative 64 u at most
+    assert torch.allclose(r.log_prob.double(), p.gather(1, labels[:, None])[:, 0].log(), atol=64 * U) and torch.allclose(r.entropy.double(), -(p * p.log()).sum(1), atol=5 * 64 * U)
+    assert torch.allclose(r.top_log_prob.double(), p.topk(2, 1).values.log(), atol=64 * U)
+    with pytest.raises(TypeError):
+        bst.predict_log_probs(X)
+    binary = fb.train({"objective": "binary", "num_leaves": 7, "device_type": "cuda", "verbosity": -1}, fb.Dataset(X, (y > 2).astype("float32")), 2)
+    with pytest.raises(fb.FalcataError):
+        binary.predict_log_probs(Xd)
+
+
 def test_custom_objective_from_class_log_probs():
     """The training scores that a custom objective sees are class-major; the gradient goes back without a copy."""
     import falcata_b200 as fb
