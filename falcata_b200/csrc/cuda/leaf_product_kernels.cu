@@ -622,8 +622,10 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafGramNarrowKernel(LeafGr
   }
 }
 
-// Adds the sums of the slices of each leaf that has several, always in the same order: a warp has 32 neighbouring sums and an eighth of
-// the slices, the eighths are added up at the end.
+// Adds the sums of the slices of each leaf that has several, always in the same order. Few slices: a thread adds all of its four sums'
+// slices. More: a warp has 32 neighbouring sums and an eighth of the slices, the eighths are added up at the end (the only form before:
+// 31 slices of 15 leaves' 513 x 1000 sums, half of them joined, took 151 us, a block's two barriers for every 32 sums).
+constexpr int kFewSlices = 16;
 template <typename O>
 __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int rows_per_slice, const float* __restrict__ partial) {
   __shared__ float s_part[8][32];
@@ -633,12 +635,31 @@ __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int ro
     long long b, e; LeafWindow(a.leaves, g, &b, &e);
     if (e - b <= rows_per_slice) continue;
     const int slices = static_cast<int>((e - b + rows_per_slice - 1) / rows_per_slice), each = (slices + 7) / 8, first = warp * each, last = min(slices, first + each);
+    const float* of_leaf = partial + 2 * (b / rows_per_slice) * size;      // first slice here, the others one place and two places apart
+    if (slices <= kFewSlices) {
+      const long long on = 2 * size;
+      for (long long i0 = static_cast<long long>(blockIdx.x) * 1024 + threadIdx.x; i0 < size; i0 += static_cast<long long>(gridDim.x) * 1024) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = i0 + 256 * j < size ? __ldg(of_leaf + i0 + 256 * j) : 0.f;
+        const float* from = of_leaf + size + i0;
+#pragma unroll 2
+        for (int s = 1; s < slices; ++s) {
+          from += on;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) if (i0 + 256 * j < size) v[j] += __ldg(from + 256 * j);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (i0 + 256 * j < size) static_cast<O*>(a.out)[g * size + i0 + 256 * j] = FromFloat<O>(v[j]);
+      }
+      continue;
+    }
     for (long long i0 = static_cast<long long>(blockIdx.x) * 32; i0 < size; i0 += static_cast<long long>(gridDim.x) * 32) {
       const long long i = i0 + lane;
       float v = 0.f;
       if (i < size) {
 #pragma unroll 8
-        for (int s = first; s < last; ++s) v += __ldg(partial + (2 * (b / rows_per_slice + s) + (s == 0 ? 0 : 1)) * size + i);
+        for (int s = first; s < last; ++s) v += __ldg(of_leaf + (2 * s + (s == 0 ? 0 : 1)) * size + i);
       }
       s_part[warp][lane] = v;
       __syncthreads();
@@ -694,7 +715,7 @@ __global__ void __launch_bounds__(256) PackLinesKernel(const unsigned short* __r
 // reach only outputs that are not stored; in a Gram's last step, where they would be summed, the copying warps bring the rows
 // that belong to the slice and zeros (unless the slice ends at a multiple of 16 rows, the depth of an instruction).
 // Warps: 0-3 store the accumulators, 4-11 copy, 12 issues the matrix instructions. Every wait is bounded; one that gives up
-// makes all roles leave, the tile's outputs NaN and the device's status word 1.
+// makes all roles leave; the outputs of every tile that is not finished are NaN then.
 constexpr int kDepthTc = 64, kTileM = 128, kMostN = 256;
 constexpr int kCopyWarps = 8, kCopyThreads = 32 * kCopyWarps, kTcThreads = 128 + kCopyThreads + 32;
 constexpr int kMostStages = 8;
@@ -704,7 +725,6 @@ constexpr int kABytes = kTileM * 128;
 // row is stored by neighbouring lanes (stored by its own lane, value by value, 200000 x 100 -> 100 took 130 us, of it 100 for the stores).
 constexpr int kStorePitch = 33, kStoreBytes = 4 * 32 * kStorePitch * 4;      // words: a row's 64 values and one to spare
 
-__device__ unsigned int g_product_status;
 
 __device__ __forceinline__ void BarInit(unsigned long long* bar, unsigned int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(Smem32(bar)), "r"(count) : "memory"); }
 __device__ __forceinline__ void BarArrive(unsigned long long* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(Smem32(bar)) : "memory"); }
@@ -716,7 +736,7 @@ __device__ __forceinline__ bool BarTry(unsigned long long* bar, unsigned int par
 // false: the budget ran out, here or in another role
 __device__ __forceinline__ bool BarWait(unsigned long long* bar, unsigned int parity, volatile int* stop) {
   for (int i = 0; i < (1 << 20); ++i) { if (BarTry(bar, parity)) return true; if (*stop != 0) return false; }
-  *stop = 1; atomicExch(&g_product_status, 1u);
+  *stop = 1;
   return false;
 }
 __device__ __forceinline__ void MmaCommit(unsigned long long* bar) {
@@ -731,7 +751,7 @@ __device__ __forceinline__ void Mma16(unsigned int d, unsigned long long da, uns
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
                ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(0u) : "memory");
 }
-__device__ __forceinline__ void TmemLoad16(unsigned int addr, unsigned int (&v)[16]) {
+__device__ __forceinline__ void TmemLoad16(unsigned int addr, unsigned int* v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                : "r"(addr) : "memory");
@@ -1040,28 +1060,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
           }
           __syncwarp();
         }
-      } else
-      for (int n0 = 0; n0 < n_end; n0 += 16) {
-        unsigned int v[16];
-        if (tile.depth > 0 && ok) {
-          TmemLoad16(tmem + acc * (a.tmem_cols / 2) + (static_cast<unsigned int>(warp * 32) << 16) + n0, v);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        } else {
+      } else {
+        // columns at a time: 32 took 50000 x 512 -> 1000 from 95 to 85 us, a Gram of 2000 x 1000 from 440 to 450
+        constexpr int kOnce = MODE == kGram ? 16 : 32;
+        for (int c0 = 0; c0 < n_end; c0 += kOnce) {
+          unsigned int v[kOnce];
+          if (tile.depth > 0 && ok) {
+            const unsigned int from = tmem + acc * (a.tmem_cols / 2) + (static_cast<unsigned int>(warp * 32) << 16) + c0;
+            TmemLoad16(from, v);
+            if constexpr (kOnce == 32) { if (c0 + 16 < a.n) TmemLoad16(from + 16, v + 16); }
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = ok ? 0u : 0x7fc00000u;
-        }
-        if (m >= m_end) continue;
-        if (part != nullptr) {
+            for (int j = 0; j < kOnce; ++j) v[j] = ok ? 0u : 0x7fc00000u;
+          }
+          if (m < m_end) {
+            if (part != nullptr) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) if (n0 + j < n_end) part[(n0 + j) * a.out_col_stride] = __uint_as_float(v[j]);
-        } else if (a.out_col_stride == 1 && sizeof(O) == 2 && n0 + 16 <= n_end && (reinterpret_cast<uintptr_t>(out + n0) & 15) == 0) {
-          union { O o[16]; uint4 q[2]; } u;
+              for (int j = 0; j < kOnce; ++j) if (c0 + j < n_end) part[(c0 + j) * a.out_col_stride] = __uint_as_float(v[j]);
+            } else if (MODE != kGram) {
+              // 16-byte pieces: out rows start on their boundaries here (others went through shared memory, or are zeros and NaN of few rows)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) u.o[j] = FromFloat<O>(__uint_as_float(v[j]));
-          reinterpret_cast<uint4*>(out + n0)[0] = u.q[0]; reinterpret_cast<uint4*>(out + n0)[1] = u.q[1];
-        } else {
+              for (int h = 0; h < kOnce / 8; ++h) {
+                const int n0 = c0 + 8 * h;
+                if (n0 + 8 <= n_end && (reinterpret_cast<uintptr_t>(out + n0) & 15) == 0) {
+                  union { O o[8]; uint4 q; } u;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) if (n0 + j < n_end) out[(n0 + j) * a.out_col_stride] = FromFloat<O>(__uint_as_float(v[j]));
+                  for (int j = 0; j < 8; ++j) u.o[j] = FromFloat<O>(__uint_as_float(v[8 * h + j]));
+                  *reinterpret_cast<uint4*>(out + n0) = u.q;
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) if (n0 + j < n_end) out[n0 + j] = FromFloat<O>(__uint_as_float(v[8 * h + j]));
+                }
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < kOnce; ++j) if (c0 + j < n_end) out[(c0 + j) * a.out_col_stride] = FromFloat<O>(__uint_as_float(v[j]));
+            }
+          }
+          __syncwarp();      // the next read of tensor memory is one of the whole warp
         }
       }
       if (tile.depth > 0 && ok) {

@@ -286,7 +286,7 @@ def _near(got, want, size, terms, dtype):
 
 
 SHAPES = [(1, 1, 1, 1), (3, 5, 2, 4), (100, 28, 10, 7), (257, 33, 17, 3), (1000, 136, 1, 31), (513, 100, 100, 5), (64, 130, 257, 2), (2000, 8, 64, 255), (300, 257, 129, 4), (40, 2000, 30, 40),
-          (1200, 64, 256, 3), (700, 200, 520, 2), (1500, 135, 259, 3), (5000, 40, 70, 4)]
+          (1200, 64, 256, 3), (700, 200, 520, 2), (1500, 135, 259, 3), (5000, 40, 70, 4), (2000, 272, 296, 2), (1999, 640, 128, 3), (1100, 264, 520, 1)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -375,6 +375,23 @@ def test_leaf_products_rows_outside_the_leaves(dtype):
     assert ops.leaf_products(x[:0], w, torch.zeros(4, dtype=torch.int32, device="cuda")).shape == (0, 12)
     assert bool((ops.leaf_gram(d[:0], x[:0], torch.zeros(4, dtype=torch.int32, device="cuda")) == 0).all())
     assert bool((ops.leaf_products(x, w, torch.zeros(4, dtype=torch.int32, device="cuda")) == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,a_cols,b_cols", [(257, 8, 4), (2048, 8, 4), (2049, 8, 4), (6000, 9, 5), (9000, 70, 50), (1500, 130, 270), (20000, 130, 270)])
+def test_leaf_gram_of_long_leaves(dtype, rows, a_cols, b_cols):
+    """Leaves of few and of many slices side by side, and one of a single slice."""
+    from falcata_b200 import ops
+    g = _gen(12)
+    n = rows + 2 * (rows // 3) + 60
+    a = torch.randn((n, a_cols), generator=g, device="cuda").to(dtype); b = torch.randn((n, b_cols), generator=g, device="cuda").to(dtype)
+    begin = torch.tensor([0, rows // 3, rows // 3 + rows, n - 60, n], device="cuda")
+    for out in (dtype, torch.float32):
+        p = ops.leaf_gram(a, b, begin, dtype=out)
+        at = begin.tolist()
+        for leaf, (lo, hi) in enumerate(zip(at[:-1], at[1:])):
+            _near(p[leaf], a[lo:hi].double().t() @ b[lo:hi].double(), a[lo:hi].double().abs().t() @ b[lo:hi].double().abs(), hi - lo, out)
+        assert torch.equal(p, ops.leaf_gram(a, b, begin, dtype=out))
 
 
 def test_leaf_products_autograd():
