@@ -721,8 +721,9 @@ constexpr int kCopyWarps = 8, kCopyThreads = 32 * kCopyWarps, kTcThreads = 128 +
 constexpr int kMostStages = 8;
 constexpr int kLag = 5, kLagFew = 2;               // a stage is handed over when so many younger ones are on their way (of 8; of fewer stages)
 constexpr int kABytes = kTileM * 128;
-// Outputs whose rows do not start on 16-byte boundaries go through shared memory, 64 columns of a warp's 32 rows at a time, so that a
-// row is stored by neighbouring lanes (stored by its own lane, value by value, 200000 x 100 -> 100 took 130 us, of it 100 for the stores).
+// Outputs go through shared memory, 64 columns of a warp's 32 rows at a time, so that a row is stored by neighbouring lanes: eight with 16
+// bytes each, or value by value where rows do not start on 16-byte boundaries (stored by its own lane, value by value, 200000 x 100 -> 100
+// took 130 us, of it 100 for the stores; by its own lane in 16-byte pieces, 50000 x 512 -> 1000 took 88 us, so 77).
 constexpr int kStorePitch = 33, kStoreBytes = 4 * 32 * kStorePitch * 4;      // words: a row's 64 values and one to spare
 
 
@@ -1021,33 +1022,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         ++set;
       }
-      const int m = warp * 32 + lane, m_end = MODE == kGram ? min(kTileM, a.a_size - tile.m0) : tile.end - tile.row0, n_end = min(a.n, a.b_size - tile.n0);
-      const long long at = MODE == kGram ? (tile.m0 + m) * a.out_row_stride + tile.n0 * a.out_col_stride : (tile.row0 + m) * a.out_row_stride + tile.n0;
-      const int slot = MODE == kGram ? SliceSlot(a.leaves, tile.leaf, tile.row0, a.tile_rows) : -1;
-      O* out = static_cast<O*>(a.out) + (MODE == kGram ? static_cast<long long>(tile.leaf) * a.a_size * a.b_size : 0) + at;
-      float* part = slot >= 0 ? a.partial + static_cast<long long>(slot) * a.a_size * a.b_size + at : nullptr;
-      if (MODE != kGram && !(reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row_stride % 8 == 0) && tile.depth > 0 && ok) {
+      const unsigned int sums = tmem + acc * (a.tmem_cols / 2) + (static_cast<unsigned int>(warp * 32) << 16);
+      const int n_end = min(a.n, a.b_size - tile.n0);
+      if constexpr (MODE != kGram) {
+        const bool pieces = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row_stride % 8 == 0;
         unsigned int* s_words = reinterpret_cast<unsigned int*>(stages + static_cast<size_t>(a.stages) * a.stage_bytes) + warp * 32 * kStorePitch;
         O* rows_out = static_cast<O*>(a.out) + (tile.row0 + warp * 32) * a.out_row_stride + tile.n0;
-        const int rows = max(0, min(32, m_end - warp * 32));
+        const int rows = max(0, min(32, tile.end - tile.row0 - warp * 32));
         for (int c0 = 0; c0 < n_end; c0 += 64) {
+#pragma unroll 1
+          for (int h = 0; h < 2 && c0 + 32 * h < a.n; ++h) {
+            unsigned int v[32];
+            if (ok) {
+              TmemLoad16(sums + c0 + 32 * h, v);
+              if (c0 + 32 * h + 16 < a.n) TmemLoad16(sums + c0 + 32 * h + 16, v + 16);
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            } else {
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            if (c0 + 16 * h >= a.n) break;
-            unsigned int v[16];
-            TmemLoad16(tmem + acc * (a.tmem_cols / 2) + (static_cast<unsigned int>(warp * 32) << 16) + c0 + 16 * h, v);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+              for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              union { O o[2]; unsigned int w; } u;
-              u.o[0] = FromFloat<O>(__uint_as_float(v[2 * j])); u.o[1] = FromFloat<O>(__uint_as_float(v[2 * j + 1]));
-              s_words[lane * kStorePitch + 8 * h + j] = u.w;
+            for (int p = 0; p < 4; ++p) {
+              union { O o[8]; unsigned int w[4]; uint4 q; } u;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) u.o[j] = FromFloat<O>(__uint_as_float(v[8 * p + j]));
+              if (pieces) reinterpret_cast<uint4*>(s_words)[8 * lane + ((4 * h + p) ^ (lane & 7))] = u.q;      // eight lanes then write to all banks
+              else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s_words[lane * kStorePitch + 16 * h + 4 * p + j] = u.w[j];
+              }
             }
           }
           __syncwarp();
           const int cols = min(64, n_end - c0);
           const O* s_row = reinterpret_cast<const O*>(s_words);
-          if (cols > 32) {
+          if (pieces) {
+            const int p = lane & 7;
+            if (8 * p < cols) {
+#pragma unroll
+              for (int r = lane >> 3; r < 32; r += 4)
+                if (r < rows) *reinterpret_cast<uint4*>(rows_out + r * a.out_row_stride + c0 + 8 * p) = reinterpret_cast<const uint4*>(s_words)[8 * r + (p ^ (r & 7))];
+            }
+          } else if (cols > 32) {
             for (int r = 0; r < rows; ++r) {
               O* to = rows_out + static_cast<long long>(r) * a.out_row_stride + c0; const O* from = s_row + r * 2 * kStorePitch;
               to[lane] = from[lane];
@@ -1061,41 +1077,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
           __syncwarp();
         }
       } else {
-        // columns at a time: 32 took 50000 x 512 -> 1000 from 95 to 85 us, a Gram of 2000 x 1000 from 440 to 450
-        constexpr int kOnce = MODE == kGram ? 16 : 32;
-        for (int c0 = 0; c0 < n_end; c0 += kOnce) {
-          unsigned int v[kOnce];
+        const int m = warp * 32 + lane, m_end = min(kTileM, a.a_size - tile.m0);
+        const long long at = (tile.m0 + m) * a.out_row_stride + tile.n0 * a.out_col_stride;
+        const int slot = SliceSlot(a.leaves, tile.leaf, tile.row0, a.tile_rows);
+        O* out = static_cast<O*>(a.out) + static_cast<long long>(tile.leaf) * a.a_size * a.b_size + at;
+        float* part = slot >= 0 ? a.partial + static_cast<long long>(slot) * a.a_size * a.b_size + at : nullptr;
+        for (int c0 = 0; c0 < n_end; c0 += 16) {
+          unsigned int v[16];
           if (tile.depth > 0 && ok) {
-            const unsigned int from = tmem + acc * (a.tmem_cols / 2) + (static_cast<unsigned int>(warp * 32) << 16) + c0;
-            TmemLoad16(from, v);
-            if constexpr (kOnce == 32) { if (c0 + 16 < a.n) TmemLoad16(from + 16, v + 16); }
+            TmemLoad16(sums + c0, v);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           } else {
 #pragma unroll
-            for (int j = 0; j < kOnce; ++j) v[j] = ok ? 0u : 0x7fc00000u;
+            for (int j = 0; j < 16; ++j) v[j] = ok ? 0u : 0x7fc00000u;
           }
           if (m < m_end) {
             if (part != nullptr) {
 #pragma unroll
-              for (int j = 0; j < kOnce; ++j) if (c0 + j < n_end) part[(c0 + j) * a.out_col_stride] = __uint_as_float(v[j]);
-            } else if (MODE != kGram) {
-              // 16-byte pieces: out rows start on their boundaries here (others went through shared memory, or are zeros and NaN of few rows)
-#pragma unroll
-              for (int h = 0; h < kOnce / 8; ++h) {
-                const int n0 = c0 + 8 * h;
-                if (n0 + 8 <= n_end && (reinterpret_cast<uintptr_t>(out + n0) & 15) == 0) {
-                  union { O o[8]; uint4 q; } u;
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) u.o[j] = FromFloat<O>(__uint_as_float(v[8 * h + j]));
-                  *reinterpret_cast<uint4*>(out + n0) = u.q;
-                } else {
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) if (n0 + j < n_end) out[n0 + j] = FromFloat<O>(__uint_as_float(v[8 * h + j]));
-                }
-              }
+              for (int j = 0; j < 16; ++j) if (c0 + j < n_end) part[(c0 + j) * a.out_col_stride] = __uint_as_float(v[j]);
             } else {
 #pragma unroll
-              for (int j = 0; j < kOnce; ++j) if (c0 + j < n_end) out[(c0 + j) * a.out_col_stride] = FromFloat<O>(__uint_as_float(v[j]));
+              for (int j = 0; j < 16; ++j) if (c0 + j < n_end) out[(c0 + j) * a.out_col_stride] = FromFloat<O>(__uint_as_float(v[j]));
             }
           }
           __syncwarp();      // the next read of tensor memory is one of the whole warp
