@@ -86,13 +86,19 @@ __device__ __forceinline__ float Exp2(float x) { float r; asm("ex2.approx.ftz.f3
 constexpr float kLog2E = 1.44269504088896340736f;
 
 // Exponents are taken to base 2 against the rounded product B = m log2 e: x_j = s_j log2 e - B is one fused multiply-add. The rounding
-// of B shifts all x alike, and the results are put together from the same x and B, so it drops out (scores far from 0 lose
-// nothing). Where B overflows (|m| > kHugeScore: scores that differ at all differ by more than e^x can hold) x = (s_j - m) log2 e.
-constexpr float kHugeScore = 1e36f;
+// of B shifts all x alike, by half a step of B at most, and the results are put together from the same x and B, so it drops out as
+// long as 2^shift is far from fp32's ends. Up to |m| = 2^24 the shift is at most 1 (at 2^31 it would pass 64, at 2^33 every term
+// overflow or vanish). Beyond kHugeScore x = (s_j - m) log2 e, without a shift: neighbouring scores differ by 2 or more there, and
+// the subtraction loses nothing that e^x could show.
+constexpr float kHugeScore = 16777216.f;
 __device__ __forceinline__ bool Huge(float m) { return !(fabsf(m) <= kHugeScore); }
-__device__ __forceinline__ float Exponent(float v, float m) { return Huge(m) ? (v - m) * kLog2E : fmaf(v, kLog2E, -(m * kLog2E)); }
-// how much lower the exponents are when the maximum goes from m to `to` (> m)
-__device__ __forceinline__ float Lower(float m, float to) { return fmaxf(Huge(m) || Huge(to) ? (m - to) * kLog2E : __fsub_rn(__fmul_rn(m, kLog2E), __fmul_rn(to, kLog2E)), kLowestExponent); }
+__device__ __forceinline__ float Exponent(float v, float m) { return Huge(m) ? (v - m) * kLog2E : fmaf(v, kLog2E, -__fmul_rn(m, kLog2E)); }
+// what the exponents of a part with maximum m are too high by: m log2 e - B
+__device__ __forceinline__ float Shift(float m) { return Huge(m) ? 0.f : fmaf(m, kLog2E, -__fmul_rn(m, kLog2E)); }
+// how much lower the exponents are when the maximum goes from m to `to` (> m); with one side beyond kHugeScore the other's shift counts
+__device__ __forceinline__ float Lower(float m, float to) {
+  return fmaxf(Huge(m) || Huge(to) ? (m - to) * kLog2E - Shift(m) + Shift(to) : __fsub_rn(__fmul_rn(m, kLog2E), __fmul_rn(to, kLog2E)), kLowestExponent);
+}
 
 // The running sums of a part of a row, relative to its maximum m (-inf: nothing yet; a NaN or +inf among the scores makes s NaN):
 // s = sum 2^x, t = sum 2^x x.
@@ -124,11 +130,11 @@ struct Sums {
 };
 // The same for 16 bytes of scores at a time, two sums side by side.
 // In a pair's product 2^x * x a ruled-out score must not give 0 * (-inf): 16-bit scores are lifted to a finite low value first, two
-// per instruction. That is exact as long as the maximum is far above that value; elsewhere every exponent is clamped by itself.
+// per instruction. That is exact as long as the maximum is far above that value, and needs exponents by one multiply-add: maxima up
+// to kMost in size; elsewhere every exponent is clamped by itself.
 template <typename T> struct FarBelow;
-template <> struct FarBelow<float> { static constexpr float kFar = INFINITY; };
-template <> struct FarBelow<__half> { static constexpr unsigned int kLow = 0xfbfffbffu; static constexpr float kFar = -60000.f; };               // -65504
-template <> struct FarBelow<__nv_bfloat16> { static constexpr unsigned int kLow = 0xf14af14au; static constexpr float kFar = -1e29f; };          // -1.0e30
+template <> struct FarBelow<__half> { static constexpr unsigned int kLow = 0xfbfffbffu; static constexpr float kMost = 60000.f; };               // -65504
+template <> struct FarBelow<__nv_bfloat16> { static constexpr unsigned int kLow = 0xf14af14au; static constexpr float kMost = kHugeScore; };     // -1.0e30
 template <typename T>
 struct PairSums {
   float m = -INFINITY; F2 s = MakeF2(0.f, 0.f), t = MakeF2(0.f, 0.f);
@@ -149,9 +155,9 @@ struct PairSums {
     const float base = m == -INFINITY ? 0.f : m;
     const T* type = nullptr;
     if constexpr (sizeof(T) == 2) {
-      if (base > FarBelow<T>::kFar && base <= kHugeScore) {
+      if (fabsf(base) <= FarBelow<T>::kMost) {
         const unsigned int low = FarBelow<T>::kLow;
-        const float minus_b = -(base * kLog2E);
+        const float minus_b = -__fmul_rn(base, kLog2E);
         const F2 minus_base = MakeF2(minus_b, minus_b), scale = MakeF2(kLog2E, kLog2E);
 #pragma unroll
         for (int u = 0; u < COUNT; ++u) {
@@ -192,14 +198,13 @@ __device__ __forceinline__ float MaxOf(const uint4 (&q)[COUNT], const T* t) {
 
 // The results of a row from its sums.
 struct RowResult {
-  float m, log_sum, entropy; bool none, bad;      // log_sum: to base 2
+  float m, log_sum, shift, entropy; bool none, bad;      // log_sum: to base 2, with the exponents' shift
   __device__ explicit RowResult(const Sums& r) {
     none = r.m == -INFINITY && !(r.s != r.s); bad = !none && !(fabsf(r.m) < InfF() && r.s < InfF());   // a NaN sum fails the comparison
-    m = r.m; log_sum = log2f(r.s); entropy = none ? 0.f : bad ? NanF() : fmaxf((log_sum - r.t / r.s) * kLn2, 0.f);
+    m = r.m; log_sum = log2f(r.s); shift = Shift(m); entropy = none ? 0.f : bad ? NanF() : fmaxf((log_sum - r.t / r.s) * kLn2, 0.f);
   }
-  __device__ __forceinline__ float LogProb(float v) const { return none || v == -INFINITY ? (bad ? NanF() : -INFINITY) : bad ? NanF() : Huge(m) || Huge(v) ? (v - m) - log_sum * kLn2 : fminf((Exponent(v, m) - log_sum) * kLn2, 0.f); }
-  // m + the rest: what B lacks of m log2 e is put back
-  __device__ __forceinline__ float LogNorm() const { return none ? -INFINITY : bad ? NanF() : m + (log_sum + (Huge(m) ? 0.f : fmaf(-m, kLog2E, __fmul_rn(m, kLog2E)))) * kLn2; }
+  __device__ __forceinline__ float LogProb(float v) const { return none || v == -INFINITY ? (bad ? NanF() : -INFINITY) : bad ? NanF() : Huge(m) || Huge(v) ? (v - m) - (log_sum - shift) * kLn2 : fminf((Exponent(v, m) - log_sum) * kLn2, 0.f); }
+  __device__ __forceinline__ float LogNorm() const { return none ? -INFINITY : bad ? NanF() : m + (log_sum - shift) * kLn2; }
   __device__ __forceinline__ void Store(const ClassScoresArgs& a, long long row, long long y, float label_score) const {
     a.log_norm[row] = LogNorm(); a.entropy[row] = entropy;
     if (a.log_prob != nullptr) a.log_prob[row] = y < 0 ? 0.f : y >= a.classes ? NanF() : LogProb(label_score);
@@ -925,8 +930,8 @@ struct RowGrad {
   __device__ __forceinline__ float Soft(float v) const { const float lp = MaxNan((v - m) - log_sum, kLowestExponent); return Exp2(lp * kLog2E) * fmaf(-h, lp, a); }
   // with the label's own gradient
   __device__ __forceinline__ float At(float v, int j) const { const float d = Soft(v); return none ? 0.f : j == label ? d + g_label : d; }
-  // log sum e^(s - m), with what B lacks of m log2 e
-  __device__ __forceinline__ static float AgainLog(const Sums& r) { return (log2f(r.s) + (Huge(r.m) ? 0.f : fmaf(-r.m, kLog2E, __fmul_rn(r.m, kLog2E)))) * kLn2; }
+  // log sum e^(s - m)
+  __device__ __forceinline__ static float AgainLog(const Sums& r) { return (log2f(r.s) - Shift(r.m)) * kLn2; }
   // one thread walks the row
   template <typename T>
   __device__ __forceinline__ void TakeAgain(const ClassScoresArgs& s, const T* row) {

@@ -522,3 +522,71 @@ def test_operators_in_a_graph_and_on_streams():
         for got, ref in ((captured[0][2], want[1]), (captured[1][2], want[2]), (eager, want[0])):
             for a, b in zip(got, ref):
                 assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------- scores of large magnitude ----
+def _large_scores(k, dtype, layout, value, seed):
+    """Rows around `value` a few steps of the type apart, rows of one value, and ordinary rows with classes masked by -|value|."""
+    g = _gen(seed)
+    steps = torch.randint(0, 6, (18, k), generator=g, device="cuda").double()
+    s = value * (1 + torch.finfo(dtype).eps * steps)
+    usual = torch.randn((18, k), generator=g, device="cuda").double() * 2.5
+    mask = -abs(value)
+    s[8] = value
+    s[9] = value; s[9, k // 2] = value + abs(value) / 2
+    s[10] = usual[10]; s[10, : 3 * k // 4] = mask          # runs, as a padded class list has them
+    s[11] = usual[11]; s[11, k // 4:] = mask
+    s[12] = usual[12]; s[12, 1::2] = mask
+    s[13] = mask; s[13, k - 1] = 1.5
+    s[14] = mask
+    s[15] = usual[15]; s[15, 0] = abs(value)
+    s[16] = -math.inf; s[16, k // 3] = value; s[16, k // 2] = mask
+    s[17] = torch.where(steps[17] < 2, mask, usual[17])
+    s = s.to(dtype)
+    return s.t().contiguous().t() if layout == "class" else s
+
+
+def _check_large(s, top):
+    """log p = (s_j - m) - log sum e^(s - m): s_j - m rounds by u of its size, the sum as for any scores; nothing grows with |m|."""
+    from falcata_b200 import ops
+    n, k = s.shape
+    labels = torch.randint(0, k, (n,), generator=_gen(1), device="cuda")
+    got = ops.class_log_probs(s, labels, top_k=top)
+    want, logp = _reference(s, labels, top)
+    tol = U * (k / 32 + 128)
+    assert torch.equal(got.top_class, want["top_class"])
+    for name, scale in (("log_prob", 1.0), ("top_log_prob", 1.0), ("entropy", 1 + math.log(k)), ("log_norm", 1.0)):
+        off = (getattr(got, name).double() - want[name]).abs() / (tol * scale + 4 * U * want[name].abs())
+        assert bool((off.nan_to_num(math.inf) <= 1)[torch.isfinite(want[name])].all()), (name, off)
+        assert torch.equal(getattr(got, name)[~torch.isfinite(want[name])].double(), want[name][~torch.isfinite(want[name])])
+    g = torch.full((n,), 0.5, device="cuda"); g_top = torch.full((n, top), 0.125, device="cuda")
+    grad = ops.class_log_probs_grad(s, got.log_norm, got.entropy, labels=labels, top_class=got.top_class, grad_log_prob=2 * g, grad_log_norm=g, grad_entropy=-g / 2, grad_top_log_prob=g_top).double()
+    p = torch.exp(logp)
+    plogp = torch.where(p > 0, p * logp, 0.0)
+    named = (want["top_class"] >= 0)
+    ref = p * (0.5 - 1.0 - 0.125 * named.sum(1, keepdim=True)) + 0.25 * (plogp + p * want["entropy"][:, None])
+    ref[torch.arange(n, device="cuda"), labels] += 1.0
+    ref.scatter_add_(1, want["top_class"].long().clamp(min=0), torch.where(named, 0.125, 0.0).double())
+    # |a| + |b| (|log p| + entropy) is at most 6 + log K, p's own error U (K / 32 + 128) + 4 U |log p|
+    bound = p * (6 + math.log(k)) * (U * (k / 32 + 128) + 8 * U * (16 + logp.abs().clamp(max=200))) + 32 * U + _half_step(s.dtype) * ref.abs()
+    assert bool(((grad - ref).abs() <= bound).all()), float(((grad - ref).abs() - bound).max())
+
+
+LARGE_ROWS = [("row", 10), ("row", 60), ("row", 300), ("row", 5000), ("row", 40000), ("class", 10), ("class", 100), ("class", 2000), ("class", 20000)]
+
+
+@pytest.mark.parametrize("layout,k", LARGE_ROWS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value", [1e8, -1e8, 3e9, 5e9, -5e9, 1e10, -1e10, 1e15, 1e20, -1e20, 1e30, -1e30, 7e35, -7e35])
+def test_class_log_probs_of_large_scores(layout, k, dtype, value):
+    """Scores far from zero that are no powers of two, and classes masked by a large finite value."""
+    _check_large(_large_scores(k, dtype, layout, value, seed=k), min(k, 20))
+
+
+@pytest.mark.parametrize("layout,k", LARGE_ROWS)
+@pytest.mark.parametrize("border", [2.0 ** exponent * sign for exponent in (20, 22, 23, 24, 25) for sign in (1, -1)])
+def test_class_log_probs_around_powers_of_two(layout, k, border):
+    """fp32 scores on both sides of a power of two, a few steps apart: parts of one row whose maxima lie on different sides."""
+    step = max(1.0, abs(border) * 2.0 ** -24)
+    s = (border + step * torch.randint(-5, 6, (18, k), generator=_gen(k), device="cuda").double()).float()
+    _check_large(s.t().contiguous().t() if layout == "class" else s, min(k, 20))
