@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(256, 4) ClassLogProbsWarpKernel(ClassScoresArg
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) { keys[u] = OrderKey<T>(walk.best[u]); second[u] = OrderKey<T>(walk.second[u]); }
       const int have = alt.Find(keys, second, walk.best_at);
-      if (lane < a.top_k) { const Entry e = alt.sh.list[lane]; res.StoreTop(a, row * a.top_k + lane, lane < have ? e.v : -INFINITY, e.cls); }
+      if (lane < a.top_k) { const Entry e = alt.sh.list[lane]; res.StoreTop(a, static_cast<long long>(row) * a.top_k + lane, lane < have ? e.v : -INFINITY, e.cls); }
       __syncwarp();
     }
     y = y_next;
@@ -762,7 +762,7 @@ __global__ void __launch_bounds__(kBlockThreads, 4) ClassLogProbsBlockKernel(Cla
     if (part == 0) {
       const RowResult res(sums);
       if (lane == 0) res.Store(a, row, y, given);
-      if constexpr (TOP) if (lane < a.top_k) { const Entry e = parts > 1 ? s_joined[lane] : alt.sh.list[lane]; res.StoreTop(a, row * a.top_k + lane, lane < have ? e.v : -INFINITY, e.cls); }
+      if constexpr (TOP) if (lane < a.top_k) { const Entry e = parts > 1 ? s_joined[lane] : alt.sh.list[lane]; res.StoreTop(a, static_cast<long long>(row) * a.top_k + lane, lane < have ? e.v : -INFINITY, e.cls); }
     }
     __syncwarp();
     y = y_next;

@@ -590,3 +590,21 @@ def test_class_log_probs_around_powers_of_two(layout, k, border):
     step = max(1.0, abs(border) * 2.0 ** -24)
     s = (border + step * torch.randint(-5, 6, (18, k), generator=_gen(k), device="cuda").double()).float()
     _check_large(s.t().contiguous().t() if layout == "class" else s, min(k, 20))
+
+
+@pytest.mark.parametrize("k", [257, 8200])
+def test_class_log_probs_more_alternatives_than_32_bits_count(k):
+    """Rows x alternatives beyond 2^32: every window of one long vector is a row, so a result at a wrapped place is another row's."""
+    from falcata_b200 import ops
+    n, top = (1 << 27) + 5, 32
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    values = torch.randn(n + k, generator=_gen(k), device="cuda", dtype=torch.bfloat16)
+    got = ops.class_log_probs(values.as_strided((n, k), (1, 1)), top_k=top)
+    for first in (0, n // 2, n - 8):
+        want, _ = _reference(values[first:].as_strided((8, k), (1, 1)), None, top)
+        assert torch.equal(got.top_class[first:first + 8], want["top_class"])
+        for name in ("log_norm", "entropy", "top_log_prob"):
+            assert torch.allclose(getattr(got, name)[first:first + 8].double(), want[name], rtol=U, atol=U * (k / 32 + 128) * (1 + math.log(k)))
+    del got
+    torch.cuda.empty_cache()
