@@ -383,5 +383,7 @@ void LaunchLeafProducts(const LeafProductsArgs& a, float* workspace, cudaStream_
 long long LeafGramWorkspace(const LeafGramArgs& a);
 int LeafGramSliceRows(const LeafGramArgs& a);
 void LaunchLeafGram(const LeafGramArgs& a, float* workspace, cudaStream_t s);
+// How often the tensor-core kernel's waits try before they give up, from the next launch on (0: as at first); returns the number before.
+int SetLeafWaitTries(int tries);
 
 }  // namespace fb

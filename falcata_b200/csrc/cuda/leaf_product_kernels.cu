@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <type_traits>
 
 namespace fb {
@@ -714,8 +715,10 @@ __global__ void __launch_bounds__(256) PackLinesKernel(const unsigned short* __r
 // others go through the copying warps in pieces of 8 or 4 bytes or single values. Rows of a neighbouring leaf in an x tile
 // reach only outputs that are not stored; in a Gram's last step, where they would be summed, the copying warps bring the rows
 // that belong to the slice and zeros (unless the slice ends at a multiple of 16 rows, the depth of an instruction).
-// Warps: 0-3 store the accumulators, 4-11 copy, 12 issues the matrix instructions. Every wait is bounded; one that gives up
-// makes all roles leave; the outputs of every tile that is not finished are NaN then.
+// Warps: 0-3 store the accumulators, 4-11 copy, 12 issues the matrix instructions. Every wait is bounded (a try lasts 4 us: 4 s); one
+// that gives up makes all roles leave, and no role waits again: a phase that never completes would look complete to the wait for the
+// next one but one, whose parity is the other. The outputs of every tile that is not finished are NaN then. What is in flight is waited
+// for before the block ends.
 constexpr int kDepthTc = 64, kTileM = 128, kMostN = 256;
 constexpr int kCopyWarps = 8, kCopyThreads = 32 * kCopyWarps, kTcThreads = 128 + kCopyThreads + 32;
 constexpr int kMostStages = 8;
@@ -734,9 +737,10 @@ __device__ __forceinline__ bool BarTry(unsigned long long* bar, unsigned int par
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(Smem32(bar)), "r"(parity) : "memory");
   return ok != 0;
 }
-// false: the budget ran out, here or in another role
-__device__ __forceinline__ bool BarWait(unsigned long long* bar, unsigned int parity, volatile int* stop) {
-  for (int i = 0; i < (1 << 20); ++i) { if (BarTry(bar, parity)) return true; if (*stop != 0) return false; }
+constexpr int kWaitTries = 1 << 20, kDrainTries = 1 << 12;
+// false: the tries ran out, here or in another role
+__device__ __forceinline__ bool BarWait(unsigned long long* bar, unsigned int parity, int tries, volatile int* stop) {
+  do { if (BarTry(bar, parity)) return true; if (*stop != 0) return false; } while (--tries > 0);
   *stop = 1;
   return false;
 }
@@ -827,7 +831,7 @@ struct TensorArgs {
   const unsigned short *a, *b; long long a_stride, b_stride, b_leaf_stride;
   int a_tma, b_tma, b_leaf_on;                                  // operand by tensor map; 1: its third coordinate is the leaf
   int a_vec, b_vec, a_size, b_size, depth;                      // columns of a Gram's sides; outputs (b_size) and features (depth) of products
-  int n, across_a, across_b, stages, stage_bytes, tmem_cols;
+  int n, across_a, across_b, stages, stage_bytes, tmem_cols, wait_tries;
   unsigned int idesc;
   void* out; float* partial; long long out_row_stride, out_col_stride;
 };
@@ -861,6 +865,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
   volatile int* stop = &s_stop;
   const int across = a.across_a * a.across_b;
   const int tiles = map.Total() * across;
+  int issued = 0, last_stage = 0; unsigned int last_parity = 0;      // steps copied (first copying thread) or multiplied (issuing thread); the latter's last stage
   // Products: the row tiles of the leaves, `across_b` output tiles each. Gram: slices, across_a x across_b tiles each.
   struct Tile { int leaf, which, m0, n0, depth, row0, end; };
   int span = 0;
@@ -925,7 +930,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
         const int steps = (tile.depth + kDepthTc - 1) / kDepthTc, cut = MODE == kGram && (tile.depth & 15) != 0 ? 1 : 0;
         if (tid == 0) {
           for (int i = 0; i < steps - cut; ++i) {
-            if (it >= a.stages && !BarWait(s_empty + fill, fill_parity, stop)) { ok = false; break; }
+            if (it >= a.stages && !BarWait(s_empty + fill, fill_parity, a.wait_tries, stop)) { ok = false; break; }
             BarArriveExpect(s_full + fill, a_bytes + b_bytes);
             load(true, true, fill, i * kDepthTc);
             ++it;
@@ -934,9 +939,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
         }
         if (cut != 0) {
           // the filling thread alone knows when the stage is free: the others skip steps, and a parity tells neighbouring uses apart only
-          if (tid == 0 && ok) { if (it >= a.stages) ok = BarWait(s_empty + fill, fill_parity, stop); if (ok) { s_go_stage = fill; BarArrive(&s_go); } }
+          if (tid == 0 && ok) { if (it >= a.stages) ok = BarWait(s_empty + fill, fill_parity, a.wait_tries, stop); if (ok) { s_go_stage = fill; BarArrive(&s_go); } }
           __syncwarp();
-          ok = ok && BarWait(&s_go, cuts & 1, stop);
+          ok = ok && BarWait(&s_go, cuts & 1, a.wait_tries, stop);
           ok = __all_sync(0xffffffffu, ok) != 0;
           if (ok) {
             const int st = *const_cast<volatile int*>(&s_go_stage);
@@ -946,7 +951,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
             __syncwarp();
             if (lane == 0) BarArrive(&s_cut);
             if (tid == 0) {
-              ok = BarWait(&s_cut, cuts & 1, stop);
+              ok = BarWait(&s_cut, cuts & 1, a.wait_tries, stop);
               if (ok) { BarArrive(s_full + st); ++it; if (++fill == a.stages) { fill = 0; fill_parity ^= 1u; } }
             }
             ok = __all_sync(0xffffffffu, ok) != 0;
@@ -956,7 +961,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
       } else {
         for (int k0 = 0; k0 < tile.depth; k0 += kDepthTc, ++it) {
           const int st = it % a.stages;
-          if (it >= a.stages) ok = __all_sync(0xffffffffu, BarWait(s_empty + st, ((it / a.stages) - 1) & 1, stop)) != 0;      // one decision per warp
+          if (it >= a.stages) ok = __all_sync(0xffffffffu, BarWait(s_empty + st, ((it / a.stages) - 1) & 1, a.wait_tries, stop)) != 0;      // one decision per warp
           if (!ok) break;
           const bool cut = MODE == kGram && ((tile.depth - k0) & 15) != 0 && tile.depth - k0 < kDepthTc;
           const bool ta = a.a_tma != 0 && !cut, tb = a.b_tma != 0 && !cut;
@@ -967,15 +972,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
       }
     }
     CopyWait<0>();
-    if (ok && !both) for (int step = max(0, it - lag); step < it; ++step) hand_over(step);
-    if (!ok && tid == 0 && (a.a_tma != 0 || a.b_tma != 0))      // the copies in flight still write shared memory
-      for (int step = max(0, it - a.stages); step < it; ++step)
-        for (int i = 0; i < (1 << 16) && !BarTry(s_full + step % a.stages, (step / a.stages) & 1); ++i) {}
+    if (!both) for (int step = max(0, it - lag); step < it; ++step) hand_over(step);
+    issued = it;
   } else if (warp == 12) {
     if (lane == 0) {
       // One thread feeds the tensor cores: its own instructions must take less time than the matrix instructions that they issue (512
       // cycles a step), so stages, parities and descriptors are carried along by adding (worked out anew: 1000 cycles a step).
-      int set = 0, st = 0, steps = 0;
+      int set = 0, st = 0;
       unsigned int parity = 0;
       bool ok = true;
       const unsigned long long a_desc0 = OperandDesc(Smem32(stages), MODE == kGram ? 8192 : 16), b_desc0 = OperandDesc(Smem32(stages) + kABytes, MODE == kProductsK ? 16 : 8192);
@@ -986,38 +989,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
         const Tile tile = tile_of(t);
         if (tile.depth == 0) continue;
         const int acc = set & 1;
-        if (set >= 2 && !BarWait(s_free + acc, ((set >> 1) - 1) & 1, stop)) { ok = false; break; }
+        if (set >= 2 && !BarWait(s_free + acc, ((set >> 1) - 1) & 1, a.wait_tries, stop)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const unsigned int d = tmem + acc * (a.tmem_cols / 2);
         bool fresh = true;
         for (int left = tile.depth; left > 0; left -= kDepthTc) {
-          if (!BarWait(s_full + st, parity, stop)) { ok = false; break; }
+          if (!BarWait(s_full + st, parity, a.wait_tries, stop)) { ok = false; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const unsigned long long da = a_desc0 + static_cast<unsigned long long>(st * stage_on), db = b_desc0 + static_cast<unsigned long long>(st * stage_on);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             if (16 * k < left) { Mma16(d, da + k * kAOn, db + k * kBOn, a.idesc, !fresh); fresh = false; }
           MmaCommit(s_empty + st);
-          ++steps;
+          ++issued;
           if (++st == a.stages) { st = 0; parity ^= 1u; }
         }
         if (ok) { MmaCommit(s_done + acc); ++set; }
       }
-      if (!ok && steps > 0) {      // the matrix instructions in flight still read shared memory
-        const int last = st == 0 ? a.stages - 1 : st - 1;
-        const unsigned int last_parity = st == 0 ? parity ^ 1u : parity;
-        for (int i = 0; i < (1 << 20) && !BarTry(s_empty + last, last_parity); ++i) {}
-      }
+      last_stage = st == 0 ? a.stages - 1 : st - 1; last_parity = st == 0 ? parity ^ 1u : parity;
     }
     __syncwarp();
   } else {
     int set = 0;
+    bool ok = true;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
       const Tile tile = tile_of(t);
       const int acc = set & 1;
-      bool ok = true;
       if (tile.depth > 0) {
-        ok = BarWait(s_done + acc, (set >> 1) & 1, stop);
+        ok = ok && BarWait(s_done + acc, (set >> 1) & 1, a.wait_tries, stop);
         ok = __all_sync(0xffffffffu, ok);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         ++set;
@@ -1089,7 +1088,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = ok ? 0u : 0x7fc00000u;
+            for (int j = 0; j < 16; ++j) v[j] = tile.depth == 0 ? 0u : 0x7fc00000u;
           }
           if (m < m_end) {
             if (part != nullptr) {
@@ -1112,8 +1111,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (*stop != 0) {      // a role left early: copies in flight still write shared memory, matrix instructions still read it and write their sums
+    if (threadIdx.x == 128 && (a.a_tma != 0 || a.b_tma != 0))
+      for (int step = max(0, issued - a.stages); step < issued; ++step)
+        for (int i = 0; i < kDrainTries && !BarTry(s_full + step % a.stages, (step / a.stages) & 1); ++i) {}
+    if (warp == 12 && lane == 0 && issued > 0) for (int i = 0; i < kDrainTries && !BarTry(s_empty + last_stage, last_parity); ++i) {}
+    __syncthreads();
+  }
   if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
 }
+
+std::atomic<int> g_wait_tries{kWaitTries};
 
 template <typename F> void DispatchHalf(int dtype, F&& f) {
   switch (dtype) {
@@ -1182,6 +1190,7 @@ void LaunchTensor(TensorArgs a, long long most_tiles, cudaStream_t s) {
   // D fp32; A, B fp16 (0) or bf16 (1), their majors; N, M
   const unsigned int type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   a.idesc = (1u << 4) | (type << 7) | (type << 10) | (MODE == kGram ? 1u << 15 : 0u) | (MODE != kProductsK ? 1u << 16 : 0u) | (static_cast<unsigned int>(a.n >> 3) << 17) | (static_cast<unsigned int>(kTileM >> 4) << 24);
+  a.wait_tries = g_wait_tries.load(std::memory_order_relaxed);
   CheckTiles(most_tiles);
   const int bytes = a.stages * a.stage_bytes + 1024 + store_bytes;
   static PerDevice allowed;
@@ -1316,6 +1325,8 @@ struct ProductsPacking {
 };
 
 }  // namespace
+
+int SetLeafWaitTries(int tries) { return g_wait_tries.exchange(tries < 1 ? kWaitTries : tries); }
 
 // Rows of a leaf that one block (narrow: one warp) sums up. Slices short enough that uneven leaves even out (4 per SM, 2 per warp), long
 // enough that a slice's work outweighs its sums' way through the workspace, and that the workspace stays within 128 MB.

@@ -282,6 +282,9 @@ int FB_OpLeafGram(const void* a_rows, long long a_stride, const void* b_rows, lo
   OPS_END();
 }
 
+// The tries of the tensor-core kernel's waits (0: the default), for tests of what a launch leaves when they run out.
+int FB_OpLeafWaitTries(int tries, int* before) { *before = SetLeafWaitTries(tries); return 0; }
+
 int FB_OpLaunchCount(long long* out) { *out = LaunchCounter().load(); return 0; }
 
 }  // extern "C"

@@ -608,3 +608,51 @@ def test_class_log_probs_more_alternatives_than_32_bits_count(k):
             assert torch.allclose(getattr(got, name)[first:first + 8].double(), want[name], rtol=U, atol=U * (k / 32 + 128) * (1 + math.log(k)))
     del got
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------ waits that run out ----
+class _WaitTries:
+    """The tensor-core kernel's waits give up after so many tries (each some microseconds); as at first again at the end."""
+
+    def __init__(self, tries):
+        self.tries = tries
+
+    def _set(self, tries):
+        import ctypes
+        from falcata_b200.basic import _lib
+        before = ctypes.c_int(0)
+        assert _lib().FB_OpLeafWaitTries(ctypes.c_int(tries), ctypes.byref(before)) == 0
+
+    def __enter__(self):
+        self._set(self.tries)
+
+    def __exit__(self, *exc):
+        torch.cuda.synchronize()
+        self._set(0)
+
+
+def _near_or_nan(got, want, size, terms, dtype):
+    """Where it is not NaN: as _near."""
+    given = ~torch.isnan(got)
+    _near(torch.where(given, got, want.to(dtype)), want, size, terms, dtype)
+    return given
+
+
+@pytest.mark.parametrize("side", ["tma", "x copied", "maps copied", "maps by output"])
+@pytest.mark.parametrize("tries", [1, 2, 6])
+def test_leaf_products_whose_waits_run_out(side, tries):
+    """Several tiles per block, each longer than a try: what is not finished is NaN, never what an accumulator happened to hold."""
+    from falcata_b200 import ops
+    n, f, k, leaves = 128 * 148 * 5, 2048, 96, 3
+    g = _gen(2)
+    x = torch.randn((n, f + 1), generator=g, device="cuda", dtype=torch.bfloat16)
+    x = x[:, 1:] if side == "x copied" else x[:, :f].contiguous()
+    w = torch.randn((leaves, k, f + (1 if side == "maps copied" else 0)), generator=g, device="cuda", dtype=torch.bfloat16)[:, :, :f]
+    if side == "maps by output":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    begin = torch.tensor([0, n // 3, n // 2, n], device="cuda")
+    want, size = _ref_products(x, w, begin)
+    with _WaitTries(tries):
+        given = _near_or_nan(ops.leaf_products(x, w, begin), want, size, f, torch.bfloat16)
+        assert tries > 1 or not bool(given.any())          # every block's first tile takes longer than one try
+    _near(ops.leaf_products(x, w, begin), want, size, f, torch.bfloat16)
