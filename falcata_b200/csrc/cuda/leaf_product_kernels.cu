@@ -937,9 +937,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
             if (++fill == a.stages) { fill = 0; fill_parity ^= 1u; }
           }
         }
-        if (cut != 0) {
+        ok = __all_sync(0xffffffffu, ok) != 0;      // the filling thread's warp leaves as a whole: it meets at barriers below
+        if (cut != 0 && ok) {
           // the filling thread alone knows when the stage is free: the others skip steps, and a parity tells neighbouring uses apart only
-          if (tid == 0 && ok) { if (it >= a.stages) ok = BarWait(s_empty + fill, fill_parity, a.wait_tries, stop); if (ok) { s_go_stage = fill; BarArrive(&s_go); } }
+          if (tid == 0) { if (it >= a.stages) ok = BarWait(s_empty + fill, fill_parity, a.wait_tries, stop); if (ok) { s_go_stage = fill; BarArrive(&s_go); } }
           __syncwarp();
           ok = ok && BarWait(&s_go, cuts & 1, a.wait_tries, stop);
           ok = __all_sync(0xffffffffu, ok) != 0;

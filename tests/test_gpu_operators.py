@@ -656,3 +656,25 @@ def test_leaf_products_whose_waits_run_out(side, tries):
         given = _near_or_nan(ops.leaf_products(x, w, begin), want, size, f, torch.bfloat16)
         assert tries > 1 or not bool(given.any())          # every block's first tile takes longer than one try
     _near(ops.leaf_products(x, w, begin), want, size, f, torch.bfloat16)
+
+
+@pytest.mark.parametrize("side", ["tma", "copied"])
+@pytest.mark.parametrize("tries", [1, 2, 6])
+def test_leaf_gram_whose_waits_run_out(side, tries):
+    """Slices that end inside a step, for which all copying warps come together: a role that leaves takes its whole warp along."""
+    from falcata_b200 import ops
+    n, ac, bc = 150003, 264, 120 if side == "copied" else 520
+    g = _gen(3)
+    a = torch.randn((n, ac + 1), generator=g, device="cuda", dtype=torch.float16)
+    a = a[:, :ac].contiguous() if side == "tma" else a[:, 1:]
+    b = torch.randn((n, bc), generator=g, device="cuda", dtype=torch.float16)
+    begin = torch.tensor([0, 5, 40001, 40001, 41007, 100000, n], device="cuda")
+    at = list(zip(begin.tolist()[:-1], begin.tolist()[1:]))
+    want = torch.stack([a[lo:hi].double().t() @ b[lo:hi].double() for lo, hi in at])
+    size = torch.stack([a[lo:hi].double().abs().t() @ b[lo:hi].double().abs() for lo, hi in at])
+    with _WaitTries(tries):
+        for dtype in (torch.float32, torch.float16):
+            given = _near_or_nan(ops.leaf_gram(a, b, begin, dtype=dtype), want, size, n, dtype)
+            assert bool(given[2].all())                        # no rows, nothing to wait for
+    for dtype in (torch.float32, torch.float16):
+        _near(ops.leaf_gram(a, b, begin, dtype=dtype), want, size, n, dtype)
