@@ -33,41 +33,61 @@ template <> __device__ __forceinline__ __nv_bfloat16 FromFloat<__nv_bfloat16>(fl
 
 constexpr int kSms = 148;
 
-// Window of leaf g inside [0, rows): whatever the caller's boundaries hold, no access leaves the arrays.
-__device__ __forceinline__ void LeafWindow(const LeafWindows& w, int g, long long* begin, long long* end) {
-  const long long b = w.begin_bits == 32 ? static_cast<const int*>(w.begin)[g] : static_cast<const long long*>(w.begin)[g];
-  const long long e = w.begin_bits == 32 ? static_cast<const int*>(w.begin)[g + 1] : static_cast<const long long*>(w.begin)[g + 1];
-  *begin = min(max(b, 0LL), w.rows); *end = min(max(e, *begin), w.rows);
+// Boundary i inside [0, rows).
+__device__ __forceinline__ int Boundary(const LeafWindows& w, int i) {
+  const long long b = w.begin_bits == 32 ? static_cast<const int*>(w.begin)[i] : static_cast<const long long*>(w.begin)[i];
+  return static_cast<int>(min(max(b, 0LL), w.rows));
 }
+// Tiles of `rows` rows in [b, e); `least`: tiles of a leaf without rows.
+__device__ __forceinline__ int TilesIn(int b, int e, int rows, int least) { return max(least, static_cast<int>((static_cast<unsigned int>(e - b) + static_cast<unsigned int>(rows) - 1u) / static_cast<unsigned int>(rows))); }
 
 // The tiles of all leaves one behind the other: `rows` rows each, a leaf's last one shorter. Up to kSpans leaves are looked up by
 // bisection; more are counted in spans of several leaves.
+// A leaf starts where the one before it ended. That is its own boundary unless boundaries fall again: then a row belongs to the first
+// leaf that has it, so no boundaries make more tiles than rows / tile rows + leaves, or rows that two leaves work on.
 constexpr int kSpans = 1024;
 struct TileMap {
   int before[kSpans + 1];        // tiles before span i
-  int row[kSpans + 1];           // with a leaf per span: its first row
+  int row[kSpans + 1];           // its first row
   int per, spans, first_row, last_row;      // rows of all leaves: [first_row, last_row)
-  __device__ __forceinline__ static int Count(const LeafWindows& w, int g, int rows, int least) {
-    long long b, e; LeafWindow(w, g, &b, &e);
-    return max(least, static_cast<int>((e - b + rows - 1) / rows));
+  // tiles of span i (its leaves: [i * p, end)), whose first row is *b; *b: the row behind it. falls: whether a boundary fell again
+  __device__ __forceinline__ static int CountSpan(const LeafWindows& w, int i, int p, int rows, int least, int* b, int* falls) {
+    int c = 0;
+    for (int g = i * p; g < min(w.leaves, (i + 1) * p); ++g) {
+      const int next = Boundary(w, g + 1), e = max(*b, next);
+      *falls |= next < *b ? 1 : 0;
+      c += TilesIn(*b, e, rows, least);
+      *b = e;
+    }
+    return c;
   }
   // All threads of the block; `least`: tiles of a leaf without rows.
   __device__ void Build(const LeafWindows& w, int rows, int least) {
     const int p = (w.leaves + kSpans - 1) / kSpans, n = (w.leaves + p - 1) / p;
     if (threadIdx.x == 0) { per = p; spans = n; }
+    int falls = 0;
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      int c = 0;
-      long long b = 0, e = 0;
-      for (int g = i * p; g < min(w.leaves, (i + 1) * p); ++g) {
-        LeafWindow(w, g, &b, &e);
-        if (g == i * p) row[i] = static_cast<int>(b);
-        c += max(least, static_cast<int>((e - b + rows - 1) / rows));
-      }
-      before[i + 1] = c;
-      if (i == 0) first_row = row[0];
-      if (i == n - 1) row[n] = last_row = static_cast<int>(e);      // with several leaves per span only the last use of row[] is this one
+      int b = Boundary(w, i * p);
+      row[i] = b;
+      if (i == 0) first_row = b;
+      before[i + 1] = CountSpan(w, i, p, rows, least, &b, &falls);
+      if (i == n - 1) row[n] = last_row = b;
     }
-    __syncthreads();
+    if (__syncthreads_or(falls) != 0) {
+      // where spans start when rows before them have been taken: the highest boundary so far
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n; i += blockDim.x) { int b = Boundary(w, i * p); CountSpan(w, i, p, rows, least, &b, &falls); before[i + 1] = b; }
+      __syncthreads();
+      if (threadIdx.x == 0) {
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) row[i + 1] = max(row[i], before[i + 1]);
+        last_row = row[n];
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n; i += blockDim.x) { int b = row[i]; before[i + 1] = CountSpan(w, i, p, rows, least, &b, &falls); }
+      __syncthreads();
+    }
     if (threadIdx.x < 32) {
       const int each = (n + 31) / 32, lo = min(n, static_cast<int>(threadIdx.x) * each), hi = min(n, lo + each);
       int sum = 0;
@@ -82,27 +102,21 @@ struct TileMap {
     __syncthreads();
   }
   __device__ __forceinline__ int Total() const { return before[spans]; }
-  // tile -> leaf, its first row and the end of the rows that it covers. `span`: where the last search of an earlier tile ended (0 at
-  // first); the next tile is mostly a few leaves on.
-  __device__ __forceinline__ void Find(const LeafWindows& w, int tile, int rows, int least, int* span, int* leaf, int* first, int* end) const {
+  // the row behind leaf g, which starts at row b
+  __device__ __forceinline__ int End(const LeafWindows& w, int g, int b) const { return per == 1 ? row[g + 1] : max(b, Boundary(w, g + 1)); }
+  // tile -> leaf, its first row and the end of the rows that it covers, and the rows [begin, last) of the whole leaf. `span`: where the last
+  // search of an earlier tile ended (0 at first); the next tile is mostly a few leaves on.
+  __device__ __forceinline__ void Find(const LeafWindows& w, int tile, int rows, int least, int* span, int* leaf, int* first, int* end, int* begin, int* last) const {
     int lo = *span;
     if (before[lo + 1] <= tile && lo + 1 < spans) ++lo;
     if (before[lo + 1] <= tile) { int hi = spans; while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (before[mid] <= tile) lo = mid; else hi = mid; } }
     *span = lo;
-    int g = lo * per, left = tile - before[lo], b = row[lo], e = row[lo + 1];
+    int g = lo * per, left = tile - before[lo], b = row[lo], e = End(w, g, b);
     if (per > 1) {
-      for (int c = Count(w, g, rows, least); left >= c; c = Count(w, g, rows, least)) { left -= c; ++g; }
-      long long b64, e64; LeafWindow(w, g, &b64, &e64);
-      b = static_cast<int>(b64); e = static_cast<int>(e64);
+      for (int c = TilesIn(b, e, rows, least); left >= c && g + 1 < w.leaves; c = TilesIn(b, e, rows, least)) { left -= c; ++g; b = e; e = End(w, g, b); }
     }
-    e = max(e, b);
-    *leaf = g; *first = static_cast<int>(min(static_cast<long long>(e), b + static_cast<long long>(left) * rows)); *end = static_cast<int>(min(static_cast<long long>(e), static_cast<long long>(*first) + rows));
-  }
-  // the rows of leaf g
-  __device__ __forceinline__ void Rows(const LeafWindows& w, int g, int* b, int* e) const {
-    if (per == 1) { *b = row[g]; *e = max(row[g], row[g + 1]); return; }
-    long long b64, e64; LeafWindow(w, g, &b64, &e64);
-    *b = static_cast<int>(b64); *e = static_cast<int>(e64);
+    *leaf = g; *begin = b; *last = e;
+    *first = static_cast<int>(min(static_cast<long long>(e), b + static_cast<long long>(left) * rows)); *end = static_cast<int>(min(static_cast<long long>(e), static_cast<long long>(*first) + rows));
   }
 };
 
@@ -194,9 +208,9 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
   const CopyPlan<Tile::THREADS> x_plan(Tile::ROWS, shape.width, pitch, shape.x_vec), w_plan(Tile::OUTS, shape.width, pitch, shape.w_vec);
   struct At { int t, span, row0, leaf, rows, out0, f0; };
   auto find = [&](At& at) {
-    int end;
+    int end, begin, last;
     const int which = at.t / across;
-    map.Find(a.leaves, which, Tile::ROWS, 0, &at.span, &at.leaf, &at.row0, &end);
+    map.Find(a.leaves, which, Tile::ROWS, 0, &at.span, &at.leaf, &at.row0, &end, &begin, &last);
     at.rows = end - at.row0; at.out0 = (at.t - which * across) * Tile::OUTS; at.f0 = 0;
   };
   auto advance = [&](At& at) { at.f0 += shape.width; if (at.f0 >= a.features) { at.t += grid; if (at.t < tiles) find(at); } };
@@ -295,10 +309,7 @@ __global__ void __launch_bounds__(32 * WR * WO, 512 / (32 * WR * WO)) LeafProduc
 
 // Where the sums of a slice go: -1 straight to the output (its leaf has no other), else a place of the workspace. Of the leaves with
 // several slices, first slices start more than a slice apart, and so do the others: 2 places per `rows` rows are enough.
-__device__ __forceinline__ int SliceSlot(const LeafWindows& w, int leaf, int row0, int rows) {
-  long long b, e; LeafWindow(w, leaf, &b, &e);
-  return e - b <= rows ? -1 : 2 * (row0 / rows) + (row0 == b ? 0 : 1);
-}
+__device__ __forceinline__ int SliceSlot(int leaf_begin, int leaf_end, int row0, int rows) { return leaf_end - leaf_begin <= rows ? -1 : 2 * (row0 / rows) + (row0 == leaf_begin ? 0 : 1); }
 
 // Gram matrices. Tile: AC = TA * GA columns of a x BC = TB * GB columns of b, RD rows a step through a ring of kRing buffers; SLICES
 // groups of GA * GB threads take every SLICES-th row each and are added up at the end, in order.
@@ -320,8 +331,8 @@ __global__ void __launch_bounds__(GA * GB * SLICES, 2) LeafGramFloatKernel(LeafG
   int span = 0;
   for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
     const int which = t / across, rest = t - which * across;
-    int leaf, row0, end;
-    map.Find(a.leaves, which, rows_per_slice, 1, &span, &leaf, &row0, &end);
+    int leaf, row0, end, leaf_begin, leaf_end;
+    map.Find(a.leaves, which, rows_per_slice, 1, &span, &leaf, &row0, &end, &leaf_begin, &leaf_end);
     const int a0 = rest / across_b * Tile::AC, b0 = rest % across_b * Tile::BC, a_in = min(Tile::AC, a.a_cols - a0), b_in = min(Tile::BC, a.b_cols - b0);
     const CopyPlan<Tile::THREADS> a_plan(RD, (a_in + 3) & ~3, Tile::AC, a_vec), b_plan(RD, (b_in + 3) & ~3, Tile::BC, b_vec);
     const float* pa = static_cast<const float*>(a.a) + row0 * a.a_stride + a0; const float* pb = static_cast<const float*>(a.b) + row0 * a.b_stride + b0;
@@ -366,7 +377,7 @@ __global__ void __launch_bounds__(GA * GB * SLICES, 2) LeafGramFloatKernel(LeafG
     }
     CopyWait<0>();
     __syncthreads();
-    const int slot = SliceSlot(a.leaves, leaf, row0, rows_per_slice);
+    const int slot = SliceSlot(leaf_begin, leaf_end, row0, rows_per_slice);
     float* to = slot >= 0 ? partial + static_cast<long long>(slot) * a.a_cols * a.b_cols : static_cast<float*>(a.out) + static_cast<long long>(leaf) * a.a_cols * a.b_cols;
     if constexpr (SLICES == 1) {
 #pragma unroll
@@ -445,19 +456,19 @@ template <typename T> __device__ __forceinline__ void Pairs(const uint4& q, F2 (
 
 // A warp's share of the tiles of `rows` rows, one behind the other: [first, last) of them.
 struct WarpTiles {
-  int left, leaf, row, leaf_end, least;
+  int left, leaf, row, leaf_begin, leaf_end, least;
   __device__ __forceinline__ WarpTiles(const TileMap& map, const LeafWindows& w, int rows, int least_) {
     least = least_;
     const int total = map.Total(), warps = gridDim.x * kNarrowWarps, me = blockIdx.x * kNarrowWarps + threadIdx.x / 32;
     const int each = total / warps, more = total - each * warps, first = me * each + min(me, more);
-    left = each + (me < more ? 1 : 0); leaf = row = leaf_end = 0;
-    if (left > 0) { int span = 0, end, begin; map.Find(w, first, rows, least, &span, &leaf, &row, &end); map.Rows(w, leaf, &begin, &leaf_end); }
+    left = each + (me < more ? 1 : 0); leaf = row = leaf_begin = leaf_end = 0;
+    if (left > 0) { int span = 0, end; map.Find(w, first, rows, least, &span, &leaf, &row, &end, &leaf_begin, &leaf_end); }
   }
   __device__ __forceinline__ void Next(const TileMap& map, const LeafWindows& w, int rows) {
     if (--left <= 0) return;
     if (leaf_end - row > rows) row += rows;
     else {
-      do { ++leaf; map.Rows(w, leaf, &row, &leaf_end); } while (least == 0 && row >= leaf_end && leaf + 1 < w.leaves);
+      do { ++leaf; row = leaf_begin = leaf_end; leaf_end = map.End(w, leaf, row); } while (least == 0 && row >= leaf_end && leaf + 1 < w.leaves);
     }
   }
 };
@@ -606,7 +617,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) LeafGramNarrowKernel(LeafGr
     }
     CopyWait<0>();
     __syncwarp();
-    const int slot = SliceSlot(a.leaves, slice.leaf, slice.row, rows_per_slice);
+    const int slot = SliceSlot(slice.leaf_begin, slice.leaf_end, slice.row, rows_per_slice);
     const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -633,10 +644,10 @@ __global__ void __launch_bounds__(256) LeafGramJoinKernel(LeafGramArgs a, int ro
   const long long size = static_cast<long long>(a.a_cols) * a.b_cols;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   for (int g = blockIdx.y; g < a.leaves.leaves; g += gridDim.y) {
-    long long b, e; LeafWindow(a.leaves, g, &b, &e);
+    const int b = Boundary(a.leaves, g), e = max(b, Boundary(a.leaves, g + 1));      // where boundaries fall again: any slices of the workspace
     if (e - b <= rows_per_slice) continue;
-    const int slices = static_cast<int>((e - b + rows_per_slice - 1) / rows_per_slice), each = (slices + 7) / 8, first = warp * each, last = min(slices, first + each);
-    const float* of_leaf = partial + 2 * (b / rows_per_slice) * size;      // first slice here, the others one place and two places apart
+    const int slices = TilesIn(b, e, rows_per_slice, 1), each = (slices + 7) / 8, first = warp * each, last = min(slices, first + each);
+    const float* of_leaf = partial + 2LL * (b / rows_per_slice) * size;      // first slice here, the others one place and two places apart
     if (slices <= kFewSlices) {
       const long long on = 2 * size;
       for (long long i0 = static_cast<long long>(blockIdx.x) * 1024 + threadIdx.x; i0 < size; i0 += static_cast<long long>(gridDim.x) * 1024) {
@@ -867,13 +878,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
   const int tiles = map.Total() * across;
   int issued = 0, last_stage = 0; unsigned int last_parity = 0;      // steps copied (first copying thread) or multiplied (issuing thread); the latter's last stage
   // Products: the row tiles of the leaves, `across_b` output tiles each. Gram: slices, across_a x across_b tiles each.
-  struct Tile { int leaf, which, m0, n0, depth, row0, end; };
+  struct Tile { int leaf, which, m0, n0, depth, row0, end, leaf_begin, leaf_end; };
   int span = 0;
   auto tile_of = [&](int t) {
     Tile r;
     r.which = t / across;
     const int rest = t - r.which * across;
-    map.Find(a.leaves, r.which, a.tile_rows, a.least, &span, &r.leaf, &r.row0, &r.end);
+    map.Find(a.leaves, r.which, a.tile_rows, a.least, &span, &r.leaf, &r.row0, &r.end, &r.leaf_begin, &r.leaf_end);
     r.m0 = MODE == kGram ? rest / a.across_b * kTileM : 0; r.n0 = rest % a.across_b * a.n;
     r.depth = MODE == kGram ? r.end - r.row0 : a.depth;
     return r;
@@ -1079,7 +1090,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) LeafTensorKernel(const __grid_c
       } else {
         const int m = warp * 32 + lane, m_end = min(kTileM, a.a_size - tile.m0);
         const long long at = (tile.m0 + m) * a.out_row_stride + tile.n0 * a.out_col_stride;
-        const int slot = SliceSlot(a.leaves, tile.leaf, tile.row0, a.tile_rows);
+        const int slot = SliceSlot(tile.leaf_begin, tile.leaf_end, tile.row0, a.tile_rows);
         O* out = static_cast<O*>(a.out) + static_cast<long long>(tile.leaf) * a.a_size * a.b_size + at;
         float* part = slot >= 0 ? a.partial + static_cast<long long>(slot) * a.a_size * a.b_size + at : nullptr;
         for (int c0 = 0; c0 < n_end; c0 += 16) {

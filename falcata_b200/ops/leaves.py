@@ -74,8 +74,9 @@ def leaf_products(x: torch.Tensor, weight: torch.Tensor, leaf_begin: torch.Tenso
     """``y[i] = weight[leaf of row i] @ x[i]``: [rows, outputs] from ``x`` [rows, features] and ``weight`` [leaves, outputs, features].
 
     float32 / float16 / bfloat16, one type. ``weight`` may have any strides (a transposed view gives the gradient in ``x``). Rows
-    before the first and behind the last leaf get zeros. Boundaries outside the rows are clamped to them; boundaries that fall
-    again leave the rows concerned unspecified. Differentiable in ``x`` and ``weight`` (once); runs on the current stream.
+    before the first and behind the last leaf get zeros. Boundaries outside the rows are clamped to them; where boundaries fall
+    again, a row that several leaves claim belongs to the first of them. Differentiable in ``x`` and ``weight`` (once); runs on
+    the current stream.
     """
     _rows("x", x)
     require_tensor("weight", weight)
@@ -94,8 +95,9 @@ def leaf_gram(a: torch.Tensor, b: torch.Tensor, leaf_begin: torch.Tensor, dtype:
     """``out[g] = sum over the rows i of leaf g of a[i] b[i]^T``: [leaves, columns of a, columns of b], leaves without rows zero.
 
     With the gradient of ``leaf_products`` for ``a`` and its ``x`` for ``b`` this is the gradient in the weights; with ``h * x`` and
-    ``x`` the normal equations of linear leaves. ``dtype``: the inputs' type (default) or float32. Not differentiable; runs on the
-    current stream, the same sums on every run.
+    ``x`` the normal equations of linear leaves. ``dtype``: the inputs' type (default) or float32. Boundaries are clamped to the
+    rows; where they fall again, the sums of the leaves concerned are unspecified. Not differentiable; runs on the current
+    stream, the same sums on every run.
     """
     _rows("a", a); _rows("b", b)
     if a.dtype != b.dtype:

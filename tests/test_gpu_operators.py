@@ -678,3 +678,91 @@ def test_leaf_gram_whose_waits_run_out(side, tries):
             assert bool(given[2].all())                        # no rows, nothing to wait for
     for dtype in (torch.float32, torch.float16):
         _near(ops.leaf_gram(a, b, begin, dtype=dtype), want, size, n, dtype)
+
+
+# ------------------------------------------------------------------------- many leaves, boundaries that fall ----
+def _check_leaves(x, w, d, begin, begin_given=None):
+    """Products, transposed products and Gram sums of rows that lie leaf by leaf; rows outside the leaves are zero."""
+    from falcata_b200 import ops
+    dtype, (n, f), (leaves, k) = x.dtype, x.shape, w.shape[:2]
+    b = begin.long()
+    row = torch.arange(n, device="cuda")
+    leaf = torch.searchsorted(b, row, right=True) - 1
+    there = ((leaf >= 0) & (leaf < leaves)).double()[:, None]
+    leaf = leaf.clamp(0, leaves - 1)
+    given = begin if begin_given is None else begin_given
+
+    def products(a, m):
+        parts = [(torch.einsum("nf,nkf->nk", a[i:i + 4096].double(), m[leaf[i:i + 4096]].double()), torch.einsum("nf,nkf->nk", a[i:i + 4096].double().abs(), m[leaf[i:i + 4096]].double().abs())) for i in range(0, n, 4096)]
+        return torch.cat([p[0] for p in parts]) * there, torch.cat([p[1] for p in parts]) * there
+
+    want, size = products(x, w)
+    y = ops.leaf_products(x, w, given)
+    _near(y, want, size, f, dtype)
+    assert bool((y[there[:, 0] == 0] == 0).all())
+    want, size = products(d, w.transpose(1, 2))
+    _near(ops.leaf_products(d, w.transpose(1, 2), given), want, size, k, dtype)
+    if begin_given is not None:
+        return
+    want, size = torch.zeros((leaves, k, f), dtype=torch.float64, device="cuda"), torch.zeros((leaves, k, f), dtype=torch.float64, device="cuda")
+    for i in range(0, n, 2048):
+        outer = torch.einsum("nk,nf->nkf", d[i:i + 2048].double(), x[i:i + 2048].double()) * there[i:i + 2048, :, None]
+        want.index_add_(0, leaf[i:i + 2048], outer); size.index_add_(0, leaf[i:i + 2048], outer.abs())
+    for out in {dtype, torch.float32}:
+        p = ops.leaf_gram(d, x, given, dtype=out)
+        _near(p, want, size, int((b[1:] - b[:-1]).max()), out)
+        assert torch.equal(p, ops.leaf_gram(d, x, given, dtype=out))
+
+
+def _many_leaves(leaves, n, long_leaf, seed):
+    """Boundaries of leaves of which many are empty, one is long, and some rows lie before the first and behind the last."""
+    g = torch.Generator(); g.manual_seed(seed)
+    size = torch.randint(0, 4, (leaves,), generator=g) * (torch.rand(leaves, generator=g) < 0.6)
+    size[leaves // 3: leaves // 3 + 70] = 0                    # a run of empty ones, across spans
+    size[leaves // 2] = long_leaf
+    begin = torch.cat([torch.zeros(1, dtype=torch.long), torch.cumsum(size, 0)]) + 7
+    assert int(begin[-1]) + 5 <= n
+    return begin.cuda()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("leaves,f,k,long_leaf", [(1024, 9, 5, 700), (1025, 9, 5, 700), (3000, 12, 7, 6000), (5000, 28, 10, 300), (1025, 70, 50, 600), (3000, 40, 33, 3000), (2049, 130, 40, 5000), (1500, 48, 200, 2500)])
+def test_more_leaves_than_spans(dtype, leaves, f, k, long_leaf):
+    """More leaves than the tile map has places: several per place, looked up leaf by leaf."""
+    n = 2 * leaves + long_leaf + 400
+    g = _gen(leaves)
+    begin = _many_leaves(leaves, n, long_leaf, seed=f)
+    x, d = torch.randn((n, f), generator=g, device="cuda").to(dtype), torch.randn((n, k), generator=g, device="cuda").to(dtype)
+    w = torch.randn((leaves, k, f), generator=g, device="cuda").mul(f ** -0.5).to(dtype)
+    _check_leaves(x, w, d, begin.int() if leaves % 2 else begin)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("leaves,f,k", [(9, 9, 5), (9, 70, 50), (9, 130, 140), (2600, 9, 5), (2600, 70, 50)])
+def test_leaf_products_of_falling_boundaries(dtype, leaves, f, k):
+    """A row that several leaves claim belongs to the first of them; the others' rows are what they would be anyway."""
+    g = _gen(f)
+    n = 4 * leaves + 900
+    given = _many_leaves(leaves, n, 500, seed=k)
+    given[leaves // 4] = n - 11; given[leaves // 4 + 1] = 3      # up and down again
+    given[1::7] -= 20
+    begin = torch.cummax(given.clamp(0, n), 0).values
+    x, d = torch.randn((n, f), generator=g, device="cuda").to(dtype), torch.randn((n, k), generator=g, device="cuda").to(dtype)
+    w = torch.randn((leaves, k, f), generator=g, device="cuda").mul(f ** -0.5).to(dtype)
+    _check_leaves(x, w, d, begin, given)
+    from falcata_b200 import ops
+    assert ops.leaf_gram(d, x, given).shape == (leaves, k, f)
+
+
+@pytest.mark.parametrize("f,k", [(4, 2), (40, 36)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_leaf_products_of_all_rows_claimed_over_and_over(dtype, f, k):
+    """As many leaves as would make more tiles than 31 bits count if each had the rows that it claims."""
+    from falcata_b200 import ops
+    n, leaves = 1 << 20, 300_001
+    g = _gen(f)
+    given = torch.zeros(leaves + 1, dtype=torch.int32, device="cuda"); given[1::2] = n
+    x = torch.randn((n, f), generator=g, device="cuda").to(dtype); w = torch.randn((1, k, f), generator=g, device="cuda").to(dtype)
+    y = ops.leaf_products(x, w.expand(leaves, k, f), given)
+    _near(y, x.double() @ w[0].double().t(), x.double().abs() @ w[0].double().abs().t(), f, dtype)
+    assert ops.leaf_gram(x[:, :1], x[:, :2], given).shape == (leaves, 1, 2)
