@@ -7,11 +7,12 @@ device predict output) and for rank bootstrap; all training state lives in the C
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import json
 import os
 from pathlib import Path
-from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple, Union
+from typing import Any, Callable, Dict, Iterator, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 
@@ -125,6 +126,20 @@ def _is_cuda_array(x: Any) -> bool:
     if _is_torch_tensor(x):
         return x.is_cuda
     return hasattr(x, "__cuda_array_interface__")
+
+
+@contextlib.contextmanager
+def _default_stream_of(t: Any) -> Iterator[None]:
+    """The native core works on the default stream of the current device and waits for it: ``t``'s device is current inside, and its
+    default stream waits for what the caller's stream has been given so far (the tensors handed over, and earlier uses of
+    their memory)."""
+    import torch
+
+    with torch.cuda.device(t.device):
+        default, current = torch.cuda.default_stream(), torch.cuda.current_stream()
+        if current != default:
+            default.wait_stream(current)
+        yield
 
 
 def _to_numpy_2d(data: Any) -> np.ndarray:
@@ -1226,8 +1241,9 @@ class Booster:
             _safe_call(lib.FB_BoosterCalcNumPredict(self._handle, 1, 2, start_iteration, num_iteration, ctypes.byref(per_row)))
             out = torch.zeros((nrow, max(1, per_row.value)), dtype=torch.int32, device=t.device)
             code = {torch.float32: 0, torch.float64: 1, torch.float16: 6}[t.dtype]
-            rc = lib.FB_BoosterPredictForDeviceMat(self._handle, ctypes.c_void_p(t.data_ptr()), code, ctypes.c_int32(nrow), ctypes.c_int32(ncol), 1,
-                                                   2, start_iteration, num_iteration, ctypes.c_void_p(out.data_ptr()))
+            with _default_stream_of(t):
+                rc = lib.FB_BoosterPredictForDeviceMat(self._handle, ctypes.c_void_p(t.data_ptr()), code, ctypes.c_int32(nrow), ctypes.c_int32(ncol), 1,
+                                                       2, start_iteration, num_iteration, ctypes.c_void_p(out.data_ptr()))
             if rc == 0:
                 return out
             host = self.predict(t.detach().cpu().numpy(), start_iteration=start_iteration, num_iteration=num_iteration, pred_leaf=True)
@@ -1242,8 +1258,9 @@ class Booster:
             nrow, ncol = t.shape
             out = torch.empty((k, nrow), dtype=torch.float32, device=t.device)
             code = {torch.float32: 0, torch.float64: 1, torch.float16: 6}[t.dtype]
-            _safe_call(lib.FB_BoosterPredictForDeviceMat(self._handle, ctypes.c_void_p(t.data_ptr()), code, ctypes.c_int32(nrow), ctypes.c_int32(ncol), 1,
-                                                         ptype, start_iteration, num_iteration, ctypes.c_void_p(out.data_ptr())))
+            with _default_stream_of(t):
+                _safe_call(lib.FB_BoosterPredictForDeviceMat(self._handle, ctypes.c_void_p(t.data_ptr()), code, ctypes.c_int32(nrow), ctypes.c_int32(ncol), 1,
+                                                             ptype, start_iteration, num_iteration, ctypes.c_void_p(out.data_ptr())))
             return out[0] if k == 1 else out.t().contiguous()
         if hasattr(data, "tocsr") and not isinstance(data, np.ndarray):
             # scipy sparse input: the rows are densified in blocks inside the library, never as one matrix; contributions

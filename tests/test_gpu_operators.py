@@ -766,3 +766,38 @@ def test_leaf_products_of_all_rows_claimed_over_and_over(dtype, f, k):
     y = ops.leaf_products(x, w.expand(leaves, k, f), given)
     _near(y, x.double() @ w[0].double().t(), x.double().abs() @ w[0].double().abs().t(), f, dtype)
     assert ops.leaf_gram(x[:, :1], x[:, :2], given).shape == (leaves, 1, 2)
+
+
+# ------------------------------------------------------------------------------- the booster's calls on streams ----
+def _late(values, big):
+    """`values`, written by the current stream only after a while of other work."""
+    x = torch.full_like(values, math.nan)
+    for _ in range(4):
+        big = big @ big
+    return x.copy_(torch.where(big[0, 0].isnan(), values, values))
+
+
+def test_booster_predictions_on_a_side_stream():
+    """Rows that the caller's stream is still to write, results whose memory it has used before: as on the default stream."""
+    import falcata_b200 as fb
+    from util import make_multiclass
+    X, y = make_multiclass(n=20000, f=8, k=5)
+    bst = fb.train({"objective": "multiclass", "num_class": 5, "num_leaves": 15, "device_type": "cuda", "verbosity": -1}, fb.Dataset(X, y), 3)
+    Xd, labels = torch.from_numpy(X).float().cuda(), torch.from_numpy(y).cuda().long()
+    big = torch.randn((4096, 4096), generator=_gen(1), device="cuda").mul_(1e-3)
+    rows = [Xd.roll(i, 0).contiguous() for i in range(8)]
+    want = [(bst.predict_log_probs(r, labels, top_k=2), bst.predict(r), bst.predict(r, pred_leaf=True)) for r in rows]
+    torch.cuda.synchronize()
+    side, got = torch.cuda.Stream(), []
+    for _ in range(2):
+        for r in rows:
+            with torch.cuda.stream(side):
+                a = bst.predict_log_probs(_late(r, big), labels, top_k=2)
+                b = bst.predict(_late(r, big))
+                got.append((a, b, bst.predict(_late(r, big), pred_leaf=True)))
+    torch.cuda.synchronize()
+    for (a, b, c), (u, v, w) in zip(got, want + want):
+        assert all(torch.equal(p, q) for p, q in zip(a, u)) and torch.equal(b, v) and torch.equal(c, w)
+    for empty in (Xd[:0],):
+        r = bst.predict_log_probs(empty, labels[:0], top_k=2)
+        assert r.log_prob.shape == (0,) and r.top_class.shape == (0, 2)
