@@ -1058,7 +1058,8 @@ class Booster:
 
             g = grad.detach().to(torch.float32).contiguous().reshape(-1)
             h = hess.detach().to(torch.float32).contiguous().reshape(-1)
-            _safe_call(lib.FB_BoosterUpdateOneIterCustom(self._handle, ctypes.c_void_p(g.data_ptr()), ctypes.c_void_p(h.data_ptr()), 1, ctypes.byref(fin)))
+            with _default_stream_of(g):
+                _safe_call(lib.FB_BoosterUpdateOneIterCustom(self._handle, ctypes.c_void_p(g.data_ptr()), ctypes.c_void_p(h.data_ptr()), 1, ctypes.byref(fin)))
             torch.cuda.synchronize()
         else:
             if _is_torch_tensor(grad):
@@ -1074,7 +1075,8 @@ class Booster:
                 import torch
 
                 gt = torch.from_numpy(g).cuda(); ht = torch.from_numpy(h).cuda()
-                _safe_call(lib.FB_BoosterUpdateOneIterCustom(self._handle, ctypes.c_void_p(gt.data_ptr()), ctypes.c_void_p(ht.data_ptr()), 1, ctypes.byref(fin)))
+                with _default_stream_of(gt):
+                    _safe_call(lib.FB_BoosterUpdateOneIterCustom(self._handle, ctypes.c_void_p(gt.data_ptr()), ctypes.c_void_p(ht.data_ptr()), 1, ctypes.byref(fin)))
                 torch.cuda.synchronize()
             else:
                 _safe_call(lib.FB_BoosterUpdateOneIterCustom(self._handle, g.ctypes.data_as(ctypes.c_void_p), h.ctypes.data_as(ctypes.c_void_p), 0, ctypes.byref(fin)))

@@ -801,3 +801,32 @@ def test_booster_predictions_on_a_side_stream():
     for empty in (Xd[:0],):
         r = bst.predict_log_probs(empty, labels[:0], top_k=2)
         assert r.log_prob.shape == (0,) and r.top_class.shape == (0, 2)
+
+
+def test_custom_objective_on_a_side_stream():
+    """Gradients that the caller's stream is still to write when the booster takes them: the same model as on the default stream.
+
+    The booster adds fp32 gradients in any order, so that two trainings on one stream differ in the last bits. Multiples of 1/64 up to
+    1 in size add up exactly (20000 of them stay below 2^24 / 64), and equal sums give equal models."""
+    import falcata_b200 as fb
+    from falcata_b200 import ops
+    from util import make_multiclass
+    X, y = make_multiclass(n=20000, f=10, k=3)
+    labels = torch.from_numpy(y).cuda().int()
+    big = torch.randn((4096, 4096), generator=_gen(1), device="cuda").mul_(1e-3)
+
+    def train(stream):
+        def objective(scores, _):
+            r = ops.class_log_probs(scores, labels)
+            grad = ops.class_log_probs_grad(scores, r.log_norm, r.entropy, labels=labels, grad_log_prob=torch.full_like(r.log_prob, -1.0))
+            p = torch.exp(scores - r.log_norm[:, None])
+            return _late((grad * 64).round().div(64).t(), big), _late((96 * p * (1 - p)).round().add(1).div(64).t().contiguous(), big)
+
+        bst = fb.Booster({"num_class": 3, "num_leaves": 7, "device_type": "cuda", "verbosity": -1, "objective": "none"}, fb.Dataset(X, y))
+        with torch.cuda.stream(stream):
+            for _ in range(4):
+                bst.update(fobj=objective)
+        torch.cuda.synchronize()
+        return bst.model_to_string()
+
+    assert train(torch.cuda.Stream()) == train(torch.cuda.default_stream())
