@@ -2,9 +2,10 @@
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import Callable, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from ..basic import _lib
 
@@ -58,6 +59,33 @@ def one_device(**tensors: Optional[torch.Tensor]) -> None:
             if device is not None:
                 raise ValueError(f"{name}: on {where}, the other tensors are on {device}")
             device = where
+
+
+def no_tangents(operator: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode derivatives are refused, not dropped."""
+    if getattr(forward_ad, "_current_level", 0) < 0:      # outside forward-mode differentiation: nothing to look for
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{operator}: forward-mode derivatives are not available")
+
+
+class _NoDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, operator, compute, *tensors):
+        ctx.operator = operator
+        return compute()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(f"{ctx.operator}: its result has no derivative; detach it or the inputs")
+
+
+def without_derivative(operator: str, compute: Callable[[], torch.Tensor], *tensors: Optional[torch.Tensor]) -> torch.Tensor:
+    """``compute()``; where a gradient is wanted in one of the tensors, a backward pass through the result raises."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return _NoDerivative.apply(operator, compute, *tensors)
+    return compute()
 
 
 # The stream's handle without the Python object around it, where torch offers that (1 us less per call).

@@ -10,7 +10,7 @@ from typing import Optional
 
 import torch
 
-from ._call import bind, check, device_and_stream, one_device, ptr, require_tensor, type_code
+from ._call import bind, check, device_and_stream, no_tangents, one_device, ptr, require_tensor, type_code, without_derivative
 
 __all__ = ["leaf_gram", "leaf_products"]
 
@@ -85,6 +85,7 @@ def leaf_products(x: torch.Tensor, weight: torch.Tensor, leaf_begin: torch.Tenso
     _begin(leaf_begin)
     if weight.dim() != 3 or weight.shape[0] != leaf_begin.numel() - 1 or weight.shape[1] < 1 or weight.shape[2] != x.shape[1]:
         raise ValueError(f"weight: [{leaf_begin.numel() - 1} leaves, outputs, {x.shape[1]} features] is wanted, got shape {tuple(weight.shape)}")
+    no_tangents("leaf_products", x, weight)
     one_device(x=x, weight=weight, leaf_begin=leaf_begin)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _LeafProducts.apply(x, weight, leaf_begin)
@@ -96,8 +97,8 @@ def leaf_gram(a: torch.Tensor, b: torch.Tensor, leaf_begin: torch.Tensor, dtype:
 
     With the gradient of ``leaf_products`` for ``a`` and its ``x`` for ``b`` this is the gradient in the weights; with ``h * x`` and
     ``x`` the normal equations of linear leaves. ``dtype``: the inputs' type (default) or float32. Boundaries are clamped to the
-    rows; where they fall again, the sums of the leaves concerned are unspecified. Not differentiable; runs on the current
-    stream, the same sums on every run.
+    rows; where they fall again, the sums of the leaves concerned are unspecified. Not differentiable (a backward
+    pass through the result raises); runs on the current stream, the same sums on every run.
     """
     _rows("a", a); _rows("b", b)
     if a.dtype != b.dtype:
@@ -108,7 +109,12 @@ def leaf_gram(a: torch.Tensor, b: torch.Tensor, leaf_begin: torch.Tensor, dtype:
     if dtype not in (a.dtype, torch.float32):
         raise TypeError(f"dtype: {a.dtype} or float32 is wanted, got {dtype}")
     _begin(leaf_begin)
+    no_tangents("leaf_gram", a, b)
     one_device(a=a, b=b, leaf_begin=leaf_begin)
+    return without_derivative("leaf_gram", lambda: _sums(a, b, leaf_begin, dtype), a, b)
+
+
+def _sums(a: torch.Tensor, b: torch.Tensor, leaf_begin: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     a, b, leaf_begin = _inner_contiguous(a), _inner_contiguous(b), leaf_begin.contiguous()
     leaves = leaf_begin.numel() - 1
     out = a.new_empty((leaves, a.shape[1], b.shape[1]), dtype=dtype)

@@ -17,7 +17,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from ._call import bind, check, device_and_stream, one_device, ptr, require_tensor, type_code
+from ._call import bind, check, device_and_stream, no_tangents, one_device, ptr, require_tensor, type_code, without_derivative
 
 MAX_TOP_CLASSES = 32
 
@@ -109,6 +109,7 @@ def class_log_probs(scores: torch.Tensor, labels: Optional[torch.Tensor] = None,
     top_k = int(top_k)
     if not 0 <= top_k <= min(MAX_TOP_CLASSES, scores.shape[1]):
         raise ValueError(f"top_k: 0 to {min(MAX_TOP_CLASSES, scores.shape[1])} alternatives of {scores.shape[1]} classes, got {top_k}")
+    no_tangents("class_log_probs", scores)
     one_device(scores=scores, labels=labels)
     if scores.requires_grad and torch.is_grad_enabled():
         return ClassLogProbs(*_ClassLogProbs.apply(scores, labels, top_k))
@@ -122,6 +123,7 @@ def class_log_probs_grad(scores: torch.Tensor, log_norm: torch.Tensor, entropy: 
 
     ``log_norm``, ``entropy``, ``top_class``: those results. The gradient has the type of the scores and their order in memory
     (class-major scores give a class-major gradient, whose transpose is what ``Booster.update`` takes from a custom objective).
+    It has no derivative itself: a backward pass through it raises.
     """
     _scores(scores)
     labels = _labels(labels, scores)
@@ -143,9 +145,16 @@ def class_log_probs_grad(scores: torch.Tensor, log_norm: torch.Tensor, entropy: 
     else:
         top_class = None
     grads = [_row_values(name, t, (n,)) for name, t in (("grad_log_prob", grad_log_prob), ("grad_log_norm", grad_log_norm), ("grad_entropy", grad_entropy))]
+    inputs = (scores, log_norm, entropy, *grads, grad_top_log_prob)
+    no_tangents("class_log_probs_grad", *inputs)
     one_device(scores=scores, labels=labels, log_norm=log_norm, entropy=entropy, top_class=top_class, grad_log_prob=grads[0], grad_log_norm=grads[1], grad_entropy=grads[2],
                grad_top_log_prob=grad_top_log_prob)
-    log_norm, entropy, grad_top_log_prob, *grads = (None if t is None else (t if t.dtype is torch.float32 else t.float()).contiguous() for t in (log_norm, entropy, grad_top_log_prob, *grads))
+    return without_derivative("class_log_probs_grad", lambda: _gradient(scores, labels, top_k, top_class, log_norm, entropy, grad_top_log_prob, *grads), *inputs)
+
+
+def _gradient(scores: torch.Tensor, labels: Optional[torch.Tensor], top_k: int, top_class: Optional[torch.Tensor], *values: Optional[torch.Tensor]) -> torch.Tensor:
+    n, k = scores.shape
+    log_norm, entropy, grad_top_log_prob, *grads = (None if t is None else (t if t.dtype is torch.float32 else t.float()).contiguous() for t in values)
     labels, top_class = (None if t is None else t.contiguous() for t in (labels, top_class))
     by_class = scores.stride(0) < scores.stride(1)
     out = scores.new_empty((k, n)).t() if by_class else scores.new_empty((n, k))

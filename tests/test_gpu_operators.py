@@ -830,3 +830,28 @@ def test_custom_objective_on_a_side_stream():
         return bst.model_to_string()
 
     assert train(torch.cuda.Stream()) == train(torch.cuda.default_stream())
+
+
+def test_results_without_a_derivative_say_so():
+    """A backward pass through a Gram sum or a gradient raises where it would have lost a derivative; their values are as ever."""
+    from falcata_b200 import ops
+    x, d = (torch.randn((50, 6), generator=_gen(i), device="cuda") for i in range(2))
+    begin = torch.tensor([0, 20, 50], device="cuda")
+    plain = ops.leaf_gram(d, x, begin)
+    assert not plain.requires_grad
+    p = ops.leaf_gram(d, x.clone().requires_grad_(), begin)
+    assert torch.equal(p, plain)
+    with pytest.raises(NotImplementedError, match="leaf_gram"):
+        p.sum().backward()
+    f = ops.class_log_probs(x)
+    z = x.clone().requires_grad_()
+    g = ops.class_log_probs_grad(z, f.log_norm, f.entropy, grad_entropy=torch.ones(50, device="cuda"))
+    assert torch.equal(g, ops.class_log_probs_grad(x, f.log_norm, f.entropy, grad_entropy=torch.ones(50, device="cuda")))
+    with pytest.raises(NotImplementedError, match="class_log_probs_grad"):
+        (g * z).sum().backward()
+    with torch.no_grad():
+        assert not ops.leaf_gram(d, z, begin).requires_grad
+    for transform in (lambda s: torch.func.jvp(lambda t: ops.class_log_probs(t).entropy, (s,), (torch.ones_like(s),)), lambda s: torch.func.grad(lambda t: ops.class_log_probs(t).entropy.sum())(s),
+                      lambda s: torch.func.vmap(lambda t: ops.class_log_probs(t).entropy)(s.reshape(5, 10, 6))):
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            transform(x)

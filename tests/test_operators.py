@@ -98,3 +98,19 @@ def test_native_entry_points_return_errors():
     assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(16), I(2), L(4), I(3), I(5), I(0), P(), P(), P(), I(0), P()) == -1 and b"boundaries" in lib.FB_OpsLastError()
     assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(32), I(2), L(4), I(0), I(5), I(0), P(), P(), P(), I(0), P()) == -1 and b"feature" in lib.FB_OpsLastError()
     assert lib.FB_OpLeafGram(P(), L(3), P(), L(3), P(), I(32), I(2), L(4), I(0), I(3), I(0), I(0), P(), P(), P(), I(0), P()) == -1 and b"column" in lib.FB_OpsLastError()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent would be lost without a word; outside forward mode, and for tensors without a tangent, nothing changes."""
+    from torch.autograd import forward_ad
+
+    half = torch.zeros(4)
+    with forward_ad.dual_level():
+        s, x, w = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (S, X, W))
+        z = forward_ad.make_dual(Z, torch.ones_like(Z))
+        for call in (lambda: ops.class_log_probs(s, Y), lambda: ops.class_log_probs_grad(s, Z, Z), lambda: ops.class_log_probs_grad(S, z, Z), lambda: ops.class_log_probs_grad(S, Z, Z, grad_entropy=z),
+                     lambda: ops.leaf_products(x, W, B), lambda: ops.leaf_products(X, w, B), lambda: ops.leaf_gram(x, X, B), lambda: ops.leaf_gram(X, x, B)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.class_log_probs_grad(S, half, half)
