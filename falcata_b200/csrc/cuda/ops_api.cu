@@ -56,8 +56,9 @@ void CheckClassScores(long long rows, long long classes, int label_bits, int top
   if (label_bits != 0 && label_bits != 32 && label_bits != 64) Log::Fatal("class scores: labels of %d bits", label_bits);
   if (top_k < 0 || top_k > kMaxTopClasses || top_k > classes) Log::Fatal("class scores: %d alternatives of %lld classes (at most %d)", top_k, classes, kMaxTopClasses);
 }
+constexpr int kMostLeafSize = 1 << 28;      // leaves, columns: steps beyond them and bytes of a row are counted in 32 bits
 void CheckLeafWindows(int begin_bits, int leaves, long long rows) {
-  if (rows < 0 || rows > 0x7fffffffLL || leaves < 1) Log::Fatal("leaf products: %lld rows in %d leaves are not covered", rows, leaves);
+  if (rows < 0 || rows > 0x7fffffffLL || leaves < 1 || leaves > kMostLeafSize) Log::Fatal("leaf products: %lld rows in %d leaves are not covered", rows, leaves);
   if (begin_bits != 32 && begin_bits != 64) Log::Fatal("leaf products: boundaries of %d bits", begin_bits);
 }
 }  // namespace
@@ -258,7 +259,7 @@ int FB_OpLeafProducts(const void* x, long long x_stride, const void* weight, lon
                       int begin_bits, int leaves, long long rows, int features, int outputs, int dtype, void* y, void* workspace, long long* workspace_floats, int device, void* stream) {
   OPS_BEGIN();
   CheckLeafWindows(begin_bits, leaves, rows);
-  if (features < 1 || outputs < 1) Log::Fatal("leaf products: at least one feature and one output (got %d, %d)", features, outputs);
+  if (features < 1 || outputs < 1 || features > kMostLeafSize || outputs > kMostLeafSize) Log::Fatal("leaf products: at least one feature and one output, at most 2^28 (got %d, %d)", features, outputs);
   LeafProductsArgs a{{begin, begin_bits, leaves, rows}, x, weight, y, dtype, features, outputs, x_stride, weight_leaf_stride, weight_out_stride, weight_in_stride};
   const long long floats = LeafProductsWorkspace(a);
   if (workspace_floats != nullptr) { *workspace_floats = floats; if (floats > 0) return 0; }
@@ -272,7 +273,7 @@ int FB_OpLeafGram(const void* a_rows, long long a_stride, const void* b_rows, lo
                   int dtype, int out_dtype, void* out, void* workspace, long long* workspace_floats, int device, void* stream) {
   OPS_BEGIN();
   CheckLeafWindows(begin_bits, leaves, rows);
-  if (a_cols < 1 || b_cols < 1) Log::Fatal("leaf Gram: at least one column on each side (got %d, %d)", a_cols, b_cols);
+  if (a_cols < 1 || b_cols < 1 || a_cols > kMostLeafSize || b_cols > kMostLeafSize) Log::Fatal("leaf Gram: at least one column on each side, at most 2^28 (got %d, %d)", a_cols, b_cols);
   LeafGramArgs a{{begin, begin_bits, leaves, rows}, a_rows, b_rows, out, dtype, out_dtype, a_cols, b_cols, a_stride, b_stride};
   const long long floats = LeafGramWorkspace(a);
   if (workspace_floats != nullptr) { *workspace_floats = floats; if (floats > 0) return 0; }

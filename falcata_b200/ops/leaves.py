@@ -15,10 +15,15 @@ from ._call import bind, check, device_and_stream, no_tangents, one_device, ptr,
 __all__ = ["leaf_gram", "leaf_products"]
 
 
+MAX_COLUMNS = MAX_LEAVES = 1 << 28      # the native call counts them, and a row's bytes, in 32 bits
+
+
 def _begin(leaf_begin: torch.Tensor) -> None:
     require_tensor("leaf_begin", leaf_begin)
     if leaf_begin.dtype not in (torch.int32, torch.int64) or leaf_begin.dim() != 1 or leaf_begin.numel() < 2:
         raise ValueError(f"leaf_begin: int32 or int64 of [leaves + 1], at least one leaf, is wanted, got {leaf_begin.dtype} {tuple(leaf_begin.shape)}")
+    if leaf_begin.numel() - 1 > MAX_LEAVES:
+        raise ValueError(f"leaf_begin: at most {MAX_LEAVES} leaves are covered, got {leaf_begin.numel() - 1}")
 
 
 def _rows(name: str, t: torch.Tensor) -> None:
@@ -26,6 +31,8 @@ def _rows(name: str, t: torch.Tensor) -> None:
     type_code(name, t)
     if t.dim() != 2 or t.shape[1] < 1:
         raise ValueError(f"{name}: [rows, columns] with at least one column is wanted, got shape {tuple(t.shape)}")
+    if t.shape[1] > MAX_COLUMNS:
+        raise ValueError(f"{name}: at most {MAX_COLUMNS} columns are covered, got {t.shape[1]}")
 
 
 def _inner_contiguous(t: torch.Tensor) -> torch.Tensor:
@@ -85,6 +92,8 @@ def leaf_products(x: torch.Tensor, weight: torch.Tensor, leaf_begin: torch.Tenso
     _begin(leaf_begin)
     if weight.dim() != 3 or weight.shape[0] != leaf_begin.numel() - 1 or weight.shape[1] < 1 or weight.shape[2] != x.shape[1]:
         raise ValueError(f"weight: [{leaf_begin.numel() - 1} leaves, outputs, {x.shape[1]} features] is wanted, got shape {tuple(weight.shape)}")
+    if weight.shape[1] > MAX_COLUMNS:
+        raise ValueError(f"weight: at most {MAX_COLUMNS} outputs are covered, got {weight.shape[1]}")
     no_tangents("leaf_products", x, weight)
     one_device(x=x, weight=weight, leaf_begin=leaf_begin)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):

@@ -114,3 +114,23 @@ def test_forward_mode_derivatives_are_refused():
                 call()
         with pytest.raises(ValueError, match="CUDA"):
             ops.class_log_probs_grad(S, half, half)
+
+
+def test_sizes_beyond_the_native_call_are_refused():
+    """The native call takes leaves and columns as 32-bit numbers: 2^32 + 3 of them must not pass as 3."""
+    from falcata_b200.basic import _lib
+
+    many = (1 << 32) + 3
+    one = torch.zeros(1, 1)
+    wide, begin = one.expand(1, many), torch.zeros(1, dtype=torch.int32)
+    for call, word in ((lambda: ops.leaf_products(wide, one[None].expand(2, 5, many), B), "columns"), (lambda: ops.leaf_products(X, one[None].expand(2, many, 3), B), "outputs"),
+                       (lambda: ops.leaf_gram(wide, one, B), "columns"), (lambda: ops.leaf_gram(one, wide, B), "columns"), (lambda: ops.leaf_gram(X, X, begin.expand(many + 1)), "leaves"),
+                       (lambda: ops.leaf_products(X, one[None].expand(many, 5, 3), begin.expand(many + 1)), "leaves")):
+        with pytest.raises(ValueError, match=f"{word} are covered"):
+            call()
+    lib, L, I, P = _lib(), ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p
+    lib.FB_OpsLastError.restype = ctypes.c_char_p
+    over = (1 << 28) + 1
+    for leaves, f, k in ((over, 3, 5), (2, over, 5), (2, 3, over)):
+        assert lib.FB_OpLeafProducts(P(), L(3), P(), L(15), L(3), L(1), P(), I(32), I(leaves), L(4), I(f), I(k), I(0), P(), P(), P(), I(0), P()) == -1 and (b"leaves" if leaves == over else b"2^28") in lib.FB_OpsLastError()
+        assert lib.FB_OpLeafGram(P(), L(3), P(), L(3), P(), I(32), I(leaves), L(4), I(f), I(k), I(0), I(0), P(), P(), P(), I(0), P()) == -1
