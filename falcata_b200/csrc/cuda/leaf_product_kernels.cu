@@ -316,7 +316,7 @@ __device__ __forceinline__ int SliceSlot(int leaf_begin, int leaf_end, int row0,
 template <int TA, int TB, int GA, int GB, int SLICES, int RD>
 struct FloatGramTile {
   static constexpr int AC = TA * GA, BC = TB * GB, GROUP = GA * GB, THREADS = GROUP * SLICES;
-  static constexpr int kLoad = kRing * RD * (AC + BC) * 4, kSum = SLICES > 1 ? SLICES * AC * BC * 4 : 0, kBytes = kLoad > kSum ? kLoad : kSum;
+  static constexpr int kLoad = kRing * RD * (AC + BC) * 4, kSum = SLICES * AC * BC * 4, kBytes = kLoad > kSum ? kLoad : kSum;
 };
 // A leaf of one slice is written to out; the sums of the slices of longer leaves go to partial [slot][a_cols][b_cols].
 template <int TA, int TB, int GA, int GB, int SLICES, int RD>
@@ -379,39 +379,25 @@ __global__ void __launch_bounds__(GA * GB * SLICES, 2) LeafGramFloatKernel(LeafG
     __syncthreads();
     const int slot = SliceSlot(leaf_begin, leaf_end, row0, rows_per_slice);
     float* to = slot >= 0 ? partial + static_cast<long long>(slot) * a.a_cols * a.b_cols : static_cast<float*>(a.out) + static_cast<long long>(leaf) * a.a_cols * a.b_cols;
-    if constexpr (SLICES == 1) {
+    float* s_sum = s_float;                  // the row buffers are free now
 #pragma unroll
-      for (int i = 0; i < TA; ++i)
+    for (int i = 0; i < TA; ++i)
 #pragma unroll
-        for (int j = 0; j < TB / 2; ++j) {
-          float v[2]; Split(acc[i][j], v[0], v[1]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int ca = ga * TA + i, cb = gb * TB + 2 * j + h;
-            if (ca < a_in && cb < b_in) to[static_cast<long long>(a0 + ca) * a.b_cols + b0 + cb] = v[h];
-          }
-        }
-    } else {
-      float* s_sum = s_float;                  // the row buffers are free now
-#pragma unroll
-      for (int i = 0; i < TA; ++i)
-#pragma unroll
-        for (int j = 0; j < TB / 2; ++j) {
-          float v0, v1; Split(acc[i][j], v0, v1);
-          float* p = s_sum + (slice * Tile::AC + ga * TA + i) * Tile::BC + gb * TB + 2 * j;
-          p[0] = v0; p[1] = v1;
-        }
-      __syncthreads();
-      for (int e = threadIdx.x; e < Tile::AC * Tile::BC; e += Tile::THREADS) {
-        const int ca = e / Tile::BC, cb = e % Tile::BC;
-        if (ca >= a_in || cb >= b_in) continue;
-        float v = 0.f;
-#pragma unroll
-        for (int s = 0; s < SLICES; ++s) v += s_sum[s * Tile::AC * Tile::BC + e];
-        to[static_cast<long long>(a0 + ca) * a.b_cols + b0 + cb] = v;
+      for (int j = 0; j < TB / 2; ++j) {
+        float v0, v1; Split(acc[i][j], v0, v1);
+        float* p = s_sum + (slice * Tile::AC + ga * TA + i) * Tile::BC + gb * TB + 2 * j;
+        p[0] = v0; p[1] = v1;
       }
-      __syncthreads();
+    __syncthreads();
+    for (int e = threadIdx.x; e < Tile::AC * Tile::BC; e += Tile::THREADS) {
+      const int ca = e / Tile::BC, cb = e % Tile::BC;
+      if (ca >= a_in || cb >= b_in) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int s = 0; s < SLICES; ++s) v += s_sum[s * Tile::AC * Tile::BC + e];
+      to[static_cast<long long>(a0 + ca) * a.b_cols + b0 + cb] = v;
     }
+    __syncthreads();
   }
 }
 
