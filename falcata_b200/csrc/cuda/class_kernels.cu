@@ -11,7 +11,8 @@
 // A row whose scores are all -inf has no distribution: log_norm and log probabilities -inf, entropy 0, no alternatives, gradient 0.
 // A row with a NaN or +inf has NaN everywhere and no alternatives.
 //
-// All kernels read every score once from memory, the gradient kernels write every value once: they are bound by bandwidth.
+// The forward kernels read every score once from memory, and so do the gradient kernels as long as log_norm is small enough to hold
+// the probabilities (kTrustedLogNorm), and write every value once: bound by bandwidth, in 16-bit types shared with the exponentials.
 // (S, T) are kept relative to a running maximum and rescaled when it grows, so partial results of any split of a row can be
 // joined. Which threads share a row goes by the number of classes and by what is contiguous:
 //   few classes                 a thread per row, the row in registers           (ClassLogProbsFewKernel)
@@ -33,7 +34,9 @@ namespace fb {
 
 namespace {
 
-// log_norm in fp32 gives p to a relative 2^-24 |log_norm|: beyond this size the gradient takes the row's maximum and sum again.
+// log_norm in fp32 gives p to a relative 2^-24 |log_norm|: beyond this size the gradient takes the row's maximum and sum again, once per
+// block of a row's chunks, or, where a thread has a row, once per slice of its classes. That costs much more than the gradient itself:
+// scores shifted by 100 take 1354 us instead of 206 at 8191 x 32001 bf16, 1167 instead of 26 at 4099 x 2000 fp32 class-major.
 constexpr float kTrustedLogNorm = 64.f;
 constexpr float kLowestExponent = -200.f;     // 2^x is 0 in fp32 from here on; keeps 0 * (-inf) out of T
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -771,7 +774,7 @@ __global__ void __launch_bounds__(kBlockThreads, 4) ClassLogProbsBlockKernel(Cla
 
 // ----------------------------------------------------------------------------------------- contiguous columns ----
 // A block turns tile_rows rows of class-major scores (or of any strides) into rows in shared memory, read as they lie: neighbouring
-// lanes have neighbouring rows. Then a warp per row, as above. Rows up to kTileBytes / 8 classes' worth of bytes long.
+// lanes have neighbouring rows. Then a warp per row, as above. Rows of up to kTileMostBytes / 8 bytes.
 // (Against the kernel below, which keeps a list per thread: 2479 x 2000 fp32 with 32 alternatives 230 -> 36 us.)
 constexpr int kTileBytes = 72 * 1024, kTileMostBytes = 200 * 1024;
 // PER > 0: at most 8 PER classes, 8 lanes per row.

@@ -3,7 +3,9 @@
 The functions in this file each run exactly one kernel of the training path (on the default stream, waiting for it) and serve
 the numerics tests. The operators on class scores (``class_log_probs`` and its gradient) and on rows grouped by leaf
 (``leaf_products``, ``leaf_gram``) are for programs: they run on the current stream without waiting, can be captured into a
-CUDA graph and are differentiable. If the native library is missing all of them raise: there is no PyTorch fallback on this path.
+CUDA graph and are differentiable. (Capture a backward pass by ``torch.autograd.grad``, or while no eager graph of the same leaves
+lives: torch joins the two at the leaves, which a capture does not survive.) If the native library is missing all of them raise:
+there is no PyTorch fallback on this path.
 """
 from __future__ import annotations
 

@@ -1,7 +1,9 @@
 """Matrix products of rows grouped by leaf: one linear map per leaf, leaves of any number of rows.
 
-``leaf_begin`` [leaves + 1] (int32 / int64, on the device, non-decreasing) gives leaf g the rows [leaf_begin[g], leaf_begin[g + 1]),
-as a partition of the rows by ``Booster.predict(..., pred_leaf=True)`` leaves them. Sums are fp32, rounded once to the output's type.
+``leaf_begin`` [leaves + 1] (int32 / int64, on the device, non-decreasing) gives leaf g the rows [leaf_begin[g], leaf_begin[g + 1]): the
+rows lie leaf by leaf. For the leaf numbers that ``Booster.predict(..., pred_leaf=True)`` gives in row order,
+``order = torch.argsort(leaf, stable=True)`` groups the rows, and ``torch.searchsorted(leaf[order], torch.arange(leaves + 1))``, of
+one type and on the device, gives their boundaries. Sums are fp32, rounded once to the output's type.
 """
 from __future__ import annotations
 
