@@ -855,3 +855,32 @@ def test_results_without_a_derivative_say_so():
                       lambda s: torch.func.vmap(lambda t: ops.class_log_probs(t).entropy)(s.reshape(5, 10, 6))):
         with pytest.raises((NotImplementedError, RuntimeError)):
             transform(x)
+
+
+@pytest.mark.parametrize("n,k", [(3, 60000), (19000, 60000), (40, 500), (40, 20000)])
+@pytest.mark.parametrize("step", [0.37, 0.61, 5.3])
+@pytest.mark.parametrize("shift", [0.0, 1000.0, 1e8])
+def test_class_log_probs_of_many_equal_terms(n, k, step, shift):
+    """Equal terms that fp32 does not hold exactly, where every rounding of a long sum goes the same way: sums must not run on in one
+    thread. (Classes far apart in memory, one vector for all rows, the highest scores where each thread starts.)"""
+    from falcata_b200 import ops
+    values = torch.full((k,), shift, device="cuda")
+    if shift == 1e8:
+        values[:64] += 8.0
+    else:
+        values[:64] += step
+    s = torch.stack([values, values], 1).reshape(-1).as_strided((n, k), (0, 2))
+    logp = (values.double() - torch.logsumexp(values.double() - shift, 0)) - shift
+    want = {"log_norm": torch.logsumexp(values.double() - shift, 0) + shift, "entropy": -(logp.exp() * logp).sum()}
+    got = ops.class_log_probs(s)
+    tol = U * (k / 32 + 128)
+    for name, w in want.items():
+        off = (getattr(got, name).double() - w).abs() - 2 * U * w.abs()
+        assert bool((off <= tol * (1 + math.log(k) * (name == "entropy"))).all()), (name, float(off.max()), tol)
+    if n * k > 10 ** 8:
+        return
+    grad = ops.class_log_probs_grad(s, got.log_norm, got.entropy, labels=torch.zeros(n, dtype=torch.int32, device="cuda"), grad_log_prob=torch.ones(n, device="cuda")).double()
+    ref = -logp.exp().expand(n, k).clone()
+    ref[:, 0] += 1
+    bound = logp.exp() * (U * (k / 32 + 256) + 8 * U * (16 + logp.abs())) + 4 * U * ref.abs()
+    assert bool(((grad - ref).abs() <= bound).all()), float(((grad - ref).abs() / bound).max())
